@@ -58,9 +58,11 @@ extern "C" {
 
 enum gptoss_attn_dtype {
     GPTOSS_ATTN_BF16 = 0, /* 2-byte bfloat16 tensors, bf16 MFMA products, fp32 accumulation: the fast path */
-    GPTOSS_ATTN_FP32 = 1  /* 4-byte float tensors, fp32 MFMA products (the reference's fp32 mode,
+    GPTOSS_ATTN_FP32 = 1, /* 4-byte float tensors, fp32 MFMA products (the reference's fp32 mode,
                              attention_kernel.py is dtype-generic), at a sixteenth of the bf16 matrix rate;
                              larger calls with scratch: gptoss_attn_split_bytes */
+    GPTOSS_ATTN_E4M3 = 2  /* storage of a paged cache only: 8-bit numbers (sign, 4 exponent and 3 mantissa bits, largest
+                             448, no infinity) with a power of two for each row of 64 */
 };
 
 enum gptoss_attn_status {
@@ -77,7 +79,9 @@ enum gptoss_attn_status {
     GPTOSS_ATTN_ERR_ALIGNMENT = -7,     /* a tensor base or stride breaks 16-byte row alignment */
     GPTOSS_ATTN_ERR_STRIDE = -8,        /* a sequence stride smaller than D or larger than 2^24 elements */
     GPTOSS_ATTN_ERR_ABI = -9,           /* struct_size does not match this library */
-    GPTOSS_ATTN_ERR_WORKSPACE = -10     /* gptoss_attn_bwd_static: 24*B*H*Sq bytes do not fit the built-in scratch */
+    GPTOSS_ATTN_ERR_WORKSPACE = -10,    /* gptoss_attn_bwd_static: 24*B*H*Sq bytes do not fit the built-in scratch */
+    GPTOSS_ATTN_ERR_PAGES = -11         /* paged cache: page_size no power of two from 16 to 1024, pages or table_width <= 0,
+                                           table_stride < 0, or table_width * page_size above 2^30 */
 };
 
 /* Size of the device array gptoss_attn_bwd_static keeps its row statistics in: 24 bytes per row must
@@ -317,6 +321,85 @@ int64_t gptoss_attn_stream_probe(int mix, int waves_per_simd, int iters, float *
  * requires the backward tensors.  Callable without a GPU.
  */
 int gptoss_attn_validate(const gptoss_attn_params *params, int need_bwd);
+
+/* ---- a key / value cache in pages --------------------------------------------------------------------------------
+ *
+ * The serving side of the same layer; the reference has no counterpart (its generate.py leaves the cache to transformers,
+ * one contiguous tensor per layer).  Keys and values of all sequences live in one pool of pages:
+ *   k_pages, v_pages (pages, G, page_size, 64) in `storage`: the model's type (`dtype`), or GPTOSS_ATTN_E4M3
+ *   k_exp, v_exp     (pages, G, page_size) bytes, E4M3 only: row values are code * 2^(byte - 127)
+ *   page_table       (B, table_width) int32, rows table_stride apart: token t of row b is slot t % page_size of page
+ *                    page_table[b][t / page_size].  An entry outside 0 .. pages - 1 names no page: what would be written
+ *                    there is dropped, what would be read from there is 0, its keys are invisible.
+ * Strides are in elements, (page, KV head, token); rows of 64 are contiguous and start on 16-byte boundaries.  Several rows
+ * of the table may name one page (a common prefix) for reading; where two rows of one call write the same slot, or a call
+ * writes what another one that may run at the same time reads, the outcome is unspecified.
+ *
+ * E4M3: a row's power of two is the smallest 2^s (s >= -64) with its largest finite number at most 448 * 2^s; the numbers
+ * divided by it are rounded to nearest, ties to even, so each is within 2^-4 of itself, or 2^(s-10) where that is more.
+ * Numbers that would come back as 2^128 are stored as 1.875 * 2^127, infinities and NaN as NaN.  What is read back is exact in bfloat16 as in float32.
+ */
+typedef struct gptoss_attn_paged_params {
+    uint32_t struct_size;   /* sizeof(gptoss_attn_paged_params), checked by every call */
+    int32_t dtype;          /* GPTOSS_ATTN_BF16 or GPTOSS_ATTN_FP32: type of q, o, k and v */
+    int32_t storage;        /* = dtype, or GPTOSS_ATTN_E4M3 */
+    int32_t sinks_dtype;    /* GPTOSS_ATTN_FP32 or GPTOSS_ATTN_BF16 */
+
+    int32_t B, H, G, Sq, D; /* Sq: query rows (fwd), new tokens of a row (write), rows of the result (read); H: fwd only */
+    int32_t pages, page_size, table_width;
+    int32_t window;         /* fwd: 0 = full causal; else sliding window length */
+    int32_t max_len;        /* fwd: a length that no sequence passes, if the caller knows one (0: not).  Only the division
+                               of the work goes by it; longer sequences are right too */
+    float scale;            /* fwd: softmax scale */
+    int32_t reserved0;
+
+    void *k_pages, *v_pages;        /* written by write only */
+    uint8_t *k_exp, *v_exp;
+    const int32_t *page_table;
+    const int32_t *seqlens;         /* (B): fwd, read: tokens of each row in the cache.  write: new tokens of each row, the rest
+                                       of its Sq is padding (NULL: all Sq) */
+    const int32_t *start;           /* (B): position of the row's first query / new token / row of the result.  fwd: NULL =
+                                       seqlens - Sq; read: NULL = 0 */
+    const void *q;                  /* (B, H, Sq, 64) */
+    const void *sinks;              /* (H), optional as in gptoss_attn_params */
+    void *o;                        /* (B, Sq, H, 64) through its strides */
+    float *lse;                     /* (B, H, Sq) */
+    void *k, *v;                    /* (B, G, Sq, 64): read by write, written by read */
+    void *scratch;                  /* fwd: gptoss_attn_paged_workspace_bytes() bytes, 16-byte aligned, of this call alone until it has run */
+    size_t scratch_bytes;
+
+    gptoss_attn_strides q_stride, o_stride, k_stride, v_stride;
+    gptoss_attn_strides k_page_stride, v_page_stride, k_exp_stride, v_exp_stride;
+    int64_t table_stride;
+} gptoss_attn_paged_params;
+
+/*
+ * New tokens into their pages: token i of row b, i < seqlens[b], goes to position start[b] + i.  Positions below 0, behind the
+ * table or on an entry that names no page are dropped.  Nothing but the written rows (and their bytes of k_exp, v_exp) is touched.
+ */
+int gptoss_attn_paged_write(const gptoss_attn_paged_params *params, void *stream);
+
+/*
+ * Rows back: row i of k and v is position start[b] + i, zero where that is below 0, at or behind seqlens[b] or the table's end, or on
+ * an entry that names no page.  Every row of the result is written.
+ */
+int gptoss_attn_paged_read(const gptoss_attn_paged_params *params, void *stream);
+
+/*
+ * Attention of a row's Sq queries over its pages, O and logsumexp.  Query i stands at position p = start[b] + i; it sees key j iff
+ * j <= p, j < n, window == 0 or j > p - window, and j's page exists, n = min(seqlens[b], table_width * page_size).  A query behind
+ * the sequence (p >= n), in front of it (p < 0) or without a visible key gives O = 0, lse = sink.  What stands in rows that a query
+ * does not see has no part in its result, infinities and NaN included.
+ * Any number of queries is right; the cache is read once for each 64 (query, head of the group) pairs, so the many queries of a
+ * prompt's chunk are better served by gptoss_attn_paged_read and gptoss_attn_fwd.
+ */
+int gptoss_attn_paged_fwd(const gptoss_attn_paged_params *params, void *stream);
+
+/* Bytes of scratch gptoss_attn_paged_fwd needs for this block (0: none; 0 for a NULL or shapeless block).  Host-only. */
+size_t gptoss_attn_paged_workspace_bytes(const gptoss_attn_paged_params *params);
+
+/* Host-only argument check that each of the three calls starts with; `call`: 0 fwd, 1 write, 2 read. */
+int gptoss_attn_paged_validate(const gptoss_attn_paged_params *params, int call);
 
 #ifdef __cplusplus
 }

@@ -12,6 +12,15 @@ from .attention_kernel import (  # noqa: F401
     hip_flash_attention,
     triton_flash_attention,
 )
+from .paged_cache import (  # noqa: F401
+    PagedCache,
+    paged_attention,
+    paged_attention_forward,
+    paged_cache,
+    paged_cache_read,
+    paged_cache_write,
+)
 
 __all__ = ["attention", "attention_forward", "attention_backward", "doc_start_from_position_ids",
-           "hip_flash_attention", "triton_flash_attention"]
+           "hip_flash_attention", "triton_flash_attention",
+           "PagedCache", "paged_cache", "paged_cache_write", "paged_cache_read", "paged_attention", "paged_attention_forward"]

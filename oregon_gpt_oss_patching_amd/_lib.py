@@ -16,6 +16,7 @@ TORCH_LIBRARY = os.path.join(_HERE, "libgptoss_torch.so")    # the PyTorch opera
 ABI_VERSION = 4
 DTYPE_BF16 = 0
 DTYPE_FP32 = 1
+DTYPE_E4M3 = 2          # storage of a paged cache only
 
 EXPORTS = (
     "gptoss_attn_version",
@@ -37,6 +38,11 @@ EXPORTS = (
     "gptoss_attn_bwd_static",
     "gptoss_attn_static_scratch_bytes",
     "gptoss_attn_doc_start",
+    "gptoss_attn_paged_fwd",
+    "gptoss_attn_paged_write",
+    "gptoss_attn_paged_read",
+    "gptoss_attn_paged_workspace_bytes",
+    "gptoss_attn_paged_validate",
     "gptoss_attn_mfma_rate_probe",
     "gptoss_attn_stream_probe",
 )
@@ -71,6 +77,36 @@ class Params(ctypes.Structure):
         ("q_stride", Strides), ("k_stride", Strides), ("v_stride", Strides), ("o_stride", Strides),
         ("do_stride", Strides), ("dq_stride", Strides), ("dk_stride", Strides), ("dv_stride", Strides),
         ("q_offset_dev", ctypes.c_void_p),
+    ]
+
+
+class PagedParams(ctypes.Structure):
+    """Mirror of `gptoss_attn_paged_params`; field order and types must match the header."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32), ("storage", ctypes.c_int32), ("sinks_dtype", ctypes.c_int32),
+        ("B", ctypes.c_int32), ("H", ctypes.c_int32), ("G", ctypes.c_int32), ("Sq", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("table_width", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("reserved0", ctypes.c_int32),
+        ("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p),
+        ("k_exp", ctypes.c_void_p), ("v_exp", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("seqlens", ctypes.c_void_p),
+        ("start", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("sinks", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("scratch", ctypes.c_void_p),
+        ("scratch_bytes", ctypes.c_size_t),
+        ("q_stride", Strides), ("o_stride", Strides), ("k_stride", Strides), ("v_stride", Strides),
+        ("k_page_stride", Strides), ("v_page_stride", Strides), ("k_exp_stride", Strides), ("v_exp_stride", Strides),
+        ("table_stride", ctypes.c_int64),
     ]
 
 
@@ -131,6 +167,14 @@ def load() -> ctypes.CDLL:
                                                 ctypes.c_void_p]
         lib.gptoss_attn_split_bytes.restype = ctypes.c_size_t
         lib.gptoss_attn_split_bytes.argtypes = [ctypes.POINTER(Params), ctypes.c_int]
+        for name in ("gptoss_attn_paged_fwd", "gptoss_attn_paged_write", "gptoss_attn_paged_read"):
+            fn = getattr(lib, name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(PagedParams), ctypes.c_void_p]
+        lib.gptoss_attn_paged_workspace_bytes.restype = ctypes.c_size_t
+        lib.gptoss_attn_paged_workspace_bytes.argtypes = [ctypes.POINTER(PagedParams)]
+        lib.gptoss_attn_paged_validate.restype = ctypes.c_int
+        lib.gptoss_attn_paged_validate.argtypes = [ctypes.POINTER(PagedParams), ctypes.c_int]
         if lib.gptoss_attn_version() != ABI_VERSION:
             raise RuntimeError("libgptoss_attn.so ABI version mismatch; rebuild the library")
         _lib = lib

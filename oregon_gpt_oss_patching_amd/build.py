@@ -12,8 +12,10 @@ import sysconfig
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCE = os.path.join(_HERE, "csrc", "gptoss_attn.hip")
+PAGED_SOURCE = os.path.join(_HERE, "csrc", "gptoss_paged.hip")
 LIBRARY = os.path.join(_HERE, "libgptoss_attn.so")
 TORCH_SOURCE = os.path.join(_HERE, "csrc", "torch_ops.cpp")
+TORCH_PAGED_SOURCE = os.path.join(_HERE, "csrc", "torch_paged.cpp")
 TORCH_LIBRARY = os.path.join(_HERE, "libgptoss_torch.so")
 
 HIPCC_FLAGS = [
@@ -46,7 +48,7 @@ def _run(cmd, verbose: bool) -> None:
 
 
 def build_library(verbose: bool = False) -> str:
-    _run([hipcc_path(), *HIPCC_FLAGS, "-o", LIBRARY, SOURCE], verbose)
+    _run([hipcc_path(), *HIPCC_FLAGS, "-o", LIBRARY, SOURCE, PAGED_SOURCE], verbose)
     return LIBRARY
 
 
@@ -58,7 +60,7 @@ def build_torch_ops(verbose: bool = False) -> str:
     _run([shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
           "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
-          "-isystem", os.path.join(rocm, "include"), "-isystem", sysconfig.get_paths()["include"], "-o", TORCH_LIBRARY, TORCH_SOURCE,
+          "-isystem", os.path.join(rocm, "include"), "-isystem", sysconfig.get_paths()["include"], "-o", TORCH_LIBRARY, TORCH_SOURCE, TORCH_PAGED_SOURCE,
           "-L" + os.path.join(root, "lib"), "-lc10", "-ltorch_cpu", "-lc10_hip", "-ltorch_hip", "-L" + _HERE, "-lgptoss_attn", "-Wl,-rpath,$ORIGIN"], verbose)
     return TORCH_LIBRARY
 

@@ -688,6 +688,7 @@ const char *gptoss_attn_status_string(int status) {
         case GPTOSS_ATTN_ERR_STRIDE: return "sequence stride smaller than head_dim or larger than 2^24 elements";
         case GPTOSS_ATTN_ERR_ABI: return "struct_size does not match this library";
         case GPTOSS_ATTN_ERR_WORKSPACE: return "the problem needs more scratch than the library's built-in array holds (gptoss_attn_static_scratch_bytes)";
+        case GPTOSS_ATTN_ERR_PAGES: return "page_size must be a power of two from 16 to 1024, pages and table_width positive, table_stride not negative, and table_width * page_size at most 2^30";
         default: return status > 0 ? "HIP runtime error (status is the hipError_t)" : "unknown status";
     }
 }

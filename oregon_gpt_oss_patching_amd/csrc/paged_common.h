@@ -1,0 +1,92 @@
+// A key / value cache in pages: what its kernels share (the arguments, the page of a token, rows of 64 as they are stored).
+//
+// A stored row is 64 numbers of the model's type, or 64 e4m3 codes and a byte e: the row is code * 2^(e - 127).  A power of two
+// makes both directions exact but for the one rounding to e4m3: codes widen to bf16 (four significant bits), and so do their
+// products with 2^s.  A divisor of largest / 448, which fills the format's range, would save at most one bit in the numbers below
+// 2^-15 of the row's largest, and cost a rounding in each direction.
+#pragma once
+#include "attn_common.h"
+
+namespace gptoss {
+
+struct PagedArgs {
+    const void *q, *sinks;
+    void *o;
+    float *lse;
+    char *k_pages, *v_pages;
+    uint8_t *k_exp, *v_exp;
+    const int32_t *table, *seqlens, *start;
+    char *k, *v;                 // rows to write, or the result of reading
+    Strides qs, os, ks, vs;      // elements
+    Strides kps, vps, kes, ves;  // (page, KV head, token), elements
+    int64_t table_stride;
+    int B, H, G, r, Sq;
+    int pages, page_shift, width, window;
+    int blocks;                  // workgroups of a batch row (write), of a row and KV head (read)
+    float scale_log2;
+    bool sinks_bf16;
+};
+
+constexpr int kExpBias = 127, kMinExp = -64, kMaxExp = 120;       // exponent bytes; the powers of two of rows
+constexpr float kLowest = -3.0e38f;                // start of a running maximum: finite, so that -inf - (it) is -inf and not NaN
+
+__device__ __forceinline__ float paged_sink(const PagedArgs &a, int head) {
+    if (!a.sinks) return 0.0f;
+    return a.sinks_bf16 ? (float)static_cast<const bf16 *>(a.sinks)[head] : static_cast<const float *>(a.sinks)[head];
+}
+
+// Page of token t of a row, -1 where there is none (t outside the table, an entry outside the pool).
+__device__ __forceinline__ int paged_page(const PagedArgs &a, int b, int t) {
+    if (t < 0 || (t >> a.page_shift) >= a.width) return -1;
+    const int page = a.table[(int64_t)b * a.table_stride + (t >> a.page_shift)];
+    return (unsigned)page < (unsigned)a.pages ? page : -1;
+}
+
+// Tokens of a row in the cache.
+__device__ __forceinline__ int paged_length(const PagedArgs &a, int b) {
+    return min(max(a.seqlens[b], 0), a.width << a.page_shift);
+}
+
+__device__ __forceinline__ float exp_of_byte(uint32_t e) { return __uint_as_float(e << 23); }        // 2^(e - 127), e >= 1
+
+// Element offset of slot t of a page.
+__device__ __forceinline__ int64_t slot_offset(const Strides &s, int page, int g, int t, int page_shift) {
+    return page * s.b + g * s.h + (int64_t)(t & ((1 << page_shift) - 1)) * s.s;
+}
+
+struct e4m3 { uint8_t code; };
+
+// Eight numbers of a row.
+__device__ __forceinline__ void load8(const bf16 *p, float (&x)[8]) {
+    const bf16x8 v = as_bf16x8(*reinterpret_cast<const u32x4 *>(p));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+}
+__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
+    const f32x4 u = *reinterpret_cast<const f32x4 *>(p), w = *reinterpret_cast<const f32x4 *>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[i] = u[i]; x[4 + i] = w[i]; }
+}
+__device__ __forceinline__ void load8(const e4m3 *p, float (&x)[8]) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(p);
+    x[0] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 0);
+    x[1] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 1);
+    x[2] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 2);
+    x[3] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 3);
+    x[4] = __builtin_amdgcn_cvt_f32_fp8((int)w.y, 0);
+    x[5] = __builtin_amdgcn_cvt_f32_fp8((int)w.y, 1);
+    x[6] = __builtin_amdgcn_cvt_f32_fp8((int)w.y, 2);
+    x[7] = __builtin_amdgcn_cvt_f32_fp8((int)w.y, 3);
+}
+__device__ __forceinline__ void store8(bf16 *p, const float (&x)[8]) {
+    union { bf16x8 v; u32x4 u; } out;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out.v[i] = (bf16)x[i];
+    *reinterpret_cast<u32x4 *>(p) = out.u;
+}
+__device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
+    *reinterpret_cast<f32x4 *>(p) = f32x4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<f32x4 *>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+}
+
+}  // namespace gptoss

@@ -9,38 +9,12 @@
 // (an autograd.Function around two Python custom operators and a ctypes call each: 250 us per forward + backward
 // whatever the size; the same calls through this file take 60 to 90 us for two rows of 383 tokens, 88 for a sliding-window layer of
 // 4096, of which 64 and 83 are kernels, and a decoding step 13 us instead of 44).  This file is built against torch; the kernels are not.
-#include <ATen/ATen.h>
-#include <ATen/hip/EmptyTensor.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <pybind11/pybind11.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/library.h>
 
-#include "../../include/gptoss_attn.h"
+#include "torch_common.h"
 
 namespace {
-
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-using c10::SymInt;
-
-constexpr int64_t kMaxSeqStride = int64_t(1) << 24;   // elements; the library refuses larger sequence strides (ERR_STRIDE)
-
-// The kernels need unit stride along head_dim, 16-byte aligned rows and a sequence stride of at least head_dim and at most
-// 2^24 elements; anything else is copied.
-Tensor row_contiguous(const Tensor &t, int64_t seq_dim) {
-    const auto st = t.strides();
-    const int64_t eb = t.element_size();
-    const bool ok = st[3] == 1 && (st[0] * eb) % 16 == 0 && (st[1] * eb) % 16 == 0 && (st[2] * eb) % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 && st[seq_dim] >= t.size(3) && st[seq_dim] <= kMaxSeqStride;
-    return ok ? t : t.contiguous();
-}
-
-void require_on(const Tensor &q, const char *name, const Tensor &t) {
-    TORCH_CHECK(t.device() == q.device(), name, " is on ", t.device(), " but q is on ", q.device(), ": every tensor must be on q's GPU");
-}
 
 // What can be looked at without a size (a traced call's sizes are symbols, and reading one as a number would tie the traced
 // program to it).
@@ -63,17 +37,6 @@ void check_inputs(const Tensor &q, const Tensor &k, const Tensor &v, const OptTe
     }
     require_on(q, "k", k);
     require_on(q, "v", v);
-}
-
-// Memory for a result or for scratch, without the dispatcher: every value of it is written before it is read.  A call's allocations are a tenth of its host time.
-Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor &like) {
-    return Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt));
-}
-
-void set(gptoss_attn_strides &s, const Tensor &t, bool bshd) {
-    s.b = t.stride(0);
-    s.h = t.stride(bshd ? 2 : 1);
-    s.s = t.stride(bshd ? 1 : 2);
 }
 
 // The parameter block and the tensors it points into.
@@ -133,15 +96,6 @@ void fill(Call &c, const Tensor &q, const Tensor &k, const Tensor &v, const OptT
 }
 
 void *stream_of(const Call &c) { return c10::hip::getCurrentHIPStream(c.q.device().index()).stream(); }
-
-// A failed library call is the package's GptossAttnError wherever it happens: in a call, a backward or a traced program.
-void check(const char *name, int rc) {
-    if (rc == 0) return;
-    const pybind11::gil_scoped_acquire gil;
-    const pybind11::object type = pybind11::module_::import("oregon_gpt_oss_patching_amd._lib").attr("GptossAttnError");
-    PyErr_SetObject(type.ptr(), type(name, rc, gptoss_attn_status_string(rc)).ptr());
-    throw pybind11::error_already_set();
-}
 
 std::tuple<Tensor, Tensor> fwd(const Tensor &q, const Tensor &k, const Tensor &v, const OptTensor &sinks, double sm_scale, int64_t window,
                                int64_t q_offset, const OptTensor &seqlens, const OptTensor &doc_start, const OptTensor &q_offset_dev) {

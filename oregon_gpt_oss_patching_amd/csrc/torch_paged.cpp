@@ -1,0 +1,234 @@
+// PyTorch operators of the key / value cache in pages (gptoss_attn_paged_* in include/gptoss_attn.h): argument checks, allocation and launch.
+//
+//   gptoss_attn::paged_write, paged_read, paged_fwd      the three library calls; none has a gradient
+//
+// Native for the same reason as attention() (torch_ops.cpp): a decoding step makes two of these calls for each layer, and each takes
+// a few microseconds on the GPU.
+#include <climits>
+
+#include "torch_common.h"
+
+namespace {
+
+int32_t size32(int64_t n) {
+    TORCH_CHECK(n <= INT_MAX, "a dimension of ", n, " is too long");
+    return static_cast<int32_t>(n);
+}
+
+int abi_dtype(at::ScalarType t) { return t == at::kFloat ? GPTOSS_ATTN_FP32 : t == at::kBFloat16 ? GPTOSS_ATTN_BF16 : t == at::kFloat8_e4m3fn ? GPTOSS_ATTN_E4M3 : -1; }
+
+void set3(gptoss_attn_strides &s, const Tensor &t) {
+    s.b = t.stride(0);
+    s.h = t.stride(1);
+    s.s = t.stride(2);
+}
+
+void require_near(const Tensor &pages, const char *name, const Tensor &t) {
+    TORCH_CHECK(t.device() == pages.device(), name, " is on ", t.device(), " but the cache is on ", pages.device(), ": every tensor must be on the cache's GPU");
+}
+
+// The parameter block and the tensors it points into.
+struct PagedCall {
+    gptoss_attn_paged_params p{};
+    Tensor table, seqlens, start, sinks, q, k, v, scratch;
+};
+
+Tensor lengths_of(const Tensor &t, const Tensor &pages, int64_t batch, const char *name) {
+    TORCH_CHECK(!t.is_floating_point() && t.numel() == batch, name, " must hold one integer per batch row");
+    return t.to(pages.device(), at::kInt).contiguous();
+}
+
+// The cache, the table and what all calls have; `dtype`: the model's type.
+void fill(PagedCall &c, const Tensor &k_pages, const Tensor &v_pages, const OptTensor &k_exp, const OptTensor &v_exp, const Tensor &page_table,
+          at::ScalarType dtype, int64_t batch) {
+    TORCH_CHECK(k_pages.is_cuda(), "gptoss attention runs on the GPU only (HIP kernels); the cache is on ", k_pages.device());
+    require_near(k_pages, "v of the cache", v_pages);
+    const auto storage = k_pages.scalar_type();
+    TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "unsupported dtype ", dtype, ": bfloat16 or float32");
+    TORCH_CHECK(v_pages.scalar_type() == storage && (storage == dtype || storage == at::kFloat8_e4m3fn), "a cache of ", storage, "/", v_pages.scalar_type(),
+                " does not go with tensors of ", dtype, ": it holds their type or float8_e4m3fn");
+    TORCH_CHECK(k_pages.dim() == 4 && k_pages.sizes() == v_pages.sizes() && k_pages.size(3) == 64, "the cache's k and v must both be (pages, G, page_size, 64), got ",
+                k_pages.sizes(), " and ", v_pages.sizes());
+    gptoss_attn_paged_params &p = c.p;
+    p.struct_size = sizeof(p);
+    p.dtype = abi_dtype(dtype);
+    p.storage = abi_dtype(storage);
+    if (storage == at::kFloat8_e4m3fn) {
+        TORCH_CHECK(k_exp && v_exp, "a float8_e4m3fn cache needs its exponents");
+        for (const auto &[name, t, e] : {std::tuple<const char *, const Tensor &, uint8_t **>("k_exp", *k_exp, &p.k_exp), {"v_exp", *v_exp, &p.v_exp}}) {
+            require_near(k_pages, name, t);
+            TORCH_CHECK(t.scalar_type() == at::kByte && t.sizes() == k_pages.sizes().slice(0, 3), name, " must be uint8 (pages, G, page_size), got ", t.scalar_type(), " ", t.sizes());
+            *e = const_cast<uint8_t *>(t.const_data_ptr<uint8_t>());
+        }
+        set3(p.k_exp_stride, *k_exp);
+        set3(p.v_exp_stride, *v_exp);
+    }
+    p.pages = size32(k_pages.size(0));
+    p.G = size32(k_pages.size(1));
+    p.page_size = size32(k_pages.size(2));
+    p.D = 64;
+    p.B = size32(batch);
+    p.k_pages = const_cast<void *>(k_pages.const_data_ptr());
+    p.v_pages = const_cast<void *>(v_pages.const_data_ptr());
+    set3(p.k_page_stride, k_pages);
+    set3(p.v_page_stride, v_pages);
+    TORCH_CHECK(page_table.dim() == 2 && page_table.size(0) == batch && !page_table.is_floating_point(), "page_table must be (B, pages of a row) integers, got ",
+                page_table.sizes(), " for ", batch, " rows");
+    c.table = page_table.to(k_pages.device(), at::kInt);
+    if (c.table.stride(1) != 1 && c.table.size(1) > 1) c.table = c.table.contiguous();
+    p.table_width = size32(c.table.size(1));
+    p.table_stride = c.table.stride(0);
+    p.page_table = c.table.const_data_ptr<int32_t>();
+}
+
+// Rows (B, G, S, 64) or (B, H, S, 64) as the kernels take them; a dimension of one element has a stride that says nothing.
+Tensor rows_of(const Tensor &t, gptoss_attn_strides &s) {
+    const bool one = t.size(2) == 1 && t.stride(2) < 64;
+    const Tensor r = one ? row_contiguous(t.as_strided(t.sizes(), {t.stride(0), t.stride(1), 64, t.stride(3)}), 2) : row_contiguous(t, 2);
+    set3(s, r);
+    return r;
+}
+
+void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+void paged_write(const Tensor &k_pages, const Tensor &v_pages, const OptTensor &k_exp, const OptTensor &v_exp, const Tensor &k_, const Tensor &v_,
+                 const Tensor &page_table, const Tensor &start, const OptTensor &seqlens) {
+    const c10::OptionalDeviceGuard guard(k_pages.device());
+    TORCH_CHECK(k_.scalar_type() == v_.scalar_type(), "k and v must be of one type, got ", k_.scalar_type(), " and ", v_.scalar_type());
+    TORCH_CHECK(k_.dim() == 4 && k_.sizes() == v_.sizes(), "k and v must both be (B, G, S, 64), got ", k_.sizes(), " and ", v_.sizes());
+    const bool half = k_.scalar_type() == at::kHalf;
+    PagedCall c;
+    fill(c, k_pages, v_pages, k_exp, v_exp, page_table, half ? at::kBFloat16 : k_.scalar_type(), k_.size(0));
+    TORCH_CHECK(k_.size(1) == c.p.G && k_.size(3) == 64, "k and v must be (B, ", c.p.G, ", S, 64) for this cache, got ", k_.sizes());
+    require_near(k_pages, "k", k_);
+    require_near(k_pages, "v", v_);
+    c.k = rows_of(half ? k_.to(at::kBFloat16) : k_, c.p.k_stride);
+    c.v = rows_of(half ? v_.to(at::kBFloat16) : v_, c.p.v_stride);
+    c.p.k = const_cast<void *>(c.k.const_data_ptr());
+    c.p.v = const_cast<void *>(c.v.const_data_ptr());
+    c.p.Sq = size32(k_.size(2));
+    c.start = lengths_of(start, k_pages, c.p.B, "start");
+    c.p.start = c.start.const_data_ptr<int32_t>();
+    if (seqlens) {
+        c.seqlens = lengths_of(*seqlens, k_pages, c.p.B, "seqlens");
+        c.p.seqlens = c.seqlens.const_data_ptr<int32_t>();
+    }
+    check("gptoss_attn_paged_write", gptoss_attn_paged_write(&c.p, stream_of(k_pages)));
+    for (const Tensor *t : {&k_pages, &v_pages, k_exp ? &*k_exp : nullptr, v_exp ? &*v_exp : nullptr})
+        if (t) t->unsafeGetTensorImpl()->bump_version();
+}
+
+std::tuple<Tensor, Tensor> paged_read(const Tensor &k_pages, const Tensor &v_pages, const OptTensor &k_exp, const OptTensor &v_exp, const Tensor &page_table,
+                                      const Tensor &seqlens, int64_t max_len, const OptTensor &start, at::ScalarType dtype) {
+    const c10::OptionalDeviceGuard guard(k_pages.device());
+    const bool half = dtype == at::kHalf;
+    const int64_t batch = seqlens.numel();
+    PagedCall c;
+    fill(c, k_pages, v_pages, k_exp, v_exp, page_table, half ? at::kBFloat16 : dtype, batch);
+    TORCH_CHECK(max_len > 0, "max_len must be positive, got ", max_len);
+    c.p.Sq = size32(max_len);
+    c.seqlens = lengths_of(seqlens, k_pages, batch, "seqlens");
+    c.p.seqlens = c.seqlens.const_data_ptr<int32_t>();
+    if (start) {
+        c.start = lengths_of(*start, k_pages, batch, "start");
+        c.p.start = c.start.const_data_ptr<int32_t>();
+    }
+    Tensor k = new_tensor({batch, c.p.G, max_len, 64}, half ? at::kBFloat16 : dtype, k_pages), v = new_tensor(k.sizes(), k.scalar_type(), k_pages);
+    set3(c.p.k_stride, k);
+    set3(c.p.v_stride, v);
+    c.p.k = k.data_ptr();
+    c.p.v = v.data_ptr();
+    check("gptoss_attn_paged_read", gptoss_attn_paged_read(&c.p, stream_of(k_pages)));
+    return half ? std::make_tuple(k.to(dtype), v.to(dtype)) : std::make_tuple(k, v);
+}
+
+std::tuple<Tensor, Tensor> paged_fwd(const Tensor &q_, const Tensor &k_pages, const Tensor &v_pages, const OptTensor &k_exp, const OptTensor &v_exp,
+                                     const Tensor &page_table, const Tensor &seqlens, const OptTensor &start, const OptTensor &sinks, double sm_scale,
+                                     int64_t window, int64_t max_len) {
+    const c10::OptionalDeviceGuard guard(k_pages.device());
+    TORCH_CHECK(q_.dim() == 4 && q_.size(3) == 64, "q must be (B, H, S, 64), got ", q_.sizes());
+    const bool half = q_.scalar_type() == at::kHalf;
+    const int64_t b = q_.size(0), h = q_.size(1), s = q_.size(2);
+    PagedCall c;
+    fill(c, k_pages, v_pages, k_exp, v_exp, page_table, half ? at::kBFloat16 : q_.scalar_type(), b);
+    require_near(k_pages, "q", q_);
+    gptoss_attn_paged_params &p = c.p;
+    c.q = rows_of(half ? q_.to(at::kBFloat16) : q_, p.q_stride);
+    p.q = c.q.const_data_ptr();
+    p.H = size32(h);
+    p.Sq = size32(s);
+    TORCH_CHECK(window >= 0 && window <= INT_MAX && max_len >= 0, "the window and max_len must not be negative");
+    p.window = static_cast<int32_t>(window);
+    p.max_len = static_cast<int32_t>(std::min<int64_t>(max_len, INT_MAX));
+    p.scale = static_cast<float>(sm_scale);
+    c.seqlens = lengths_of(seqlens, k_pages, b, "seqlens");
+    p.seqlens = c.seqlens.const_data_ptr<int32_t>();
+    if (start) {
+        c.start = lengths_of(*start, k_pages, b, "start");
+        p.start = c.start.const_data_ptr<int32_t>();
+    }
+    p.sinks_dtype = GPTOSS_ATTN_FP32;
+    if (sinks) {
+        require_near(k_pages, "sinks", *sinks);
+        TORCH_CHECK(sinks->numel() == h, "sinks must hold one logit per query head");
+        const bool bf16 = sinks->scalar_type() == at::kBFloat16;
+        c.sinks = (bf16 ? *sinks : sinks->to(at::kFloat)).contiguous();
+        p.sinks_dtype = bf16 ? GPTOSS_ATTN_BF16 : GPTOSS_ATTN_FP32;
+        p.sinks = c.sinks.const_data_ptr();
+    }
+    Tensor o = new_tensor({b, s, h, 64}, c.q.scalar_type(), k_pages), lse = new_tensor({b, h, s}, at::kFloat, k_pages);
+    set(p.o_stride, o, true);
+    p.o = o.data_ptr();
+    p.lse = lse.data_ptr<float>();
+    p.scratch_bytes = gptoss_attn_paged_workspace_bytes(&p);
+    if (p.scratch_bytes) {
+        c.scratch = new_tensor({static_cast<int64_t>(p.scratch_bytes / sizeof(float))}, at::kFloat, k_pages);
+        p.scratch = c.scratch.data_ptr();
+    }
+    check("gptoss_attn_paged_fwd", gptoss_attn_paged_fwd(&p, stream_of(k_pages)));
+    return {half ? o.to(at::kHalf) : o, lse};
+}
+
+// Tensors that want a gradient are refused, as these calls would drop it without a word.
+void refuse_gradients(const c10::OperatorHandle &op, c10::DispatchKeySet keys, torch::jit::Stack *stack) {
+    if (at::GradMode::is_enabled()) {
+        const size_t n = op.schema().arguments().size();
+        for (size_t i = stack->size() - n; i < stack->size(); ++i)
+            TORCH_CHECK(!(*stack)[i].isTensor() || !(*stack)[i].toTensor().requires_grad(), op.schema().name(),
+                        " has no gradient: call it under torch.no_grad() (argument ", op.schema().arguments()[i + n - stack->size()].name(), " requires one)");
+    }
+    const at::AutoDispatchBelowADInplaceOrView below;
+    op.redispatchBoxed(keys & c10::after_ADInplaceOrView_keyset, stack);
+}
+
+void refuse_cpu(const c10::OperatorHandle &, torch::jit::Stack *) {
+    TORCH_CHECK(false, "gptoss attention runs on the GPU only (HIP kernels); got CPU tensors");
+}
+
+void refuse_vmap(const c10::OperatorHandle &, torch::jit::Stack *) {
+    TORCH_CHECK(false, "gptoss attention cannot be vmapped: its tensors have a batch dimension of their own");
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(gptoss_attn, m) {
+    m.def("paged_write(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_exp, Tensor(d!)? v_exp, Tensor k, Tensor v, Tensor page_table, Tensor start, "
+          "Tensor? seqlens) -> ()");
+    m.def("paged_read(Tensor k_pages, Tensor v_pages, Tensor? k_exp, Tensor? v_exp, Tensor page_table, Tensor seqlens, SymInt max_len, Tensor? start, "
+          "ScalarType dtype) -> (Tensor, Tensor)");
+    m.def("paged_fwd(Tensor q, Tensor k_pages, Tensor v_pages, Tensor? k_exp, Tensor? v_exp, Tensor page_table, Tensor seqlens, Tensor? start, Tensor? sinks, "
+          "float sm_scale, SymInt window, SymInt max_len) -> (Tensor, Tensor)");
+}
+TORCH_LIBRARY_IMPL(gptoss_attn, CUDA, m) {
+    m.impl("paged_write", &paged_write);
+    m.impl("paged_read", &paged_read);
+    m.impl("paged_fwd", &paged_fwd);
+}
+#define GPTOSS_PAGED_IMPL(KEY, FN)                                                        \
+    TORCH_LIBRARY_IMPL(gptoss_attn, KEY, m) {                                             \
+        for (const char *name : {"paged_write", "paged_read", "paged_fwd"})               \
+            m.impl(name, torch::CppFunction::makeFromBoxedFunction<&FN>());               \
+    }
+GPTOSS_PAGED_IMPL(Autograd, refuse_gradients)
+GPTOSS_PAGED_IMPL(CPU, refuse_cpu)
+GPTOSS_PAGED_IMPL(FuncTorchBatched, refuse_vmap)

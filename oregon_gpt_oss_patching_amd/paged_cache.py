@@ -1,0 +1,132 @@
+"""A key / value cache in pages and the attention that reads it, for decoding with the layers that `attention` trains.
+
+The sequences of a serving batch share one pool of pages per layer, `PagedCache`, and each has a row of page numbers in a
+`page_table` (B, pages of a row): token t stands in slot t % page_size of page page_table[b, t // page_size].  An entry outside
+the pool (-1, say) names no page.  The pool holds the model's type, or 8-bit e4m3 numbers with a power of two for each row of
+64: half of bfloat16's memory and traffic, each number within 2^-4 of itself.
+
+    cache = paged_cache(pages, kv_heads, page_size=64, storage=torch.float8_e4m3fn)
+    paged_cache_write(cache, k, v, page_table, start)                     # new tokens' keys and values, (B, G, S, 64)
+    out = paged_attention(q, cache, page_table, start + S, sinks, scale, window)      # (B, S, H, 64), as attention()
+    k, v = paged_cache_read(cache, page_table, seqlens, max_len)          # rows back, for attention() of a long prompt's chunk
+
+Everything that says where tokens stand (`page_table`, `start`, `seqlens`) stays on the GPU and is read there: the calls do not
+synchronise and can be captured into a graph that is replayed with other contents.  None has a gradient.
+
+The reference has no counterpart: its generate.py leaves the cache to transformers (generate.py:1-30).
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from . import attention_kernel as _ak
+
+__all__ = ["PagedCache", "paged_cache", "paged_cache_write", "paged_cache_read", "paged_attention", "paged_attention_forward"]
+
+
+class PagedCache(NamedTuple):
+    """k, v: (pages, G, page_size, 64), bfloat16, float32 or float8_e4m3fn, page_size a power of two from 16 to 1024; rows of 64 must be
+    contiguous and start on 16-byte boundaries, the other strides are free.  k_exp, v_exp: float8_e4m3fn only, (pages, G, page_size)
+    uint8, a row's values are its numbers times 2^(byte - 127)."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_exp: Optional[torch.Tensor] = None
+    v_exp: Optional[torch.Tensor] = None
+
+
+def paged_cache(pages, kv_heads, page_size=64, storage=torch.bfloat16, device="cuda") -> PagedCache:
+    """An empty cache (all zeros) of one layer."""
+    if storage not in (torch.bfloat16, torch.float32, torch.float8_e4m3fn):
+        raise RuntimeError(f"unsupported storage {storage}: bfloat16, float32 or float8_e4m3fn")
+    if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+        raise RuntimeError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
+    shape = (pages, kv_heads, page_size)
+    k, v = (torch.zeros((*shape, 64), dtype=storage, device=device) for _ in range(2))
+    if storage != torch.float8_e4m3fn:
+        return PagedCache(k, v)
+    return PagedCache(k, v, *(torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2)))
+
+
+_ready = False
+_write = _read = _fwd = None
+
+
+def _register_ops() -> None:
+    global _ready, _write, _read, _fwd
+    _lib.load_torch_ops()
+    ops = torch.ops.gptoss_attn
+
+    @torch.library.register_fake(f"{_ak.OP_NAMESPACE}::paged_write")
+    def _write_fake(k_pages, v_pages, k_exp, v_exp, k, v, page_table, start, seqlens):
+        return None
+
+    @torch.library.register_fake(f"{_ak.OP_NAMESPACE}::paged_read")
+    def _read_fake(k_pages, v_pages, k_exp, v_exp, page_table, seqlens, max_len, start, dtype):
+        shape = (page_table.shape[0], k_pages.shape[1], max_len, 64)
+        return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+
+    @torch.library.register_fake(f"{_ak.OP_NAMESPACE}::paged_fwd")
+    def _fwd_fake(q, k_pages, v_pages, k_exp, v_exp, page_table, seqlens, start, sinks, sm_scale, window, max_len):
+        b, h, s, d = q.shape
+        return q.new_empty((b, s, h, d)), q.new_empty((b, h, s), dtype=torch.float32)
+
+    _write, _read, _fwd = ops.paged_write.default, ops.paged_read.default, ops.paged_fwd.default
+    _ready = True
+
+
+try:
+    _register_ops()
+except Exception:       # not built yet: importing has to work for the build itself; the first call tries again and raises
+    pass
+
+
+def _ints(x, like):
+    return x if x is None or torch.is_tensor(x) else torch.as_tensor(x, dtype=torch.int32, device=like.device)
+
+
+def paged_cache_write(cache: PagedCache, k, v, page_table, start, seqlens=None) -> None:
+    """Writes new tokens: k, v (B, G, S, 64), any strides; token i of row b goes to position start[b] + i.  `seqlens`: how many of its S
+    tokens each row has, the rest being padding, which is not written.  Positions in front of 0, behind the table, or on an entry that
+    names no page are dropped; nothing else of the cache is touched.  float16 tensors are rounded to bfloat16 on the way in.
+
+    Two rows of one call must not write the same slot, and nothing that runs at the same time may read what is being written."""
+    if not _ready:
+        _register_ops()
+    _write(cache.k, cache.v, cache.k_exp, cache.v_exp, k, v, _ints(page_table, cache.k), _ints(start, cache.k), _ints(seqlens, cache.k))
+
+
+def paged_cache_read(cache: PagedCache, page_table, seqlens, max_len, start=None, dtype=None):
+    """Rows back out of the pages: k, v (B, G, max_len, 64), row i being position start[b] + i (start: 0).  Zero at and behind seqlens[b], in
+    front of 0 and where an entry names no page.  `dtype`: the cache's, or of an e4m3 cache bfloat16 (exact), float32 or float16.
+
+    The keys and values that a chunk of a long prompt sees, for `attention(q, k, v, sinks, scale, window, start_q)`."""
+    if not _ready:
+        _register_ops()
+    if dtype is None:
+        dtype = torch.bfloat16 if cache.k.dtype == torch.float8_e4m3fn else cache.k.dtype
+    return _read(cache.k, cache.v, cache.k_exp, cache.v_exp, _ints(page_table, cache.k), _ints(seqlens, cache.k), int(max_len), _ints(start, cache.k), dtype)
+
+
+def paged_attention_forward(q, cache: PagedCache, page_table, seqlens, sinks, sm_scale, bandwidth=None, start=None, max_len=None):
+    """`paged_attention` that returns (o, lse (B, H, S) float32)."""
+    if not _ready:
+        _register_ops()
+    return _fwd(q, cache.k, cache.v, cache.k_exp, cache.v_exp, _ints(page_table, q), _ints(seqlens, q), _ints(start, q), sinks, float(sm_scale),
+                int(bandwidth or 0), int(max_len or 0))
+
+
+def paged_attention(q, cache: PagedCache, page_table, seqlens, sinks, sm_scale, bandwidth=None, start=None, max_len=None):
+    """Attention of each row's new queries q (B, H, S, 64) over the row's tokens in the cache, the new ones among them: (B, S, H, 64).
+
+    `seqlens` (B): tokens of each row in the cache.  Query i of row b stands at position start[b] + i (start: seqlens - S, the last S tokens)
+    and sees the keys at and before it, with `bandwidth` the last so many of them.  Queries at or behind seqlens[b] are padding: they
+    give 0, as does a query that sees no key.  What stands in rows that a query does not see has no part in its result.
+    `sinks`, `sm_scale`, `bandwidth`: as in `attention` (sinks=None: a logit of 0; logits of -inf: no sink).
+    `max_len`: a length that no row passes, if the caller knows one shorter than the table; it only helps to divide the work.
+
+    The cache is read once for each 64 pairs of a query and a head of its KV head's group; the many queries of a prompt's chunk are better
+    served by `paged_cache_read` and `attention`."""
+    return paged_attention_forward(q, cache, page_table, seqlens, sinks, sm_scale, bandwidth, start, max_len)[0]
