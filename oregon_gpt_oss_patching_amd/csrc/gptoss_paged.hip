@@ -62,6 +62,39 @@ int launch(Kernel kernel, int64_t workgroups, int threads, void *stream, const P
     return e == hipSuccess ? GPTOSS_ATTN_OK : static_cast<int>(e);
 }
 
+// How the attention's work is divided: column blocks of 16 pairs, blocks of pairs of a row, (row, block) units, shares of all units'
+// tiles for each KV head beside one for each unit (0: units stay whole), and the scratch that takes.
+constexpr int kMinTiles = 8;
+struct PagedDivision { int nb, blocks, shares; int64_t units; size_t plan_bytes, bytes; };
+
+PagedDivision paged_division(const gptoss_attn_paged_params *p) {
+    PagedDivision d{};
+    const int64_t pairs = (int64_t)p->Sq * (p->H / p->G);
+    const int most = p->dtype == GPTOSS_ATTN_FP32 ? paged_pairs<float>() : paged_pairs<bf16>();
+    d.nb = pairs <= 16 ? 1 : pairs <= 32 || most == 32 ? 2 : 4;
+    const int64_t blocks = (pairs + 16 * d.nb - 1) / (16 * d.nb);
+    d.blocks = (int)(blocks < 0x7fffffff ? blocks : 0x7fffffff);
+    d.units = blocks * p->B;
+    // the most tiles that a unit can have
+    int64_t keys = (int64_t)p->table_width * p->page_size;
+    if (p->max_len > 0 && p->max_len < keys) keys = p->max_len;
+    const int64_t queries = (16 * d.nb - 1) / (p->H / p->G) + 2;                   // that a unit's pairs touch
+    if (p->window > 0 && p->window + queries + 2 * kPagedKeys < keys) keys = p->window + queries + 2 * kPagedKeys;
+    const int64_t tiles = (keys + kPagedKeys - 1) / kPagedKeys;
+    if (d.units > kPagedMaxUnits || tiles <= kMinTiles) return d;
+    d.shares = 1024 / p->G > 0 ? 1024 / p->G : 1;
+    d.plan_bytes = ((size_t)d.units * 2 * sizeof(int) + 15) & ~(size_t)15;
+    d.bytes = d.plan_bytes + (size_t)(d.shares + d.units) * p->G * paged_partial_floats(d.nb) * sizeof(float);
+    return d;
+}
+
+template <typename T, typename ST, int NB>
+int attend(const PagedDivision &d, void *stream, const PagedArgs &a) {
+    const int s = launch(attn_paged_kernel<T, ST, NB>, (d.shares + d.units) * a.G, 64 * kPagedWaves, stream, a);
+    if (s || !d.shares) return s;
+    return launch(attn_paged_combine_kernel<T, NB>, ((int64_t)a.B * a.H * a.Sq + 3) / 4, 256, stream, a);
+}
+
 }  // namespace
 
 extern "C" {
@@ -99,16 +132,34 @@ int gptoss_attn_paged_validate(const gptoss_attn_paged_params *p, int call) {
     return GPTOSS_ATTN_OK;
 }
 
-size_t gptoss_attn_paged_workspace_bytes(const gptoss_attn_paged_params *) { return 0; }
+size_t gptoss_attn_paged_workspace_bytes(const gptoss_attn_paged_params *p) {
+    if (!p || p->B <= 0 || p->G <= 0 || p->H <= 0 || p->H % p->G || p->Sq <= 0 || p->table_width <= 0 || p->page_size <= 0) return 0;
+    return paged_division(p).bytes;
+}
 
 int gptoss_attn_paged_fwd(const gptoss_attn_paged_params *p, void *stream) {
     const int rc = gptoss_attn_paged_validate(p, kFwd);
     if (rc) return rc;
-    const PagedArgs a = make_args(p);
-    const int64_t grid = (int64_t)a.B * a.H * a.Sq;
-    if (p->dtype == GPTOSS_ATTN_BF16)
-        return p->storage == GPTOSS_ATTN_E4M3 ? launch(attn_paged_kernel<bf16, e4m3>, grid, 256, stream, a) : launch(attn_paged_kernel<bf16, bf16>, grid, 256, stream, a);
-    return p->storage == GPTOSS_ATTN_E4M3 ? launch(attn_paged_kernel<float, e4m3>, grid, 256, stream, a) : launch(attn_paged_kernel<float, float>, grid, 256, stream, a);
+    PagedArgs a = make_args(p);
+    const PagedDivision d = paged_division(p);
+    if (d.units > 0x7fffffff) return GPTOSS_ATTN_ERR_SHAPE;
+    a.blocks = d.blocks;
+    a.units = (int)d.units;
+    a.shares = d.shares;
+    a.min_tiles = kMinTiles;
+    if (d.shares) {
+        a.plan = static_cast<int *>(p->scratch);
+        a.partial = reinterpret_cast<float *>(static_cast<char *>(p->scratch) + d.plan_bytes);
+    }
+    const bool codes = p->storage == GPTOSS_ATTN_E4M3;
+    if (p->dtype == GPTOSS_ATTN_BF16) {
+#define GPTOSS_PAGED(NB) (codes ? attend<bf16, e4m3, NB>(d, stream, a) : attend<bf16, bf16, NB>(d, stream, a))
+        return d.nb == 1 ? GPTOSS_PAGED(1) : d.nb == 2 ? GPTOSS_PAGED(2) : GPTOSS_PAGED(4);
+#undef GPTOSS_PAGED
+    }
+#define GPTOSS_PAGED(NB) (codes ? attend<float, e4m3, NB>(d, stream, a) : attend<float, float, NB>(d, stream, a))
+    return d.nb == 1 ? GPTOSS_PAGED(1) : GPTOSS_PAGED(2);
+#undef GPTOSS_PAGED
 }
 
 int gptoss_attn_paged_write(const gptoss_attn_paged_params *p, void *stream) {

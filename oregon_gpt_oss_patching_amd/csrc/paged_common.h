@@ -22,7 +22,12 @@ struct PagedArgs {
     int64_t table_stride;
     int B, H, G, r, Sq;
     int pages, page_shift, width, window;
-    int blocks;                  // workgroups of a batch row (write), of a row and KV head (read)
+    int blocks;                  // workgroups of a batch row (write), of a row and KV head (read); blocks of pairs of a row (attention)
+    // attention: (row, block of pairs) units, into how many shares their work is cut (0: not), of how many tiles at least; the shares'
+    // partial results and, for each unit, its first share and their number
+    int units, shares, min_tiles;
+    float *partial;
+    int *plan;
     float scale_log2;
     bool sinks_bf16;
 };
