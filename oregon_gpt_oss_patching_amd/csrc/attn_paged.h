@@ -26,10 +26,12 @@
 
 namespace gptoss {
 
-constexpr int kPagedKeys = 32, kPagedWaves = 4, kPagedMaxUnits = 1024;
+constexpr int kPagedWaves = 4, kPagedMaxUnits = 1024;
 constexpr int kPagedRow = kD + 2;               // floats of a merged row: O, m, l
 constexpr float kRaise = 8.0f;                  // in the exponent of two
 
+// Blocks of 16 keys in a tile: what a wavefront has under way is a tile, so rows of fewer bytes come more at a time.
+template <typename T, typename ST, int NB> __host__ __device__ constexpr int paged_tile_blocks() { return sizeof(T) == 2 && sizeof(ST) == 1 && NB == 1 ? 4 : 2; }
 // Pairs (query, head of the group) that one workgroup may take.
 template <typename T> __host__ __device__ constexpr int paged_pairs() { return sizeof(T) == 2 ? 64 : 32; }
 // floats of a share's partial result: rows of O, then (m, l) of each
@@ -41,59 +43,85 @@ struct PagedSpan {
     int pos0, pos1;              // first and last position of queries that exist
     int lo, hi, t_first, tiles;  // keys lo .. hi - 1, in tiles
 };
-__device__ __forceinline__ PagedSpan paged_span(const PagedArgs &a, int unit, int pairs) {
-    PagedSpan s;
-    s.b = unit / a.blocks;
-    s.pair0 = (unit - s.b * a.blocks) * pairs;
-    s.n = paged_length(a, s.b);
+__device__ __forceinline__ int paged_base(const PagedArgs &a, int b, int n) {
     // (positions beyond +-2^30 exist in no row)
-    s.base = a.start ? min(max(a.start[s.b], -(1 << 30)), (1 << 30) - 1) : s.n - a.Sq;
-    const int i0 = s.pair0 / a.r, i1 = min(a.Sq - 1, (s.pair0 + pairs - 1) / a.r);
-    s.pos0 = max(s.base + i0, 0);
-    s.pos1 = min(s.base + i1, s.n - 1);
+    return a.start ? min(max(a.start[b], -(1 << 30)), (1 << 30) - 1) : n - a.Sq;
+}
+template <int PAIRS, int KEYS>
+__device__ __forceinline__ PagedSpan paged_span(const PagedArgs &a, int b, int block, int n, int base) {
+    PagedSpan s;
+    s.b = b;
+    s.pair0 = block * PAIRS;
+    s.n = n;
+    s.base = base;
+    const int i0 = a.by_r.quotient(s.pair0), i1 = min(a.Sq - 1, a.by_r.quotient(s.pair0 + PAIRS - 1));
+    s.pos0 = max(base + i0, 0);
+    s.pos1 = min(base + i1, n - 1);
     const bool any = s.pos0 <= s.pos1;
     s.lo = any && a.window ? max(0, s.pos0 - a.window + 1) : 0;
     s.hi = any ? s.pos1 + 1 : 0;
-    s.t_first = s.lo / kPagedKeys;
-    s.tiles = any ? (s.hi + kPagedKeys - 1) / kPagedKeys - s.t_first : 0;
+    s.t_first = s.lo / KEYS;
+    s.tiles = any ? (s.hi + KEYS - 1) / KEYS - s.t_first : 0;
     return s;
+}
+
+// x + (x of all lanes below), over the wavefront, without LDS: within rows of 16 lanes, then over the rows
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);        // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);        // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);        // row_bcast:31 into rows 2 and 3
+    return x;
 }
 
 // Which share of which unit a workgroup takes.  All units' tiles are cut into shares of `chunk`, the smallest length of at least
 // a.min_tiles with which they number no more than a.shares and one for each unit, which is what the grid and the scratch hold.
 struct PagedShare { int unit, index, count, first; };     // first: number of the unit's first share; unit < 0: nothing left
-__device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int slot, int pairs) {
-    if (!a.shares) return PagedShare{slot, 0, 1, slot};
+template <int PAIRS, int KEYS>
+__device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int slot, PagedSpan &sp) {
     const int lane = threadIdx.x & 63;
-    int64_t all = 0;
-    if (a.units <= 64) {
-        uint32_t x = lane < a.units ? (uint32_t)paged_span(a, lane, pairs).tiles : 0u;      // at most 2^25 each
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) x += (uint32_t)__shfl_xor((int)x, d);
-        all = x;
-    } else {
-        for (int u = lane; u < a.units; u += 64) all += paged_span(a, u, pairs).tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) all += __shfl_xor((long long)all, d);
+    if (!a.shares) {
+        const int b = a.by_blocks.quotient(slot), n = paged_length(a, b);
+        sp = paged_span<PAIRS, KEYS>(a, b, slot - b * a.blocks, n, paged_base(a, b, n));
+        return PagedShare{slot, 0, 1, slot};
     }
-    const int64_t even = (all + a.shares - 1) / a.shares;
-    const int chunk = max(a.min_tiles, (int)(even < (1 << 30) ? even : (1 << 30)));      // (more tiles than a unit can have)
+    // a lane's unit, the first 64 of them kept
+    auto mine = [&](int u, int &n, int &base) __attribute__((always_inline)) {
+        n = base = 0;
+        if (u >= a.units) return 0;
+        const int b = a.by_blocks.quotient(u);
+        n = paged_length(a, b);
+        base = paged_base(a, b, n);
+        return paged_span<PAIRS, KEYS>(a, b, u - b * a.blocks, n, base).tiles;
+    };
+    int n, base;
+    const int tiles0 = mine(lane, n, base);
+    const int sum0 = __builtin_amdgcn_readlane(wave_scan(tiles0), 63);      // (as unsigned: at most 2^25 tiles each)
+    int chunk;
+    if (a.units <= 64) {
+        chunk = (int)(((uint32_t)sum0 + (uint32_t)a.shares - 1u) / (uint32_t)a.shares);
+    } else {
+        int64_t all = (uint32_t)sum0;
+        for (int u0 = 64; u0 < a.units; u0 += 64) {
+            int x, y;
+            all += (uint32_t)__builtin_amdgcn_readlane(wave_scan(mine(u0 + lane, x, y)), 63);
+        }
+        const int64_t even = (all + a.shares - 1) / a.shares;
+        chunk = (int)(even < (1 << 30) ? even : (1 << 30));                 // (more tiles than a unit can have)
+    }
+    chunk = max(a.min_tiles, chunk);
     int before = 0;
     for (int u0 = 0; u0 < a.units; u0 += 64) {
-        const int u = u0 + lane;
-        const int mine = u < a.units ? max(1, (paged_span(a, u, pairs).tiles + chunk - 1) / chunk) : 0;
-        int incl = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int y = __shfl_up(incl, d);
-            if (lane >= d) incl += y;
-        }
-        const int first = before + incl - mine;
-        const unsigned long long who = __builtin_amdgcn_ballot_w64(slot >= first && slot < first + mine);
+        const int tiles = u0 ? mine(u0 + lane, n, base) : tiles0;
+        const int shares = u0 + lane < a.units ? max(1, (int)((uint32_t)(tiles + chunk - 1) / (uint32_t)chunk)) : 0;
+        const int incl = wave_scan(shares), first = before + incl - shares;
+        const unsigned long long who = __builtin_amdgcn_ballot_w64(slot >= first && slot < first + shares);
         if (who) {
-            const int l = __builtin_ctzll(who);
-            const int f = __builtin_amdgcn_readlane(first, l);
-            return PagedShare{u0 + l, slot - f, __builtin_amdgcn_readlane(mine, l), f};
+            const int l = __builtin_ctzll(who), f = __builtin_amdgcn_readlane(first, l), b = a.by_blocks.quotient(u0 + l);
+            sp = paged_span<PAIRS, KEYS>(a, b, u0 + l - b * a.blocks, __builtin_amdgcn_readlane(n, l), __builtin_amdgcn_readlane(base, l));
+            return PagedShare{u0 + l, slot - f, __builtin_amdgcn_readlane(shares, l), f};
         }
         before += __builtin_amdgcn_readlane(incl, 63);
     }
@@ -130,24 +158,24 @@ __device__ __forceinline__ bf16x8 widen8(uint32_t w0, uint32_t w1, float f) {
 
 // A tile's K and V as they are loaded, and what is done with them.  `kb` / `vb`: scalar addresses of the first row of a block of 16 keys;
 // lanes: l16 = lane % 16, quad = lane / 16.
-template <typename T, typename ST, int NB> struct PagedTile;
+template <typename T, typename ST, int NB, int KB> struct PagedTile;
 
 // ---- bfloat16 products -----------------------------------------------------------------------------------------------
-template <typename ST, int NB>
-struct PagedTile<bf16, ST, NB> {
+template <typename ST, int NB, int KB>
+struct PagedTile<bf16, ST, NB, KB> {
     static constexpr bool kCodes = sizeof(ST) == 1;
-    static constexpr int kStage = kPagedKeys * kRowBytes;        // LDS bytes of a wavefront
+    static constexpr int kStage = 16 * KB * kRowBytes;           // LDS bytes of a wavefront
     static constexpr int kVecs = kCodes ? 1 : 2;                 // 16-byte loads per lane and block
-    u32x4 k[2][kVecs], v[2][kVecs];
-    uint32_t ke[2], ve[2];
+    u32x4 k[KB][kVecs], v[KB][kVecs];
+    uint32_t ke[KB], ve[KB];
     bf16x8 q[NB][2];
     f32x4 o[NB][4];
-    uint32_t tr[4], wr[2];
+    uint32_t tr[4], wr[2], k_at, v_at[kVecs], ke_at, ve_at;
 
     __device__ __forceinline__ static int v_row(int lane, int i) { return kCodes ? lane >> 2 : (lane >> 3) + 8 * i; }
 
-    __device__ __forceinline__ void init(uint32_t stage, int lane) {
-        const int i = lane & 15, row = 4 * (lane >> 4) + (i >> 2);
+    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage, int lane) {
+        const int i = lane & 15, quad = lane >> 4, row = 4 * quad + (i >> 2);
 #pragma unroll
         for (int d = 0; d < 4; ++d) tr[d] = stage + row * kRowBytes + (((2 * d + ((i & 3) >> 1)) ^ swz(row)) * 16) + (i & 1) * 8;
 #pragma unroll
@@ -155,6 +183,11 @@ struct PagedTile<bf16, ST, NB> {
             const int r = v_row(lane, e), c = kCodes ? 2 * (lane & 3) + e : lane & 7;
             wr[e] = stage + r * kRowBytes + ((c ^ swz(r)) * 16);
         }
+        k_at = i * a.kp.s + 16 * quad;
+#pragma unroll
+        for (int e = 0; e < kVecs; ++e) v_at[e] = v_row(lane, e) * a.vp.s + 16 * (kCodes ? lane & 3 : lane & 7);
+        ke_at = i * a.ke.s;
+        ve_at = v_row(lane, 0) * a.ve.s;
     }
     __device__ __forceinline__ void load_q(int nb, const bf16 *row, bool there, int quad) {
 #pragma unroll
@@ -165,22 +198,19 @@ struct PagedTile<bf16, ST, NB> {
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[nb][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    __device__ __forceinline__ void load_k(int blk, const char *kb, const uint8_t *eb, const PagedArgs &a, int lane) {
-        const int l16 = lane & 15, quad = lane >> 4;
-        const uint32_t at = (uint32_t)(l16 * (int)a.kps.s * (kCodes ? 1 : 2) + 16 * quad);
+    __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb) {
 #pragma unroll
-        for (int s = 0; s < kVecs; ++s) k[blk][s] = *reinterpret_cast<const u32x4 *>(kb + at + 64 * s);
-        if constexpr (kCodes) ke[blk] = eb[(uint32_t)(l16 * (int)a.kes.s)];
+        for (int s = 0; s < kVecs; ++s) k[blk][s] = *reinterpret_cast<const u32x4 *>(kb + k_at + 64 * s);
+        if constexpr (kCodes) ke[blk] = (uint8_t)eb[ke_at];
     }
-    __device__ __forceinline__ void load_v(int blk, const char *vb, const uint8_t *eb, const PagedArgs &a, int lane) {
+    __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb) {
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i)
-            v[blk][i] = *reinterpret_cast<const u32x4 *>(vb + (uint32_t)(v_row(lane, i) * (int)a.vps.s * (kCodes ? 1 : 2) + 16 * (kCodes ? lane & 3 : lane & 7)));
-        if constexpr (kCodes) ve[blk] = eb[(uint32_t)(v_row(lane, 0) * (int)a.ves.s)];
+        for (int i = 0; i < kVecs; ++i) v[blk][i] = *reinterpret_cast<const u32x4 *>(vb + v_at[i]);
+        if constexpr (kCodes) ve[blk] = (uint8_t)eb[ve_at];
     }
-    __device__ __forceinline__ void logits(f32x4 (&s)[NB][2]) const {
+    __device__ __forceinline__ void logits(f32x4 (&s)[NB][KB]) const {
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
+        for (int blk = 0; blk < KB; ++blk) {
             bf16x8 f[2];
             if constexpr (kCodes) {
                 const float p = exp_of_byte(ke[blk]);
@@ -200,8 +230,25 @@ struct PagedTile<bf16, ST, NB> {
     // V into the stage; rows outside first .. last - 1 of the tile as zeros where `edge`, and whether a row inside holds no finite number
     __device__ __forceinline__ bool stage_v(bool edge, int first, int last, unsigned there, int lane) {
         bool odd = false;
+        if (edge) {
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
+            for (int blk = 0; blk < KB; ++blk)
+#pragma unroll
+                for (int i = 0; i < kVecs; ++i) {
+                    const int r = 16 * blk + v_row(lane, i);
+                    const bool in = r >= first && r < last && (there >> blk & 1);
+                    if constexpr (kCodes) ve[blk] = in ? ve[blk] : (uint32_t)kExpBias;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t x = in ? v[blk][i][e] : 0u;
+                        v[blk][i][e] = x;
+                        if constexpr (kCodes) odd = odd || (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;        // 0x7f: NaN
+                        else odd = odd || (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+                    }
+                }
+        }
+#pragma unroll
+        for (int blk = 0; blk < KB; ++blk)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 u32x4 x;
@@ -212,32 +259,26 @@ struct PagedTile<bf16, ST, NB> {
                 } else {
                     x = v[blk][i];
                 }
-                if (edge) {
-                    const int r = 16 * blk + v_row(lane, i);
-                    const bool in = r >= first && r < last && (there >> blk & 1);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[e] = in ? x[e] : 0u;
-                        odd = odd || (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
-                    }
-                }
                 *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>((uintptr_t)(wr[i] + 16 * blk * kRowBytes)) = x;
             }
         return odd;
     }
-    __device__ __forceinline__ void product(const f32x4 (&s)[NB][2]) {
-        bf16x8 p[NB];
+    __device__ __forceinline__ void product(const f32x4 (&s)[NB][KB]) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int h = 0; h < KB / 2; ++h) {
+            bf16x8 p[NB];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { p[nb][e] = (bf16)s[nb][0][e]; p[nb][4 + e] = (bf16)s[nb][1][e]; }
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            union { struct { s16x4 a, b; } s; bf16x8 v; } x;
-            x.s.a = lds_load_tr64(tr[d], 0);
-            x.s.b = lds_load_tr64(tr[d], 16 * kRowBytes);
+                for (int e = 0; e < 4; ++e) { p[nb][e] = (bf16)s[nb][2 * h][e]; p[nb][4 + e] = (bf16)s[nb][2 * h + 1][e]; }
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) o[nb][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb], o[nb][d], 0, 0, 0);
+            for (int d = 0; d < 4; ++d) {
+                union { struct { s16x4 a, b; } s; bf16x8 v; } x;
+                x.s.a = lds_load_tr64(tr[d], 32 * h * kRowBytes);
+                x.s.b = lds_load_tr64(tr[d], (32 * h + 16) * kRowBytes);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) o[nb][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb], o[nb][d], 0, 0, 0);
+            }
         }
     }
     // column of o[.][d][e] in the lane's row
@@ -250,20 +291,31 @@ struct PagedTile<bf16, ST, NB> {
 };
 
 // ---- float32 products ------------------------------------------------------------------------------------------------
-template <typename ST, int NB>
-struct PagedTile<float, ST, NB> {
+template <typename ST, int NB, int KB>
+struct PagedTile<float, ST, NB, KB> {
     static constexpr bool kCodes = sizeof(ST) == 1;
-    static constexpr int kStage = kPagedKeys * kD * 4;           // used where V holds infinities or NaN only
+    static constexpr int kStage = 16 * KB * kD * 4;              // used where V holds infinities or NaN only
     static constexpr int kVecs = kCodes ? 1 : 4;
     typedef typename std::conditional<kCodes, uint32_t, f32x4>::type vec;       // four numbers of a row of V
-    u32x4 k[2][kVecs];
-    vec v[2][4];
-    uint32_t ke[2], ve[2][4];
+    u32x4 k[KB][kVecs];
+    vec v[KB][4];
+    uint32_t ke[KB], ve[KB][4];
     float q[NB][16];
     f32x4 o[NB][4];
-    uint32_t stage;
+    f32x4 w[KB][4];              // V as numbers
+    uint32_t stage, k_at, ke_at, v_at[4], ve_at[4];
 
-    __device__ __forceinline__ void init(uint32_t stage_, int) { stage = stage_; }
+    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage_, int lane) {
+        const int l16 = lane & 15, quad = lane >> 4;
+        stage = stage_;
+        k_at = l16 * a.kp.s + 16 * quad;
+        ke_at = l16 * a.ke.s;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v_at[e] = (4 * quad + e) * a.vp.s + 4 * (uint32_t)sizeof(ST) * l16;
+            ve_at[e] = (4 * quad + e) * a.ve.s;
+        }
+    }
     __device__ __forceinline__ static int q_index(int t, int quad) { return kCodes ? 16 * quad + t : 16 * (t >> 2) + 4 * quad + (t & 3); }
     __device__ __forceinline__ void load_q(int nb, const float *row, bool there, int quad) {
 #pragma unroll
@@ -275,24 +327,25 @@ struct PagedTile<float, ST, NB> {
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[nb][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    __device__ __forceinline__ void load_k(int blk, const char *kb, const uint8_t *eb, const PagedArgs &a, int lane) {
-        const int l16 = lane & 15, quad = lane >> 4;
-        const uint32_t at = (uint32_t)(l16 * (int)a.kps.s * (kCodes ? 1 : 4) + 16 * quad);
+    __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb) {
 #pragma unroll
-        for (int s = 0; s < kVecs; ++s) k[blk][s] = *reinterpret_cast<const u32x4 *>(kb + at + 64 * s);
-        if constexpr (kCodes) ke[blk] = eb[(uint32_t)(l16 * (int)a.kes.s)];
+        for (int s = 0; s < kVecs; ++s) k[blk][s] = *reinterpret_cast<const u32x4 *>(kb + k_at + 64 * s);
+        if constexpr (kCodes) ke[blk] = (uint8_t)eb[ke_at];
     }
-    __device__ __forceinline__ void load_v(int blk, const char *vb, const uint8_t *eb, const PagedArgs &a, int lane) {
-        const int l16 = lane & 15, quad = lane >> 4;
+    __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            v[blk][e] = *reinterpret_cast<const vec *>(vb + (uint32_t)((4 * quad + e) * (int)a.vps.s * (kCodes ? 1 : 4) + (kCodes ? 4 : 16) * l16));
-            if constexpr (kCodes) ve[blk][e] = eb[(uint32_t)((4 * quad + e) * (int)a.ves.s)];
+            v[blk][e] = *reinterpret_cast<const vec *>(vb + v_at[e]);
+            if constexpr (kCodes) ve[blk][e] = (uint8_t)eb[ve_at[e]];
         }
     }
-    __device__ __forceinline__ void logits(f32x4 (&s)[NB][2]) const {
+    __device__ __forceinline__ static float code(uint32_t w, int i) {
+        return i == 0 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 0) : i == 1 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 1)
+               : i == 2 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 2) : __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+    }
+    __device__ __forceinline__ void logits(f32x4 (&s)[NB][KB]) const {
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
+        for (int blk = 0; blk < KB; ++blk) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) s[nb][blk] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             float p = 1.0f;
@@ -307,16 +360,10 @@ struct PagedTile<float, ST, NB> {
             }
         }
     }
-    __device__ __forceinline__ static float code(uint32_t w, int i) {
-        return i == 0 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 0) : i == 1 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 1)
-               : i == 2 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 2) : __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
-    }
-    f32x4 w[2][4];       // V as numbers
     __device__ __forceinline__ bool stage_v(bool edge, int first, int last, unsigned there, int lane) {
-        bool odd = false;
         const int l16 = lane & 15, quad = lane >> 4;
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
+        for (int blk = 0; blk < KB; ++blk)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if constexpr (kCodes) {
@@ -326,7 +373,13 @@ struct PagedTile<float, ST, NB> {
                 } else {
                     w[blk][e] = v[blk][e];
                 }
-                if (edge) {
+            }
+        bool odd = false;
+        if (edge) {
+#pragma unroll
+            for (int blk = 0; blk < KB; ++blk)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
                     const int r = 16 * blk + 4 * quad + e;
                     const bool in = r >= first && r < last && (there >> blk & 1);
 #pragma unroll
@@ -336,12 +389,12 @@ struct PagedTile<float, ST, NB> {
                     }
                     *reinterpret_cast<__attribute__((address_space(3))) f32x4 *>((uintptr_t)(stage + (r * kD + 4 * l16) * 4)) = w[blk][e];
                 }
-            }
+        }
         return odd;
     }
-    __device__ __forceinline__ void product(const f32x4 (&s)[NB][2]) {
+    __device__ __forceinline__ void product(const f32x4 (&s)[NB][KB]) {
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
+        for (int blk = 0; blk < KB; ++blk)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -355,133 +408,139 @@ struct PagedTile<float, ST, NB> {
     }
 };
 
-template <typename T, typename ST, int NB>
-constexpr int paged_lds_bytes() {
-    constexpr int merge = kPagedWaves * 16 * (NB > 2 ? 2 : NB) * kPagedRow * 4, stages = kPagedWaves * PagedTile<T, ST, NB>::kStage;
-    return stages > merge ? stages : merge;
-}
-
-// Eight columns of a finished row: weights' sum l and products `acc` relative to the maximum `top`, the sink not yet among them.
+// Eight columns of a finished row: weights' sum l and products `acc` relative to the maximum `top`, the sink not yet among them.  `none`: no
+// query, or no key that it sees.
 template <typename T>
-__device__ __forceinline__ void paged_finish(const PagedArgs &a, const PagedSpan &sp, int row, int head, int c8, float top, float l, const float (&acc)[8]) {
-    const float sink = paged_sink(a, head), sink2 = sink * kLog2e;
+__device__ __forceinline__ void paged_finish(const PagedArgs &a, int b, int row, int head, int c8, float sink, bool none, float top, float l, const float (&acc)[8]) {
+    const float sink2 = sink * kLog2e;
     // (the larger one's weight is 1 and not the power of a difference with itself, which a fused multiply-add of the logit would not make 0)
     const bool by_sink = sink2 >= top;
     const float ref = by_sink ? sink2 : top, f = by_sink ? fast_exp2(top - sink2) : 1.0f;
     const float z = l * f + (by_sink ? 1.0f : fast_exp2(sink2 - top));
-    const int pos = sp.base + row;
-    const bool none = pos < 0 || pos >= sp.n || l == 0.0f;          // no query, or no key that it sees
     const float mul = none ? 0.0f : f / z;
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = none ? 0.0f : acc[e] * mul;
-    store8(static_cast<T *>(a.o) + sp.b * a.os.b + head * a.os.h + row * a.os.s + c8, x);
-    if (c8 == 0) a.lse[((int64_t)sp.b * a.H + head) * a.Sq + row] = none ? sink : (ref + fast_log2(z)) * kLn2;
+    store8(static_cast<T *>(a.o) + b * a.os.b + head * a.os.h + row * a.os.s + c8, x);
+    if (c8 == 0) a.lse[((int64_t)b * a.H + head) * a.Sq + row] = none ? sink : (ref + fast_log2(z)) * kLn2;
+}
+
+// column blocks that are merged at a time
+template <int NB> constexpr int paged_merge_blocks() { return NB == 4 ? 2 : NB; }
+template <typename T, typename ST, int NB>
+constexpr int paged_lds_bytes() {
+    constexpr int merge = kPagedWaves * 16 * paged_merge_blocks<NB>() * kPagedRow * 4;
+    constexpr int stages = kPagedWaves * PagedTile<T, ST, NB, paged_tile_blocks<T, ST, NB>()>::kStage;
+    return stages > merge ? stages : merge;
 }
 
 template <typename T, typename ST, int NB>
-__global__ __launch_bounds__(64 * kPagedWaves, NB == 1 && sizeof(T) == 2 ? 4 : 2) void attn_paged_kernel(const PagedArgs a) {
-    using Tile = PagedTile<T, ST, NB>;
-    constexpr int NW = kPagedWaves, kPairs = 16 * NB;
+__global__ __launch_bounds__(64 * kPagedWaves, NB == 1 && sizeof(T) == 2 ? (sizeof(ST) == 1 ? 3 : 4) : 2) void attn_paged_kernel(const PagedArgs a) {
+    constexpr int NW = kPagedWaves, kPairs = 16 * NB, KB = paged_tile_blocks<T, ST, NB>(), kKeys = 16 * KB;
+    using Tile = PagedTile<T, ST, NB, KB>;
     __shared__ __attribute__((aligned(128))) char smem[paged_lds_bytes<T, ST, NB>()];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, quad = lane >> 4;
-    const int g = blockIdx.x % a.G;
-    const PagedShare share = paged_share(a, blockIdx.x / a.G, kPairs);
-    const int unit = __builtin_amdgcn_readfirstlane(share.unit);
-    if (unit < 0) return;
-    const PagedSpan sp = paged_span(a, unit, kPairs);
-    const int t_lo = sp.t_first + (int)((int64_t)sp.tiles * share.index / share.count);
-    const int n_wg = sp.t_first + (int)((int64_t)sp.tiles * (share.index + 1) / share.count) - t_lo;
+    const int slot = a.by_g.quotient(blockIdx.x), g = blockIdx.x - slot * a.G;
+    PagedSpan sp;
+    const PagedShare share = paged_share<kPairs, kKeys>(a, slot, sp);
+    if (share.unit < 0) return;
+    // the unit's tiles in even parts, the first ones a tile longer where it does not come out even
+    const int part_tiles = (int)((uint32_t)sp.tiles / (uint32_t)share.count), longer = sp.tiles - part_tiles * share.count;
+    const int t_lo = sp.t_first + part_tiles * share.index + min(share.index, longer), n_wg = part_tiles + (share.index < longer ? 1 : 0);
     const int n_it = n_wg > w ? (n_wg - w + NW - 1) / NW : 0;       // this wavefront's tiles: t_lo + w + NW j
     const int pairs = min(a.Sq * a.r - sp.pair0, kPairs);
 
+    const int32_t *table = a.table + sp.b * a.table_stride;
+    const int in_page = (1 << a.page_shift) - 1, weff = a.window ? a.window : 0x3fffffff;
+    int entry[KB];                           // pages of the wavefront's next 64 tiles, one a lane, for each 16 keys of a tile
+    auto entries = [&](int j) __attribute__((always_inline)) {
+        const int n0 = (t_lo + w + NW * (j + lane)) * kKeys;
+#pragma unroll
+        for (int blk = 0; blk < KB; ++blk) {
+            if (blk && (16 * blk & in_page)) {
+                entry[blk] = entry[blk - 1];
+            } else {
+                const int i = (n0 + 16 * blk) >> a.page_shift;
+                int page = -1;
+                if (j + lane < n_it && i < a.width) page = table[i];
+                entry[blk] = (unsigned)page < (unsigned)a.pages ? page : -1;
+            }
+        }
+    };
+    if (n_it > 0) entries(0);
+
     Tile tile;
     const uint32_t stage = lds_addr(smem) + w * Tile::kStage;
-    tile.init(stage, lane);
+    tile.init(a, stage, lane);
     int pq[NB];                // position of the column's query
     float m[NB], l[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const bool ok = 16 * nb + l16 < pairs;
-        const int pair = sp.pair0 + (ok ? 16 * nb + l16 : 0), row = pair / a.r, head = g * a.r + pair % a.r;
+        const int pair = sp.pair0 + (ok ? 16 * nb + l16 : 0), row = a.by_r.quotient(pair), head = g * a.r + pair - row * a.r;
         pq[nb] = sp.base + row;
         tile.load_q(nb, static_cast<const T *>(a.q) + sp.b * a.qs.b + head * a.qs.h + row * a.qs.s, ok, quad);
         m[nb] = kLowest;
         l[nb] = 0.0f;
     }
 
-    const int32_t *table = a.table + sp.b * a.table_stride;
-    const int in_page = (1 << a.page_shift) - 1, weff = a.window ? a.window : 0x3fffffff;
-    int entry0 = 0, entry1 = 0;              // pages of the wavefront's next 64 tiles, one a lane: their first and second 16 keys
-    unsigned there = 0;                      // of the tile under way: which of the two exist
-    auto entry = [&](int token) {
-        const int i = token >> a.page_shift;
-        const int page = i < a.width ? table[i] : -1;
-        return (unsigned)page < (unsigned)a.pages ? page : -1;
-    };
-    auto entries = [&](int j) __attribute__((always_inline)) {
-        if ((j & 63) == 0) {
-            const int n0 = (t_lo + w + NW * (j + lane)) * kPagedKeys;
-            const bool mine = j + lane < n_it;
-            entry0 = mine ? entry(n0) : -1;
-            entry1 = mine ? (a.page_shift > 4 ? entry0 : entry(n0 + 16)) : -1;
-        }
-    };
-    auto page_of = [&](int j, int blk) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(blk ? entry1 : entry0, j & 63); };
-    auto fetch_k = [&](int j) __attribute__((always_inline)) {
-        const int n0 = (t_lo + w + NW * j) * kPagedKeys;
+    const char *k_base = a.kp.head(g), *v_base = a.vp.head(g), *ke_base = a.ke.head(g), *ve_base = a.ve.head(g);
+    auto page_of = [&](int j, int blk) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(entry[blk], j & 63); };
+    // (page, slot) -> load(block, address of the rows, of their exponents); blocks behind the first of a page follow it
+    auto fetch = [&](int j, const char *base, const PagedPool &rows, const char *ebase, const PagedPool &exps, auto load) __attribute__((always_inline)) {
+        const int n0 = (t_lo + w + NW * j) * kKeys;
+        const char *p = nullptr, *e = nullptr;
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-            const int page = max(page_of(j, blk), 0), slot = (n0 + 16 * blk) & in_page;
-            tile.load_k(blk, a.k_pages + (page * a.kps.b + g * a.kps.h + slot * a.kps.s) * (int)sizeof(ST),
-                        Tile::kCodes ? a.k_exp + page * a.kes.b + g * a.kes.h + slot * a.kes.s : nullptr, a, lane);
+        for (int blk = 0; blk < KB; ++blk) {
+            if (blk && (16 * blk & in_page)) {
+                p += 16 * (uint64_t)rows.s;
+                if constexpr (Tile::kCodes) e += 16 * exps.s;
+            } else {
+                const int page = max(page_of(j, blk), 0), at = (n0 + 16 * blk) & in_page;
+                p = base + rows.at(page, at);
+                if constexpr (Tile::kCodes) e = ebase + exps.at(page, at);
+            }
+            load(blk, p, e);
         }
     };
-    auto fetch_v = [&](int j) __attribute__((always_inline)) {
-        const int n0 = (t_lo + w + NW * j) * kPagedKeys;
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-            const int page = max(page_of(j, blk), 0), slot = (n0 + 16 * blk) & in_page;
-            tile.load_v(blk, a.v_pages + (page * a.vps.b + g * a.vps.h + slot * a.vps.s) * (int)sizeof(ST),
-                        Tile::kCodes ? a.v_exp + page * a.ves.b + g * a.ves.h + slot * a.ves.s : nullptr, a, lane);
-        }
-    };
+    auto fetch_k = [&](int j) __attribute__((always_inline)) { fetch(j, k_base, a.kp, ke_base, a.ke, [&](int blk, const char *p, const char *e) { tile.load_k(blk, p, e); }); };
+    auto fetch_v = [&](int j) __attribute__((always_inline)) { fetch(j, v_base, a.vp, ve_base, a.ve, [&](int blk, const char *p, const char *e) { tile.load_v(blk, p, e); }); };
 
     if (n_it > 0) {
-        entries(0);
         fetch_k(0);
         fetch_v(0);
     }
     for (int j = 0; j < n_it; ++j) {
-        const int n0 = (t_lo + w + NW * j) * kPagedKeys;
-        there = (page_of(j, 0) >= 0 ? 1u : 0u) | (page_of(j, 1) >= 0 ? 2u : 0u);
-        const bool edge = !(n0 + kPagedKeys - 1 <= sp.pos0 && n0 > sp.pos1 - weff && there == 3u);
-        f32x4 s[NB][2];
+        const int n0 = (t_lo + w + NW * j) * kKeys;
+        unsigned there = 0;                  // which of the tile's blocks have a page
+#pragma unroll
+        for (int blk = 0; blk < KB; ++blk) there |= page_of(j, blk) >= 0 ? 1u << blk : 0u;
+        const bool edge = !(n0 + kKeys - 1 <= sp.pos0 && n0 > sp.pos1 - weff && there == (1u << KB) - 1);
+        f32x4 s[NB][KB];
         tile.logits(s);
         const bool more = j + 1 < n_it;
         if (more) {
-            entries(j + 1);
+            if (((j + 1) & 63) == 0) entries(j + 1);
             fetch_k(j + 1);
         }
         const bool odd = tile.stage_v(edge, sp.lo - n0, sp.hi - n0, there, lane);
         if (more) fetch_v(j + 1);
-        // (a key that one query sees and another does not: only where there are several)
-        const bool by_hand = edge && sp.pos0 != sp.pos1 && __builtin_amdgcn_ballot_w64(odd) != 0ull;
-
+        if (edge) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            if (edge) {
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int blk = 0; blk < 2; ++blk)
+                for (int blk = 0; blk < KB; ++blk)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int key = n0 + 16 * blk + 4 * quad + e;
                         s[nb][blk][e] = key <= pq[nb] && key > pq[nb] - weff && (there >> blk & 1) ? s[nb][blk][e] : -INFINITY;
                     }
-            }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
             float mx = s[nb][0][0];
 #pragma unroll
-            for (int e = 1; e < 8; ++e) mx = fast_max(mx, s[nb][e >> 2][e & 3]);
+            for (int e = 1; e < 4 * KB; ++e) mx = fast_max(mx, s[nb][e >> 2][e & 3]);
             mx *= a.scale_log2;
             if (__builtin_amdgcn_ballot_w64(mx > m[nb] + kRaise) != 0ull) {
                 const float m_new = fast_max(m[nb], quad_max(mx)), alpha = fast_exp2(m[nb] - m_new);
@@ -490,30 +549,32 @@ __global__ __launch_bounds__(64 * kPagedWaves, NB == 1 && sizeof(T) == 2 ? 4 : 2
                 for (int d = 0; d < 4; ++d) tile.o[nb][d] *= alpha;
                 m[nb] = m_new;
             }
-            float sum = 0.0f;
+            float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 4 * KB; ++e) {
                 const float p = fast_exp2(fmaf(s[nb][e >> 2][e & 3], a.scale_log2, -m[nb]));
                 s[nb][e >> 2][e & 3] = p;
-                sum += p;
+                if (e & 1) sum1 += p;
+                else sum0 += p;
             }
-            l[nb] += sum;
+            l[nb] += sum0 + sum1;
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        if (!by_hand) {
+        // (a key that one query sees and another does not: only where there are several)
+        if (__builtin_expect(!edge || sp.pos0 == sp.pos1 || __builtin_amdgcn_ballot_w64(odd) == 0ull, 1)) {
             tile.product(s);
         } else {
             // infinities or NaN in V: key by key, and only for the queries that see it (0 times infinity is NaN)
 #pragma unroll 1
-            for (int key = 0; key < kPagedKeys; ++key) {
+            for (int key = 0; key < kKeys; ++key) {
                 const int from = ((key >> 2 & 3) << 4) | l16, reg = (key >> 4) * 4 + (key & 3);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                     float p = s[nb][0][0];
 #pragma unroll
-                    for (int e = 1; e < 8; ++e) p = reg == e ? s[nb][e >> 2][e & 3] : p;
+                    for (int e = 1; e < 4 * KB; ++e) p = reg == e ? s[nb][e >> 2][e & 3] : p;
                     p = __shfl(p, from);
                     if (n0 + key <= pq[nb] && n0 + key > pq[nb] - weff && (there >> (key >> 4) & 1)) {
 #pragma unroll
@@ -529,17 +590,17 @@ __global__ __launch_bounds__(64 * kPagedWaves, NB == 1 && sizeof(T) == 2 ? 4 : 2
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 
-    // ---- merge the wavefronts, up to 32 pairs at a time: rows [wavefront][pair][64 + (m, l)] in LDS ----
-    constexpr int kHalf = NB > 2 ? 2 : NB;
+    // ---- merge the wavefronts: rows [wavefront][pair][64 + (m, l)] in LDS ----
+    constexpr int kMerge = paged_merge_blocks<NB>();
     float *red = reinterpret_cast<float *>(smem);
     float *part = a.partial + ((int64_t)(share.first + share.index) * a.G + g) * paged_partial_floats(NB);
 #pragma unroll
-    for (int h = 0; h < NB / kHalf; ++h) {
+    for (int h = 0; h < NB / kMerge; ++h) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i) {
-            const int nb = h * kHalf + i;
-            float *row = red + (w * 16 * kHalf + 16 * i + l16) * kPagedRow;
+        for (int i = 0; i < kMerge; ++i) {
+            const int nb = h * kMerge + i;
+            float *row = red + (w * 16 * kMerge + 16 * i + l16) * kPagedRow;
             const float l_tot = quad_sum(l[nb]);
 #pragma unroll
             for (int d = 0; d < 4; ++d)
@@ -549,50 +610,57 @@ __global__ __launch_bounds__(64 * kPagedWaves, NB == 1 && sizeof(T) == 2 ? 4 : 2
         }
         __syncthreads();
         // eight lanes per row, eight columns each
-        const int c8 = (tid & 7) * 8, local = tid >> 3;
-        const int slot = h * 16 * kHalf + local;
-        if (local < 16 * kHalf && slot < pairs) {
+        const int c8 = (tid & 7) * 8;
+#pragma unroll
+        for (int local = tid >> 3; local < 16 * kMerge; local += 8 * NW) {
+            const int mine = h * 16 * kMerge + local;
+            if (mine >= pairs) break;
             float top = kLowest, l_all = 0.0f, acc[8];
 #pragma unroll
-            for (int k = 0; k < NW; ++k) top = fast_max(top, red[(k * 16 * kHalf + local) * kPagedRow + kD]);
+            for (int k = 0; k < NW; ++k) top = fast_max(top, red[(k * 16 * kMerge + local) * kPagedRow + kD]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
 #pragma unroll
             for (int k = 0; k < NW; ++k) {
-                const float *row = red + (k * 16 * kHalf + local) * kPagedRow;
+                const float *row = red + (k * 16 * kMerge + local) * kPagedRow;
                 const float f = fast_exp2(row[kD] - top);
                 l_all += f * row[kD + 1];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) acc[e] += f * row[c8 + e];
             }
             if (share.count > 1) {
-                *reinterpret_cast<f32x4 *>(part + slot * kD + c8) = f32x4{acc[0], acc[1], acc[2], acc[3]};
-                *reinterpret_cast<f32x4 *>(part + slot * kD + c8 + 4) = f32x4{acc[4], acc[5], acc[6], acc[7]};
-                if (c8 == 0) { part[kPairs * kD + 2 * slot] = top; part[kPairs * kD + 2 * slot + 1] = l_all; }
+                *reinterpret_cast<f32x4 *>(part + mine * kD + c8) = f32x4{acc[0], acc[1], acc[2], acc[3]};
+                *reinterpret_cast<f32x4 *>(part + mine * kD + c8 + 4) = f32x4{acc[4], acc[5], acc[6], acc[7]};
+                if (c8 == 0) { part[kPairs * kD + 2 * mine] = top; part[kPairs * kD + 2 * mine + 1] = l_all; }
             } else {
-                const int pair = sp.pair0 + slot, row = pair / a.r, head = g * a.r + pair % a.r;
-                paged_finish<T>(a, sp, row, head, c8, top, l_all, acc);
+                const int pair = sp.pair0 + mine, row = a.by_r.quotient(pair), head = g * a.r + pair - row * a.r, pos = sp.base + row;
+                paged_finish<T>(a, sp.b, row, head, c8, paged_sink(a, head), pos < 0 || pos >= sp.n || l_all == 0.0f, top, l_all, acc);
             }
         }
     }
-    if (a.plan && share.index == 0 && g == 0 && tid == 0) {
-        a.plan[2 * unit] = share.first;
-        a.plan[2 * unit + 1] = share.count;
+    if (a.shares && share.index == 0 && g == 0 && tid == 0) {
+        a.plan[2 * share.unit] = share.first;
+        a.plan[2 * share.unit + 1] = share.count;
     }
 }
 
-// Shares of one (batch row, head, query) row, one wavefront per row: lane = (group of shares, 8 columns), added in an order that
+// Shares of one (batch row, KV head, pair) row, one wavefront per row: lane = (group of shares, 8 columns), added in an order that
 // depends on their number only.
 template <typename T, int NB>
 __global__ __launch_bounds__(256) void attn_paged_combine_kernel(const PagedArgs a) {
     constexpr int kPairs = 16 * NB;
     const int lane = threadIdx.x & 63, c8 = (lane & 7) * 8, sg = lane >> 3;
-    const int64_t idx = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t per_head = (int64_t)a.Sq * a.r;
-    if (idx >= (int64_t)a.B * a.G * per_head) return;
-    const int pair = (int)(idx % per_head), g = (int)(idx / per_head % a.G), b = (int)(idx / per_head / a.G);
-    const int unit = b * a.blocks + pair / kPairs, slot = pair % kPairs;
+    // workgroups: four pairs of a (batch row, KV head)
+    const int per_head = a.Sq * a.r, quads = (per_head + 3) / 4;
+    int bid = a.by_quads.quotient(blockIdx.x);
+    const int pair = (blockIdx.x - bid * quads) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = a.by_g.quotient(bid), g = bid - b * a.G;
+    if (pair >= per_head) return;
+    const int block = pair / kPairs, slot = pair % kPairs, row = a.by_r.quotient(pair), head = g * a.r + pair - row * a.r;
+    const int unit = b * a.blocks + block;
     const int first = a.plan[2 * unit], count = a.plan[2 * unit + 1];
+    const float sink = paged_sink(a, head);
+    const int n = paged_length(a, b), pos = paged_base(a, b, n) + row;
     if (count == 1) return;
     const float *part = a.partial + ((int64_t)first * a.G + g) * paged_partial_floats(NB);
     const int64_t step = a.G * paged_partial_floats(NB);
@@ -621,7 +689,7 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(const PagedArgs
         acc[e] *= f;
         acc[e] += __shfl_xor(acc[e], 8); acc[e] += __shfl_xor(acc[e], 16); acc[e] += __shfl_xor(acc[e], 32);
     }
-    if (sg == 0) paged_finish<T>(a, paged_span(a, unit, kPairs), pair / a.r, g * a.r + pair % a.r, c8, top, l, acc);
+    if (sg == 0) paged_finish<T>(a, b, row, head, c8, sink, pos < 0 || pos >= n || l == 0.0f, top, l, acc);
 }
 
 }  // namespace gptoss

@@ -23,23 +23,28 @@ int check_rows(const void *p, const gptoss_attn_strides &s, int eb) {
 
 Strides cvt(const gptoss_attn_strides &s) { return Strides{s.b, s.h, s.s}; }
 
+PagedPool pool(void *base, const gptoss_attn_strides &s, int eb) { return PagedPool{static_cast<char *>(base), s.h * eb, (uint32_t)(s.b * eb), (uint32_t)(s.s * eb)}; }
+
+// Strides that the kernels keep in 32 bits.
+bool pool_fits(const gptoss_attn_strides &s, int eb) { return s.b >= 0 && s.b * eb <= 0xffffffffll && s.s >= 0 && s.s <= (1 << 24); }
+
 PagedArgs make_args(const gptoss_attn_paged_params *p) {
     PagedArgs a{};
     a.q = p->q;
     a.sinks = p->sinks;
     a.o = p->o;
     a.lse = p->lse;
-    a.k_pages = static_cast<char *>(p->k_pages);
-    a.v_pages = static_cast<char *>(p->v_pages);
-    a.k_exp = p->k_exp;
-    a.v_exp = p->v_exp;
+    const int eb = p->storage == GPTOSS_ATTN_E4M3 ? 1 : p->storage == GPTOSS_ATTN_FP32 ? 4 : 2;
+    a.kp = pool(p->k_pages, p->k_page_stride, eb);
+    a.vp = pool(p->v_pages, p->v_page_stride, eb);
+    a.ke = pool(p->k_exp, p->k_exp_stride, 1);
+    a.ve = pool(p->v_exp, p->v_exp_stride, 1);
     a.table = p->page_table;
     a.seqlens = p->seqlens;
     a.start = p->start;
     a.k = static_cast<char *>(p->k);
     a.v = static_cast<char *>(p->v);
     a.qs = cvt(p->q_stride); a.os = cvt(p->o_stride); a.ks = cvt(p->k_stride); a.vs = cvt(p->v_stride);
-    a.kps = cvt(p->k_page_stride); a.vps = cvt(p->v_page_stride); a.kes = cvt(p->k_exp_stride); a.ves = cvt(p->v_exp_stride);
     a.table_stride = p->table_stride;
     a.B = p->B; a.H = p->H; a.G = p->G; a.Sq = p->Sq;
     a.r = p->H > 0 ? p->H / p->G : 0;
@@ -64,7 +69,7 @@ int launch(Kernel kernel, int64_t workgroups, int threads, void *stream, const P
 
 // How the attention's work is divided: column blocks of 16 pairs, blocks of pairs of a row, (row, block) units, shares of all units'
 // tiles for each KV head beside one for each unit (0: units stay whole), and the scratch that takes.
-constexpr int kMinTiles = 8;
+constexpr int kMinKeys = 256;
 struct PagedDivision { int nb, blocks, shares; int64_t units; size_t plan_bytes, bytes; };
 
 PagedDivision paged_division(const gptoss_attn_paged_params *p) {
@@ -75,13 +80,12 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     const int64_t blocks = (pairs + 16 * d.nb - 1) / (16 * d.nb);
     d.blocks = (int)(blocks < 0x7fffffff ? blocks : 0x7fffffff);
     d.units = blocks * p->B;
-    // the most tiles that a unit can have
+    // the most keys that a unit can see
     int64_t keys = (int64_t)p->table_width * p->page_size;
     if (p->max_len > 0 && p->max_len < keys) keys = p->max_len;
     const int64_t queries = (16 * d.nb - 1) / (p->H / p->G) + 2;                   // that a unit's pairs touch
-    if (p->window > 0 && p->window + queries + 2 * kPagedKeys < keys) keys = p->window + queries + 2 * kPagedKeys;
-    const int64_t tiles = (keys + kPagedKeys - 1) / kPagedKeys;
-    if (d.units > kPagedMaxUnits || tiles <= kMinTiles) return d;
+    if (p->window > 0 && p->window + queries < keys) keys = p->window + queries;
+    if (d.units > kPagedMaxUnits || keys <= kMinKeys) return d;
     d.shares = 1024 / p->G > 0 ? 1024 / p->G : 1;
     d.plan_bytes = ((size_t)d.units * 2 * sizeof(int) + 15) & ~(size_t)15;
     d.bytes = d.plan_bytes + (size_t)(d.shares + d.units) * p->G * paged_partial_floats(d.nb) * sizeof(float);
@@ -89,10 +93,11 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
 }
 
 template <typename T, typename ST, int NB>
-int attend(const PagedDivision &d, void *stream, const PagedArgs &a) {
+int attend(const PagedDivision &d, void *stream, PagedArgs &a) {
+    a.min_tiles = kMinKeys / (16 * paged_tile_blocks<T, ST, NB>());
     const int s = launch(attn_paged_kernel<T, ST, NB>, (d.shares + d.units) * a.G, 64 * kPagedWaves, stream, a);
     if (s || !d.shares) return s;
-    return launch(attn_paged_combine_kernel<T, NB>, ((int64_t)a.B * a.H * a.Sq + 3) / 4, 256, stream, a);
+    return launch(attn_paged_combine_kernel<T, NB>, (int64_t)a.B * a.G * (((int64_t)a.Sq * a.r + 3) / 4), 256, stream, a);
 }
 
 }  // namespace
@@ -116,6 +121,8 @@ int gptoss_attn_paged_validate(const gptoss_attn_paged_params *p, int call) {
     if ((rc = check_rows(p->k_pages, p->k_page_stride, codes ? 1 : eb))) return rc;
     if ((rc = check_rows(p->v_pages, p->v_page_stride, codes ? 1 : eb))) return rc;
     if (!p->page_table || (codes && (!p->k_exp || !p->v_exp))) return GPTOSS_ATTN_ERR_NULL_TENSOR;
+    if (!pool_fits(p->k_page_stride, codes ? 1 : eb) || !pool_fits(p->v_page_stride, codes ? 1 : eb)) return GPTOSS_ATTN_ERR_STRIDE;
+    if (codes && (!pool_fits(p->k_exp_stride, 1) || !pool_fits(p->v_exp_stride, 1))) return GPTOSS_ATTN_ERR_STRIDE;
     if (!aligned(p->page_table, 4) || !aligned(p->seqlens, 4) || !aligned(p->start, 4)) return GPTOSS_ATTN_ERR_ALIGNMENT;
     if (call == kWrite ? !p->start : !p->seqlens) return GPTOSS_ATTN_ERR_NULL_TENSOR;
     if (call != kFwd) {
@@ -142,11 +149,14 @@ int gptoss_attn_paged_fwd(const gptoss_attn_paged_params *p, void *stream) {
     if (rc) return rc;
     PagedArgs a = make_args(p);
     const PagedDivision d = paged_division(p);
-    if (d.units > 0x7fffffff) return GPTOSS_ATTN_ERR_SHAPE;
+    if (d.units > 0x7fffffff || (int64_t)a.Sq * a.r > (1 << 30)) return GPTOSS_ATTN_ERR_SHAPE;
     a.blocks = d.blocks;
     a.units = (int)d.units;
     a.shares = d.shares;
-    a.min_tiles = kMinTiles;
+    a.by_r = div_by(a.r);
+    a.by_g = div_by(a.G);
+    a.by_blocks = div_by(a.blocks);
+    a.by_quads = div_by(((int64_t)a.Sq * a.r + 3) / 4);
     if (d.shares) {
         a.plan = static_cast<int *>(p->scratch);
         a.partial = reinterpret_cast<float *>(static_cast<char *>(p->scratch) + d.plan_bytes);

@@ -37,12 +37,12 @@ __device__ __forceinline__ uint2 e4m3_codes(const float (&x)[8], int s) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store_quantised(char *pages, int64_t at, uint8_t *exps, int64_t exp_at, int c8, const T *src) {
+__device__ __forceinline__ void store_quantised(char *row, char *exp, int c8, const T *src) {
     float x[8];
     load8(src + c8, x);
     const int s = row_exponent(x);
-    *reinterpret_cast<uint2 *>(pages + at + c8) = e4m3_codes(x, s);
-    if (c8 == 0) exps[exp_at] = (uint8_t)(s + kExpBias);
+    *reinterpret_cast<uint2 *>(row + c8) = e4m3_codes(x, s);
+    if (c8 == 0) *exp = (char)(s + kExpBias);
 }
 
 template <typename T>
@@ -63,25 +63,26 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const PagedArgs a) {
     if (page < 0) return;
     const T *k = reinterpret_cast<const T *>(a.k) + b * a.ks.b + g * a.ks.h + i * a.ks.s;
     const T *v = reinterpret_cast<const T *>(a.v) + b * a.vs.b + g * a.vs.h + i * a.vs.s;
-    const int64_t ka = slot_offset(a.kps, page, g, (int)pos, a.page_shift), va = slot_offset(a.vps, page, g, (int)pos, a.page_shift);
+    const int at = (int)pos & ((1 << a.page_shift) - 1);
+    char *kr = a.kp.head(g) + a.kp.at(page, at), *vr = a.vp.head(g) + a.vp.at(page, at);
     if constexpr (E4M3) {
-        store_quantised(a.k_pages, ka, a.k_exp, slot_offset(a.kes, page, g, (int)pos, a.page_shift), c8, k);
-        store_quantised(a.v_pages, va, a.v_exp, slot_offset(a.ves, page, g, (int)pos, a.page_shift), c8, v);
+        store_quantised(kr, a.ke.head(g) + a.ke.at(page, at), c8, k);
+        store_quantised(vr, a.ve.head(g) + a.ve.at(page, at), c8, v);
     } else {
-        copy8(reinterpret_cast<T *>(a.k_pages) + ka + c8, k + c8);
-        copy8(reinterpret_cast<T *>(a.v_pages) + va + c8, v + c8);
+        copy8(reinterpret_cast<T *>(kr) + c8, k + c8);
+        copy8(reinterpret_cast<T *>(vr) + c8, v + c8);
     }
 }
 
 template <typename T, typename ST>
-__device__ __forceinline__ void read8(T *dst, const char *pages, int64_t at, const uint8_t *exps, int64_t exp_at, int c8, bool there) {
+__device__ __forceinline__ void read8(T *dst, const char *row, const char *exp, int c8, bool there) {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = 0.0f;
     if (there) {
-        load8(reinterpret_cast<const ST *>(pages) + at + c8, x);
+        load8(reinterpret_cast<const ST *>(row) + c8, x);
         if constexpr (sizeof(ST) == 1) {
-            const float f = exp_of_byte(exps[exp_at]);
+            const float f = exp_of_byte(*reinterpret_cast<const uint8_t *>(exp));
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] *= f;
         }
@@ -100,11 +101,9 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const PagedArgs a) {
     const int64_t pos = (a.start ? (int64_t)a.start[b] : 0) + i;
     const int page = pos >= 0 && pos < paged_length(a, b) ? paged_page(a, b, (int)pos) : -1;
     const bool there = page >= 0;
-    const int t = there ? (int)pos : 0, p = there ? page : 0;
-    read8<T, ST>(reinterpret_cast<T *>(a.k) + b * a.ks.b + g * a.ks.h + i * a.ks.s, a.k_pages, slot_offset(a.kps, p, g, t, a.page_shift), a.k_exp,
-                 slot_offset(a.kes, p, g, t, a.page_shift), c8, there);
-    read8<T, ST>(reinterpret_cast<T *>(a.v) + b * a.vs.b + g * a.vs.h + i * a.vs.s, a.v_pages, slot_offset(a.vps, p, g, t, a.page_shift), a.v_exp,
-                 slot_offset(a.ves, p, g, t, a.page_shift), c8, there);
+    const int at = (int)pos & ((1 << a.page_shift) - 1), p = there ? page : 0;
+    read8<T, ST>(reinterpret_cast<T *>(a.k) + b * a.ks.b + g * a.ks.h + i * a.ks.s, a.kp.head(g) + a.kp.at(p, at), a.ke.head(g) + a.ke.at(p, at), c8, there);
+    read8<T, ST>(reinterpret_cast<T *>(a.v) + b * a.vs.b + g * a.vs.h + i * a.vs.s, a.vp.head(g) + a.vp.at(p, at), a.ve.head(g) + a.ve.at(p, at), c8, there);
 }
 
 }  // namespace gptoss

@@ -9,16 +9,36 @@
 
 namespace gptoss {
 
+// Quotients of numbers below 2^31 by a number that the host knows: one multiplication.  With s = ceil(log2 d) and mul = ceil(2^(31 + s) / d) the
+// product is too large by less than x * 2^s / d, which is less than 2^(31 + s) / d: never by a whole quotient.
+struct Div {
+    uint32_t mul, shift;
+    __host__ __device__ __forceinline__ int quotient(int x) const { return (int)(((uint64_t)(uint32_t)x * mul) >> shift); }
+};
+inline Div div_by(int64_t d) {
+    uint32_t s = 0;
+    while (((int64_t)1 << s) < d) ++s;
+    return Div{(uint32_t)((((uint64_t)1 << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d), 31 + s};
+}
+
+// A pool of pages: strides in bytes, of pages and tokens below 2^32.
+struct PagedPool {
+    char *base;
+    int64_t h;
+    uint32_t b, s;
+    __device__ __forceinline__ char *head(int g) const { return base + g * h; }
+    __device__ __forceinline__ int64_t at(int page, int slot) const { return (int64_t)((uint64_t)(uint32_t)page * b + (uint64_t)(uint32_t)slot * s); }
+};
+
 struct PagedArgs {
     const void *q, *sinks;
     void *o;
     float *lse;
-    char *k_pages, *v_pages;
-    uint8_t *k_exp, *v_exp;
+    PagedPool kp, vp;            // rows in bytes
+    PagedPool ke, ve;            // their exponents
     const int32_t *table, *seqlens, *start;
     char *k, *v;                 // rows to write, or the result of reading
     Strides qs, os, ks, vs;      // elements
-    Strides kps, vps, kes, ves;  // (page, KV head, token), elements
     int64_t table_stride;
     int B, H, G, r, Sq;
     int pages, page_shift, width, window;
@@ -26,6 +46,7 @@ struct PagedArgs {
     // attention: (row, block of pairs) units, into how many shares their work is cut (0: not), of how many tiles at least; the shares'
     // partial results and, for each unit, its first share and their number
     int units, shares, min_tiles;
+    Div by_r, by_g, by_blocks, by_quads;        // by r, G, blocks, and a row and KV head's workgroups of the sum over shares
     float *partial;
     int *plan;
     float scale_log2;
@@ -53,11 +74,6 @@ __device__ __forceinline__ int paged_length(const PagedArgs &a, int b) {
 }
 
 __device__ __forceinline__ float exp_of_byte(uint32_t e) { return __uint_as_float(e << 23); }        // 2^(e - 127), e >= 1
-
-// Element offset of slot t of a page.
-__device__ __forceinline__ int64_t slot_offset(const Strides &s, int page, int g, int t, int page_shift) {
-    return page * s.b + g * s.h + (int64_t)(t & ((1 << page_shift) - 1)) * s.s;
-}
 
 struct e4m3 { uint8_t code; };
 
