@@ -32,6 +32,8 @@ constexpr float kRaise = 8.0f;                  // in the exponent of two
 
 // Blocks of 16 keys in a tile: what a wavefront has under way is a tile, so rows of fewer bytes come more at a time.
 template <typename T, typename ST, int NB> __host__ __device__ constexpr int paged_tile_blocks() { return sizeof(T) == 2 && sizeof(ST) == 1 && NB == 1 ? 4 : 2; }
+// Workgroups of a kernel that a compute unit holds (wavefronts per SIMD): what its registers leave.
+template <typename T, typename ST, int NB> __host__ __device__ constexpr int paged_occupancy() { return sizeof(T) == 4 || NB > 1 ? 2 : sizeof(ST) == 1 ? 3 : 4; }
 // Pairs (query, head of the group) that one workgroup may take.
 template <typename T> __host__ __device__ constexpr int paged_pairs() { return sizeof(T) == 2 ? 64 : 32; }
 // floats of a share's partial result: rows of O, then (m, l) of each
@@ -156,6 +158,14 @@ __device__ __forceinline__ bf16x8 widen8(uint32_t w0, uint32_t w1, float f) {
     return x.v;
 }
 
+// Rows that no other workgroup reads bypass the caches' retention: 16 x 8192 tokens 54.1 -> 48.5 us, 4 x 65536 101 -> 89.7 (6.0 TB/s), 32 rows of
+// 6000 to 16384 in e4m3 73.8 -> 68.7.  A row of more pairs than a workgroup takes is read again by the next one (NB = 4, and two blocks in 32 bits).
+template <bool ONCE, typename V>
+__device__ __forceinline__ V load_rows(const char *p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
+    else return *reinterpret_cast<const V *>(p);
+}
+
 // A tile's K and V as they are loaded, and what is done with them.  `kb` / `vb`: scalar addresses of the first row of a block of 16 keys;
 // lanes: l16 = lane % 16, quad = lane / 16.
 template <typename T, typename ST, int NB, int KB> struct PagedTile;
@@ -163,7 +173,7 @@ template <typename T, typename ST, int NB, int KB> struct PagedTile;
 // ---- bfloat16 products -----------------------------------------------------------------------------------------------
 template <typename ST, int NB, int KB>
 struct PagedTile<bf16, ST, NB, KB> {
-    static constexpr bool kCodes = sizeof(ST) == 1;
+    static constexpr bool kCodes = sizeof(ST) == 1, kOnce = NB < 4;
     static constexpr int kStage = 16 * KB * kRowBytes;           // LDS bytes of a wavefront
     static constexpr int kVecs = kCodes ? 1 : 2;                 // 16-byte loads per lane and block
     u32x4 k[KB][kVecs], v[KB][kVecs];
@@ -200,12 +210,12 @@ struct PagedTile<bf16, ST, NB, KB> {
     }
     __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb) {
 #pragma unroll
-        for (int s = 0; s < kVecs; ++s) k[blk][s] = *reinterpret_cast<const u32x4 *>(kb + k_at + 64 * s);
+        for (int s = 0; s < kVecs; ++s) k[blk][s] = load_rows<kOnce, u32x4>(kb + k_at + 64 * s);
         if constexpr (kCodes) ke[blk] = (uint8_t)eb[ke_at];
     }
     __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb) {
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) v[blk][i] = *reinterpret_cast<const u32x4 *>(vb + v_at[i]);
+        for (int i = 0; i < kVecs; ++i) v[blk][i] = load_rows<kOnce, u32x4>(vb + v_at[i]);
         if constexpr (kCodes) ve[blk] = (uint8_t)eb[ve_at];
     }
     __device__ __forceinline__ void logits(f32x4 (&s)[NB][KB]) const {
@@ -293,7 +303,7 @@ struct PagedTile<bf16, ST, NB, KB> {
 // ---- float32 products ------------------------------------------------------------------------------------------------
 template <typename ST, int NB, int KB>
 struct PagedTile<float, ST, NB, KB> {
-    static constexpr bool kCodes = sizeof(ST) == 1;
+    static constexpr bool kCodes = sizeof(ST) == 1, kOnce = NB < 2;
     static constexpr int kStage = 16 * KB * kD * 4;              // used where V holds infinities or NaN only
     static constexpr int kVecs = kCodes ? 1 : 4;
     typedef typename std::conditional<kCodes, uint32_t, f32x4>::type vec;       // four numbers of a row of V
@@ -329,13 +339,13 @@ struct PagedTile<float, ST, NB, KB> {
     }
     __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb) {
 #pragma unroll
-        for (int s = 0; s < kVecs; ++s) k[blk][s] = *reinterpret_cast<const u32x4 *>(kb + k_at + 64 * s);
+        for (int s = 0; s < kVecs; ++s) k[blk][s] = load_rows<kOnce, u32x4>(kb + k_at + 64 * s);
         if constexpr (kCodes) ke[blk] = (uint8_t)eb[ke_at];
     }
     __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            v[blk][e] = *reinterpret_cast<const vec *>(vb + v_at[e]);
+            v[blk][e] = load_rows<kOnce, vec>(vb + v_at[e]);
             if constexpr (kCodes) ve[blk][e] = (uint8_t)eb[ve_at[e]];
         }
     }
@@ -435,7 +445,7 @@ constexpr int paged_lds_bytes() {
 }
 
 template <typename T, typename ST, int NB>
-__global__ __launch_bounds__(64 * kPagedWaves, NB == 1 && sizeof(T) == 2 ? (sizeof(ST) == 1 ? 3 : 4) : 2) void attn_paged_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<T, ST, NB>())) void attn_paged_kernel(const PagedArgs a) {
     constexpr int NW = kPagedWaves, kPairs = 16 * NB, KB = paged_tile_blocks<T, ST, NB>(), kKeys = 16 * KB;
     using Tile = PagedTile<T, ST, NB, KB>;
     __shared__ __attribute__((aligned(128))) char smem[paged_lds_bytes<T, ST, NB>()];

@@ -86,7 +86,16 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     const int64_t queries = (16 * d.nb - 1) / (p->H / p->G) + 2;                   // that a unit's pairs touch
     if (p->window > 0 && p->window + queries < keys) keys = p->window + queries;
     if (d.units > kPagedMaxUnits || keys <= kMinKeys) return d;
-    d.shares = 1024 / p->G > 0 ? 1024 / p->G : 1;
+    // As many workgroups as a 256-CU part holds at a time: they start and end together.  A unit's last share is half of one on average; at
+    // least half of the workgroups are shares all the same, so that a long row among many is cut.
+    const bool codes = p->storage == GPTOSS_ATTN_E4M3;
+    const int per_cu = p->dtype == GPTOSS_ATTN_FP32 ? paged_occupancy<float, float, 1>()
+                       : d.nb > 1                   ? paged_occupancy<bf16, bf16, 2>()
+                       : codes                      ? paged_occupancy<bf16, e4m3, 1>()
+                                                    : paged_occupancy<bf16, bf16, 1>();
+    const int64_t held = 256 * per_cu / p->G, left = held - d.units / 2;
+    d.shares = (int)(left > held / 2 ? left : held / 2);
+    if (d.shares < 1) d.shares = 1;
     d.plan_bytes = ((size_t)d.units * 2 * sizeof(int) + 15) & ~(size_t)15;
     d.bytes = d.plan_bytes + (size_t)(d.shares + d.units) * p->G * paged_partial_floats(d.nb) * sizeof(float);
     return d;
