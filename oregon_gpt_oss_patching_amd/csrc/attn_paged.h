@@ -26,14 +26,16 @@
 
 namespace gptoss {
 
-constexpr int kPagedWaves = 4, kPagedMaxUnits = 1024;
+constexpr int kPagedMaxUnits = 1024;
 constexpr int kPagedRow = kD + 2;               // floats of a merged row: O, m, l
 constexpr float kRaise = 8.0f;                  // in the exponent of two
 
+// Wavefronts of a workgroup: four, or (NW) up to as many as a compute unit runs where one workgroup walks a unit alone.
+constexpr int kPagedWaves = 4;
 // Blocks of 16 keys in a tile: what a wavefront has under way is a tile, so rows of fewer bytes come more at a time.
-template <typename T, typename ST, int NB> __host__ __device__ constexpr int paged_tile_blocks() { return sizeof(T) == 2 && sizeof(ST) == 1 && NB == 1 ? 4 : 2; }
-// Workgroups of a kernel that a compute unit holds (wavefronts per SIMD): what its registers leave.
-template <typename T, typename ST, int NB> __host__ __device__ constexpr int paged_occupancy() { return sizeof(T) == 4 || NB > 1 ? 2 : sizeof(ST) == 1 ? 3 : 4; }
+template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_tile_blocks() { return sizeof(T) == 2 && sizeof(ST) == 1 && NB == 1 && NW == kPagedWaves ? 4 : 2; }
+// Wavefronts per SIMD, of what the registers leave.
+template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_occupancy() { return sizeof(T) == 4 || NB > 1 ? 2 : sizeof(ST) == 1 && NW == kPagedWaves ? 3 : 4; }
 // Pairs (query, head of the group) that one workgroup may take.
 template <typename T> __host__ __device__ constexpr int paged_pairs() { return sizeof(T) == 2 ? 64 : 32; }
 // floats of a share's partial result: rows of O, then (m, l) of each
@@ -435,20 +437,21 @@ __device__ __forceinline__ void paged_finish(const PagedArgs &a, int b, int row,
     if (c8 == 0) a.lse[((int64_t)b * a.H + head) * a.Sq + row] = none ? sink : (ref + fast_log2(z)) * kLn2;
 }
 
-// column blocks that are merged at a time
+// column blocks and wavefronts that are merged at a time
 template <int NB> constexpr int paged_merge_blocks() { return NB == 4 ? 2 : NB; }
-template <typename T, typename ST, int NB>
+template <int NW> constexpr int paged_merge_waves() { return NW < 8 ? NW : 8; }
+template <typename T, typename ST, int NB, int NW>
 constexpr int paged_lds_bytes() {
-    constexpr int merge = kPagedWaves * 16 * paged_merge_blocks<NB>() * kPagedRow * 4;
-    constexpr int stages = kPagedWaves * PagedTile<T, ST, NB, paged_tile_blocks<T, ST, NB>()>::kStage;
+    constexpr int merge = paged_merge_waves<NW>() * 16 * paged_merge_blocks<NB>() * kPagedRow * 4;
+    constexpr int stages = NW * PagedTile<T, ST, NB, paged_tile_blocks<T, ST, NB, NW>()>::kStage;
     return stages > merge ? stages : merge;
 }
 
-template <typename T, typename ST, int NB>
-__global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<T, ST, NB>())) void attn_paged_kernel(const PagedArgs a) {
-    constexpr int NW = kPagedWaves, kPairs = 16 * NB, KB = paged_tile_blocks<T, ST, NB>(), kKeys = 16 * KB;
+template <typename T, typename ST, int NB, int NW>
+__global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void attn_paged_kernel(const PagedArgs a) {
+    constexpr int kPairs = 16 * NB, KB = paged_tile_blocks<T, ST, NB, NW>(), kKeys = 16 * KB;
     using Tile = PagedTile<T, ST, NB, KB>;
-    __shared__ __attribute__((aligned(128))) char smem[paged_lds_bytes<T, ST, NB>()];
+    __shared__ __attribute__((aligned(128))) char smem[paged_lds_bytes<T, ST, NB, NW>()];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, quad = lane >> 4;
     const int slot = a.by_g.quotient(blockIdx.x), g = blockIdx.x - slot * a.G;
     PagedSpan sp;
@@ -601,8 +604,32 @@ __global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<T, ST, NB>())) v
     }
 
     // ---- merge the wavefronts: rows [wavefront][pair][64 + (m, l)] in LDS ----
-    constexpr int kMerge = paged_merge_blocks<NB>();
+    constexpr int kMerge = paged_merge_blocks<NB>(), MW = paged_merge_waves<NW>();
     float *red = reinterpret_cast<float *>(smem);
+    if constexpr (NW > MW) {
+        // LDS holds half of them: the upper ones hand theirs over first
+        static_assert(NW == 2 * MW && NB == 1, "one block of columns, two halves");
+        float *row = red + ((w % MW) * 16 + l16) * kPagedRow;
+        const float l_tot = quad_sum(l[0]);
+        __syncthreads();
+        if (w >= MW) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) row[Tile::column(d, e, quad)] = tile.o[0][d][e];
+            if (quad == 0) { row[kD] = m[0]; row[kD + 1] = l_tot; }
+        }
+        __syncthreads();
+        if (w < MW) {
+            const float top = fast_max(m[0], row[kD]), f = fast_exp2(m[0] - top), f2 = fast_exp2(row[kD] - top);
+            l[0] = l[0] * f + (quad == 0 ? f2 * row[kD + 1] : 0.0f);
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) tile.o[0][d][e] = tile.o[0][d][e] * f + f2 * row[Tile::column(d, e, quad)];
+            m[0] = top;
+        }
+    }
     float *part = a.partial + ((int64_t)(share.first + share.index) * a.G + g) * paged_partial_floats(NB);
 #pragma unroll
     for (int h = 0; h < NB / kMerge; ++h) {
@@ -612,6 +639,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<T, ST, NB>())) v
             const int nb = h * kMerge + i;
             float *row = red + (w * 16 * kMerge + 16 * i + l16) * kPagedRow;
             const float l_tot = quad_sum(l[nb]);
+            if (NW > MW && w >= MW) continue;
 #pragma unroll
             for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -627,11 +655,11 @@ __global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<T, ST, NB>())) v
             if (mine >= pairs) break;
             float top = kLowest, l_all = 0.0f, acc[8];
 #pragma unroll
-            for (int k = 0; k < NW; ++k) top = fast_max(top, red[(k * 16 * kMerge + local) * kPagedRow + kD]);
+            for (int k = 0; k < MW; ++k) top = fast_max(top, red[(k * 16 * kMerge + local) * kPagedRow + kD]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < NW; ++k) {
+            for (int k = 0; k < MW; ++k) {
                 const float *row = red + (k * 16 * kMerge + local) * kPagedRow;
                 const float f = fast_exp2(row[kD] - top);
                 l_all += f * row[kD + 1];
@@ -654,16 +682,16 @@ __global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<T, ST, NB>())) v
     }
 }
 
-// Shares of one (batch row, KV head, pair) row, one wavefront per row: lane = (group of shares, 8 columns), added in an order that
-// depends on their number only.
-template <typename T, int NB>
+// Shares of one (batch row, KV head, pair) row, WR wavefronts per row (one: four rows to a workgroup): lane = (group of shares, 8 columns),
+// added in an order that depends on their number only.
+template <typename T, int NB, int WR>
 __global__ __launch_bounds__(256) void attn_paged_combine_kernel(const PagedArgs a) {
-    constexpr int kPairs = 16 * NB;
-    const int lane = threadIdx.x & 63, c8 = (lane & 7) * 8, sg = lane >> 3;
-    // workgroups: four pairs of a (batch row, KV head)
-    const int per_head = a.Sq * a.r, quads = (per_head + 3) / 4;
-    int bid = a.by_quads.quotient(blockIdx.x);
-    const int pair = (blockIdx.x - bid * quads) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int kPairs = 16 * NB, kRows = 4 / WR, kGroups = 8 * WR;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c8 = (lane & 7) * 8;
+    // workgroups: kRows pairs of a (batch row, KV head)
+    const int per_head = a.Sq * a.r, wgs = (per_head + kRows - 1) / kRows;
+    const int bid = a.by_wgs.quotient(blockIdx.x);
+    const int pair = (blockIdx.x - bid * wgs) * kRows + (WR == 1 ? w : 0);
     const int b = a.by_g.quotient(bid), g = bid - b * a.G;
     if (pair >= per_head) return;
     const int block = pair / kPairs, slot = pair % kPairs, row = a.by_r.quotient(pair), head = g * a.r + pair - row * a.r;
@@ -677,7 +705,7 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(const PagedArgs
     float m = kLowest, l = 0.0f, acc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-    for (int s = sg; s < count; s += 8) {
+    for (int s = (WR == 1 ? 0 : 8 * w) + (lane >> 3); s < count; s += kGroups) {
         const float *p = part + s * step;
         const float ms = p[kPairs * kD + 2 * slot], ls = p[kPairs * kD + 2 * slot + 1];
         const f32x4 x = *reinterpret_cast<const f32x4 *>(p + slot * kD + c8), y = *reinterpret_cast<const f32x4 *>(p + slot * kD + c8 + 4);
@@ -691,7 +719,7 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(const PagedArgs
     top = fast_max(top, __shfl_xor(top, 8));
     top = fast_max(top, __shfl_xor(top, 16));
     top = fast_max(top, __shfl_xor(top, 32));
-    const float f = fast_exp2(m - top);
+    float f = fast_exp2(m - top);
     l *= f;
     l += __shfl_xor(l, 8); l += __shfl_xor(l, 16); l += __shfl_xor(l, 32);
 #pragma unroll
@@ -699,7 +727,31 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(const PagedArgs
         acc[e] *= f;
         acc[e] += __shfl_xor(acc[e], 8); acc[e] += __shfl_xor(acc[e], 16); acc[e] += __shfl_xor(acc[e], 32);
     }
-    if (sg == 0) paged_finish<T>(a, b, row, head, c8, sink, pos < 0 || pos >= n || l == 0.0f, top, l, acc);
+    if constexpr (WR > 1) {
+        __shared__ float red[WR][kPagedRow];
+        if (lane < 8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) red[w][c8 + e] = acc[e];
+            if (lane == 0) { red[w][kD] = top; red[w][kD + 1] = l; }
+        }
+        __syncthreads();
+        if (w != 0) return;
+        float all = kLowest;
+#pragma unroll
+        for (int k = 0; k < WR; ++k) all = fast_max(all, red[k][kD]);
+        l = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < WR; ++k) {
+            f = fast_exp2(red[k][kD] - all);
+            l += f * red[k][kD + 1];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] += f * red[k][c8 + e];
+        }
+        top = all;
+    }
+    if (lane < 8) paged_finish<T>(a, b, row, head, c8, sink, pos < 0 || pos >= n || l == 0.0f, top, l, acc);
 }
 
 }  // namespace gptoss

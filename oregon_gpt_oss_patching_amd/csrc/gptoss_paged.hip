@@ -68,14 +68,15 @@ int launch(Kernel kernel, int64_t workgroups, int threads, void *stream, const P
 }
 
 // How the attention's work is divided: column blocks of 16 pairs, blocks of pairs of a row, (row, block) units, shares of all units'
-// tiles for each KV head beside one for each unit (0: units stay whole), and the scratch that takes.
-constexpr int kMinKeys = 256;
-struct PagedDivision { int nb, blocks, shares; int64_t units; size_t plan_bytes, bytes; };
+// tiles for each KV head beside one for each unit (0: units stay whole, each walked by `alone` wavefronts), keys that a share has at least, and
+// the scratch that takes.
+struct PagedDivision { int nb, blocks, shares, alone, min_keys; int64_t units; size_t plan_bytes, bytes; };
 
 PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     PagedDivision d{};
-    const int64_t pairs = (int64_t)p->Sq * (p->H / p->G);
-    const int most = p->dtype == GPTOSS_ATTN_FP32 ? paged_pairs<float>() : paged_pairs<bf16>();
+    const bool f32 = p->dtype == GPTOSS_ATTN_FP32, codes = p->storage == GPTOSS_ATTN_E4M3;
+    const int64_t r = p->H / p->G, pairs = (int64_t)p->Sq * r;
+    const int most = f32 ? paged_pairs<float>() : paged_pairs<bf16>();
     d.nb = pairs <= 16 ? 1 : pairs <= 32 || most == 32 ? 2 : 4;
     const int64_t blocks = (pairs + 16 * d.nb - 1) / (16 * d.nb);
     d.blocks = (int)(blocks < 0x7fffffff ? blocks : 0x7fffffff);
@@ -83,19 +84,29 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     // the most keys that a unit can see
     int64_t keys = (int64_t)p->table_width * p->page_size;
     if (p->max_len > 0 && p->max_len < keys) keys = p->max_len;
-    const int64_t queries = (16 * d.nb - 1) / (p->H / p->G) + 2;                   // that a unit's pairs touch
+    const int64_t queries = (16 * d.nb - 1) / r + 2;                   // that a unit's pairs touch
     if (p->window > 0 && p->window + queries < keys) keys = p->window + queries;
-    if (d.units > kPagedMaxUnits || keys <= kMinKeys) return d;
+    d.min_keys = f32 ? 128 : 256;
+    // Short rows: a workgroup walks a unit alone, as many wavefronts as its keys and the compute unit's share of the workgroups have room
+    // for, and there is nothing to add in a second launch.  us, cut / alone, 64 heads on 8 KV heads: 1 x 500 tokens 10.3 / 7.7, 1 x 1025 10.3 /
+    // 9.7, but 1 x 1500 10.3 / 12.2; 32 x 1000 18.9 / 14.9, 128 x 250 18.0 / 14.2, 64 x 500 of which most are short 13.0 / 9.7; with two
+    // workgroups to a unit and more the others' rows fill the time that a long one takes: 64 x 2000 48.9 / 43.5, with one of 2000 among shorter ones
+    // 21.3 / 21.7 (32 rows 15.3 / 19.4).  In 32 bits 1 x 257 10.5 / 9.8, but 8 x 500 11.1 / 13.7; 128 x 500 on two KV heads 21.7 / 16.4.
+    const int64_t wgs = d.units * p->G;
+    const bool full = wgs > (f32 ? 128 : 256);
+    d.alone = d.nb > 1 || keys <= 128 || wgs > (f32 ? 256 : 512) ? kPagedWaves : f32 || full || keys <= 256 ? 8 : 16;
+    if (d.units > kPagedMaxUnits || keys <= (f32 ? 288 : 1152) * (full ? 2 : 1)) return d;
+    d.alone = kPagedWaves;
     // As many workgroups as a 256-CU part holds at a time: they start and end together.  A unit's last share is half of one on average; at
-    // least half of the workgroups are shares all the same, so that a long row among many is cut.
-    const bool codes = p->storage == GPTOSS_ATTN_E4M3;
-    const int per_cu = p->dtype == GPTOSS_ATTN_FP32 ? paged_occupancy<float, float, 1>()
-                       : d.nb > 1                   ? paged_occupancy<bf16, bf16, 2>()
-                       : codes                      ? paged_occupancy<bf16, e4m3, 1>()
-                                                    : paged_occupancy<bf16, bf16, 1>();
-    const int64_t held = 256 * per_cu / p->G, left = held - d.units / 2;
-    d.shares = (int)(left > held / 2 ? left : held / 2);
-    if (d.shares < 1) d.shares = 1;
+    // least half of the workgroups are shares all the same, so that a long row among many is cut.  No more than the units can have.
+    const int per_cu = f32        ? paged_occupancy<float, float, 1, kPagedWaves>()
+                       : d.nb > 1 ? paged_occupancy<bf16, bf16, 2, kPagedWaves>()
+                       : codes    ? paged_occupancy<bf16, e4m3, 1, kPagedWaves>()
+                                  : paged_occupancy<bf16, bf16, 1, kPagedWaves>();
+    const int64_t held = 256 * per_cu / p->G, left = held - d.units / 2, can = d.units * ((keys + d.min_keys - 1) / d.min_keys);
+    int64_t shares = left > held / 2 ? left : held / 2;
+    if (shares > can) shares = can;
+    d.shares = shares > 1 ? (int)shares : 1;
     d.plan_bytes = ((size_t)d.units * 2 * sizeof(int) + 15) & ~(size_t)15;
     d.bytes = d.plan_bytes + (size_t)(d.shares + d.units) * p->G * paged_partial_floats(d.nb) * sizeof(float);
     return d;
@@ -103,10 +114,19 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
 
 template <typename T, typename ST, int NB>
 int attend(const PagedDivision &d, void *stream, PagedArgs &a) {
-    a.min_tiles = kMinKeys / (16 * paged_tile_blocks<T, ST, NB>());
-    const int s = launch(attn_paged_kernel<T, ST, NB>, (d.shares + d.units) * a.G, 64 * kPagedWaves, stream, a);
+    if constexpr (NB == 1) {
+        if constexpr (sizeof(T) == 2)
+            if (d.alone == 16) return launch(attn_paged_kernel<T, ST, NB, 16>, d.units * a.G, 1024, stream, a);
+        if (d.alone == 8) return launch(attn_paged_kernel<T, ST, NB, 8>, d.units * a.G, 512, stream, a);
+    }
+    a.min_tiles = d.min_keys / (16 * paged_tile_blocks<T, ST, NB, kPagedWaves>());
+    const int s = launch(attn_paged_kernel<T, ST, NB, kPagedWaves>, (d.shares + d.units) * a.G, 64 * kPagedWaves, stream, a);
     if (s || !d.shares) return s;
-    return launch(attn_paged_combine_kernel<T, NB>, (int64_t)a.B * a.G * (((int64_t)a.Sq * a.r + 3) / 4), 256, stream, a);
+    // a workgroup for each row where they are few and their shares may be many
+    const int64_t heads = (int64_t)a.B * a.G, pairs = (int64_t)a.Sq * a.r;
+    const int64_t wgs = heads * pairs <= 1024 ? pairs : (pairs + 3) / 4;
+    a.by_wgs = div_by(wgs);
+    return wgs == pairs ? launch(attn_paged_combine_kernel<T, NB, 4>, heads * wgs, 256, stream, a) : launch(attn_paged_combine_kernel<T, NB, 1>, heads * wgs, 256, stream, a);
 }
 
 }  // namespace
@@ -165,7 +185,6 @@ int gptoss_attn_paged_fwd(const gptoss_attn_paged_params *p, void *stream) {
     a.by_r = div_by(a.r);
     a.by_g = div_by(a.G);
     a.by_blocks = div_by(a.blocks);
-    a.by_quads = div_by(((int64_t)a.Sq * a.r + 3) / 4);
     if (d.shares) {
         a.plan = static_cast<int *>(p->scratch);
         a.partial = reinterpret_cast<float *>(static_cast<char *>(p->scratch) + d.plan_bytes);

@@ -46,7 +46,7 @@ struct PagedArgs {
     // attention: (row, block of pairs) units, into how many shares their work is cut (0: not), of how many tiles at least; the shares'
     // partial results and, for each unit, its first share and their number
     int units, shares, min_tiles;
-    Div by_r, by_g, by_blocks, by_quads;        // by r, G, blocks, and a row and KV head's workgroups of the sum over shares
+    Div by_r, by_g, by_blocks, by_wgs;          // by r, G, blocks, and a row and KV head's workgroups of the sum over shares
     float *partial;
     int *plan;
     float scale_log2;
