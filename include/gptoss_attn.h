@@ -363,7 +363,7 @@ typedef struct gptoss_attn_paged_params {
     const void *q;                  /* (B, H, Sq, 64) */
     const void *sinks;              /* (H), optional as in gptoss_attn_params */
     void *o;                        /* (B, Sq, H, 64) through its strides */
-    float *lse;                     /* (B, H, Sq) */
+    float *lse;                     /* (B, H, Sq), optional */
     void *k, *v;                    /* (B, G, Sq, 64): read by write, written by read */
     void *scratch;                  /* fwd: gptoss_attn_paged_workspace_bytes() bytes, 16-byte aligned, of this call alone until it has run */
     size_t scratch_bytes;

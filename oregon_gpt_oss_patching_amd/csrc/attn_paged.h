@@ -212,12 +212,12 @@ struct PagedTile<bf16, ST, NB, KB> {
     }
     __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb) {
 #pragma unroll
-        for (int s = 0; s < kVecs; ++s) k[blk][s] = load_rows<kOnce, u32x4>(kb + k_at + 64 * s);
+        for (int s = 0; s < kVecs; ++s) k[blk][s] = load16<kOnce>(kb + k_at + 64 * s);
         if constexpr (kCodes) ke[blk] = (uint8_t)eb[ke_at];
     }
     __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb) {
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) v[blk][i] = load_rows<kOnce, u32x4>(vb + v_at[i]);
+        for (int i = 0; i < kVecs; ++i) v[blk][i] = load16<kOnce>(vb + v_at[i]);
         if constexpr (kCodes) ve[blk] = (uint8_t)eb[ve_at];
     }
     __device__ __forceinline__ void logits(f32x4 (&s)[NB][KB]) const {
@@ -341,7 +341,7 @@ struct PagedTile<float, ST, NB, KB> {
     }
     __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb) {
 #pragma unroll
-        for (int s = 0; s < kVecs; ++s) k[blk][s] = load_rows<kOnce, u32x4>(kb + k_at + 64 * s);
+        for (int s = 0; s < kVecs; ++s) k[blk][s] = load16<kOnce>(kb + k_at + 64 * s);
         if constexpr (kCodes) ke[blk] = (uint8_t)eb[ke_at];
     }
     __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb) {
@@ -434,7 +434,7 @@ __device__ __forceinline__ void paged_finish(const PagedArgs &a, int b, int row,
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = none ? 0.0f : acc[e] * mul;
     store8(static_cast<T *>(a.o) + b * a.os.b + head * a.os.h + row * a.os.s + c8, x);
-    if (c8 == 0) a.lse[((int64_t)b * a.H + head) * a.Sq + row] = none ? sink : (ref + fast_log2(z)) * kLn2;
+    if (c8 == 0 && a.lse) a.lse[((int64_t)b * a.H + head) * a.Sq + row] = none ? sink : (ref + fast_log2(z)) * kLn2;
 }
 
 // column blocks and wavefronts that are merged at a time

@@ -162,8 +162,7 @@ int gptoss_attn_paged_validate(const gptoss_attn_paged_params *p, int call) {
     if (p->window < 0 || p->window > (1 << 30) || p->max_len < 0 || !(p->scale > 0.0f) || !(p->scale < 3.0e38f)) return GPTOSS_ATTN_ERR_SHAPE;
     if ((rc = check_rows(p->q, p->q_stride, eb))) return rc;
     if ((rc = check_rows(p->o, p->o_stride, eb))) return rc;
-    if (!p->lse) return GPTOSS_ATTN_ERR_NULL_TENSOR;
-    if (!aligned(p->scratch, 16)) return GPTOSS_ATTN_ERR_ALIGNMENT;
+    if (!aligned(p->lse, 4) || !aligned(p->scratch, 16)) return GPTOSS_ATTN_ERR_ALIGNMENT;
     if (p->scratch_bytes < gptoss_attn_paged_workspace_bytes(p) || (!p->scratch && gptoss_attn_paged_workspace_bytes(p))) return GPTOSS_ATTN_ERR_WORKSPACE;
     return GPTOSS_ATTN_OK;
 }
@@ -204,25 +203,31 @@ int gptoss_attn_paged_write(const gptoss_attn_paged_params *p, void *stream) {
     const int rc = gptoss_attn_paged_validate(p, kWrite);
     if (rc) return rc;
     PagedArgs a = make_args(p);
-    const int64_t blocks = ((int64_t)a.Sq * a.G + 31) / 32;
-    if (blocks * a.B > 0x7fffffff || (int64_t)a.Sq * a.G > 0x7fffffff - 32) return GPTOSS_ATTN_ERR_SHAPE;
+    const int64_t rows = (int64_t)a.Sq * a.G;
+    if (rows > (1 << 30)) return GPTOSS_ATTN_ERR_SHAPE;
+    const int64_t blocks = (rows + 31) / 32, grid = blocks * a.B;
     a.blocks = (int)blocks;
+    a.by_blocks = div_by(blocks);
+    a.by_g = div_by(a.G);
+    const bool codes = p->storage == GPTOSS_ATTN_E4M3;
     if (p->dtype == GPTOSS_ATTN_BF16)
-        return p->storage == GPTOSS_ATTN_E4M3 ? launch(paged_write_kernel<bf16, true>, blocks * a.B, 256, stream, a) : launch(paged_write_kernel<bf16, false>, blocks * a.B, 256, stream, a);
-    return p->storage == GPTOSS_ATTN_E4M3 ? launch(paged_write_kernel<float, true>, blocks * a.B, 256, stream, a) : launch(paged_write_kernel<float, false>, blocks * a.B, 256, stream, a);
+        return codes ? launch(paged_write_kernel<bf16, true>, grid, 256, stream, a) : launch(paged_write_kernel<bf16, false>, grid, 256, stream, a);
+    return codes ? launch(paged_write_kernel<float, true>, grid, 256, stream, a) : launch(paged_write_kernel<float, false>, grid, 256, stream, a);
 }
 
 int gptoss_attn_paged_read(const gptoss_attn_paged_params *p, void *stream) {
     const int rc = gptoss_attn_paged_validate(p, kRead);
     if (rc) return rc;
     PagedArgs a = make_args(p);
-    const int64_t blocks = ((int64_t)a.Sq + 31) / 32;
-    if (blocks * a.G * a.B > 0x7fffffff) return GPTOSS_ATTN_ERR_SHAPE;
+    const int64_t blocks = ((int64_t)a.Sq + 31) / 32, grid = blocks * a.G * a.B;
+    if ((int64_t)a.G * a.B > 0x7fffffff) return GPTOSS_ATTN_ERR_SHAPE;
     a.blocks = (int)blocks;
-    const int64_t grid = blocks * a.G * a.B;
+    a.by_blocks = div_by(blocks);
+    a.by_g = div_by(a.G);
+    const bool codes = p->storage == GPTOSS_ATTN_E4M3;
     if (p->dtype == GPTOSS_ATTN_BF16)
-        return p->storage == GPTOSS_ATTN_E4M3 ? launch(paged_read_kernel<bf16, e4m3>, grid, 256, stream, a) : launch(paged_read_kernel<bf16, bf16>, grid, 256, stream, a);
-    return p->storage == GPTOSS_ATTN_E4M3 ? launch(paged_read_kernel<float, e4m3>, grid, 256, stream, a) : launch(paged_read_kernel<float, float>, grid, 256, stream, a);
+        return codes ? launch(paged_read_kernel<bf16, e4m3>, grid, 256, stream, a) : launch(paged_read_kernel<bf16, bf16>, grid, 256, stream, a);
+    return codes ? launch(paged_read_kernel<float, e4m3>, grid, 256, stream, a) : launch(paged_read_kernel<float, float>, grid, 256, stream, a);
 }
 
 }  // extern "C"

@@ -77,17 +77,32 @@ __device__ __forceinline__ float exp_of_byte(uint32_t e) { return __uint_as_floa
 
 struct e4m3 { uint8_t code; };
 
+// 16 bytes; ONCE: past the caches' retention, for what a kernel streams through.
+template <bool ONCE>
+__device__ __forceinline__ u32x4 load16(const void *p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(static_cast<const u32x4 *>(p));
+    else return *static_cast<const u32x4 *>(p);
+}
+template <bool ONCE>
+__device__ __forceinline__ void store16(void *p, const u32x4 x) {
+    if constexpr (ONCE) __builtin_nontemporal_store(x, static_cast<u32x4 *>(p));
+    else *static_cast<u32x4 *>(p) = x;
+}
+
 // Eight numbers of a row.
+template <bool ONCE = false>
 __device__ __forceinline__ void load8(const bf16 *p, float (&x)[8]) {
-    const bf16x8 v = as_bf16x8(*reinterpret_cast<const u32x4 *>(p));
+    const bf16x8 v = as_bf16x8(load16<ONCE>(p));
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
 }
+template <bool ONCE = false>
 __device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
-    const f32x4 u = *reinterpret_cast<const f32x4 *>(p), w = *reinterpret_cast<const f32x4 *>(p + 4);
+    const u32x4 u = load16<ONCE>(p), w = load16<ONCE>(p + 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { x[i] = u[i]; x[4 + i] = w[i]; }
+    for (int i = 0; i < 4; ++i) { x[i] = __uint_as_float(u[i]); x[4 + i] = __uint_as_float(w[i]); }
 }
+template <bool ONCE = false>
 __device__ __forceinline__ void load8(const e4m3 *p, float (&x)[8]) {
     const uint2 w = *reinterpret_cast<const uint2 *>(p);
     x[0] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 0);
@@ -99,15 +114,17 @@ __device__ __forceinline__ void load8(const e4m3 *p, float (&x)[8]) {
     x[6] = __builtin_amdgcn_cvt_f32_fp8((int)w.y, 2);
     x[7] = __builtin_amdgcn_cvt_f32_fp8((int)w.y, 3);
 }
+template <bool ONCE = false>
 __device__ __forceinline__ void store8(bf16 *p, const float (&x)[8]) {
     union { bf16x8 v; u32x4 u; } out;
 #pragma unroll
     for (int i = 0; i < 8; ++i) out.v[i] = (bf16)x[i];
-    *reinterpret_cast<u32x4 *>(p) = out.u;
+    store16<ONCE>(p, out.u);
 }
+template <bool ONCE = false>
 __device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
-    *reinterpret_cast<f32x4 *>(p) = f32x4{x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<f32x4 *>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) store16<ONCE>(p + i, u32x4{__float_as_uint(x[i]), __float_as_uint(x[i + 1]), __float_as_uint(x[i + 2]), __float_as_uint(x[i + 3])});
 }
 
 }  // namespace gptoss

@@ -1,6 +1,7 @@
 // PyTorch operators of the key / value cache in pages (gptoss_attn_paged_* in include/gptoss_attn.h): argument checks, allocation and launch.
 //
-//   gptoss_attn::paged_write, paged_read, paged_fwd      the three library calls; none has a gradient
+//   gptoss_attn::paged_write, paged_read, paged_fwd      the three library calls; none has a gradient (an operator cannot return None: an empty
+//                                                        lse stands for "not requested")
 //
 // Native for the same reason as attention() (torch_ops.cpp): a decoding step makes two of these calls for each layer, and each takes
 // a few microseconds on the GPU.
@@ -33,9 +34,14 @@ struct PagedCall {
     Tensor table, seqlens, start, sinks, q, k, v, scratch;
 };
 
+// As int32 on the cache's GPU; what is so already does not go through the dispatcher (half a microsecond each).
+Tensor int32_on(const Tensor &t, const Tensor &pages) {
+    return t.scalar_type() == at::kInt && t.device() == pages.device() ? t : t.to(pages.device(), at::kInt);
+}
+
 Tensor lengths_of(const Tensor &t, const Tensor &pages, int64_t batch, const char *name) {
-    TORCH_CHECK(!t.is_floating_point() && t.numel() == batch, name, " must hold one integer per batch row");
-    return t.to(pages.device(), at::kInt).contiguous();
+    TORCH_CHECK(t.numel() == batch && !at::isFloatingType(t.scalar_type()), name, " must hold one integer per batch row");
+    return int32_on(t, pages).contiguous();
 }
 
 // The cache, the table and what all calls have; `dtype`: the model's type.
@@ -72,9 +78,9 @@ void fill(PagedCall &c, const Tensor &k_pages, const Tensor &v_pages, const OptT
     p.v_pages = const_cast<void *>(v_pages.const_data_ptr());
     set3(p.k_page_stride, k_pages);
     set3(p.v_page_stride, v_pages);
-    TORCH_CHECK(page_table.dim() == 2 && page_table.size(0) == batch && !page_table.is_floating_point(), "page_table must be (B, pages of a row) integers, got ",
+    TORCH_CHECK(page_table.dim() == 2 && page_table.size(0) == batch && !at::isFloatingType(page_table.scalar_type()), "page_table must be (B, pages of a row) integers, got ",
                 page_table.sizes(), " for ", batch, " rows");
-    c.table = page_table.to(k_pages.device(), at::kInt);
+    c.table = int32_on(page_table, k_pages);
     if (c.table.stride(1) != 1 && c.table.size(1) > 1) c.table = c.table.contiguous();
     p.table_width = size32(c.table.size(1));
     p.table_stride = c.table.stride(0);
@@ -144,7 +150,7 @@ std::tuple<Tensor, Tensor> paged_read(const Tensor &k_pages, const Tensor &v_pag
 
 std::tuple<Tensor, Tensor> paged_fwd(const Tensor &q_, const Tensor &k_pages, const Tensor &v_pages, const OptTensor &k_exp, const OptTensor &v_exp,
                                      const Tensor &page_table, const Tensor &seqlens, const OptTensor &start, const OptTensor &sinks, double sm_scale,
-                                     int64_t window, int64_t max_len) {
+                                     int64_t window, int64_t max_len, bool need_lse) {
     const c10::OptionalDeviceGuard guard(k_pages.device());
     TORCH_CHECK(q_.dim() == 4 && q_.size(3) == 64, "q must be (B, H, S, 64), got ", q_.sizes());
     const bool half = q_.scalar_type() == at::kHalf;
@@ -172,14 +178,15 @@ std::tuple<Tensor, Tensor> paged_fwd(const Tensor &q_, const Tensor &k_pages, co
         require_near(k_pages, "sinks", *sinks);
         TORCH_CHECK(sinks->numel() == h, "sinks must hold one logit per query head");
         const bool bf16 = sinks->scalar_type() == at::kBFloat16;
-        c.sinks = (bf16 ? *sinks : sinks->to(at::kFloat)).contiguous();
+        c.sinks = (bf16 || sinks->scalar_type() == at::kFloat ? *sinks : sinks->to(at::kFloat)).contiguous();
         p.sinks_dtype = bf16 ? GPTOSS_ATTN_BF16 : GPTOSS_ATTN_FP32;
         p.sinks = c.sinks.const_data_ptr();
     }
-    Tensor o = new_tensor({b, s, h, 64}, c.q.scalar_type(), k_pages), lse = new_tensor({b, h, s}, at::kFloat, k_pages);
+    Tensor o = new_tensor({b, s, h, 64}, c.q.scalar_type(), k_pages);
+    Tensor lse = need_lse ? new_tensor({b, h, s}, at::kFloat, k_pages) : new_tensor({0}, at::kFloat, k_pages);
     set(p.o_stride, o, true);
     p.o = o.data_ptr();
-    p.lse = lse.data_ptr<float>();
+    p.lse = need_lse ? lse.data_ptr<float>() : nullptr;
     p.scratch_bytes = gptoss_attn_paged_workspace_bytes(&p);
     if (p.scratch_bytes) {
         c.scratch = new_tensor({static_cast<int64_t>(p.scratch_bytes / sizeof(float))}, at::kFloat, k_pages);
@@ -217,7 +224,7 @@ TORCH_LIBRARY_FRAGMENT(gptoss_attn, m) {
     m.def("paged_read(Tensor k_pages, Tensor v_pages, Tensor? k_exp, Tensor? v_exp, Tensor page_table, Tensor seqlens, SymInt max_len, Tensor? start, "
           "ScalarType dtype) -> (Tensor, Tensor)");
     m.def("paged_fwd(Tensor q, Tensor k_pages, Tensor v_pages, Tensor? k_exp, Tensor? v_exp, Tensor page_table, Tensor seqlens, Tensor? start, Tensor? sinks, "
-          "float sm_scale, SymInt window, SymInt max_len) -> (Tensor, Tensor)");
+          "float sm_scale, SymInt window, SymInt max_len, bool need_lse=True) -> (Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(gptoss_attn, CUDA, m) {
     m.impl("paged_write", &paged_write);

@@ -69,9 +69,9 @@ def _register_ops() -> None:
         return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
 
     @torch.library.register_fake(f"{_ak.OP_NAMESPACE}::paged_fwd")
-    def _fwd_fake(q, k_pages, v_pages, k_exp, v_exp, page_table, seqlens, start, sinks, sm_scale, window, max_len):
+    def _fwd_fake(q, k_pages, v_pages, k_exp, v_exp, page_table, seqlens, start, sinks, sm_scale, window, max_len, need_lse=True):
         b, h, s, d = q.shape
-        return q.new_empty((b, s, h, d)), q.new_empty((b, h, s), dtype=torch.float32)
+        return q.new_empty((b, s, h, d)), q.new_empty((b, h, s) if need_lse else (0,), dtype=torch.float32)
 
     _write, _read, _fwd = ops.paged_write.default, ops.paged_read.default, ops.paged_fwd.default
     _ready = True
@@ -83,8 +83,11 @@ except Exception:       # not built yet: importing has to work for the build its
     pass
 
 
+_Tensor = torch.Tensor
+
+
 def _ints(x, like):
-    return x if x is None or torch.is_tensor(x) else torch.as_tensor(x, dtype=torch.int32, device=like.device)
+    return x if x is None or isinstance(x, _Tensor) else torch.as_tensor(x, dtype=torch.int32, device=like.device)
 
 
 def paged_cache_write(cache: PagedCache, k, v, page_table, start, seqlens=None) -> None:
@@ -95,7 +98,7 @@ def paged_cache_write(cache: PagedCache, k, v, page_table, start, seqlens=None) 
     Two rows of one call must not write the same slot, and nothing that runs at the same time may read what is being written."""
     if not _ready:
         _register_ops()
-    _write(cache.k, cache.v, cache.k_exp, cache.v_exp, k, v, _ints(page_table, cache.k), _ints(start, cache.k), _ints(seqlens, cache.k))
+    _write(*cache, k, v, _ints(page_table, cache.k), _ints(start, cache.k), _ints(seqlens, cache.k))
 
 
 def paged_cache_read(cache: PagedCache, page_table, seqlens, max_len, start=None, dtype=None):
@@ -107,14 +110,14 @@ def paged_cache_read(cache: PagedCache, page_table, seqlens, max_len, start=None
         _register_ops()
     if dtype is None:
         dtype = torch.bfloat16 if cache.k.dtype == torch.float8_e4m3fn else cache.k.dtype
-    return _read(cache.k, cache.v, cache.k_exp, cache.v_exp, _ints(page_table, cache.k), _ints(seqlens, cache.k), int(max_len), _ints(start, cache.k), dtype)
+    return _read(*cache, _ints(page_table, cache.k), _ints(seqlens, cache.k), int(max_len), _ints(start, cache.k), dtype)
 
 
 def paged_attention_forward(q, cache: PagedCache, page_table, seqlens, sinks, sm_scale, bandwidth=None, start=None, max_len=None):
     """`paged_attention` that returns (o, lse (B, H, S) float32)."""
     if not _ready:
         _register_ops()
-    return _fwd(q, cache.k, cache.v, cache.k_exp, cache.v_exp, _ints(page_table, q), _ints(seqlens, q), _ints(start, q), sinks, float(sm_scale),
+    return _fwd(q, *cache, _ints(page_table, q), _ints(seqlens, q), _ints(start, q), sinks, float(sm_scale),
                 int(bandwidth or 0), int(max_len or 0))
 
 
@@ -129,4 +132,7 @@ def paged_attention(q, cache: PagedCache, page_table, seqlens, sinks, sm_scale, 
 
     The cache is read once for each 64 pairs of a query and a head of its KV head's group; the many queries of a prompt's chunk are better
     served by `paged_cache_read` and `attention`."""
-    return paged_attention_forward(q, cache, page_table, seqlens, sinks, sm_scale, bandwidth, start, max_len)[0]
+    if not _ready:
+        _register_ops()
+    return _fwd(q, *cache, _ints(page_table, q), _ints(seqlens, q), _ints(start, q), sinks, float(sm_scale),
+                int(bandwidth or 0), int(max_len or 0), False)[0]

@@ -81,6 +81,9 @@ def check(A, cache, table, n, q, sinks, window=0, start=None, max_len=None, scal
     again, lse2 = A.paged_attention_forward(q.to(DEV), cache, table, n, None if sinks is None else sinks.to(DEV), scale, window or None,
                                             None if start is None else torch.tensor(start, dtype=torch.int32, device=DEV), max_len)
     assert torch.equal(o, again) and torch.equal(lse, lse2)
+    alone = A.paged_attention(q.to(DEV), cache, table, n, None if sinks is None else sinks.to(DEV), scale, window or None,
+                              None if start is None else torch.tensor(start, dtype=torch.int32, device=DEV), max_len)
+    assert torch.equal(o, alone)
     ref, ref_lse, terms = P.attention(q, *values(cache), table.cpu(), n.cpu(), sinks, scale, window, start)
     assert o.dtype == q.dtype and o.shape == ref.shape and lse.shape == ref_lse.shape
     tol, tol_lse = P.bounds(ref, ref_lse, terms, q.dtype)

@@ -88,7 +88,7 @@ ALL = (FWD, WRITE, READ)
     (lambda p: setattr(p.v_stride, "s", 0), -8, (WRITE, READ)),
     (lambda p: setattr(p, "q", 0x1004), -7, (FWD,)),
     (lambda p: setattr(p, "o", None), -2, (FWD,)),
-    (lambda p: setattr(p, "lse", None), -2, (FWD,)),
+    (lambda p: setattr(p, "lse", 0x1002), -7, (FWD,)),
     (lambda p: setattr(p, "sinks_dtype", 2), -6, (FWD,)),
     (lambda p: setattr(p, "window", -1), -5, (FWD,)),
     (lambda p: setattr(p, "max_len", -1), -5, (FWD,)),
