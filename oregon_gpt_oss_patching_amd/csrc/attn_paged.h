@@ -32,10 +32,15 @@ constexpr float kRaise = 8.0f;                  // in the exponent of two
 
 // Wavefronts of a workgroup: four, or (NW) up to as many as a compute unit runs where one workgroup walks a unit alone.
 constexpr int kPagedWaves = 4;
-// Blocks of 16 keys in a tile: what a wavefront has under way is a tile, so rows of fewer bytes come more at a time.
-template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_tile_blocks() { return sizeof(T) == 2 && sizeof(ST) == 1 && NB == 1 && NW == kPagedWaves ? 4 : 2; }
+// Blocks of 16 keys in a tile: what a wavefront has under way is a tile, so rows of fewer bytes come more at a time; two columns' worth of
+// float32 numbers leave registers for one block.
+template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_tile_blocks() {
+    return sizeof(T) == 4 ? (sizeof(ST) == 4 && NB > 1 ? 1 : 2) : sizeof(ST) == 1 && NB == 1 && NW == kPagedWaves ? 4 : 2;
+}
 // Wavefronts per SIMD, of what the registers leave.
-template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_occupancy() { return sizeof(T) == 4 || NB > 1 ? 2 : sizeof(ST) == 1 && NW == kPagedWaves ? 3 : 4; }
+template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_occupancy() {
+    return sizeof(T) == 4 ? ((sizeof(ST) == 1) == (NB == 1) && NW == kPagedWaves ? 3 : 2) : NB == 1 ? 4 : NB == 2 || (NB == 3 && sizeof(ST) == 1) ? 3 : 2;
+}
 // Pairs (query, head of the group) that one workgroup may take.
 template <typename T> __host__ __device__ constexpr int paged_pairs() { return sizeof(T) == 2 ? 64 : 32; }
 // floats of a share's partial result: rows of O, then (m, l) of each
@@ -239,8 +244,9 @@ struct PagedTile<bf16, ST, NB, KB> {
             }
         }
     }
-    // V into the stage; rows outside first .. last - 1 of the tile as zeros where `edge`, and whether a row inside holds no finite number
-    __device__ __forceinline__ bool stage_v(bool edge, int first, int last, unsigned there, int lane) {
+    // V into the stage.  Where `edge`: rows outside first .. last - 1 of the tile as zeros; with `several` queries, what is not finite in the
+    // others as zeros too, and the answer is whether there was such a thing.
+    __device__ __forceinline__ bool stage_v(bool edge, bool several, int first, int last, unsigned there, int lane) {
         bool odd = false;
         if (edge) {
 #pragma unroll
@@ -252,10 +258,12 @@ struct PagedTile<bf16, ST, NB, KB> {
                     if constexpr (kCodes) ve[blk] = in ? ve[blk] : (uint32_t)kExpBias;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint32_t x = in ? v[blk][i][e] : 0u;
-                        v[blk][i][e] = x;
-                        if constexpr (kCodes) odd = odd || (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;        // 0x7f: NaN
-                        else odd = odd || (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+                        uint32_t x = in ? v[blk][i][e] : 0u, bad;
+                        if constexpr (kCodes) bad = ((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;      // 0x7f, 0xff: NaN
+                        else bad = ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+                        if (!several) bad = 0u;
+                        odd = odd || bad != 0u;
+                        v[blk][i][e] = x & ~bad;
                     }
                 }
         }
@@ -295,18 +303,13 @@ struct PagedTile<bf16, ST, NB, KB> {
     }
     // column of o[.][d][e] in the lane's row
     __device__ __forceinline__ static int column(int d, int e, int quad) { return 16 * d + 4 * quad + e; }
-    // V of row `key` and that column, out of the stage
-    __device__ __forceinline__ static float staged(uint32_t stage, int key, int col) {
-        const uint32_t at = stage + key * kRowBytes + (((col >> 3) ^ swz(key)) * 16) + (col & 7) * 2;
-        return (float)*reinterpret_cast<const __attribute__((address_space(3))) bf16 *>((uintptr_t)at);
-    }
 };
 
 // ---- float32 products ------------------------------------------------------------------------------------------------
 template <typename ST, int NB, int KB>
 struct PagedTile<float, ST, NB, KB> {
     static constexpr bool kCodes = sizeof(ST) == 1, kOnce = NB < 2;
-    static constexpr int kStage = 16 * KB * kD * 4;              // used where V holds infinities or NaN only
+    static constexpr int kStage = 0;
     static constexpr int kVecs = kCodes ? 1 : 4;
     typedef typename std::conditional<kCodes, uint32_t, f32x4>::type vec;       // four numbers of a row of V
     u32x4 k[KB][kVecs];
@@ -315,11 +318,10 @@ struct PagedTile<float, ST, NB, KB> {
     float q[NB][16];
     f32x4 o[NB][4];
     f32x4 w[KB][4];              // V as numbers
-    uint32_t stage, k_at, ke_at, v_at[4], ve_at[4];
+    uint32_t k_at, ke_at, v_at[4], ve_at[4];
 
-    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage_, int lane) {
+    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t, int lane) {
         const int l16 = lane & 15, quad = lane >> 4;
-        stage = stage_;
         k_at = l16 * a.kp.s + 16 * quad;
         ke_at = l16 * a.ke.s;
 #pragma unroll
@@ -372,8 +374,7 @@ struct PagedTile<float, ST, NB, KB> {
             }
         }
     }
-    __device__ __forceinline__ bool stage_v(bool edge, int first, int last, unsigned there, int lane) {
-        const int l16 = lane & 15, quad = lane >> 4;
+    __device__ __forceinline__ bool stage_v(bool edge, bool several, int first, int last, unsigned there, int lane) {
 #pragma unroll
         for (int blk = 0; blk < KB; ++blk)
 #pragma unroll
@@ -392,14 +393,15 @@ struct PagedTile<float, ST, NB, KB> {
             for (int blk = 0; blk < KB; ++blk)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int r = 16 * blk + 4 * quad + e;
+                    const int r = 16 * blk + 4 * (lane >> 4) + e;
                     const bool in = r >= first && r < last && (there >> blk & 1);
 #pragma unroll
                     for (int d = 0; d < 4; ++d) {
-                        w[blk][e][d] = in ? w[blk][e][d] : 0.0f;
-                        odd = odd || (__float_as_uint(w[blk][e][d]) & 0x7f800000u) == 0x7f800000u;
+                        const float x = in ? w[blk][e][d] : 0.0f;
+                        const bool bad = several && (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
+                        odd = odd || bad;
+                        w[blk][e][d] = bad ? 0.0f : x;
                     }
-                    *reinterpret_cast<__attribute__((address_space(3))) f32x4 *>((uintptr_t)(stage + (r * kD + 4 * l16) * 4)) = w[blk][e];
                 }
         }
         return odd;
@@ -415,9 +417,6 @@ struct PagedTile<float, ST, NB, KB> {
                     for (int nb = 0; nb < NB; ++nb) o[nb][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[blk][e][d], s[nb][blk][e], o[nb][d], 0, 0, 0);
     }
     __device__ __forceinline__ static int column(int d, int e, int quad) { return 16 * quad + 4 * e + d; }
-    __device__ __forceinline__ static float staged(uint32_t stage, int key, int col) {
-        return *reinterpret_cast<const __attribute__((address_space(3))) float *>((uintptr_t)(stage + (key * kD + col) * 4));
-    }
 };
 
 // Eight columns of a finished row: weights' sum l and products `acc` relative to the maximum `top`, the sink not yet among them.  `none`: no
@@ -445,6 +444,13 @@ constexpr int paged_lds_bytes() {
     constexpr int merge = paged_merge_waves<NW>() * 16 * paged_merge_blocks<NB>() * kPagedRow * 4;
     constexpr int stages = NW * PagedTile<T, ST, NB, paged_tile_blocks<T, ST, NB, NW>()>::kStage;
     return stages > merge ? stages : merge;
+}
+
+// LDS written and read by lanes of one wavefront, which executes these in order: the compiler has to keep that order too.
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 template <typename T, typename ST, int NB, int NW>
@@ -523,6 +529,8 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
         fetch_k(0);
         fetch_v(0);
     }
+    const bool several = sp.pos0 != sp.pos1;
+    bool odd = false;
     for (int j = 0; j < n_it; ++j) {
         const int n0 = (t_lo + w + NW * j) * kKeys;
         unsigned there = 0;                  // which of the tile's blocks have a page
@@ -536,7 +544,7 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
             if (((j + 1) & 63) == 0) entries(j + 1);
             fetch_k(j + 1);
         }
-        const bool odd = tile.stage_v(edge, sp.lo - n0, sp.hi - n0, there, lane);
+        odd = tile.stage_v(edge, several, sp.lo - n0, sp.hi - n0, there, lane) || odd;
         if (more) fetch_v(j + 1);
         if (edge) {
 #pragma unroll
@@ -572,35 +580,39 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
             }
             l[nb] += sum0 + sum1;
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        // (a key that one query sees and another does not: only where there are several)
-        if (__builtin_expect(!edge || sp.pos0 == sp.pos1 || __builtin_amdgcn_ballot_w64(odd) == 0ull, 1)) {
-            tile.product(s);
-        } else {
-            // infinities or NaN in V: key by key, and only for the queries that see it (0 times infinity is NaN)
+        wave_lds_order();
+        tile.product(s);
+        wave_lds_order();
+    }
+
+    // Infinities and NaN in a row of V that one query sees and another does not (0 times them is NaN) have been left out of the product.  A weight times
+    // infinity is infinity, so they are what is missing: added here to the columns that see them, from the pages, key by key.  (In the loop,
+    // whatever form it has, this costs the kernels 15 registers and more.)
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0ull, 0)) {
 #pragma unroll 1
-            for (int key = 0; key < kKeys; ++key) {
-                const int from = ((key >> 2 & 3) << 4) | l16, reg = (key >> 4) * 4 + (key & 3);
+        for (int j = 0; j < n_it; ++j) {
+            const int n0 = (t_lo + w + NW * j) * kKeys;
+            // (in a tile whose keys all queries see nothing has been left out)
+            if (n0 + kKeys - 1 <= sp.pos0 && n0 > sp.pos1 - weff && paged_page(a, sp.b, n0) >= 0 && paged_page(a, sp.b, n0 + kKeys - 16) >= 0 &&
+                (KB < 4 || (paged_page(a, sp.b, n0 + 16) >= 0 && paged_page(a, sp.b, n0 + 32) >= 0)))
+                continue;
+#pragma unroll 1
+            for (int key = max(n0, sp.lo); key < min(n0 + kKeys, sp.hi); ++key) {
+                const int page = paged_page(a, sp.b, key);
+                if (page < 0) continue;
+                const char *row = v_base + a.vp.at(page, key & in_page);
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    float p = s[nb][0][0];
+                for (int d = 0; d < 4; ++d)
 #pragma unroll
-                    for (int e = 1; e < 4 * KB; ++e) p = reg == e ? s[nb][e >> 2][e & 3] : p;
-                    p = __shfl(p, from);
-                    if (n0 + key <= pq[nb] && n0 + key > pq[nb] - weff && (there >> (key >> 4) & 1)) {
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = stored_number(reinterpret_cast<const ST *>(row) + Tile::column(d, e, quad));
+                        if ((__float_as_uint(x) & 0x7f800000u) != 0x7f800000u) continue;
 #pragma unroll
-                        for (int d = 0; d < 4; ++d)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) tile.o[nb][d][e] += p * Tile::staged(stage, key, Tile::column(d, e, quad));
+                        for (int nb = 0; nb < NB; ++nb)
+                            if (key <= pq[nb] && key > pq[nb] - weff) tile.o[nb][d][e] += x;
                     }
-                }
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 
     // ---- merge the wavefronts: rows [wavefront][pair][64 + (m, l)] in LDS ----

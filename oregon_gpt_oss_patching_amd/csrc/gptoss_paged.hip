@@ -72,12 +72,15 @@ int launch(Kernel kernel, int64_t workgroups, int threads, void *stream, const P
 // the scratch that takes.
 struct PagedDivision { int nb, blocks, shares, alone, min_keys; int64_t units; size_t plan_bytes, bytes; };
 
+// Workgroups of four wavefronts that a compute unit runs at a time.
+template <typename T, typename ST, int NB> constexpr int per_simd() { return paged_occupancy<T, ST, NB, kPagedWaves>(); }
+
 PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     PagedDivision d{};
     const bool f32 = p->dtype == GPTOSS_ATTN_FP32, codes = p->storage == GPTOSS_ATTN_E4M3;
     const int64_t r = p->H / p->G, pairs = (int64_t)p->Sq * r;
     const int most = f32 ? paged_pairs<float>() : paged_pairs<bf16>();
-    d.nb = pairs <= 16 ? 1 : pairs <= 32 || most == 32 ? 2 : 4;
+    d.nb = pairs <= 16 ? 1 : pairs <= 32 || most == 32 ? 2 : pairs <= 48 ? 3 : 4;
     const int64_t blocks = (pairs + 16 * d.nb - 1) / (16 * d.nb);
     d.blocks = (int)(blocks < 0x7fffffff ? blocks : 0x7fffffff);
     d.units = blocks * p->B;
@@ -99,10 +102,10 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     d.alone = kPagedWaves;
     // As many workgroups as a 256-CU part holds at a time: they start and end together.  A unit's last share is half of one on average; at
     // least half of the workgroups are shares all the same, so that a long row among many is cut.  No more than the units can have.
-    const int per_cu = f32        ? paged_occupancy<float, float, 1, kPagedWaves>()
-                       : d.nb > 1 ? paged_occupancy<bf16, bf16, 2, kPagedWaves>()
-                       : codes    ? paged_occupancy<bf16, e4m3, 1, kPagedWaves>()
-                                  : paged_occupancy<bf16, bf16, 1, kPagedWaves>();
+#define GPTOSS_HELD(T, NB) (codes ? per_simd<T, e4m3, NB>() : per_simd<T, T, NB>())
+    const int per_cu = f32 ? (d.nb == 1 ? GPTOSS_HELD(float, 1) : GPTOSS_HELD(float, 2))
+                           : d.nb == 1 ? GPTOSS_HELD(bf16, 1) : d.nb == 2 ? GPTOSS_HELD(bf16, 2) : d.nb == 3 ? GPTOSS_HELD(bf16, 3) : GPTOSS_HELD(bf16, 4);
+#undef GPTOSS_HELD
     const int64_t held = 256 * per_cu / p->G, left = held - d.units / 2, can = d.units * ((keys + d.min_keys - 1) / d.min_keys);
     int64_t shares = left > held / 2 ? left : held / 2;
     if (shares > can) shares = can;
@@ -191,7 +194,7 @@ int gptoss_attn_paged_fwd(const gptoss_attn_paged_params *p, void *stream) {
     const bool codes = p->storage == GPTOSS_ATTN_E4M3;
     if (p->dtype == GPTOSS_ATTN_BF16) {
 #define GPTOSS_PAGED(NB) (codes ? attend<bf16, e4m3, NB>(d, stream, a) : attend<bf16, bf16, NB>(d, stream, a))
-        return d.nb == 1 ? GPTOSS_PAGED(1) : d.nb == 2 ? GPTOSS_PAGED(2) : GPTOSS_PAGED(4);
+        return d.nb == 1 ? GPTOSS_PAGED(1) : d.nb == 2 ? GPTOSS_PAGED(2) : d.nb == 3 ? GPTOSS_PAGED(3) : GPTOSS_PAGED(4);
 #undef GPTOSS_PAGED
     }
 #define GPTOSS_PAGED(NB) (codes ? attend<float, e4m3, NB>(d, stream, a) : attend<float, float, NB>(d, stream, a))

@@ -77,6 +77,11 @@ __device__ __forceinline__ float exp_of_byte(uint32_t e) { return __uint_as_floa
 
 struct e4m3 { uint8_t code; };
 
+// A number of a row (of a code: without its power of two).
+__device__ __forceinline__ float stored_number(const bf16 *p) { return (float)*p; }
+__device__ __forceinline__ float stored_number(const float *p) { return *p; }
+__device__ __forceinline__ float stored_number(const e4m3 *p) { return __builtin_amdgcn_cvt_f32_fp8((int)p->code, 0); }
+
 // 16 bytes; ONCE: past the caches' retention, for what a kernel streams through.
 template <bool ONCE>
 __device__ __forceinline__ u32x4 load16(const void *p) {
