@@ -9,10 +9,11 @@
 // and a table that is wider than the rows costs nothing.
 //
 // In a workgroup four wavefronts take tiles in turn, each for itself (no barrier in the loop), and merge their (m, l, O) at the end.
-//  * K goes from the pages straight into the MFMA's A operand: a lane holds pieces of one key's row, and which number of the row stands in
-//    which slot of the contraction is free as long as Q has the same order.
-//  * V has to be turned (the contraction runs over keys): bf16 rows go through a stage of LDS and are read back transposed; in 32 bits each
-//    lane loads four columns of its own four keys, which is what the fp32 MFMA takes.
+//  * Loads take whole cache lines.  The MFMA's A operand wants a lane to hold pieces of one key's row, 16 rows of 64 bytes to a load: codes come so,
+//    but rows of more bytes loaded that way keep a compute unit at 37 GB/s (one workgroup of 16 wavefronts; with whole rows 131), so K goes
+//    through a stage of LDS first.  Which number of the row stands in which slot of the contraction is free as long as Q has the same order.
+//  * V has to be turned (the contraction runs over keys): for bf16 products it goes through the same stage, after K, and is read back transposed;
+//    in 32 bits each lane loads four columns of its own four keys, which is what the fp32 MFMA takes.
 //  * P leaves the S product in the layout of the PV product's B operand.
 //  * Entries of the page table are loaded 64 tiles at a time, one per lane; a tile's page is a readlane and its addresses are scalar.
 //  * e4m3 rows widen on the way into the operand: to bf16 by the instruction that takes a power of two along (exact), K's with one
@@ -173,6 +174,13 @@ __device__ __forceinline__ V load_rows(const char *p) {
     else return *reinterpret_cast<const V *>(p);
 }
 
+// A lane's 32-bit offset from a scalar address.  Hidden, as the compiler widens it once in front of the loop otherwise, and then adds 64 bits per load.
+__device__ __forceinline__ uint32_t lane_offset(uint32_t at, uint32_t mask) {
+    at &= mask;
+    asm volatile("" : "+v"(at));
+    return at;
+}
+
 // A tile's K and V as they are loaded, and what is done with them.  `kb` / `vb`: scalar addresses of the first row of a block of 16 keys;
 // lanes: l16 = lane % 16, quad = lane / 16.
 template <typename T, typename ST, int NB, int KB> struct PagedTile;
@@ -180,16 +188,20 @@ template <typename T, typename ST, int NB, int KB> struct PagedTile;
 // ---- bfloat16 products -----------------------------------------------------------------------------------------------
 template <typename ST, int NB, int KB>
 struct PagedTile<bf16, ST, NB, KB> {
-    static constexpr bool kCodes = sizeof(ST) == 1, kOnce = NB < 4;
+    static constexpr bool kCodes = sizeof(ST) == 1, kOnce = NB < 4, kStagedK = !kCodes;
     static constexpr int kStage = 16 * KB * kRowBytes;           // LDS bytes of a wavefront
     static constexpr int kVecs = kCodes ? 1 : 2;                 // 16-byte loads per lane and block
     u32x4 k[KB][kVecs], v[KB][kVecs];
     uint32_t ke[KB], ve[KB];
     bf16x8 q[NB][2];
     f32x4 o[NB][4];
-    uint32_t tr[4], wr[2], k_at, v_at[kVecs], ke_at, ve_at;
+    uint32_t tr[4], wr[2], nat[2], k_at[kVecs], v_at[kVecs], ke_at, ve_at;
 
-    __device__ __forceinline__ static int v_row(int lane, int i) { return kCodes ? lane >> 2 : (lane >> 3) + 8 * i; }
+    // (codes: rows 0, 1, 4, 5 and so on for each 16 lanes, which then write to distinct banks)
+    __device__ __forceinline__ static int v_row(int lane, int i) {
+        const int q = lane >> 2;
+        return kCodes ? (q & 9) | (q & 2) << 1 | (q & 4) >> 1 : (lane >> 3) + 8 * i;
+    }
 
     __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage, int lane) {
         const int i = lane & 15, quad = lane >> 4, row = 4 * quad + (i >> 2);
@@ -200,7 +212,10 @@ struct PagedTile<bf16, ST, NB, KB> {
             const int r = v_row(lane, e), c = kCodes ? 2 * (lane & 3) + e : lane & 7;
             wr[e] = stage + r * kRowBytes + ((c ^ swz(r)) * 16);
         }
-        k_at = i * a.kp.s + 16 * quad;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) nat[e] = stage + i * kRowBytes + (((4 * e + quad) ^ swz(i)) * 16);
+#pragma unroll
+        for (int e = 0; e < kVecs; ++e) k_at[e] = kCodes ? i * a.kp.s + 16 * quad : v_row(lane, e) * a.kp.s + 16 * (lane & 7);
 #pragma unroll
         for (int e = 0; e < kVecs; ++e) v_at[e] = v_row(lane, e) * a.vp.s + 16 * (kCodes ? lane & 3 : lane & 7);
         ke_at = i * a.ke.s;
@@ -215,15 +230,22 @@ struct PagedTile<bf16, ST, NB, KB> {
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[nb][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb) {
+    // `mask`: all ones, or 0 where there is no next tile (one address instead of a branch)
+    __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb, uint32_t mask) {
 #pragma unroll
-        for (int s = 0; s < kVecs; ++s) k[blk][s] = load16<kOnce>(kb + k_at + 64 * s);
-        if constexpr (kCodes) ke[blk] = (uint8_t)eb[ke_at];
+        for (int s = 0; s < kVecs; ++s) k[blk][s] = load16<kOnce>(kb + lane_offset(k_at[s], mask));
+        if constexpr (kCodes) ke[blk] = (uint8_t)eb[lane_offset(ke_at, mask)];
     }
-    __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb) {
+    __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb, uint32_t mask) {
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) v[blk][i] = load16<kOnce>(vb + v_at[i]);
-        if constexpr (kCodes) ve[blk] = (uint8_t)eb[ve_at];
+        for (int i = 0; i < kVecs; ++i) v[blk][i] = load16<kOnce>(vb + lane_offset(v_at[i], mask));
+        if constexpr (kCodes) ve[blk] = (uint8_t)eb[lane_offset(ve_at, mask)];
+    }
+    __device__ __forceinline__ void stage_k() const {
+#pragma unroll
+        for (int blk = 0; blk < KB; ++blk)
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>((uintptr_t)(wr[i] + 16 * blk * kRowBytes)) = k[blk][i];
     }
     __device__ __forceinline__ void logits(f32x4 (&s)[NB][KB]) const {
 #pragma unroll
@@ -234,8 +256,8 @@ struct PagedTile<bf16, ST, NB, KB> {
                 f[0] = widen8(k[blk][0][0], k[blk][0][1], p);
                 f[1] = widen8(k[blk][0][2], k[blk][0][3], p);
             } else {
-                f[0] = as_bf16x8(k[blk][0]);
-                f[1] = as_bf16x8(k[blk][1]);
+                f[0] = as_bf16x8(lds_load128(nat[0], 16 * blk * kRowBytes));
+                f[1] = as_bf16x8(lds_load128(nat[1], 16 * blk * kRowBytes));
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -308,8 +330,8 @@ struct PagedTile<bf16, ST, NB, KB> {
 // ---- float32 products ------------------------------------------------------------------------------------------------
 template <typename ST, int NB, int KB>
 struct PagedTile<float, ST, NB, KB> {
-    static constexpr bool kCodes = sizeof(ST) == 1, kOnce = NB < 2;
-    static constexpr int kStage = 0;
+    static constexpr bool kCodes = sizeof(ST) == 1, kOnce = NB < 2, kStagedK = !kCodes;
+    static constexpr int kStage = kCodes ? 0 : 16 * KB * kD * 4;
     static constexpr int kVecs = kCodes ? 1 : 4;
     typedef typename std::conditional<kCodes, uint32_t, f32x4>::type vec;       // four numbers of a row of V
     u32x4 k[KB][kVecs];
@@ -318,11 +340,18 @@ struct PagedTile<float, ST, NB, KB> {
     float q[NB][16];
     f32x4 o[NB][4];
     f32x4 w[KB][4];              // V as numbers
-    uint32_t k_at, ke_at, v_at[4], ve_at[4];
+    uint32_t k_at[kVecs], wr[kVecs], nat[kVecs], ke_at, v_at[4], ve_at[4];
 
-    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t, int lane) {
+    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage, int lane) {
         const int l16 = lane & 15, quad = lane >> 4;
-        k_at = l16 * a.kp.s + 16 * quad;
+#pragma unroll
+        for (int e = 0; e < kVecs; ++e) {
+            // rows quad + 4 e in 16 pieces, piece c of row r at c ^ r: what 16 lanes write or read is in distinct banks
+            const int r = quad + 4 * e;
+            k_at[e] = kCodes ? l16 * a.kp.s + 16 * quad : r * a.kp.s + 16 * l16;
+            wr[e] = stage + r * kD * 4 + ((l16 ^ r) * 16);
+            nat[e] = stage + l16 * kD * 4 + (((4 * e + quad) ^ l16) * 16);
+        }
         ke_at = l16 * a.ke.s;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -341,34 +370,43 @@ struct PagedTile<float, ST, NB, KB> {
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[nb][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb) {
+    __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb, uint32_t mask) {
 #pragma unroll
-        for (int s = 0; s < kVecs; ++s) k[blk][s] = load16<kOnce>(kb + k_at + 64 * s);
-        if constexpr (kCodes) ke[blk] = (uint8_t)eb[ke_at];
+        for (int s = 0; s < kVecs; ++s) k[blk][s] = load16<kOnce>(kb + lane_offset(k_at[s], mask));
+        if constexpr (kCodes) ke[blk] = (uint8_t)eb[lane_offset(ke_at, mask)];
     }
-    __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb) {
+    __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb, uint32_t mask) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            v[blk][e] = load_rows<kOnce, vec>(vb + v_at[e]);
-            if constexpr (kCodes) ve[blk][e] = (uint8_t)eb[ve_at[e]];
+            v[blk][e] = load_rows<kOnce, vec>(vb + lane_offset(v_at[e], mask));
+            if constexpr (kCodes) ve[blk][e] = (uint8_t)eb[lane_offset(ve_at[e], mask)];
         }
     }
     __device__ __forceinline__ static float code(uint32_t w, int i) {
         return i == 0 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 0) : i == 1 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 1)
                : i == 2 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 2) : __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
     }
+    __device__ __forceinline__ void stage_k() const {
+#pragma unroll
+        for (int blk = 0; blk < KB; ++blk)
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>((uintptr_t)(wr[i] + 16 * blk * kD * 4)) = k[blk][i];
+    }
     __device__ __forceinline__ void logits(f32x4 (&s)[NB][KB]) const {
 #pragma unroll
         for (int blk = 0; blk < KB; ++blk) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) s[nb][blk] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            u32x4 f[kVecs];
+#pragma unroll
+            for (int t = 0; t < kVecs; ++t) f[t] = kCodes ? k[blk][t] : lds_load128(nat[t], 16 * blk * kD * 4);
             float p = 1.0f;
             if constexpr (kCodes) p = exp_of_byte(ke[blk]);
 #pragma unroll
             for (int t = 0; t < 16; ++t) {
                 float x;
-                if constexpr (kCodes) x = p * code(k[blk][0][t >> 2], t & 3);
-                else x = __uint_as_float(k[blk][t >> 2][t & 3]);
+                if constexpr (kCodes) x = p * code(f[0][t >> 2], t & 3);
+                else x = __uint_as_float(f[t >> 2][t & 3]);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) s[nb][blk] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, q[nb][t], s[nb][blk], 0, 0, 0);
             }
@@ -522,30 +560,43 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
             load(blk, p, e);
         }
     };
-    auto fetch_k = [&](int j) __attribute__((always_inline)) { fetch(j, k_base, a.kp, ke_base, a.ke, [&](int blk, const char *p, const char *e) { tile.load_k(blk, p, e); }); };
-    auto fetch_v = [&](int j) __attribute__((always_inline)) { fetch(j, v_base, a.vp, ve_base, a.ve, [&](int blk, const char *p, const char *e) { tile.load_v(blk, p, e); }); };
+    auto fetch_k = [&](int j, uint32_t mask) __attribute__((always_inline)) { fetch(j, k_base, a.kp, ke_base, a.ke, [&](int blk, const char *p, const char *e) { tile.load_k(blk, p, e, mask); }); };
+    auto fetch_v = [&](int j, uint32_t mask) __attribute__((always_inline)) { fetch(j, v_base, a.vp, ve_base, a.ve, [&](int blk, const char *p, const char *e) { tile.load_v(blk, p, e, mask); }); };
 
     if (n_it > 0) {
-        fetch_k(0);
-        fetch_v(0);
+        fetch_k(0, ~0u);
+        fetch_v(0, ~0u);
     }
     const bool several = sp.pos0 != sp.pos1;
     bool odd = false;
     for (int j = 0; j < n_it; ++j) {
         const int n0 = (t_lo + w + NW * j) * kKeys;
-        unsigned there = 0;                  // which of the tile's blocks have a page
+        int pages = 0;                       // negative where a block of the tile has no page
+        unsigned there = 0;                  // which of them have one
 #pragma unroll
-        for (int blk = 0; blk < KB; ++blk) there |= page_of(j, blk) >= 0 ? 1u << blk : 0u;
-        const bool edge = !(n0 + kKeys - 1 <= sp.pos0 && n0 > sp.pos1 - weff && there == (1u << KB) - 1);
+        for (int blk = 0; blk < KB; ++blk) {
+            pages |= page_of(j, blk);
+            there |= page_of(j, blk) >= 0 ? 1u << blk : 0u;
+        }
+        const bool edge = n0 + kKeys - 1 > sp.pos0 || n0 <= sp.pos1 - weff || pages < 0;
+        // The next tile; behind the last one the same loads from one line of it, so that the waits for what is under way can be counted: with a branch
+        // around them every tile began with a wait for all of it.
+        const int next = min(j + 1, n_it - 1);
+        const uint32_t mask = next > j ? ~0u : 0u;
+        if ((next & 63) == 0) entries(next);
         f32x4 s[NB][KB];
-        tile.logits(s);
-        const bool more = j + 1 < n_it;
-        if (more) {
-            if (((j + 1) & 63) == 0) entries(j + 1);
-            fetch_k(j + 1);
+        if constexpr (Tile::kStagedK) {
+            tile.stage_k();
+            fetch_k(next, mask);
+            wave_lds_order();
+            tile.logits(s);
+            wave_lds_order();
+        } else {
+            tile.logits(s);
+            fetch_k(next, mask);
         }
         odd = tile.stage_v(edge, several, sp.lo - n0, sp.hi - n0, there, lane) || odd;
-        if (more) fetch_v(j + 1);
+        fetch_v(next, mask);
         if (edge) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)

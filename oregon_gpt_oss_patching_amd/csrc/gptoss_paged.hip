@@ -125,11 +125,13 @@ int attend(const PagedDivision &d, void *stream, PagedArgs &a) {
     a.min_tiles = d.min_keys / (16 * paged_tile_blocks<T, ST, NB, kPagedWaves>());
     const int s = launch(attn_paged_kernel<T, ST, NB, kPagedWaves>, (d.shares + d.units) * a.G, 64 * kPagedWaves, stream, a);
     if (s || !d.shares) return s;
-    // a workgroup for each row where they are few and their shares may be many
+    // A wavefront adds eight shares at a time; four of them for each row where a unit has more than twice that (us: 1 x 65536 tokens 33.5 / 29.6,
+    // 16 x 8192, eight shares a unit, 48.3 / 49.1, five queries on eight rows 19.2 / 21.9).
     const int64_t heads = (int64_t)a.B * a.G, pairs = (int64_t)a.Sq * a.r;
-    const int64_t wgs = heads * pairs <= 1024 ? pairs : (pairs + 3) / 4;
+    const bool many = d.shares > 16 * d.units;
+    const int64_t wgs = many ? pairs : (pairs + 3) / 4;
     a.by_wgs = div_by(wgs);
-    return wgs == pairs ? launch(attn_paged_combine_kernel<T, NB, 4>, heads * wgs, 256, stream, a) : launch(attn_paged_combine_kernel<T, NB, 1>, heads * wgs, 256, stream, a);
+    return many ? launch(attn_paged_combine_kernel<T, NB, 4>, heads * wgs, 256, stream, a) : launch(attn_paged_combine_kernel<T, NB, 1>, heads * wgs, 256, stream, a);
 }
 
 }  // namespace
