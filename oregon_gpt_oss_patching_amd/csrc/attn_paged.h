@@ -497,7 +497,9 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
     using Tile = PagedTile<T, ST, NB, KB>;
     __shared__ __attribute__((aligned(128))) char smem[paged_lds_bytes<T, ST, NB, NW>()];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, quad = lane >> 4;
-    const int slot = a.by_g.quotient(blockIdx.x), g = blockIdx.x - slot * a.G;
+    // workgroup -> (slot, KV head), heads next to each other or eight slots (a.across: the heads of a slot then run on one XCD)
+    const int line = a.across ? blockIdx.x >> 3 : blockIdx.x, line_slot = a.by_g.quotient(line), g = line - line_slot * a.G;
+    const int slot = a.across ? 8 * line_slot + (blockIdx.x & 7) : line_slot;
     PagedSpan sp;
     const PagedShare share = paged_share<kPairs, kKeys>(a, slot, sp);
     if (share.unit < 0) return;

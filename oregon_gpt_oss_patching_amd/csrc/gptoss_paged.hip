@@ -69,8 +69,8 @@ int launch(Kernel kernel, int64_t workgroups, int threads, void *stream, const P
 
 // How the attention's work is divided: column blocks of 16 pairs, blocks of pairs of a row, (row, block) units, shares of all units'
 // tiles for each KV head beside one for each unit (0: units stay whole, each walked by `alone` wavefronts), keys that a share has at least, and
-// the scratch that takes.
-struct PagedDivision { int nb, blocks, shares, alone, min_keys; int64_t units; size_t plan_bytes, bytes; };
+// the scratch that takes; `across`: a slot's KV heads on one XCD.
+struct PagedDivision { int nb, blocks, shares, alone, min_keys; bool across; int64_t units; size_t plan_bytes, bytes; };
 
 // Workgroups of four wavefronts that a compute unit runs at a time.
 template <typename T, typename ST, int NB> constexpr int per_simd() { return paged_occupancy<T, ST, NB, kPagedWaves>(); }
@@ -101,7 +101,9 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     if (d.units > kPagedMaxUnits || keys <= (f32 ? 288 : 1152) * (full ? 2 : 1)) return d;
     d.alone = kPagedWaves;
     // As many workgroups as a 256-CU part holds at a time: they start and end together.  A unit's last share is half of one on average; at
-    // least half of the workgroups are shares all the same, so that a long row among many is cut.  No more than the units can have.
+    // least half of the workgroups are shares all the same, so that a long row among many is cut.  No more than the units can have.  us with half as many,
+    // as many, twice as many: 16 x 8192 tokens 46.3 / 47.5 / 50.1, 64 x 3540 73.9 / 77.4 / 80.3, but 64 rows of 150 to 16384 103 / 81.6 / 83.5, 32 of 6000 to
+    // 16384 137 / 112 / 114, and four queries on each of those in e4m3 44.3 / 33.4 / 41.2.
 #define GPTOSS_HELD(T, NB) (codes ? per_simd<T, e4m3, NB>() : per_simd<T, T, NB>())
     const int per_cu = f32 ? (d.nb == 1 ? GPTOSS_HELD(float, 1) : GPTOSS_HELD(float, 2))
                            : d.nb == 1 ? GPTOSS_HELD(bf16, 1) : d.nb == 2 ? GPTOSS_HELD(bf16, 2) : d.nb == 3 ? GPTOSS_HELD(bf16, 3) : GPTOSS_HELD(bf16, 4);
@@ -110,6 +112,10 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     int64_t shares = left > held / 2 ? left : held / 2;
     if (shares > can) shares = can;
     d.shares = shares > 1 ? (int)shares : 1;
+    // The exponents of a page's KV heads share cache lines, which the heads' workgroups then read from one L2.  us, heads next to each other / on one
+    // XCD, e4m3: 32 rows of 6000 to 16384 tokens 65.4 / 63.5, 24 of 150 to 30000 37.1 / 35.1, 200 of up to 4000 67.5 / 64.1; but 8 of up to 6000 14.5 / 15.4,
+    // and in bfloat16 200 rows 102 / 106.
+    d.across = codes && p->B * keys >= 1 << 17;
     d.plan_bytes = ((size_t)d.units * 2 * sizeof(int) + 15) & ~(size_t)15;
     d.bytes = d.plan_bytes + (size_t)(d.shares + d.units) * p->G * paged_partial_floats(d.nb) * sizeof(float);
     return d;
@@ -123,7 +129,9 @@ int attend(const PagedDivision &d, void *stream, PagedArgs &a) {
         if (d.alone == 8) return launch(attn_paged_kernel<T, ST, NB, 8>, d.units * a.G, 512, stream, a);
     }
     a.min_tiles = d.min_keys / (16 * paged_tile_blocks<T, ST, NB, kPagedWaves>());
-    const int s = launch(attn_paged_kernel<T, ST, NB, kPagedWaves>, (d.shares + d.units) * a.G, 64 * kPagedWaves, stream, a);
+    const int64_t slots = d.shares + d.units;
+    a.across = d.across;
+    const int s = launch(attn_paged_kernel<T, ST, NB, kPagedWaves>, (a.across ? (slots + 7) / 8 * 8 : slots) * a.G, 64 * kPagedWaves, stream, a);
     if (s || !d.shares) return s;
     // A wavefront adds eight shares at a time; four of them for each row where a unit has more than twice that (us: 1 x 65536 tokens 33.5 / 29.6,
     // 16 x 8192, eight shares a unit, 48.3 / 49.1, five queries on eight rows 19.2 / 21.9).
