@@ -77,7 +77,7 @@ enum gptoss_attn_status {
                                            2^31-1 workgroups */
     GPTOSS_ATTN_ERR_DTYPE = -6,         /* dtype not in gptoss_attn_dtype */
     GPTOSS_ATTN_ERR_ALIGNMENT = -7,     /* a tensor base or stride breaks 16-byte row alignment */
-    GPTOSS_ATTN_ERR_STRIDE = -8,        /* a sequence stride smaller than D or larger than 2^24 elements */
+    GPTOSS_ATTN_ERR_STRIDE = -8,        /* a sequence stride smaller than D or larger than 2^24 elements; of pages also a stride from page to page below 0 or of 2^32 bytes and more */
     GPTOSS_ATTN_ERR_ABI = -9,           /* struct_size does not match this library */
     GPTOSS_ATTN_ERR_WORKSPACE = -10,    /* gptoss_attn_bwd_static: 24*B*H*Sq bytes do not fit the built-in scratch */
     GPTOSS_ATTN_ERR_PAGES = -11         /* paged cache: page_size no power of two from 16 to 1024, pages or table_width <= 0,

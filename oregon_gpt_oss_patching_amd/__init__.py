@@ -14,6 +14,7 @@ from .attention_kernel import (  # noqa: F401
 )
 from .paged_cache import (  # noqa: F401
     PagedCache,
+    PagedState,
     paged_attention,
     paged_attention_forward,
     paged_cache,
@@ -23,4 +24,4 @@ from .paged_cache import (  # noqa: F401
 
 __all__ = ["attention", "attention_forward", "attention_backward", "doc_start_from_position_ids",
            "hip_flash_attention", "triton_flash_attention",
-           "PagedCache", "paged_cache", "paged_cache_write", "paged_cache_read", "paged_attention", "paged_attention_forward"]
+           "PagedCache", "PagedState", "paged_cache", "paged_cache_write", "paged_cache_read", "paged_attention", "paged_attention_forward"]

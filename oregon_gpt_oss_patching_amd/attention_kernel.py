@@ -331,7 +331,15 @@ def hip_flash_attention(
     packed from several documents attend across documents, as in the reference, unless the
     caller passes `doc_start=` (see `doc_start_from_position_ids`) or packing awareness was
     switched on with `patch_flash_attention(respect_packing=True)`, in which case the
-    `position_ids` the model passes along are used."""
+    `position_ids` the model passes along are used.
+
+    With `paged=` (a `PagedState`) the layer's new keys and values go into a cache in pages, and the queries attend to what
+    stands there."""
+    paged = kwargs.get("paged")
+    if paged is not None:
+        if kwargs.get("doc_start") is not None or kwargs.get("seqlens") is not None:
+            raise RuntimeError("paged= holds the rows' lengths itself and has no documents: pass neither seqlens nor doc_start")
+        return paged.attend(module, query, key, value, scaling), None
     doc_start = kwargs.get("doc_start")
     if doc_start is None and RESPECT_PACKING and kwargs.get("position_ids") is not None:
         pos = kwargs["position_ids"]

@@ -13,18 +13,20 @@ the pool (-1, say) names no page.  The pool holds the model's type, or 8-bit e4m
 Everything that says where tokens stand (`page_table`, `start`, `seqlens`) stays on the GPU and is read there: the calls do not
 synchronise and can be captured into a graph that is replayed with other contents.  None has a gradient.
 
+A patched model takes all of this as one argument, a `PagedState`: `model(ids, position_ids=..., use_cache=False, paged=state)`.
+
 The reference has no counterpart: its generate.py leaves the cache to transformers (generate.py:1-30).
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
 from . import _lib
 from . import attention_kernel as _ak
 
-__all__ = ["PagedCache", "paged_cache", "paged_cache_write", "paged_cache_read", "paged_attention", "paged_attention_forward"]
+__all__ = ["PagedCache", "PagedState", "paged_cache", "paged_cache_write", "paged_cache_read", "paged_attention", "paged_attention_forward"]
 
 
 class PagedCache(NamedTuple):
@@ -35,6 +37,32 @@ class PagedCache(NamedTuple):
     v: torch.Tensor
     k_exp: Optional[torch.Tensor] = None
     v_exp: Optional[torch.Tensor] = None
+
+
+class PagedState(NamedTuple):
+    """Where a patched model's layers keep and find their keys and values: `hip_flash_attention(..., paged=PagedState(...))`, which is
+    `model(ids, position_ids=..., use_cache=False, paged=PagedState(...))`.
+
+    caches: a `PagedCache` for each layer, by its `layer_idx`.  page_table (B, width): the same pages in each layer's pool.
+    start (B): position of each row's first new token; None: the rows begin with this call, and attend to the new tokens as they came.
+    seqlens (B): tokens of each row with the new ones.  counts (B): how many of the call's S tokens a row has, where not all have S, the rest being
+    padding (start=None: seqlens).  max_len: as in `paged_attention`."""
+    caches: Sequence[PagedCache]
+    page_table: torch.Tensor
+    start: Optional[torch.Tensor]
+    seqlens: torch.Tensor
+    counts: Optional[torch.Tensor] = None
+    max_len: Optional[int] = None
+
+    def attend(self, module, q, k, v, sm_scale) -> torch.Tensor:
+        """A layer's new keys and values into its cache, and its queries' attention."""
+        cache, window = self.caches[module.layer_idx], module.sliding_window
+        if self.start is None:
+            n = _ints(self.seqlens, q)
+            paged_cache_write(cache, k, v, self.page_table, torch.zeros_like(n), n)
+            return _ak.attention(q, k, v, module.sinks, sm_scale, window, None, n)
+        paged_cache_write(cache, k, v, self.page_table, self.start, self.counts)
+        return paged_attention(q, cache, self.page_table, self.seqlens, module.sinks, sm_scale, window, self.start, self.max_len)
 
 
 def paged_cache(pages, kv_heads, page_size=64, storage=torch.bfloat16, device="cuda") -> PagedCache:

@@ -238,6 +238,27 @@ def test_attention_many_rows(A, dtype, storage):
 
 
 @pytest.mark.parametrize("dtype,storage", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("lens,h,g,sq,width,w", [
+    ([1024, 300, 1, 0], 16, 2, 1, 64, 0),                         # rows that many wavefronts walk without a second launch
+    ([256, 17, 255], 8, 8, 1, 16, 0),
+    ([250] * 40, 16, 8, 1, 16, 0),
+    ([2300, 40, 1153], 40, 1, 1, 144, 0),                         # 40 pairs: three blocks of columns, cut
+    ([600, 31], 24, 2, 4, 38, 0),                                 # 48, not cut (bfloat16)
+    ([2900] + [0, 37, 64, 1200, 1] * 14, 12, 3, 1, 190, 0),       # 71 rows, more than a wavefront has lanes
+    ([2100, 5] * 35, 6, 3, 3, 140, 500),
+    ([30, 0, 77] * 367, 4, 2, 1, 100, 0),                         # 1101 rows in a table of 1600 tokens
+    ([1300] + [3] * 11, 4, 1, 40, 100, 0),                        # blocks of pairs beside rows
+])
+def test_attention_divisions(A, dtype, storage, lens, h, g, sq, width, w):
+    """Sizes on both sides of what decides how the work is divided."""
+    print(f"case {dtype} {storage} rows={len(lens)} H={h} G={g} Sq={sq} width={width} window={w}", flush=True)
+    cache, table, n, q, sinks, _, _ = make(A, 23 + sum(lens) + sq, lens, h, g, sq, 16, dtype, storage)
+    wide = torch.full((len(lens), width), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    check(A, cache, wide, n, q, sinks, w)
+
+
+@pytest.mark.parametrize("dtype,storage", TYPES, ids=TYPE_IDS)
 def test_missing_pages_and_lengths_beyond_the_table(A, dtype, storage):
     """Entries of -1 and beyond the pool inside a row: their keys are invisible; a row of nothing else sees nothing.  A length behind the table's end is the
     table's end."""
@@ -458,6 +479,38 @@ def test_calls_on_two_streams(A):
         assert all(torch.equal(x, want[i]) for x in got[i])
 
 
+@pytest.mark.parametrize("storage", [BF16, E4M3])
+def test_two_graphs_that_share_a_pool(A, storage):
+    """Two captured calls of different divisions whose scratch comes from one memory pool, replayed in turn with eager calls between them."""
+    cache, table, n, q, sinks, _, _ = make(A, 24, [5000, 20, 3000], 16, 2, 1, 16, BF16, storage)
+    q, sinks = q.to(DEV), sinks.to(DEV)
+    args = [(q, table, n, None), (q[:2].contiguous(), table[:2].contiguous(), n[:2].contiguous(), 700)]
+
+    def call(i):
+        x, t, m, window = args[i]
+        return A.paged_attention_forward(x, cache, t, m, sinks, SCALE, window)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(0)
+        call(1)
+    side.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i in range(2):
+        with torch.cuda.graph(graphs[i], pool=graphs[0].pool() if i else None):
+            outs.append(call(i))
+    for step in range(4):
+        n.copy_(torch.tensor([5000 - 900 * step, 20, 3000 - 70 * step]))
+        args[1][2].copy_(n[:2])
+        for i in range(2):
+            graphs[i].replay()
+            got = [x.clone() for x in outs[i]]
+            want = call(i)
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(got, want)), (step, i)
+
+
 # ---- as they are used together ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("storage", [BF16, E4M3])
 @pytest.mark.parametrize("window", [None, 32])
@@ -483,3 +536,75 @@ def test_prompt_chunks_and_decoding(A, storage, window):
         tol = 2e-2 + 2.0 ** -8 * ref.abs() if size > 8 else P.bounds(ref, ref_lse, terms, BF16)[0]
         assert bool(((o.cpu().double() - ref).abs() <= tol).all()), at
         at = end
+
+
+@pytest.mark.parametrize("storage", [BF16, E4M3])
+def test_layers_with_a_paged_state(A, storage):
+    """A layer through hip_flash_attention(paged=): a padded prompt, padded chunks of different lengths, single tokens.  Each against the definition, on
+    what the pages hold, and the prompt against attention() itself."""
+    from types import SimpleNamespace
+    g, h, ps, b = 2, 16, 16, 2
+    gen = torch.Generator().manual_seed(25)
+    sinks = torch.randn(h, generator=gen).to(BF16).to(DEV)
+    modules = [SimpleNamespace(sinks=sinks, sliding_window=w, layer_idx=i) for i, w in enumerate((32, None))]
+    caches = [new_cache(A, 24, g, ps, storage) for _ in modules]
+    table = torch.randperm(24, generator=gen).to(torch.int32)[:22].view(2, 11).to(DEV)
+    start = torch.zeros(b, dtype=torch.int32)
+    for step, counts in enumerate(([90, 37], [7, 3], [1, 1], [1, 1], [0, 5])):
+        s, counts = max(counts), torch.tensor(counts, dtype=torch.int32)
+        seqlens = start + counts
+        state = A.PagedState(caches, table, None if step == 0 else start.to(DEV), seqlens.to(DEV), None if step in (0, 2, 3) else counts.to(DEV))
+        for module in modules:
+            q, k, v = (torch.randn(b, s, x, 64, generator=gen).to(BF16).to(DEV).transpose(1, 2) for x in (h, g, g))
+            o, none = A.hip_flash_attention(module, q, k, v, None, SCALE, paged=state)
+            assert none is None
+            if step == 0:
+                assert torch.equal(o, A.attention(q, k, v, sinks, SCALE, module.sliding_window, None, counts.to(DEV)))
+                kk, vv = A.paged_cache_read(caches[module.layer_idx], table, seqlens.to(DEV), s)
+                for x, y in ((kk, k), (vv, v)):
+                    for r in range(b):
+                        c = int(counts[r])
+                        assert torch.equal(x[r, :, :c].cpu().double(), P.stored_rows(y[r, :, :c].cpu(), storage))
+                continue
+            ref, ref_lse, terms = P.attention(q.cpu(), *values(caches[module.layer_idx]), table.cpu(), seqlens, sinks.cpu(), SCALE,
+                                              module.sliding_window or 0, start)
+            assert bool(((o.cpu().double() - ref).abs() <= P.bounds(ref, ref_lse, terms, BF16)[0]).all()), (step, module.layer_idx)
+        start = seqlens
+    with pytest.raises(RuntimeError, match="neither seqlens nor doc_start"):
+        A.hip_flash_attention(modules[0], q, k, v, None, SCALE, paged=state, seqlens=seqlens)
+
+
+def test_patched_model_decodes_on_pages(A):
+    """A patched two-layer model: a padded prompt and tokens one by one on pages give, up to the roundings of the type, the logits of whole rows at once.
+    In float32: two runs whose sums are ordered differently differ by the order of 1e-6 of logits near 1; a key too few or too many moves them by 1e-2."""
+    from transformers import GptOssConfig, GptOssForCausalLM
+    from oregon_gpt_oss_patching_amd import patching
+    cfg = GptOssConfig(vocab_size=512, hidden_size=256, intermediate_size=256, num_hidden_layers=2,
+                       num_attention_heads=16, num_key_value_heads=4, head_dim=64, num_local_experts=2,
+                       num_experts_per_tok=2, sliding_window=32, max_position_embeddings=512,
+                       layer_types=["sliding_attention", "full_attention"], attn_implementation="eager")
+    torch.manual_seed(0)
+    model = GptOssForCausalLM(cfg).to(DEV, FP32).eval()
+    lens, total = torch.tensor([50, 71]), 6
+    ids = torch.randint(0, 512, (2, 80), device=DEV)
+    table = torch.arange(10, dtype=torch.int32, device=DEV).view(2, 5)
+    caches = [A.paged_cache(10, 4, 16, FP32) for _ in range(2)]
+    patching.patch_flash_attention()
+    try:
+        with torch.no_grad():
+            whole = model(ids, use_cache=False).logits
+            s = int(lens.max())
+            state = A.PagedState(caches, table, None, lens.to(DEV))
+            out = model(ids[:, :s], use_cache=False, paged=state).logits
+            for r in range(2):
+                assert torch.allclose(out[r, :lens[r]], whole[r, :lens[r]], rtol=1e-4, atol=1e-4)
+            at = lens.to(DEV)
+            for _ in range(total):
+                state = A.PagedState(caches, table, at, at + 1)
+                new = ids.gather(1, at[:, None])
+                out = model(new, position_ids=at[:, None], use_cache=False, paged=state).logits[:, 0]
+                want = whole[torch.arange(2, device=DEV), at]
+                assert torch.allclose(out, want, rtol=1e-4, atol=1e-4), float((out - want).abs().max())
+                at = at + 1
+    finally:
+        patching.unpatch_flash_attention()

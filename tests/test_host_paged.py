@@ -113,6 +113,30 @@ def test_e4m3_needs_its_exponents():
         assert _validate(p, call) == -2
 
 
+@pytest.mark.parametrize("storage", [_lib.DTYPE_BF16, _lib.DTYPE_E4M3])
+def test_page_strides_of_32_bits(storage):
+    """A page's stride in bytes is below 2^32; what is longer, or runs backwards, is refused."""
+    most = 2 ** 31 - 8 if storage == _lib.DTYPE_BF16 else 2 ** 32 - 16
+    for call in ALL:
+        for name in ("k_page_stride", "v_page_stride") + (("k_exp_stride", "v_exp_stride") if storage == _lib.DTYPE_E4M3 else ()):
+            p = _params(storage)
+            getattr(p, name).b = most
+            assert _validate(p, call) == 0
+            for bad in (2 ** 32, -64):
+                getattr(p, name).b = bad
+                assert _validate(p, call) == -8
+
+
+def test_paged_adapter_refuses_other_lengths():
+    """hip_flash_attention(paged=) takes the rows' lengths from the state alone."""
+    import oregon_gpt_oss_patching_amd as A
+    x = torch.zeros(1, 1, 1, 64)
+    state = A.PagedState([], torch.zeros(1, 1, dtype=torch.int32), None, torch.ones(1, dtype=torch.int32))
+    for name in ("seqlens", "doc_start"):
+        with pytest.raises(RuntimeError, match="neither seqlens nor doc_start"):
+            A.hip_flash_attention(None, x, x, x, None, 0.125, paged=state, **{name: torch.ones(1, dtype=torch.int32)})
+
+
 def test_null_params():
     for call in ALL:
         assert _lib.load().gptoss_attn_paged_validate(None, call) == -1
