@@ -13,11 +13,11 @@
 //    but rows of more bytes loaded that way keep a compute unit at 37 GB/s (one workgroup of 16 wavefronts; with whole rows 131), so K goes
 //    through a stage of LDS first.  Which number of the row stands in which slot of the contraction is free as long as Q has the same order.
 //  * V has to be turned (the contraction runs over keys): for bf16 products it goes through the same stage, after K, and is read back transposed;
-//    in 32 bits each lane loads four columns of its own four keys, which is what the fp32 MFMA takes.
+//    from float32 pages each lane loads four columns of its own four keys, which is what the fp32 MFMA takes.
 //  * P leaves the S product in the layout of the PV product's B operand.
 //  * Entries of the page table are loaded 64 tiles at a time, one per lane; a tile's page is a readlane and its addresses are scalar.
 //  * e4m3 rows widen on the way into the operand: to bf16 by the instruction that takes a power of two along (exact), K's with one
-//    power per lane, V's before they are staged.
+//    power per lane, V's before they are staged; float32 queries then go in as three bf16 terms.
 // The running maximum is raised only when a logit passes it by more than 2^8 (the sums are in 32 bits and the weights keep their relative
 // precision): the reduction over the lanes and the rescaling are then rare.
 #pragma once
@@ -36,11 +36,11 @@ constexpr int kPagedWaves = 4;
 // Blocks of 16 keys in a tile: what a wavefront has under way is a tile, so rows of fewer bytes come more at a time; two columns' worth of
 // float32 numbers leave registers for one block.
 template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_tile_blocks() {
-    return sizeof(T) == 4 ? (sizeof(ST) == 4 && NB > 1 ? 1 : 2) : sizeof(ST) == 1 && NB == 1 && NW == kPagedWaves ? 4 : 2;
+    return sizeof(ST) == 4 ? (NB > 1 ? 1 : 2) : sizeof(ST) == 1 && NB == 1 && NW == kPagedWaves ? 4 : 2;
 }
 // Wavefronts per SIMD, of what the registers leave.
 template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_occupancy() {
-    return sizeof(T) == 4 ? ((sizeof(ST) == 1) == (NB == 1) && NW == kPagedWaves ? 3 : 2) : NB == 1 ? 4 : NB == 2 || (NB == 3 && sizeof(ST) == 1) ? 3 : 2;
+    return sizeof(ST) == 4 ? (NB == 2 && NW == kPagedWaves ? 3 : 2) : sizeof(T) == 4 ? 3 : NB == 1 ? 4 : NB == 2 || (NB == 3 && sizeof(ST) == 1) ? 3 : 2;
 }
 // Pairs (query, head of the group) that one workgroup may take.
 template <typename T> __host__ __device__ constexpr int paged_pairs() { return sizeof(T) == 2 ? 64 : 32; }
@@ -185,15 +185,29 @@ __device__ __forceinline__ uint32_t lane_offset(uint32_t at, uint32_t mask) {
 // lanes: l16 = lane % 16, quad = lane / 16.
 template <typename T, typename ST, int NB, int KB> struct PagedTile;
 
+// Eight numbers as their upper 16 bits, and what is left of them.
+__device__ __forceinline__ bf16x8 take_upper(float (&x)[8]) {
+    u32x4 u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = __builtin_amdgcn_perm(__float_as_uint(x[2 * e + 1]), __float_as_uint(x[2 * e]), 0x07060302u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] -= __uint_as_float(__float_as_uint(x[e]) & 0xffff0000u);
+    return as_bf16x8(u);
+}
+
 // ---- bfloat16 products -----------------------------------------------------------------------------------------------
-template <typename ST, int NB, int KB>
-struct PagedTile<bf16, ST, NB, KB> {
-    static constexpr bool kCodes = sizeof(ST) == 1, kOnce = NB < 4, kStagedK = !kCodes;
+// Of float32 queries over codes too: a code times its power of two is a bfloat16 number, and a float32 number is the sum of three (its 24 bits, eight
+// at a time), so three products of each kind take the place of the fp32 MFMA's, in a fifth of their time: 32 rows of 6000 to 16384 tokens 69 us, and 135 with those.
+// The smaller terms are added first, to 0: their roundings are then 2^-8 of the sum's.
+template <typename T, typename ST, int NB, int KB>
+struct PagedTile16 {
+    static constexpr bool kCodes = sizeof(ST) == 1, kOnce = NB < (sizeof(T) == 4 ? 2 : 4), kStagedK = !kCodes;
+    static constexpr int kTerms = sizeof(T) == 4 ? 3 : 1;
     static constexpr int kStage = 16 * KB * kRowBytes;           // LDS bytes of a wavefront
     static constexpr int kVecs = kCodes ? 1 : 2;                 // 16-byte loads per lane and block
     u32x4 k[KB][kVecs], v[KB][kVecs];
     uint32_t ke[KB], ve[KB];
-    bf16x8 q[NB][2];
+    bf16x8 q[NB][kTerms][2];     // the largest term first
     f32x4 o[NB][4];
     uint32_t tr[4], wr[2], nat[2], k_at[kVecs], v_at[kVecs], ke_at, ve_at;
 
@@ -221,11 +235,20 @@ struct PagedTile<bf16, ST, NB, KB> {
         ke_at = i * a.ke.s;
         ve_at = v_row(lane, 0) * a.ve.s;
     }
-    __device__ __forceinline__ void load_q(int nb, const bf16 *row, bool there, int quad) {
+    __device__ __forceinline__ void load_q(int nb, const T *row, bool there, int quad) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const u32x4 x = *reinterpret_cast<const u32x4 *>(row + (kCodes ? 16 * quad + 8 * s : 32 * s + 8 * quad));
-            q[nb][s] = as_bf16x8(there ? x : u32x4{0, 0, 0, 0});
+            const T *at = row + (kCodes ? 16 * quad + 8 * s : 32 * s + 8 * quad);
+            if constexpr (kTerms == 1) {
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
+                q[nb][0][s] = as_bf16x8(there ? x : u32x4{0, 0, 0, 0});
+            } else {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = there ? at[e] : 0.0f;
+#pragma unroll
+                for (int t = 0; t < kTerms; ++t) q[nb][t][s] = take_upper(x);
+            }
         }
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[nb][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -261,8 +284,13 @@ struct PagedTile<bf16, ST, NB, KB> {
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                const f32x4 z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[0], q[nb][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-                s[nb][blk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[1], q[nb][1], z, 0, 0, 0);
+                f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int t = kTerms - 1; t >= 0; --t) {
+                    z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[0], q[nb][t][0], z, 0, 0, 0);
+                    z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[1], q[nb][t][1], z, 0, 0, 0);
+                }
+                s[nb][blk] = z;
             }
         }
     }
@@ -308,39 +336,58 @@ struct PagedTile<bf16, ST, NB, KB> {
     __device__ __forceinline__ void product(const f32x4 (&s)[NB][KB]) {
 #pragma unroll
         for (int h = 0; h < KB / 2; ++h) {
-            bf16x8 p[NB];
+            bf16x8 p[NB][kTerms];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+            for (int nb = 0; nb < NB; ++nb) {
+                if constexpr (kTerms == 1) {
+                    // (one rounding of each weight, half a step of bfloat16: of the size of the rounding of o)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { p[nb][e] = (bf16)s[nb][2 * h][e]; p[nb][4 + e] = (bf16)s[nb][2 * h + 1][e]; }
+                    for (int e = 0; e < 4; ++e) { p[nb][0][e] = (bf16)s[nb][2 * h][e]; p[nb][0][4 + e] = (bf16)s[nb][2 * h + 1][e]; }
+                } else {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = s[nb][2 * h + (e >> 2)][e & 3];
+#pragma unroll
+                    for (int t = 0; t < kTerms; ++t) p[nb][t] = take_upper(x);
+                }
+            }
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
                 union { struct { s16x4 a, b; } s; bf16x8 v; } x;
                 x.s.a = lds_load_tr64(tr[d], 32 * h * kRowBytes);
                 x.s.b = lds_load_tr64(tr[d], (32 * h + 16) * kRowBytes);
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) o[nb][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb], o[nb][d], 0, 0, 0);
+                for (int nb = 0; nb < NB; ++nb) {
+                    if constexpr (kTerms == 1) {
+                        o[nb][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb][0], o[nb][d], 0, 0, 0);
+                    } else {
+                        f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int t = kTerms - 1; t >= 0; --t) z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb][t], z, 0, 0, 0);
+                        o[nb][d] += z;
+                    }
+                }
             }
         }
     }
     // column of o[.][d][e] in the lane's row
     __device__ __forceinline__ static int column(int d, int e, int quad) { return 16 * d + 4 * quad + e; }
 };
+template <typename ST, int NB, int KB> struct PagedTile<bf16, ST, NB, KB> : PagedTile16<bf16, ST, NB, KB> {};
+template <int NB, int KB> struct PagedTile<float, e4m3, NB, KB> : PagedTile16<float, e4m3, NB, KB> {};
 
 // ---- float32 products ------------------------------------------------------------------------------------------------
-template <typename ST, int NB, int KB>
-struct PagedTile<float, ST, NB, KB> {
-    static constexpr bool kCodes = sizeof(ST) == 1, kOnce = NB < 2, kStagedK = !kCodes;
-    static constexpr int kStage = kCodes ? 0 : 16 * KB * kD * 4;
-    static constexpr int kVecs = kCodes ? 1 : 4;
-    typedef typename std::conditional<kCodes, uint32_t, f32x4>::type vec;       // four numbers of a row of V
+template <int NB, int KB>
+struct PagedTile<float, float, NB, KB> {
+    static constexpr bool kCodes = false, kOnce = NB < 2, kStagedK = true;
+    static constexpr int kStage = 16 * KB * kD * 4;
+    static constexpr int kVecs = 4;
     u32x4 k[KB][kVecs];
-    vec v[KB][4];
-    uint32_t ke[KB], ve[KB][4];
+    f32x4 v[KB][4];              // four numbers of a row of V
     float q[NB][16];
     f32x4 o[NB][4];
-    f32x4 w[KB][4];              // V as numbers
-    uint32_t k_at[kVecs], wr[kVecs], nat[kVecs], ke_at, v_at[4], ve_at[4];
+    f32x4 w[KB][4];              // V without what is masked
+    uint32_t k_at[kVecs], wr[kVecs], nat[kVecs], v_at[4];
 
     __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage, int lane) {
         const int l16 = lane & 15, quad = lane >> 4;
@@ -348,43 +395,30 @@ struct PagedTile<float, ST, NB, KB> {
         for (int e = 0; e < kVecs; ++e) {
             // rows quad + 4 e in 16 pieces, piece c of row r at c ^ r: what 16 lanes write or read is in distinct banks
             const int r = quad + 4 * e;
-            k_at[e] = kCodes ? l16 * a.kp.s + 16 * quad : r * a.kp.s + 16 * l16;
+            k_at[e] = r * a.kp.s + 16 * l16;
             wr[e] = stage + r * kD * 4 + ((l16 ^ r) * 16);
             nat[e] = stage + l16 * kD * 4 + (((4 * e + quad) ^ l16) * 16);
         }
-        ke_at = l16 * a.ke.s;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v_at[e] = (4 * quad + e) * a.vp.s + 4 * (uint32_t)sizeof(ST) * l16;
-            ve_at[e] = (4 * quad + e) * a.ve.s;
-        }
+        for (int e = 0; e < 4; ++e) v_at[e] = (4 * quad + e) * a.vp.s + 16 * l16;
     }
-    __device__ __forceinline__ static int q_index(int t, int quad) { return kCodes ? 16 * quad + t : 16 * (t >> 2) + 4 * quad + (t & 3); }
     __device__ __forceinline__ void load_q(int nb, const float *row, bool there, int quad) {
 #pragma unroll
         for (int t = 0; t < 16; t += 4) {
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(row + q_index(t, quad));
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(row + 4 * t + 4 * quad);
 #pragma unroll
             for (int e = 0; e < 4; ++e) q[nb][t + e] = there ? x[e] : 0.0f;
         }
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[nb][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb, uint32_t mask) {
+    __device__ __forceinline__ void load_k(int blk, const char *kb, const char *, uint32_t mask) {
 #pragma unroll
         for (int s = 0; s < kVecs; ++s) k[blk][s] = load16<kOnce>(kb + lane_offset(k_at[s], mask));
-        if constexpr (kCodes) ke[blk] = (uint8_t)eb[lane_offset(ke_at, mask)];
     }
-    __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb, uint32_t mask) {
+    __device__ __forceinline__ void load_v(int blk, const char *vb, const char *, uint32_t mask) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[blk][e] = load_rows<kOnce, vec>(vb + lane_offset(v_at[e], mask));
-            if constexpr (kCodes) ve[blk][e] = (uint8_t)eb[lane_offset(ve_at[e], mask)];
-        }
-    }
-    __device__ __forceinline__ static float code(uint32_t w, int i) {
-        return i == 0 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 0) : i == 1 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 1)
-               : i == 2 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 2) : __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+        for (int e = 0; e < 4; ++e) v[blk][e] = load_rows<kOnce, f32x4>(vb + lane_offset(v_at[e], mask));
     }
     __device__ __forceinline__ void stage_k() const {
 #pragma unroll
@@ -399,33 +433,20 @@ struct PagedTile<float, ST, NB, KB> {
             for (int nb = 0; nb < NB; ++nb) s[nb][blk] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             u32x4 f[kVecs];
 #pragma unroll
-            for (int t = 0; t < kVecs; ++t) f[t] = kCodes ? k[blk][t] : lds_load128(nat[t], 16 * blk * kD * 4);
-            float p = 1.0f;
-            if constexpr (kCodes) p = exp_of_byte(ke[blk]);
+            for (int t = 0; t < kVecs; ++t) f[t] = lds_load128(nat[t], 16 * blk * kD * 4);
 #pragma unroll
-            for (int t = 0; t < 16; ++t) {
-                float x;
-                if constexpr (kCodes) x = p * code(f[0][t >> 2], t & 3);
-                else x = __uint_as_float(f[t >> 2][t & 3]);
+            for (int t = 0; t < 16; ++t)
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) s[nb][blk] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, q[nb][t], s[nb][blk], 0, 0, 0);
-            }
+                for (int nb = 0; nb < NB; ++nb)
+                    s[nb][blk] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f[t >> 2][t & 3]), q[nb][t], s[nb][blk], 0, 0, 0);
         }
     }
     __device__ __forceinline__ bool stage_v(bool edge, bool several, int first, int last, unsigned there, int lane) {
+        bool odd = false;
 #pragma unroll
         for (int blk = 0; blk < KB; ++blk)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if constexpr (kCodes) {
-                    const float p = exp_of_byte(ve[blk][e]);
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) w[blk][e][d] = p * code(v[blk][e], d);
-                } else {
-                    w[blk][e] = v[blk][e];
-                }
-            }
-        bool odd = false;
+            for (int e = 0; e < 4; ++e) w[blk][e] = v[blk][e];
         if (edge) {
 #pragma unroll
             for (int blk = 0; blk < KB; ++blk)

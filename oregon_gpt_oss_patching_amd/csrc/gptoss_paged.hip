@@ -77,9 +77,9 @@ template <typename T, typename ST, int NB> constexpr int per_simd() { return pag
 
 PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     PagedDivision d{};
-    const bool f32 = p->dtype == GPTOSS_ATTN_FP32, codes = p->storage == GPTOSS_ATTN_E4M3;
+    const bool codes = p->storage == GPTOSS_ATTN_E4M3, f32 = p->storage == GPTOSS_ATTN_FP32;      // f32: the fp32 MFMA
     const int64_t r = p->H / p->G, pairs = (int64_t)p->Sq * r;
-    const int most = f32 ? paged_pairs<float>() : paged_pairs<bf16>();
+    const int most = p->dtype == GPTOSS_ATTN_FP32 ? paged_pairs<float>() : paged_pairs<bf16>();
     d.nb = pairs <= 16 ? 1 : pairs <= 32 || most == 32 ? 2 : pairs <= 48 ? 3 : 4;
     const int64_t blocks = (pairs + 16 * d.nb - 1) / (16 * d.nb);
     d.blocks = (int)(blocks < 0x7fffffff ? blocks : 0x7fffffff);
@@ -105,7 +105,7 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     // as many, twice as many: 16 x 8192 tokens 46.3 / 47.5 / 50.1, 64 x 3540 73.9 / 77.4 / 80.3, but 64 rows of 150 to 16384 103 / 81.6 / 83.5, 32 of 6000 to
     // 16384 137 / 112 / 114, and four queries on each of those in e4m3 44.3 / 33.4 / 41.2.
 #define GPTOSS_HELD(T, NB) (codes ? per_simd<T, e4m3, NB>() : per_simd<T, T, NB>())
-    const int per_cu = f32 ? (d.nb == 1 ? GPTOSS_HELD(float, 1) : GPTOSS_HELD(float, 2))
+    const int per_cu = p->dtype == GPTOSS_ATTN_FP32 ? (d.nb == 1 ? GPTOSS_HELD(float, 1) : GPTOSS_HELD(float, 2))
                            : d.nb == 1 ? GPTOSS_HELD(bf16, 1) : d.nb == 2 ? GPTOSS_HELD(bf16, 2) : d.nb == 3 ? GPTOSS_HELD(bf16, 3) : GPTOSS_HELD(bf16, 4);
 #undef GPTOSS_HELD
     const int64_t held = 256 * per_cu / p->G, left = held - d.units / 2, can = d.units * ((keys + d.min_keys - 1) / d.min_keys);
@@ -124,7 +124,7 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
 template <typename T, typename ST, int NB>
 int attend(const PagedDivision &d, void *stream, PagedArgs &a) {
     if constexpr (NB == 1) {
-        if constexpr (sizeof(T) == 2)
+        if constexpr (sizeof(ST) < 4)
             if (d.alone == 16) return launch(attn_paged_kernel<T, ST, NB, 16>, d.units * a.G, 1024, stream, a);
         if (d.alone == 8) return launch(attn_paged_kernel<T, ST, NB, 8>, d.units * a.G, 512, stream, a);
     }
