@@ -54,8 +54,8 @@ struct PagedSpan {
     int lo, hi, t_first, tiles;  // keys lo .. hi - 1, in tiles
 };
 __device__ __forceinline__ int paged_base(const PagedArgs &a, int b, int n) {
-    // (positions beyond +-2^30 exist in no row)
-    return a.start ? min(max(a.start[b], -(1 << 30)), (1 << 30) - 1) : n - a.Sq;
+    // (positions of 2^30 and more exist in no row; below -2^30 no query reaches one that does)
+    return a.start ? min(max(a.start[b], -(1 << 30)), 1 << 30) : n - a.Sq;
 }
 template <int PAIRS, int KEYS>
 __device__ __forceinline__ PagedSpan paged_span(const PagedArgs &a, int b, int block, int n, int base) {
@@ -247,7 +247,12 @@ struct PagedTile16 {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = there ? at[e] : 0.0f;
 #pragma unroll
-                for (int t = 0; t < kTerms; ++t) q[nb][t][s] = take_upper(x);
+                for (int t = 0; t < kTerms; ++t) {
+                    q[nb][t][s] = take_upper(x);
+                    // (an infinity less itself is not what is left of it)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = isinf(at[e]) ? 0.0f : x[e];
+                }
             }
         }
 #pragma unroll

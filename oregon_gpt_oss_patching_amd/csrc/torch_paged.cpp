@@ -55,6 +55,7 @@ void fill(PagedCall &c, const Tensor &k_pages, const Tensor &v_pages, const OptT
                 " does not go with tensors of ", dtype, ": it holds their type or float8_e4m3fn");
     TORCH_CHECK(k_pages.dim() == 4 && k_pages.sizes() == v_pages.sizes() && k_pages.size(3) == 64, "the cache's k and v must both be (pages, G, page_size, 64), got ",
                 k_pages.sizes(), " and ", v_pages.sizes());
+    TORCH_CHECK(k_pages.stride(3) == 1 && v_pages.stride(3) == 1, "the cache's rows of 64 must be contiguous, got strides ", k_pages.strides(), " and ", v_pages.strides());
     gptoss_attn_paged_params &p = c.p;
     p.struct_size = sizeof(p);
     p.dtype = abi_dtype(dtype);
@@ -87,10 +88,17 @@ void fill(PagedCall &c, const Tensor &k_pages, const Tensor &v_pages, const OptT
     p.page_table = c.table.const_data_ptr<int32_t>();
 }
 
-// Rows (B, G, S, 64) or (B, H, S, 64) as the kernels take them; a dimension of one element has a stride that says nothing.
+// Rows (B, G, S, 64) or (B, H, S, 64) as the kernels take them, and their strides; a dimension of one element has a stride that says nothing.  What is laid out
+// otherwise is copied (a copy that is one: `contiguous` gives such a tensor back as it is, on whatever address).
 Tensor rows_of(const Tensor &t, gptoss_attn_strides &s) {
-    const bool one = t.size(2) == 1 && t.stride(2) < 64;
-    const Tensor r = one ? row_contiguous(t.as_strided(t.sizes(), {t.stride(0), t.stride(1), 64, t.stride(3)}), 2) : row_contiguous(t, 2);
+    const int64_t per16 = 16 / t.element_size();
+    s.b = t.size(0) == 1 ? 0 : t.stride(0);
+    s.h = t.size(1) == 1 ? 0 : t.stride(1);
+    s.s = t.size(2) == 1 ? 64 : t.stride(2);
+    if (t.stride(3) == 1 && s.b % per16 == 0 && s.h % per16 == 0 && s.s % per16 == 0 && s.s >= 64 && s.s <= kMaxSeqStride &&
+        reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0)
+        return t;
+    const Tensor r = t.clone(at::MemoryFormat::Contiguous);
     set3(s, r);
     return r;
 }

@@ -189,6 +189,44 @@ def test_strided_sources_and_float16(A):
         assert torch.equal(got, k.to(BF16).to(k.dtype))
 
 
+@pytest.mark.parametrize("dtype,storage", TYPES, ids=TYPE_IDS)
+def test_dimensions_of_one_and_addresses_between_16_bytes(A, dtype, storage):
+    """Strides of dimensions with one element say nothing, whatever they are; rows on other addresses are copied."""
+    gen = torch.Generator().manual_seed(26)
+    table = torch.tensor([[1, 0]], dtype=torch.int32, device=DEV)
+    for g, h, s in ((1, 1, 1), (2, 8, 1), (1, 4, 3)):
+        k, v, q = (torch.randn(1, x, s, 64, generator=gen).to(dtype).to(DEV) for x in (g, g, h))
+
+        def odd(x, strides, at=0):
+            y = torch.empty(x.numel() * 2 + 64, dtype=dtype, device=DEV)[at:].as_strided(x.shape, strides)
+            y.copy_(x)
+            return y
+
+        want = None
+        for at in (0, 1):
+            st = lambda x: (7, 5 if x.shape[1] == 1 else 64 * s, 3 if s == 1 else 64, 1)
+            kk, vv, qq = (odd(x, st(x), at) for x in (k, v, q))
+            cache = A.paged_cache(2, g, 16, storage)
+            A.paged_cache_write(cache, kk, vv, table, [5])
+            o = A.paged_attention(qq, cache, table, [5 + s], None, SCALE, None, [5])
+            if want is None:
+                plain = A.paged_cache(2, g, 16, storage)
+                A.paged_cache_write(plain, k, v, table, [5])
+                want = A.paged_attention(q, plain, table, [5 + s], None, SCALE, None, [5])
+            for x, y in zip(cache, plain):
+                assert x is None or torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+            assert torch.equal(o, want)
+
+
+def test_under_inference_mode(A):
+    with torch.inference_mode():
+        cache = A.paged_cache(2, 1, 16, E4M3)
+        table, k = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.ones(1, 1, 4, 64, dtype=BF16, device=DEV)
+        A.paged_cache_write(cache, k, k, table, [0])
+        assert torch.equal(A.paged_cache_read(cache, table, [4], 4)[0], k)
+        assert torch.equal(A.paged_attention(k[:, :, :1], cache, table, [4], torch.full((1,), -float("inf"), device=DEV), SCALE), k[:, :, :1])
+
+
 # ---- attention -------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,storage", TYPES, ids=TYPE_IDS)
 @pytest.mark.parametrize("lens,h,g,sq,ps,w", [
@@ -326,6 +364,35 @@ def test_rows_that_no_query_or_only_a_later_one_sees(A, dtype, storage, bad):
 
 
 @pytest.mark.parametrize("dtype,storage", TYPES, ids=TYPE_IDS)
+def test_infinite_queries(A, dtype, storage):
+    """A query with an infinity where all keys are negative has logits of -inf alone: no weight but the sink's."""
+    cache, table, n, q, sinks, k, v = make(A, 27, [40], 4, 1, 1, 16, dtype, storage)
+    k = k.clone()
+    k[..., 9] = -1 - k[..., 9].abs()
+    A.paged_cache_write(cache, k.to(DEV), v.to(DEV), table, [0])
+    plain = A.paged_attention(q.to(DEV), cache, table, n, sinks.to(DEV), SCALE)
+    q[:, 2, :, 9] = float("inf")
+    o, lse = A.paged_attention_forward(q.to(DEV), cache, table, n, sinks.to(DEV), SCALE)
+    assert not o[:, :, 2].any() and torch.equal(lse[0, 2].cpu(), sinks[2:3].float())
+    for h in (0, 1, 3):
+        assert torch.equal(o[:, :, h], plain[:, :, h])
+
+
+def test_positions_at_the_end_of_the_longest_table(A):
+    """2^30 tokens: the last one exists, positions behind it do not, whatever they are."""
+    table = torch.full((1, 1 << 20), -1, dtype=torch.int32, device=DEV)
+    table[0, -1] = 0
+    cache, n = A.paged_cache(1, 1, 1024), [1 << 30]
+    k = torch.ones(1, 1, 1, 64, dtype=BF16, device=DEV)
+    A.paged_cache_write(cache, k, k, table, [(1 << 30) - 1])
+    assert bool((cache.k[0, 0, -1] == 1).all()) and not cache.k[0, 0, :-1].any()
+    sinks = torch.full((1,), -float("inf"), device=DEV)
+    assert torch.equal(A.paged_attention(k, cache, table, n, sinks, SCALE, 1, [(1 << 30) - 1]), k)
+    for start in (1 << 30, 2 ** 31 - 1, -1, -2 ** 31):
+        assert not A.paged_attention(k, cache, table, n, sinks, SCALE, 1, [start]).any()
+
+
+@pytest.mark.parametrize("dtype,storage", TYPES, ids=TYPE_IDS)
 def test_layouts(A, dtype, storage):
     """A pool with the heads of a token side by side, one layer's slice of a larger pool, q out of a projection's layout, 64-bit and strided tables."""
     lens = [130, 77, 5]
@@ -400,6 +467,7 @@ def test_refusals(A):
         ("for this cache", lambda: A.paged_cache_write(cache, q, q, table, n)),
         ("both be", lambda: A.paged_cache_write(cache, k, q, table, n)),
         ("max_len", lambda: A.paged_cache_read(cache, table, n, 0)),
+        ("rows of 64 must be contiguous", lambda: A.paged_attention(q, A.PagedCache(*(torch.zeros(4, 2, 16, 128, dtype=BF16, device=DEV)[..., ::2] for _ in range(2))), table, n, None, SCALE)),
         ("exponents", lambda: A.paged_attention(q, A.PagedCache(cache.k.to(E4M3), cache.v.to(E4M3)), table, n, None, SCALE)),
         ("must not be negative", lambda: A.paged_attention(q, cache, table, n, None, SCALE, -3)),
     ):
