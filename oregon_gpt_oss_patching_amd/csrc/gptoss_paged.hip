@@ -90,15 +90,21 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     const int64_t queries = (16 * d.nb - 1) / r + 2;                   // that a unit's pairs touch
     if (p->window > 0 && p->window + queries < keys) keys = p->window + queries;
     d.min_keys = f32 ? 128 : 256;
-    // Short rows: a workgroup walks a unit alone, as many wavefronts as its keys and the compute unit's share of the workgroups have room
-    // for, and there is nothing to add in a second launch.  us, cut / alone, 64 heads on 8 KV heads: 1 x 500 tokens 10.3 / 7.7, 1 x 1025 10.3 /
-    // 9.7, but 1 x 1500 10.3 / 12.2; 32 x 1000 18.9 / 14.9, 128 x 250 18.0 / 14.2, 64 x 500 of which most are short 13.0 / 9.7; with two
-    // workgroups to a unit and more the others' rows fill the time that a long one takes: 64 x 2000 48.9 / 43.5, with one of 2000 among shorter ones
-    // 21.3 / 21.7 (32 rows 15.3 / 19.4).  In 32 bits 1 x 257 10.5 / 9.8, but 8 x 500 11.1 / 13.7; 128 x 500 on two KV heads 21.7 / 16.4.
+    // Short rows: a workgroup walks a unit alone, as many wavefronts as its keys and the compute unit's share of the workgroups have room for, and
+    // there is nothing to add in a second launch.  Rows of few bytes, and workgroups that fill the chip by themselves, do so for longer.  us, cut / alone, 64
+    // heads on 8 KV heads ("to n": rows of 50 to n tokens):
+    //   bfloat16: 1 x 1025 tokens 9.1 / 8.0, but 1 x 1500 9.0 / 11.9; 32 x 1000 18.4 / 14.6, 16 to 1100 10.0 / 10.4, 32 to 2000 14.3 / 16.1; more than a workgroup to a
+    //   compute unit: 64 x 2000 48.1 / 43.4, 64 to 2500 22.0 / 22.3, 40 to 3500 19.8 / 23.3
+    //   codes: 1 x 1500 9.4 / 9.5, 8 x 1500 12.2 / 10.2, but 4 to 2000 10.1 / 11.5; half a workgroup to a compute unit and more: 16 to 2000 11.8 / 11.2, 32 x 2000 20.5 / 16.2, but
+    //   16 to 3500 12.6 / 15.7; more than one: 64 to 3500 21.1 / 18.4, 40 to 3500 17.0 / 17.2, 40 to 4500 17.9 / 20.4
+    //   four queries a row (four wavefronts): 3 to 800 10.2 / 10.1, 3 to 1000 10.3 / 11.4, 32 x 500 16.3 / 9.4; 16 to 1000 11.4 / 10.9, 16 to 1300 12.9 / 13.2; 64 to 2000 24.9 / 20.2, 40 to
+    //   3000 22.4 / 23.5
+    //   32 bits: 1 x 300 10.2 / 9.6, 8 x 300 11.0 / 9.9, but 1 x 500 10.4 / 11.6; 128 x 500 on two KV heads 21.7 / 16.4
     const int64_t wgs = d.units * p->G;
-    const bool full = wgs > (f32 ? 128 : 256);
+    const bool full = wgs > (f32 ? 128 : 256), half = wgs >= 128;
     d.alone = d.nb > 1 || keys <= 128 || wgs > (f32 ? 256 : 512) ? kPagedWaves : f32 || full || keys <= 256 ? 8 : 16;
-    if (d.units > kPagedMaxUnits || keys <= (f32 ? 288 : 1152) * (full ? 2 : 1)) return d;
+    const int most_alone = f32 ? (full ? 576 : 288) : d.nb > 1 ? (full ? 2304 : half ? 1152 : 832) : codes ? (full ? 3456 : half ? 2304 : 1536) : full ? 2304 : 1152;
+    if (d.units > kPagedMaxUnits || keys <= most_alone) return d;
     d.alone = kPagedWaves;
     // As many workgroups as a 256-CU part holds at a time: they start and end together.  A unit's last share is half of one on average; at
     // least half of the workgroups are shares all the same, so that a long row among many is cut.  No more than the units can have.  us with half as many,

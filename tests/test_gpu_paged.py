@@ -286,6 +286,11 @@ def test_attention_many_rows(A, dtype, storage):
     ([2100, 5] * 35, 6, 3, 3, 140, 500),
     ([30, 0, 77] * 367, 4, 2, 1, 100, 0),                         # 1101 rows in a table of 1600 tokens
     ([1300] + [3] * 11, 4, 1, 40, 100, 0),                        # blocks of pairs beside rows
+    ([1536, 7], 8, 1, 1, 96, 0),                                  # codes are walked alone for longer than other rows
+    ([2304, 90] + [40] * 14, 16, 8, 1, 144, 0),
+    ([3456, 1000] + [40] * 31, 16, 8, 1, 216, 0),
+    ([832, 31], 24, 2, 2, 52, 0),
+    ([1152, 900] + [31] * 14, 24, 8, 6, 72, 0),
 ])
 def test_attention_divisions(A, dtype, storage, lens, h, g, sq, width, w):
     """Sizes on both sides of what decides how the work is divided."""
