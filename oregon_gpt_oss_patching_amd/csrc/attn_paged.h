@@ -166,14 +166,6 @@ __device__ __forceinline__ bf16x8 widen8(uint32_t w0, uint32_t w1, float f) {
     return x.v;
 }
 
-// Rows that no other workgroup reads bypass the caches' retention: 16 x 8192 tokens 54.1 -> 48.5 us, 4 x 65536 101 -> 89.7 (6.0 TB/s), 32 rows of
-// 6000 to 16384 in e4m3 73.8 -> 68.7.  A row of more pairs than a workgroup takes is read again by the next one (NB = 4, and two blocks in 32 bits).
-template <bool ONCE, typename V>
-__device__ __forceinline__ V load_rows(const char *p) {
-    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
-    else return *reinterpret_cast<const V *>(p);
-}
-
 // A lane's 32-bit offset from a scalar address.  Hidden, as the compiler widens it once in front of the loop otherwise, and then adds 64 bits per load.
 __device__ __forceinline__ uint32_t lane_offset(uint32_t at, uint32_t mask) {
     at &= mask;
@@ -181,6 +173,9 @@ __device__ __forceinline__ uint32_t lane_offset(uint32_t at, uint32_t mask) {
     return at;
 }
 
+// kOnce: rows that no other workgroup reads bypass the caches' retention, us without / with: 16 x 8192 tokens 54.6 / 47.3, 4 x 65536 101 / 87.2 (6.2 TB/s), 64 rows of 150
+// to 16384 96.7 / 84.8, 32 of 6000 to 16384 in e4m3 74.8 / 66.2.  A row of more pairs than a workgroup takes is read again by the next one (NB = 4, and two
+// blocks in 32 bits).
 // A tile's K and V as they are loaded, and what is done with them.  `kb` / `vb`: scalar addresses of the first row of a block of 16 keys;
 // lanes: l16 = lane % 16, quad = lane / 16.
 template <typename T, typename ST, int NB, int KB> struct PagedTile;
@@ -423,7 +418,7 @@ struct PagedTile<float, float, NB, KB> {
     }
     __device__ __forceinline__ void load_v(int blk, const char *vb, const char *, uint32_t mask) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[blk][e] = load_rows<kOnce, f32x4>(vb + lane_offset(v_at[e], mask));
+        for (int e = 0; e < 4; ++e) v[blk][e] = __builtin_bit_cast(f32x4, load16<kOnce>(vb + lane_offset(v_at[e], mask)));
     }
     __device__ __forceinline__ void stage_k() const {
 #pragma unroll
