@@ -192,6 +192,13 @@ def load_torch_ops() -> None:
     torch.ops.load_library(TORCH_LIBRARY)
 
 
+def direct_calls():
+    """(paged_write, paged_read, paged_fwd) of libgptoss_torch.so as Python functions that do not go through the dispatcher."""
+    f = ctypes.PyDLL(TORCH_LIBRARY).gptoss_paged_direct
+    f.restype = ctypes.py_object
+    return f()
+
+
 def status_string(status: int) -> str:
     return load().gptoss_attn_status_string(int(status)).decode()
 

@@ -80,10 +80,11 @@ def paged_cache(pages, kv_heads, page_size=64, storage=torch.bfloat16, device="c
 
 _ready = False
 _write = _read = _fwd = None
+_write_now = _read_now = _fwd_now = None        # the same without the dispatcher, NotImplemented where it is needed
 
 
 def _register_ops() -> None:
-    global _ready, _write, _read, _fwd
+    global _ready, _write, _read, _fwd, _write_now, _read_now, _fwd_now
     _lib.load_torch_ops()
     ops = torch.ops.gptoss_attn
 
@@ -101,6 +102,7 @@ def _register_ops() -> None:
         b, h, s, d = q.shape
         return q.new_empty((b, s, h, d)), q.new_empty((b, h, s) if need_lse else (0,), dtype=torch.float32)
 
+    _write_now, _read_now, _fwd_now = _lib.direct_calls()
     _write, _read, _fwd = ops.paged_write.default, ops.paged_read.default, ops.paged_fwd.default
     _ready = True
 
@@ -112,6 +114,7 @@ except Exception:       # not built yet: importing has to work for the build its
 
 
 _Tensor = torch.Tensor
+_compiling = torch.compiler.is_compiling
 
 
 def _ints(x, like):
@@ -126,7 +129,8 @@ def paged_cache_write(cache: PagedCache, k, v, page_table, start, seqlens=None) 
     Two rows of one call must not write the same slot, and nothing that runs at the same time may read what is being written."""
     if not _ready:
         _register_ops()
-    _write(*cache, k, v, _ints(page_table, cache.k), _ints(start, cache.k), _ints(seqlens, cache.k))
+    if _compiling() or _write_now(*cache, k, v, page_table, start, seqlens) is NotImplemented:
+        _write(*cache, k, v, _ints(page_table, cache.k), _ints(start, cache.k), _ints(seqlens, cache.k))
 
 
 def paged_cache_read(cache: PagedCache, page_table, seqlens, max_len, start=None, dtype=None):
@@ -138,15 +142,20 @@ def paged_cache_read(cache: PagedCache, page_table, seqlens, max_len, start=None
         _register_ops()
     if dtype is None:
         dtype = torch.bfloat16 if cache.k.dtype == torch.float8_e4m3fn else cache.k.dtype
-    return _read(*cache, _ints(page_table, cache.k), _ints(seqlens, cache.k), int(max_len), _ints(start, cache.k), dtype)
+    out = NotImplemented if _compiling() else _read_now(*cache, page_table, seqlens, max_len, start, dtype)
+    if out is NotImplemented:
+        out = _read(*cache, _ints(page_table, cache.k), _ints(seqlens, cache.k), int(max_len), _ints(start, cache.k), dtype)
+    return out
 
 
 def paged_attention_forward(q, cache: PagedCache, page_table, seqlens, sinks, sm_scale, bandwidth=None, start=None, max_len=None):
     """`paged_attention` that returns (o, lse (B, H, S) float32)."""
     if not _ready:
         _register_ops()
-    return _fwd(q, *cache, _ints(page_table, q), _ints(seqlens, q), _ints(start, q), sinks, float(sm_scale),
-                int(bandwidth or 0), int(max_len or 0))
+    out = NotImplemented if _compiling() else _fwd_now(q, *cache, page_table, seqlens, start, sinks, sm_scale, bandwidth, max_len, True)
+    if out is NotImplemented:
+        out = _fwd(q, *cache, _ints(page_table, q), _ints(seqlens, q), _ints(start, q), sinks, float(sm_scale), int(bandwidth or 0), int(max_len or 0))
+    return out
 
 
 def paged_attention(q, cache: PagedCache, page_table, seqlens, sinks, sm_scale, bandwidth=None, start=None, max_len=None):
@@ -162,5 +171,8 @@ def paged_attention(q, cache: PagedCache, page_table, seqlens, sinks, sm_scale, 
     served by `paged_cache_read` and `attention`."""
     if not _ready:
         _register_ops()
-    return _fwd(q, *cache, _ints(page_table, q), _ints(seqlens, q), _ints(start, q), sinks, float(sm_scale),
-                int(bandwidth or 0), int(max_len or 0), False)[0]
+    out = NotImplemented if _compiling() else _fwd_now(q, *cache, page_table, seqlens, start, sinks, sm_scale, bandwidth, max_len, False)
+    if out is NotImplemented:
+        out = _fwd(q, *cache, _ints(page_table, q), _ints(seqlens, q), _ints(start, q), sinks, float(sm_scale), int(bandwidth or 0), int(max_len or 0),
+                   False)[0]
+    return out

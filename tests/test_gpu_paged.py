@@ -490,6 +490,49 @@ def test_refusals(A):
         assert e.value.status == status
 
 
+def test_the_operators_are_called_where_something_watches(A):
+    """Python's calls go past the dispatcher only where nobody stands there: modes, a profiler and the compiler see the operators, and what comes out is the same.  Gradients are
+    refused either way; a parameter's are nobody's under no_grad."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    cache, table, n, q, sinks, k, v = make(A, 28, [300, 20], 8, 2, 1, 16, BF16, E4M3, 2)
+    q, sinks, k, v = q.to(DEV), torch.nn.Parameter(sinks.to(DEV)), k.to(DEV), v.to(DEV)
+    start = torch.tensor([3, 7], dtype=torch.int32, device=DEV)
+
+    def calls(k):
+        A.paged_cache_write(cache, k, v, table, start)
+        kk, vv = A.paged_cache_read(cache, table, n, 300)
+        o = A.paged_attention(q, cache, table, n, sinks, SCALE, 40)
+        return (kk, vv, o, *A.paged_attention_forward(q, cache, table, n, sinks, SCALE))
+
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    names = ["paged_write", "paged_read", "paged_fwd", "paged_fwd"]
+    with torch.no_grad():
+        want = calls(k)
+        with Watch():
+            got = [calls(k)]
+        assert [x for x in seen if "paged" in x] == [f"gptoss_attn.{x}.default" for x in names]
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+            got.append(calls(k))
+        assert {e.key for e in prof.key_averages()} >= {f"gptoss_attn::{x}" for x in names}
+        got.append(torch.compile(calls, fullgraph=True, backend="aot_eager")(k))
+        with torch.autocast("cuda", torch.bfloat16):
+            got.append(calls(k))
+    for out in got:
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        A.paged_attention(q, cache, table, n, sinks, SCALE)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        A.paged_cache_write(cache, k.clone().requires_grad_(), v, table, start)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="vmap"):
+        torch.vmap(lambda x: A.paged_attention(x, cache, table, n, None, SCALE))(q[None])
+
+
 # ---- streams and graphs ------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,storage", TYPES, ids=TYPE_IDS)
 def test_graph_of_a_decoding_step(A, dtype, storage):

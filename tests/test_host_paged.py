@@ -172,6 +172,13 @@ def test_gradients_are_refused():
         A.paged_attention(q, cache, table, n, None, 0.125)
 
 
+def test_forward_gradients_are_refused():
+    cache, table, n = _cpu_cache(), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q = torch.zeros(1, 16, 1, 64, dtype=torch.bfloat16)
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError, match="no gradient"):
+        A.paged_attention(torch.autograd.forward_ad.make_dual(q, q), cache, table, n, None, 0.125)
+
+
 def test_paged_cache_allocates_and_refuses():
     c = _cpu_cache(storage=torch.float8_e4m3fn)
     assert c.k.shape == (4, 2, 16, 64) and c.k_exp.shape == (4, 2, 16) and c.k_exp.dtype == torch.uint8
