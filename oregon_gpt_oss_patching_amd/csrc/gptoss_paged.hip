@@ -89,7 +89,6 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     if (p->max_len > 0 && p->max_len < keys) keys = p->max_len;
     const int64_t queries = (16 * d.nb - 1) / r + 2;                   // that a unit's pairs touch
     if (p->window > 0 && p->window + queries < keys) keys = p->window + queries;
-    d.min_keys = f32 ? 128 : 256;
     // Short rows: a workgroup walks a unit alone, as many wavefronts as its keys and the compute unit's share of the workgroups have room for, and
     // there is nothing to add in a second launch.  Rows of few bytes, and workgroups that fill the chip by themselves, do so for longer.  us, cut / alone, 64
     // heads on 8 KV heads ("to n": rows of 50 to n tokens):
@@ -106,6 +105,9 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     const int most_alone = f32 ? (full ? 576 : 288) : d.nb > 1 ? (full ? 2304 : half ? 1152 : 832) : codes ? (full ? 3456 : half ? 2304 : 1536) : full ? 2304 : 1152;
     if (d.units > kPagedMaxUnits || keys <= most_alone) return d;
     d.alone = kPagedWaves;
+    // Shares of 128 keys where each can have a compute unit, us with 256 / 128: 1 x 2049 tokens 9.2 / 8.4, 1 x 3500 9.3 / 8.8, 8 x 2500 on one KV head 9.6 / 8.9, four queries on 1 x 2049 10.6 / 9.8, in
+    // e4m3 10.2 / 9.7, but 1 x 4097 9.5 / 10.0, 2 x 3000 10.1 / 10.4; in 32 bits, where a tile takes longer, 1 x 2049 11.8 / 10.6, 2 x 4097 16.9 / 15.3 and 2 x 2049 12.2 / 13.4.
+    d.min_keys = f32 || wgs * ((keys + 127) / 128) <= 256 ? 128 : 256;
     // As many workgroups as a 256-CU part holds at a time: they start and end together.  A unit's last share is half of one on average; at
     // least half of the workgroups are shares all the same, so that a long row among many is cut.  No more than the units can have.  us with half as many,
     // as many, twice as many: 16 x 8192 tokens 46.3 / 47.5 / 50.1, 64 x 3540 73.9 / 77.4 / 80.3, but 64 rows of 150 to 16384 103 / 81.6 / 83.5, 32 of 6000 to
