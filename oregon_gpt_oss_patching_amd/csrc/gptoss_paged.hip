@@ -141,10 +141,10 @@ int attend(const PagedDivision &d, void *stream, PagedArgs &a) {
     a.across = d.across;
     const int s = launch(attn_paged_kernel<T, ST, NB, kPagedWaves>, (a.across ? (slots + 7) / 8 * 8 : slots) * a.G, 64 * kPagedWaves, stream, a);
     if (s || !d.shares) return s;
-    // A wavefront adds eight shares at a time; four of them for each row where a unit has more than twice that (us: 1 x 65536 tokens 32.7 / 28.7,
-    // 4 x 8193 19.8 / 19.0; 16 x 8192, eight shares a unit, 47.3 / 47.9, five queries on eight rows 19.3 / 21.9).
+    // A wavefront adds eight shares at a time; four of them for each row where a unit has more than that and rows are few, or more than twice that (us: 1 x 65536
+    // tokens 32.7 / 28.7, 1 x 1300 8.6 / 8.3, 8 of 700 to 6000 15.3 / 15.0; with eight shares a unit 16 x 8192 47.3 / 47.9, five queries on those eight rows 19.3 / 21.9).
     const int64_t heads = (int64_t)a.B * a.G, pairs = (int64_t)a.Sq * a.r;
-    const bool many = d.shares > 16 * d.units;
+    const bool many = d.shares > (heads * pairs <= 512 ? 8 : 16) * d.units;
     const int64_t wgs = many ? pairs : (pairs + 3) / 4;
     a.by_wgs = div_by(wgs);
     return many ? launch(attn_paged_combine_kernel<T, NB, 4>, heads * wgs, 256, stream, a) : launch(attn_paged_combine_kernel<T, NB, 1>, heads * wgs, 256, stream, a);
