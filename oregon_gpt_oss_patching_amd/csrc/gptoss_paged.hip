@@ -105,9 +105,11 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     const int most_alone = f32 ? (full ? 576 : 288) : d.nb > 1 ? (full ? 2304 : half ? 1152 : 832) : codes ? (full ? 3456 : half ? 2304 : 1536) : full ? 2304 : 1152;
     if (d.units > kPagedMaxUnits || keys <= most_alone) return d;
     d.alone = kPagedWaves;
-    // Shares of 128 keys where each can have a compute unit, us with 256 / 128: 1 x 2049 tokens 9.2 / 8.4, 1 x 3500 9.3 / 8.8, 8 x 2500 on one KV head 9.6 / 8.9, four queries on 1 x 2049 10.6 / 9.8, in
-    // e4m3 10.2 / 9.7, but 1 x 4097 9.5 / 10.0, 2 x 3000 10.1 / 10.4; in 32 bits, where a tile takes longer, 1 x 2049 11.8 / 10.6, 2 x 4097 16.9 / 15.3 and 2 x 2049 12.2 / 13.4.
-    d.min_keys = f32 || wgs * ((keys + 127) / 128) <= 256 ? 128 : 256;
+    // Shares of 128 keys where each can have a compute unit, of up to 384 where not: two and three tiles of a wavefront.  us with 128 / 256 / 384: 1 x 2049 tokens 8.4 / 9.2 / -, 1 x
+    // 5000 10.3 / 9.5 / 10.0, 1 x 10000 - / 11.4 / 10.5, 2 x 4000 - / 10.1 / 10.3, 4 of 700 to 6000 - / 11.8 / 11.0, under four queries - / 14.8 / 12.7, 8 of 50 to 2000 - / 9.7 / 10.1; in
+    // 32 bits 1 x 2049 10.6 / 11.8 / -, 1 x 5000 14.0 / 12.2 / 13.7, 2 x 4000 14.6 / 12.8 / 13.5, 1 x 10000 16.3 / 17.3 / -, 8 to 2000 13.8 / 12.2 / 13.2: up to 256.
+    const int64_t per_unit = (wgs * ((keys + 127) / 128) + 255) / 256, most_per_unit = f32 ? 2 : 3;
+    d.min_keys = 128 * (int)(per_unit < most_per_unit ? per_unit : most_per_unit);
     // As many workgroups as a 256-CU part holds at a time: they start and end together.  A unit's last share is half of one on average; at
     // least half of the workgroups are shares all the same, so that a long row among many is cut.  No more than the units can have.  us with half as many,
     // as many, twice as many: 16 x 8192 tokens 46.3 / 47.5 / 50.1, 64 x 3540 73.9 / 77.4 / 80.3, but 64 rows of 150 to 16384 103 / 81.6 / 83.5, 32 of 6000 to
