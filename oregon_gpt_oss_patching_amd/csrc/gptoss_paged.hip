@@ -110,10 +110,11 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     // 32 bits 1 x 2049 10.6 / 11.8 / -, 1 x 5000 14.0 / 12.2 / 13.7, 2 x 4000 14.6 / 12.8 / 13.5, 1 x 10000 16.3 / 17.3 / -, 8 to 2000 13.8 / 12.2 / 13.2: up to 256.
     const int64_t per_unit = (wgs * ((keys + 127) / 128) + 255) / 256, most_per_unit = f32 ? 2 : 3;
     d.min_keys = 128 * (int)(per_unit < most_per_unit ? per_unit : most_per_unit);
-    // Several blocks of columns cost the sum as much again each; many rows of them are cut half as often (four, five and eight queries, 384 / 768: 8 rows of 700 to 6000
-    // 16.8 / 15.8, 19.0 / 17.7 and 21.0 / 19.3, 16 of 500 to 6000 23.4 / 21.6, 23.7 / 23.7 and 25.3 / 25.6, 12 of 700 to 6000 21.5 / 20.5, 22.0 / 22.6 and 23.4 / 24.5; fewer keys in all:
-    // 20 rows of up to 6000 on two KV heads, five queries, 13.8 / 15.6).
-    if (d.nb > 1 && !f32 && per_unit >= 12) d.min_keys = 768;
+    // Many rows are cut half as often where they are long, and where several blocks of columns make the sum dear.  us, 384 / 768, one query: 8 rows of 1000 to 12000 20.9 / 19.7, 16 of
+    // 500 to 6000 20.0 / 18.9, in e4m3 17.2 / 15.7, but 12 of 700 to 6000 17.7 / 18.2, 24 of 100 to 2500 13.8 / 15.2; four, five and eight: 8 of 700 to 6000 16.8 / 15.8, 19.0 / 17.7 and 21.0 /
+    // 19.3, 12 of those 21.5 / 20.5, 22.0 / 22.6 and 23.4 / 24.5, 24 of 100 to 2000 15.7 / 15.9, 18.4 / 18.2 and 20.7 / 20.5; fewer keys in all: 20 of up to 6000 on two KV heads, five queries, 13.8 / 15.6.
+    // In 32 bits 8 of 700 to 6000 22.4 / 24.8.
+    if (!f32 && per_unit >= 12 && (d.nb > 1 || keys > 4096)) d.min_keys = 768;
     // As many workgroups as a 256-CU part holds at a time: they start and end together.  A unit's last share is half of one on average; at
     // least half of the workgroups are shares all the same, so that a long row among many is cut.  No more than the units can have.  us with half as many,
     // as many, twice as many: 16 x 8192 tokens 46.3 / 47.5 / 50.1, 64 x 3540 73.9 / 77.4 / 80.3, but 64 rows of 150 to 16384 103 / 81.6 / 83.5, 32 of 6000 to
