@@ -190,6 +190,18 @@ __device__ __forceinline__ bf16x8 take_upper(float (&x)[8]) {
     return as_bf16x8(u);
 }
 
+// Eight weights as two bfloat16 terms each: the upper 16 bits, and what is left, which is less than 2^-7 of the weight and rounded by 2^-8 of itself, so that
+// their sum is off by 2^-15 of the weight at most.  2^-20 of the weight is added to what is left, as 0 times an infinity in V would be NaN, where a weight times
+// infinity is infinity (for weights above 2^-110, as below 2^-126 for a single term).
+__device__ __forceinline__ void split_weights(const float (&x)[8], bf16x8 &hi, bf16x8 &lo) {
+    u32x4 u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = __builtin_amdgcn_perm(__float_as_uint(x[2 * e + 1]), __float_as_uint(x[2 * e]), 0x07060302u);
+    hi = as_bf16x8(u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lo[e] = (bf16)fmaf(x[e], 1.0f + 0x1p-20f, -__uint_as_float(__float_as_uint(x[e]) & 0xffff0000u));
+}
+
 // ---- bfloat16 products -----------------------------------------------------------------------------------------------
 // Of float32 queries over codes too: a code times its power of two is a bfloat16 number, and a float32 number is the sum of three (its 24 bits, eight
 // at a time), so three products of each kind take the place of the fp32 MFMA's, in a fifth of their time: 32 rows of 6000 to 16384 tokens 69 us, and 135 with those.
@@ -336,17 +348,19 @@ struct PagedTile16 {
     __device__ __forceinline__ void product(const f32x4 (&s)[NB][KB]) {
 #pragma unroll
         for (int h = 0; h < KB / 2; ++h) {
-            bf16x8 p[NB][kTerms];
+            // A bfloat16 query's weights go in as two terms: one alone, half a step of bfloat16 of each weight, adds as much to the result's error as
+            // rounding it does (relative, 2-norm: 2.2e-3 in all and not 1.7e-3).  us, one term / two: 16 x 8192 tokens 48.7 / 48.9, in e4m3 30.7 / 31.1, one row of 2049 8.5 / 8.6,
+            // five queries on eight rows of 700 to 6000 17.6 / 18.3; where the arithmetic counts, eight queries on 16 x 8192 in e4m3, 43.0 / 49.5.
+            constexpr int kWeightTerms = kTerms == 1 ? 2 : kTerms;
+            bf16x8 p[NB][kWeightTerms];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = s[nb][2 * h + (e >> 2)][e & 3];
                 if constexpr (kTerms == 1) {
-                    // (one rounding of each weight, half a step of bfloat16: of the size of the rounding of o)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { p[nb][0][e] = (bf16)s[nb][2 * h][e]; p[nb][0][4 + e] = (bf16)s[nb][2 * h + 1][e]; }
+                    split_weights(x, p[nb][0], p[nb][1]);
                 } else {
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = s[nb][2 * h + (e >> 2)][e & 3];
 #pragma unroll
                     for (int t = 0; t < kTerms; ++t) p[nb][t] = take_upper(x);
                 }
@@ -356,11 +370,14 @@ struct PagedTile16 {
                 union { struct { s16x4 a, b; } s; bf16x8 v; } x;
                 x.s.a = lds_load_tr64(tr[d], 32 * h * kRowBytes);
                 x.s.b = lds_load_tr64(tr[d], (32 * h + 16) * kRowBytes);
+                if constexpr (kTerms == 1) {
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    if constexpr (kTerms == 1) {
-                        o[nb][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb][0], o[nb][d], 0, 0, 0);
-                    } else {
+                    for (int t = kWeightTerms - 1; t >= 0; --t)
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) o[nb][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb][t], o[nb][d], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
                         f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                         for (int t = kTerms - 1; t >= 0; --t) z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb][t], z, 0, 0, 0);
