@@ -86,8 +86,24 @@ __device__ __forceinline__ int wave_scan(int x) {
     return x;
 }
 
-// Which share of which unit a workgroup takes.  All units' tiles are cut into shares of `chunk`, the smallest length of at least
-// a.min_tiles with which they number no more than a.shares and one for each unit, which is what the grid and the scratch hold.
+// The sum of the lanes' numbers, each at most 2^30 / KEYS: 64 times 2^26 (tiles of 16 keys) does not fit 32 bits.
+template <int KEYS>
+__device__ __forceinline__ uint64_t wave_total(int x) {
+    if constexpr (KEYS >= 32) return (uint32_t)__builtin_amdgcn_readlane(wave_scan(x), 63);
+    const uint32_t lo = __builtin_amdgcn_readlane(wave_scan(x & 0xffff), 63), hi = __builtin_amdgcn_readlane(wave_scan(x >> 16), 63);
+    return ((uint64_t)hi << 16) + lo;
+}
+
+// Length of the shares that `tiles` are cut into: the smallest of at least `least` with which units that have so many in all have no more than `shares`, and
+// one for each unit, which is what the grid and the scratch hold.
+__host__ __device__ __forceinline__ int paged_chunk(uint64_t tiles, int shares, int least) {
+    const uint64_t up = tiles + (uint32_t)shares - 1u;
+    const uint64_t even = up >> 32 ? up / (uint32_t)shares : (uint32_t)up / (uint32_t)shares;     // (32 bits: a quotient in a tenth of the instructions)
+    const int chunk = even < (1u << 30) ? (int)even : 1 << 30;                                    // (more tiles than a unit can have)
+    return chunk > least ? chunk : least;
+}
+
+// Which share of which unit a workgroup takes.
 struct PagedShare { int unit, index, count, first; };     // first: number of the unit's first share; unit < 0: nothing left
 template <int PAIRS, int KEYS>
 __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int slot, PagedSpan &sp) {
@@ -108,20 +124,12 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int slot, 
     };
     int n, base;
     const int tiles0 = mine(lane, n, base);
-    const int sum0 = __builtin_amdgcn_readlane(wave_scan(tiles0), 63);      // (as unsigned: at most 2^25 tiles each)
-    int chunk;
-    if (a.units <= 64) {
-        chunk = (int)(((uint32_t)sum0 + (uint32_t)a.shares - 1u) / (uint32_t)a.shares);
-    } else {
-        int64_t all = (uint32_t)sum0;
-        for (int u0 = 64; u0 < a.units; u0 += 64) {
-            int x, y;
-            all += (uint32_t)__builtin_amdgcn_readlane(wave_scan(mine(u0 + lane, x, y)), 63);
-        }
-        const int64_t even = (all + a.shares - 1) / a.shares;
-        chunk = (int)(even < (1 << 30) ? even : (1 << 30));                 // (more tiles than a unit can have)
+    uint64_t all = wave_total<KEYS>(tiles0);
+    for (int u0 = 64; u0 < a.units; u0 += 64) {
+        int x, y;
+        all += wave_total<KEYS>(mine(u0 + lane, x, y));
     }
-    chunk = max(a.min_tiles, chunk);
+    const int chunk = paged_chunk(all, a.shares, a.min_tiles);
     int before = 0;
     for (int u0 = 0; u0 < a.units; u0 += 64) {
         const int tiles = u0 ? mine(u0 + lane, n, base) : tiles0;

@@ -1,0 +1,59 @@
+"""Host check of how attention over pages divides its work (csrc/attn_paged.h, compiled here for the CPU): whatever the rows' lengths, the shares are no more than the
+grid and the scratch hold."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PROGRAM = r"""
+#include "%s"
+#include <cstdio>
+using namespace gptoss;
+int main() {
+    unsigned long long units, tiles, n = 0;
+    int shares, least;
+    // one line: units, tiles of each, shares, least -> chunk
+    while (std::scanf("%%llu %%llu %%d %%d", &units, &tiles, &shares, &least) == 4) {
+        std::printf("%%d\n", paged_chunk(units * tiles, shares, least));
+        ++n;
+    }
+    return n == 0;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def chunks(tmp_path_factory):
+    """paged_chunk of rows (units, tiles of each, shares, least)."""
+    hipcc = os.environ.get("HIPCC") or shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("hipcc not found")
+    folder = tmp_path_factory.mktemp("division")
+    source, program = folder / "unit.hip", folder / "unit"
+    source.write_text(PROGRAM % os.path.join(ROOT, "oregon_gpt_oss_patching_amd", "csrc", "attn_paged.h"))
+    proc = subprocess.run([hipcc, "-std=c++17", "-O1", "--offload-arch=gfx950", "--offload-host-only", "-o", str(program), str(source)], capture_output=True, text=True)
+    assert proc.returncode == 0, proc.stderr[-2000:]
+
+    def run(rows):
+        out = subprocess.run([str(program)], input="\n".join(" ".join(map(str, r)) for r in rows), capture_output=True, text=True, timeout=60)
+        assert out.returncode == 0, out.stderr
+        return [int(x) for x in out.stdout.split()]
+
+    return run
+
+
+def test_shares_fit_the_grid(chunks):
+    """Rows of up to 2^30 tokens in tiles of 16, 32 and 64 keys, up to 1024 of them: the shares are no more than `shares` and one for each unit.  64 rows of 2^26 tiles are
+    2^32 in all."""
+    rows = [(units, tiles, shares, least)
+            for units in (1, 2, 63, 64, 65, 1000, 1024)
+            for tiles in (0, 1, 2, 7, 8, 9, 1000, 2 ** 20 - 1, 2 ** 24, 2 ** 25, 2 ** 26 - 8, 2 ** 26 - 1, 2 ** 26)
+            for shares in (1, 2, 96, 100, 1023, 1024)
+            for least in (2, 4, 8, 24, 48)]
+    for (units, tiles, shares, least), chunk in zip(rows, chunks(rows)):
+        assert chunk >= least
+        assert units * max(1, -(-tiles // chunk)) <= shares + units, (units, tiles, shares, least, chunk)
+        assert chunk == least or units * tiles > (chunk - 1) * shares, (units, tiles, shares, least, chunk)      # (no longer than need be)
