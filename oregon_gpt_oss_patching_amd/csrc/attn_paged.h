@@ -556,7 +556,7 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
     const int pairs = min(a.Sq * a.r - sp.pair0, kPairs);
 
     const int32_t *table = a.table + sp.b * a.table_stride;
-    const int in_page = (1 << a.page_shift) - 1, weff = a.window ? a.window : 0x3fffffff;
+    const int in_page = (1 << a.page_shift) - 1, weff = a.window ? a.window : 1 << 30;
     int entry[KB];                           // pages of the wavefront's next 64 tiles, one a lane, for each 16 keys of a tile
     auto entries = [&](int j) __attribute__((always_inline)) {
         const int n0 = (t_lo + w + NW * (j + lane)) * kKeys;
