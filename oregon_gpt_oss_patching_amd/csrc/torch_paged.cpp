@@ -41,9 +41,12 @@ struct PagedCall {
     Tensor table, seqlens, start, sinks, q, k, v, scratch;
 };
 
-// As int32 on the cache's GPU; what is so already does not go through the dispatcher (half a microsecond each).
+// As int32 on the cache's GPU; what is so already does not go through the dispatcher (half a microsecond each).  Wider numbers that int32 does not hold become its
+// ends, which are no page, in front of every position and behind each (cut off, 2^32 + 3 would be page 3).
 Tensor int32_on(const Tensor &t, const Tensor &pages) {
-    return t.scalar_type() == at::kInt && t.device() == pages.device() ? t : t.to(pages.device(), at::kInt);
+    if (t.scalar_type() == at::kInt && t.device() == pages.device()) return t;
+    const bool wide = t.scalar_type() == at::kLong || t.scalar_type() == at::kUInt32 || t.scalar_type() == at::kUInt64;
+    return (wide ? t.to(at::kLong).clamp(INT_MIN, INT_MAX) : t).to(pages.device(), at::kInt);
 }
 
 Tensor lengths_of(const Tensor &t, const Tensor &pages, int64_t batch, const char *name) {
