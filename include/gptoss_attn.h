@@ -327,7 +327,8 @@ int gptoss_attn_validate(const gptoss_attn_params *params, int need_bwd);
  * The serving side of the same layer; the reference has no counterpart (its generate.py leaves the cache to transformers,
  * one contiguous tensor per layer).  Keys and values of all sequences live in one pool of pages:
  *   k_pages, v_pages (pages, G, page_size, 64) in `storage`: the model's type (`dtype`), or GPTOSS_ATTN_E4M3
- *   k_exp, v_exp     (pages, G, page_size) bytes, E4M3 only: row values are code * 2^(byte - 127)
+ *   k_exp, v_exp     (pages, G, page_size) bytes, E4M3 only: row values are code * 2^(byte - 127), infinite from 2^128 on; NaN
+ *                    where the byte is 255
  *   page_table       (B, table_width) int32, rows table_stride apart: token t of row b is slot t % page_size of page
  *                    page_table[b][t / page_size].  An entry outside 0 .. pages - 1 names no page: what would be written
  *                    there is dropped, what would be read from there is 0, its keys are invisible.

@@ -32,7 +32,7 @@ __all__ = ["PagedCache", "PagedState", "paged_cache", "paged_cache_write", "page
 class PagedCache(NamedTuple):
     """k, v: (pages, G, page_size, 64), bfloat16, float32 or float8_e4m3fn, page_size a power of two from 16 to 1024; rows of 64 must be
     contiguous and start on 16-byte boundaries, the other strides are free.  k_exp, v_exp: float8_e4m3fn only, (pages, G, page_size)
-    uint8, a row's values are its numbers times 2^(byte - 127)."""
+    uint8, a row's values are its numbers times 2^(byte - 127), NaN where the byte is 255."""
     k: torch.Tensor
     v: torch.Tensor
     k_exp: Optional[torch.Tensor] = None
