@@ -327,15 +327,31 @@ struct PagedTile16 {
                     const bool in = r >= first && r < last && (there >> blk & 1);
                     if constexpr (kCodes) ve[blk] = in ? ve[blk] : (uint32_t)kExpBias;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t x = in ? v[blk][i][e] : 0u, bad;
-                        if constexpr (kCodes) bad = ((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;      // 0x7f, 0xff: NaN
-                        else bad = ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
-                        if (!several) bad = 0u;
-                        odd = odd || bad != 0u;
-                        v[blk][i][e] = x & ~bad;
-                    }
+                    for (int e = 0; e < 4; ++e) v[blk][i][e] = in ? v[blk][i][e] : 0u;
                 }
+            if (several) {
+#pragma unroll
+                for (int blk = 0; blk < KB; ++blk) {
+                    // Added to the magnitudes of codes, what carries those that are not finite into the sign's bit: NaN, 0x7f; under 2^120 and more what comes to 2^128, from 0x78
+                    // down by 8 for each power; under the byte 255 all of them.
+                    uint32_t carry = 0x01010101u;
+                    if constexpr (kCodes) {
+                        carry = ve[blk] < 247u ? carry : ve[blk] == 255u ? 0x80808080u : 0x08080808u * (ve[blk] - 246u);
+                        ve[blk] = ve[blk] == 255u ? (uint32_t)kExpBias : ve[blk];
+                    }
+#pragma unroll
+                    for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t x = v[blk][i][e];
+                            uint32_t bad;
+                            if constexpr (kCodes) bad = ((((x & 0x7f7f7f7fu) + carry) & 0x80808080u) >> 7) * 0xffu;
+                            else bad = ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+                            odd = odd || bad != 0u;
+                            v[blk][i][e] = x & ~bad;
+                        }
+                }
+            }
         }
 #pragma unroll
         for (int blk = 0; blk < KB; ++blk)
@@ -700,11 +716,14 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
                 const int page = paged_page(a, sp.b, key);
                 if (page < 0) continue;
                 const char *row = v_base + a.vp.at(page, key & in_page);
+                uint32_t power = 0;
+                if constexpr (Tile::kCodes) power = (uint8_t)ve_base[a.ve.at(page, key & in_page)];
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float x = stored_number(reinterpret_cast<const ST *>(row) + Tile::column(d, e, quad));
+                        float x = stored_number(reinterpret_cast<const ST *>(row) + Tile::column(d, e, quad));
+                        if constexpr (Tile::kCodes) x = times_exp(x, power);
                         if ((__float_as_uint(x) & 0x7f800000u) != 0x7f800000u) continue;
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb)

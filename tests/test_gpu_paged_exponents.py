@@ -58,3 +58,30 @@ def test_attention_under_small_and_large_powers(A, dtype, byte, n):  # noqa: F81
     tol = tol - 1e-37 + 2.0 ** -133 + (n + 64) * 2.0 ** -149
     assert float(ref.abs().max()) > 10 * float(tol.max())
     assert bool(((o.cpu().double() - ref).abs() <= tol).all()) and bool(((lse.cpu().double() - ref_lse).abs() <= tol_lse).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("byte,code", [(255, 0x38), (255, 0), (254, 0x38), (254, 0x48), (248, 0x7e), (247, 0x78), (247, 0x7f)])
+@pytest.mark.parametrize("heads", [1, 8, 16])
+def test_values_that_only_a_later_query_sees(A, dtype, byte, code, heads):  # noqa: F811
+    """A row of V that is infinite or NaN by its byte: queries that do not see it are as if it were not there."""
+    gen = torch.Generator().manual_seed(77)
+    n, sq = 60, 4
+    k, v = ((torch.randn(n, 64, generator=gen) * 60).to(E4M3) for _ in range(2))
+    exps = torch.full((n,), 120, dtype=torch.uint8)
+    q = torch.randn(1, heads, sq, 64, generator=gen).to(dtype).to(DEV)
+    clean, table = cache_of(A, k, exps, v, exps)
+    want = A.paged_attention(q, clean, table, [n], None, SCALE)
+    bad, bad_exps = v.view(torch.uint8).clone(), exps.clone()
+    bad[58], bad_exps[58] = 0x30, byte
+    bad[58, 5:9] = code
+    broken, _ = cache_of(A, k, exps, bad.view(E4M3), bad_exps)
+    value = rows(bad.view(E4M3), bad_exps)[58]
+    o = A.paged_attention(q, broken, table, [n], None, SCALE)
+    # queries at 56, 57, 58, 59: the first two do not see the row
+    assert torch.equal(o[:, :2], want[:, :2])
+    for i in range(2, sq):
+        for d in range(64):
+            if not torch.isfinite(value[d]):
+                x = o[0, i, :, d].float().cpu()
+                assert bool(torch.isnan(x).all()) if torch.isnan(value[d]) else bool((x == float(value[d])).all()), (i, d)
