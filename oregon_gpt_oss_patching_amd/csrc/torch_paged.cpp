@@ -224,16 +224,20 @@ std::tuple<Tensor, Tensor> paged_fwd(const Tensor &q, const Tensor &k_pages, con
 
 using Pair = std::tuple<Tensor, Tensor>;
 
-// A gradient of either mode (most tensors have no record of any).
-bool wants_gradient(const Tensor &t) { return t.unsafeGetTensorImpl()->autograd_meta() && (t.requires_grad() || t._fw_grad(0).defined()); }
+// What a tensor asks for (most have no record of either): a gradient, which torch.no_grad() takes back, or the tangent of forward mode, which it does not.
+bool wants_gradient(const Tensor &t) { return t.unsafeGetTensorImpl()->autograd_meta() && t.requires_grad(); }
+bool has_tangent(const Tensor &t) { return t.unsafeGetTensorImpl()->autograd_meta() && t._fw_grad(0).defined(); }
 
-// Tensors that want a gradient are refused, as these calls would drop it without a word.
+// Tensors with either are refused, as these calls would drop it without a word.
 void refuse_gradients(const c10::OperatorHandle &op, c10::DispatchKeySet keys, torch::jit::Stack *stack) {
-    if (at::GradMode::is_enabled()) {
-        const size_t n = op.schema().arguments().size();
-        for (size_t i = stack->size() - n; i < stack->size(); ++i)
-            TORCH_CHECK(!(*stack)[i].isTensor() || !wants_gradient((*stack)[i].toTensor()), op.schema().name(),
-                        " has no gradient: call it under torch.no_grad() (argument ", op.schema().arguments()[i + n - stack->size()].name(), " requires one)");
+    const size_t n = op.schema().arguments().size();
+    for (size_t i = stack->size() - n; i < stack->size(); ++i) {
+        if (!(*stack)[i].isTensor()) continue;
+        const Tensor &t = (*stack)[i].toTensor();
+        TORCH_CHECK(!at::GradMode::is_enabled() || !wants_gradient(t), op.schema().name(), " has no gradient: call it under torch.no_grad() (argument ",
+                    op.schema().arguments()[i + n - stack->size()].name(), " requires one)");
+        TORCH_CHECK(!has_tangent(t), op.schema().name(), " has no gradient, forward mode's neither: argument ", op.schema().arguments()[i + n - stack->size()].name(),
+                    " has a tangent");
     }
     const at::AutoDispatchBelowADInplaceOrView below;
     op.redispatchBoxed(keys & c10::after_ADInplaceOrView_keyset, stack);
@@ -296,7 +300,7 @@ struct Arguments {
                                                  c10::getAutogradRelatedKeySetFromBackend(c10::BackendComponent::CUDABit);
         if (!THPVariable_CheckExact(args[i])) return ok = false, none;
         const Tensor &t = THPVariable_Unpack(args[i]);
-        if ((t.key_set().raw_repr() & ~plain.raw_repr()) != 0 || (grad && wants_gradient(t))) ok = false;
+        if ((t.key_set().raw_repr() & ~plain.raw_repr()) != 0 || (grad && wants_gradient(t)) || has_tangent(t)) ok = false;
         return t;
     }
     OptTensor optional(int i) { return args[i] == Py_None ? OptTensor() : OptTensor(tensor(i)); }

@@ -1,0 +1,26 @@
+"""GPU tests of what the calls of the cache in pages refuse where they go past the dispatcher."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from test_gpu_paged import BF16, DEV, SCALE, A  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents(A, grad):  # noqa: F811
+    """A forward-mode tangent is refused under torch.no_grad() too, and nothing is written; without one the same tensors pass."""
+    cache, table, n = A.paged_cache(4, 2, 16), torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    q, k = torch.ones(1, 16, 1, 64, dtype=BF16, device=DEV), torch.ones(1, 2, 1, 64, dtype=BF16, device=DEV)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        for call in (lambda d: A.paged_attention(d(q), cache, table, n, None, SCALE),
+                     lambda d: A.paged_attention_forward(q, cache, table, n, d(torch.zeros(16, device=DEV)), SCALE),
+                     lambda d: A.paged_cache_write(cache, k, d(k), table, n - 1),
+                     lambda d: A.paged_cache_read(A.PagedCache(cache.k, d(cache.v)), table, n, 4)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+            assert not cache.k.any()
+        for call in (lambda d: A.paged_attention(d(q), cache, table, n, None, SCALE), lambda d: A.paged_cache_write(cache, d(k), d(k), table, n - 1)):
+            call(lambda t: forward_ad.unpack_dual(forward_ad.make_dual(t, torch.ones_like(t))).primal)
+        assert bool((cache.k[0, :, 0] == 1).all())
