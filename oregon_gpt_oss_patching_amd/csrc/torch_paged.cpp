@@ -137,9 +137,10 @@ void paged_write(const Tensor &k_pages, const Tensor &v_pages, const OptTensor &
         c.seqlens = lengths_of(*seqlens, k_pages, c.p.B, "seqlens");
         c.p.seqlens = c.seqlens.const_data_ptr<int32_t>();
     }
-    check("gptoss_attn_paged_write", gptoss_attn_paged_write(&c.p, stream_of(k_pages)));
+    // (this refuses a cache that was made in inference mode and is written outside of it: before the launch, not after)
     for (const Tensor *t : {&k_pages, &v_pages, k_exp ? &*k_exp : nullptr, v_exp ? &*v_exp : nullptr})
         if (t) t->unsafeGetTensorImpl()->bump_version();
+    check("gptoss_attn_paged_write", gptoss_attn_paged_write(&c.p, stream_of(k_pages)));
 }
 
 std::tuple<Tensor, Tensor> paged_read(const Tensor &k_pages, const Tensor &v_pages, const OptTensor &k_exp, const OptTensor &v_exp, const Tensor &page_table,
