@@ -56,6 +56,8 @@ class PagedState(NamedTuple):
 
     def attend(self, module, q, k, v, sm_scale) -> torch.Tensor:
         """A layer's new keys and values into its cache, and its queries' attention."""
+        if k.shape[2] != q.shape[2]:
+            raise RuntimeError(f"paged= writes the new tokens' keys, as many as queries, got {k.shape[2]} for {q.shape[2]}: the pages hold the past, pass no past_key_values")
         cache, window = self.caches[module.layer_idx], module.sliding_window
         if self.start is None:
             n = _ints(self.seqlens, q)
