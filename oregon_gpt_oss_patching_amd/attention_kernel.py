@@ -312,6 +312,11 @@ class _attention:
     apply = staticmethod(attention)
 
 
+def _is_lengths(attention_mask) -> bool:
+    """Valid lengths handed over in place of the dense mask (see sft_bench.mask_free_attention_mask)."""
+    return torch.is_tensor(attention_mask) and attention_mask.dim() == 1 and not attention_mask.dtype.is_floating_point
+
+
 def hip_flash_attention(
     module,
     query: torch.Tensor,
@@ -337,8 +342,8 @@ def hip_flash_attention(
     stands there."""
     paged = kwargs.get("paged")
     if paged is not None:
-        if kwargs.get("doc_start") is not None or kwargs.get("seqlens") is not None:
-            raise RuntimeError("paged= holds the rows' lengths itself and has no documents: pass neither seqlens nor doc_start")
+        if kwargs.get("doc_start") is not None or kwargs.get("seqlens") is not None or _is_lengths(attention_mask):
+            raise RuntimeError("paged= holds the rows' lengths itself and has no documents: pass neither seqlens nor doc_start, nor lengths as attention_mask")
         return paged.attend(module, query, key, value, scaling), None
     doc_start = kwargs.get("doc_start")
     if doc_start is None and RESPECT_PACKING and kwargs.get("position_ids") is not None:
@@ -346,9 +351,7 @@ def hip_flash_attention(
         if pos.dim() == 2 and pos.shape[0] == query.shape[0] and pos.shape[1] == query.shape[2] == key.shape[2]:
             doc_start = doc_start_from_position_ids(pos)
     seqlens = kwargs.get("seqlens")
-    if (seqlens is None and torch.is_tensor(attention_mask) and attention_mask.dim() == 1
-            and not attention_mask.dtype.is_floating_point):
-        # valid lengths handed over in place of the dense mask (see sft_bench.mask_free_attention_mask)
+    if seqlens is None and _is_lengths(attention_mask):
         seqlens = attention_mask
     out = attention(query, key, value, module.sinks, scaling, module.sliding_window, None, seqlens, doc_start)
     return out, None

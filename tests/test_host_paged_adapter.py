@@ -27,3 +27,18 @@ def test_as_many_keys_as_queries_pass():
     q, k = torch.zeros(1, 16, 3, 64, dtype=torch.bfloat16), torch.zeros(1, 2, 3, 64, dtype=torch.bfloat16)
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
         A.hip_flash_attention(MODULE, q, k, k, None, 0.125, paged=_state(None))
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_lengths_as_a_mask_are_refused(dtype):
+    """Without pages a 1-D attention_mask of integers is the rows' lengths, and seqlens= is refused with them: neither is dropped."""
+    x = torch.zeros(1, 2, 3, 64, dtype=torch.bfloat16)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="lengths as attention_mask"):
+        A.hip_flash_attention(MODULE, x, x, x, torch.full((1,), 2, dtype=dtype), 0.125, paged=_state(None))
+
+
+def test_other_masks_are_ignored_as_without_pages():
+    q, k = torch.zeros(1, 16, 3, 64, dtype=torch.bfloat16), torch.zeros(1, 2, 3, 64, dtype=torch.bfloat16)
+    for mask in (torch.ones(1, 3, dtype=torch.int64), torch.zeros(1, 1, 3, 3), torch.zeros(3)):
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+            A.hip_flash_attention(MODULE, q, k, k, mask, 0.125, paged=_state(None))
