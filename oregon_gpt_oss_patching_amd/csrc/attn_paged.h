@@ -4,9 +4,10 @@
 //
 // Work.  The Sq * r (query, head of the group) pairs of a KV head are the columns of S^T, up to 16 NB of them to a workgroup (a unit), so that
 // K and V are read once.  The host does not see the lengths: a fixed number of workgroups finds, from all lengths, how long equal shares of
-// all units' 32-key tiles are and which share is its own (PagedShare); a unit with one share writes its results, the others leave fp32
+// all units' tiles (of 16, 32 or 64 keys) are and which share is its own (PagedShare); a unit with one share writes its results, the others leave fp32
 // partials that attn_paged_combine_kernel adds in the order of the shares.  So one long row among many short ones is spread over the chip,
-// and a table that is wider than the rows costs nothing.
+// and rows are divided alike in a table that fits them and in a wider one (but for the shortest, which the host sends to a workgroup each where the table says that they are:
+// gptoss_paged.hip).
 //
 // In a workgroup four wavefronts take tiles in turn, each for itself (no barrier in the loop), and merge their (m, l, O) at the end.
 //  * Loads take whole cache lines.  The MFMA's A operand wants a lane to hold pieces of one key's row, 16 rows of 64 bytes to a load: codes come so,
@@ -103,6 +104,23 @@ __host__ __device__ __forceinline__ int paged_chunk(uint64_t tiles, int shares, 
     return chunk > least ? chunk : least;
 }
 
+// The least length of a share, in 128 keys, from how many workgroups (shares of all units for all KV heads) there are with shares of one, two, three and six times that,
+// for 256 compute units: 128, 256 or 384 keys, the first with which each workgroup has a compute unit to itself; where none has, 768 if that fills the compute units evenly,
+// four fifths of whole rounds, and 384 if not.  us at 128 / 256 / 384 / 768, workgroups in brackets:
+//   1 x 2049 tokens 8.8 [136] / 9.2 / 9.8 / -, 1 x 5000 10.6 [320] / 9.6 [160] / 10.3 / -, 2 x 4000 11.5 / 10.1 [256] / 10.8 / 12.3, 1 x 10000 13.1 / 12.0 [320] / 10.7 [216] / 12.3, in
+//   32 bits 16.6 / 17.7 / 14.9 / 18.5, 20 of 100 to 6000 on two KV heads, five queries, 17.6 / 15.6 [258] / 14.7 [180] / 17.0;
+//   8 of 700 to 6000 - / 14.9 / 14.5 [464] / 14.4 [248], under five queries - / 20.3 / 20.0 / 18.7, in 32 bits - / 23.1 / 22.6 / 22.3, 16 of 500 to 6000 20.4 [824] / 19.1 [440], in e4m3
+//   17.7 / 16.0, 32 of 100 to 3000 17.4 [712] / 17.0 [440];
+//   but 24 of 100 to 2500 14.2 [480] / 15.2 [304], 4 x 8193 17.9 [704] / 18.9 [352], 12 of 700 to 6000 under five queries 22.7 [512] / 24.0 [360], under eight 24.8 / 26.5.
+__host__ __device__ __forceinline__ int paged_least(int of1, int of2, int of3, int of6) {
+    constexpr int kUnits = 256;
+    if (of1 <= kUnits) return 1;
+    if (of2 <= kUnits) return 2;
+    if (of3 <= kUnits) return 3;
+    const int rounds = (of6 + kUnits - 1) / kUnits;
+    return (int64_t)5 * of6 >= (int64_t)4 * kUnits * rounds ? 6 : 3;
+}
+
 // Which share of which unit a workgroup takes.
 struct PagedShare { int unit, index, count, first; };     // first: number of the unit's first share; unit < 0: nothing left
 template <int PAIRS, int KEYS>
@@ -125,11 +143,23 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int slot, 
     int n, base;
     const int tiles0 = mine(lane, n, base);
     uint64_t all = wave_total<KEYS>(tiles0);
+    // numbers of shares of n times 128 keys, two at a time in 16 bits (which they fit wherever they are used: at most six times a.shares, and one for each unit)
+    constexpr int k128 = 128 / KEYS;
+    auto numbers = [&](int u, int tiles, int n, int m) __attribute__((always_inline)) {
+        const int x = max(1, (tiles + n * k128 - 1) / (n * k128)), y = max(1, (tiles + m * k128 - 1) / (m * k128));
+        return __builtin_amdgcn_readlane(wave_scan(u < a.units ? x + (y << 16) : 0), 63);
+    };
+    uint32_t of12 = numbers(lane, tiles0, 1, 2), of36 = numbers(lane, tiles0, 3, 6);
     for (int u0 = 64; u0 < a.units; u0 += 64) {
         int x, y;
-        all += wave_total<KEYS>(mine(u0 + lane, x, y));
+        const int tiles = mine(u0 + lane, x, y);
+        all += wave_total<KEYS>(tiles);
+        of12 += numbers(u0 + lane, tiles, 1, 2);
+        of36 += numbers(u0 + lane, tiles, 3, 6);
     }
-    const int chunk = paged_chunk(all, a.shares, a.min_tiles);
+    int chunk = paged_chunk(all, a.shares, 1);
+    if (chunk < 6 * k128)
+        chunk = max(chunk, k128 * paged_least((of12 & 0xffff) * a.G, (of12 >> 16) * a.G, (of36 & 0xffff) * a.G, (of36 >> 16) * a.G));
     int before = 0;
     for (int u0 = 0; u0 < a.units; u0 += 64) {
         const int tiles = u0 ? mine(u0 + lane, n, base) : tiles0;

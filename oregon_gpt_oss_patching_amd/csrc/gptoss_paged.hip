@@ -68,9 +68,9 @@ int launch(Kernel kernel, int64_t workgroups, int threads, void *stream, const P
 }
 
 // How the attention's work is divided: column blocks of 16 pairs, blocks of pairs of a row, (row, block) units, shares of all units'
-// tiles for each KV head beside one for each unit (0: units stay whole, each walked by `alone` wavefronts), keys that a share has at least, and
-// the scratch that takes; `across`: a slot's KV heads on one XCD.
-struct PagedDivision { int nb, blocks, shares, alone, min_keys; bool across; int64_t units; size_t plan_bytes, bytes; };
+// tiles for each KV head that there are at most beside one for each unit (0: units stay whole, each walked by `alone` wavefronts), how many are to be expected, and
+// the scratch that takes; `across`: a slot's KV heads on one XCD.  How long shares are is the kernel's to find, from the lengths (PagedShare).
+struct PagedDivision { int nb, blocks, shares, usual, alone; bool across; int64_t units; size_t plan_bytes, bytes; };
 
 // Workgroups of four wavefronts that a compute unit runs at a time.
 template <typename T, typename ST, int NB> constexpr int per_simd() { return paged_occupancy<T, ST, NB, kPagedWaves>(); }
@@ -90,7 +90,8 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     const int64_t queries = (16 * d.nb - 1) / r + 2;                   // that a unit's pairs touch
     if (p->window > 0 && p->window + queries < keys) keys = p->window + queries;
     // Short rows: a workgroup walks a unit alone, as many wavefronts as its keys and the compute unit's share of the workgroups have room for, and
-    // there is nothing to add in a second launch.  Rows of few bytes, and workgroups that fill the chip by themselves, do so for longer.  us, cut / alone, 64
+    // there is nothing to add in a second launch.  What counts is what the host knows of the lengths: in a table far wider than the rows, without max_len, these are cut too, 32 x 1000
+    // tokens 18.7 and not 15.3, with four queries 23.1 / 15.7, 32 x 2000 in codes 21.8 / 16.0.  Rows of few bytes, and workgroups that fill the chip by themselves, go alone for longer.  us, cut / alone, 64
     // heads on 8 KV heads ("to n": rows of 50 to n tokens):
     //   bfloat16: 1 x 1025 tokens 9.1 / 8.0, but 1 x 1500 9.0 / 11.9; 32 x 1000 18.4 / 14.6, 16 to 1100 10.0 / 10.4, 32 to 2000 14.3 / 16.1; more than a workgroup to a
     //   compute unit: 64 x 2000 48.1 / 43.4, 64 to 2500 22.0 / 22.3, 40 to 3500 19.8 / 23.3
@@ -105,28 +106,21 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     const int most_alone = f32 ? (full ? 576 : 288) : d.nb > 1 ? (full ? 2304 : half ? 1152 : 832) : codes ? (full ? 3456 : half ? 2304 : 1536) : full ? 2304 : 1152;
     if (d.units > kPagedMaxUnits || keys <= most_alone) return d;
     d.alone = kPagedWaves;
-    // Shares of 128 keys where each can have a compute unit, of up to 384 where not: two and three tiles of a wavefront.  us with 128 / 256 / 384: 1 x 2049 tokens 8.4 / 9.2 / -, 1 x
-    // 5000 10.3 / 9.5 / 10.0, 1 x 10000 - / 11.4 / 10.5, 2 x 4000 - / 10.1 / 10.3, 4 of 700 to 6000 - / 11.8 / 11.0, under four queries - / 14.8 / 12.7, 8 of 50 to 2000 - / 9.7 / 10.1; in
-    // 32 bits 1 x 2049 10.6 / 11.8 / -, 1 x 5000 14.0 / 12.2 / 13.7, 2 x 4000 14.6 / 12.8 / 13.5, 1 x 10000 16.3 / 17.3 / -, 8 to 2000 13.8 / 12.2 / 13.2: up to 256.
-    const int64_t per_unit = (wgs * ((keys + 127) / 128) + 255) / 256, most_per_unit = f32 ? 2 : 3;
-    d.min_keys = 128 * (int)(per_unit < most_per_unit ? per_unit : most_per_unit);
-    // Many rows are cut half as often where they are long, and where several blocks of columns make the sum dear.  us, 384 / 768, one query: 8 rows of 1000 to 12000 20.9 / 19.7, 16 of
-    // 500 to 6000 20.0 / 18.9, in e4m3 17.2 / 15.7, but 12 of 700 to 6000 17.7 / 18.2, 24 of 100 to 2500 13.8 / 15.2; four, five and eight: 8 of 700 to 6000 16.8 / 15.8, 19.0 / 17.7 and 21.0 /
-    // 19.3, 12 of those 21.5 / 20.5, 22.0 / 22.6 and 23.4 / 24.5, 24 of 100 to 2000 15.7 / 15.9, 18.4 / 18.2 and 20.7 / 20.5; fewer keys in all: 20 of up to 6000 on two KV heads, five queries, 13.8 / 15.6.
-    // In 32 bits 8 of 700 to 6000 22.4 / 24.8.
-    if (!f32 && per_unit >= 12 && (d.nb > 1 || keys > 4096)) d.min_keys = 768;
     // As many workgroups as a 256-CU part holds at a time: they start and end together.  A unit's last share is half of one on average; at
     // least half of the workgroups are shares all the same, so that a long row among many is cut.  No more than the units can have.  us with half as many,
     // as many, twice as many: 16 x 8192 tokens 46.3 / 47.5 / 50.1, 64 x 3540 73.9 / 77.4 / 80.3, but 64 rows of 150 to 16384 103 / 81.6 / 83.5, 32 of 6000 to
     // 16384 137 / 112 / 114, and four queries on each of those in e4m3 44.3 / 33.4 / 41.2.
 #define GPTOSS_HELD(T, NB) (codes ? per_simd<T, e4m3, NB>() : per_simd<T, T, NB>())
-    const int per_cu = p->dtype == GPTOSS_ATTN_FP32 ? (d.nb == 1 ? GPTOSS_HELD(float, 1) : GPTOSS_HELD(float, 2))
+    const int at_a_time = p->dtype == GPTOSS_ATTN_FP32 ? (d.nb == 1 ? GPTOSS_HELD(float, 1) : GPTOSS_HELD(float, 2))
                            : d.nb == 1 ? GPTOSS_HELD(bf16, 1) : d.nb == 2 ? GPTOSS_HELD(bf16, 2) : d.nb == 3 ? GPTOSS_HELD(bf16, 3) : GPTOSS_HELD(bf16, 4);
 #undef GPTOSS_HELD
-    const int64_t held = 256 * per_cu / p->G, left = held - d.units / 2, can = d.units * ((keys + d.min_keys - 1) / d.min_keys);
+    const int64_t held = 256 * at_a_time / p->G, left = held - d.units / 2, can = d.units * ((keys + 127) / 128);
     int64_t shares = left > held / 2 ? left : held / 2;
     if (shares > can) shares = can;
     d.shares = shares > 1 ? (int)shares : 1;
+    // (of rows as long as can be, in shares of 128 to 384 keys)
+    const int64_t per_cu = (wgs * ((keys + 127) / 128) + 255) / 256, least = 128 * (per_cu < 3 ? per_cu : 3), usual = d.units * ((keys + least - 1) / least);
+    d.usual = usual < shares ? (int)usual : d.shares;
     // The exponents of a page's KV heads share cache lines, which the heads' workgroups then read from one L2.  us, heads next to each other / on one
     // XCD, e4m3: 32 rows of 6000 to 16384 tokens 65.4 / 63.5, 24 of 150 to 30000 37.1 / 35.1, 200 of up to 4000 67.5 / 64.1; but 8 of up to 6000 14.5 / 15.4,
     // and in bfloat16 200 rows 102 / 106.
@@ -143,7 +137,6 @@ int attend(const PagedDivision &d, void *stream, PagedArgs &a) {
             if (d.alone == 16) return launch(attn_paged_kernel<T, ST, NB, 16>, d.units * a.G, 1024, stream, a);
         if (d.alone == 8) return launch(attn_paged_kernel<T, ST, NB, 8>, d.units * a.G, 512, stream, a);
     }
-    a.min_tiles = d.min_keys / (16 * paged_tile_blocks<T, ST, NB, kPagedWaves>());
     const int64_t slots = d.shares + d.units;
     a.across = d.across;
     const int s = launch(attn_paged_kernel<T, ST, NB, kPagedWaves>, (a.across ? (slots + 7) / 8 * 8 : slots) * a.G, 64 * kPagedWaves, stream, a);
@@ -151,7 +144,7 @@ int attend(const PagedDivision &d, void *stream, PagedArgs &a) {
     // A wavefront adds eight shares at a time; four of them for each row where a unit has more than that and rows are few, or more than twice that (us: 1 x 65536
     // tokens 32.7 / 28.7, 1 x 1300 8.6 / 8.3, 8 of 700 to 6000 15.3 / 15.0; with eight shares a unit 16 x 8192 47.3 / 47.9, five queries on those eight rows 19.3 / 21.9).
     const int64_t heads = (int64_t)a.B * a.G, pairs = (int64_t)a.Sq * a.r;
-    const bool many = d.shares > (heads * pairs <= 512 ? 8 : 16) * d.units;
+    const bool many = d.usual > (heads * pairs <= 512 ? 8 : 16) * d.units;
     const int64_t wgs = many ? pairs : (pairs + 3) / 4;
     a.by_wgs = div_by(wgs);
     return many ? launch(attn_paged_combine_kernel<T, NB, 4>, heads * wgs, 256, stream, a) : launch(attn_paged_combine_kernel<T, NB, 1>, heads * wgs, 256, stream, a);

@@ -45,7 +45,7 @@ struct PagedArgs {
     int blocks;                  // workgroups of a batch row (write), of a row and KV head (read); blocks of pairs of a row (attention)
     // attention: (row, block of pairs) units, into how many shares their work is cut (0: not), of how many tiles at least; the shares'
     // partial results and, for each unit, its first share and their number
-    int units, shares, min_tiles;
+    int units, shares;
     bool across;                 // eight slots of workgroups next to each other, not the heads of one
     Div by_r, by_g, by_blocks, by_wgs;          // by r, G, blocks, and a row and KV head's workgroups of the sum over shares
     float *partial;

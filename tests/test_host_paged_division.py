@@ -1,5 +1,5 @@
 """Host check of how attention over pages divides its work (csrc/attn_paged.h, compiled here for the CPU): whatever the rows' lengths, the shares are no more than the
-grid and the scratch hold."""
+grid and the scratch hold, and how long they are follows the workgroups that they come to."""
 import os
 import shutil
 import subprocess
@@ -15,9 +15,13 @@ using namespace gptoss;
 int main() {
     unsigned long long units, tiles, n = 0;
     int shares, least;
-    // one line: units, tiles of each, shares, least -> chunk
-    while (std::scanf("%%llu %%llu %%d %%d", &units, &tiles, &shares, &least) == 4) {
-        std::printf("%%d\n", paged_chunk(units * tiles, shares, least));
+    // one line: c units, tiles of each, shares, least -> chunk; l workgroups with shares of 1, 2, 3 and 6 times 128 keys -> least
+    char what;
+    int of[4];
+    while (std::scanf(" %%c", &what) == 1) {
+        if (what == 'c' && std::scanf("%%llu %%llu %%d %%d", &units, &tiles, &shares, &least) == 4) std::printf("%%d\n", paged_chunk(units * tiles, shares, least));
+        else if (what == 'l' && std::scanf("%%d %%d %%d %%d", of, of + 1, of + 2, of + 3) == 4) std::printf("%%d\n", paged_least(of[0], of[1], of[2], of[3]));
+        else return 1;
         ++n;
     }
     return n == 0;
@@ -27,7 +31,7 @@ int main() {
 
 @pytest.fixture(scope="module")
 def chunks(tmp_path_factory):
-    """paged_chunk of rows (units, tiles of each, shares, least)."""
+    """What the functions give for lines of arguments, the first a letter."""
     hipcc = os.environ.get("HIPCC") or shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     if not os.path.exists(hipcc):
         pytest.skip("hipcc not found")
@@ -48,12 +52,29 @@ def chunks(tmp_path_factory):
 def test_shares_fit_the_grid(chunks):
     """Rows of up to 2^30 tokens in tiles of 16, 32 and 64 keys, up to 1024 of them: the shares are no more than `shares` and one for each unit.  64 rows of 2^26 tiles are
     2^32 in all."""
-    rows = [(units, tiles, shares, least)
+    rows = [("c", units, tiles, shares, least)
             for units in (1, 2, 63, 64, 65, 1000, 1024)
             for tiles in (0, 1, 2, 7, 8, 9, 1000, 2 ** 20 - 1, 2 ** 24, 2 ** 25, 2 ** 26 - 8, 2 ** 26 - 1, 2 ** 26)
             for shares in (1, 2, 96, 100, 1023, 1024)
             for least in (2, 4, 8, 24, 48)]
-    for (units, tiles, shares, least), chunk in zip(rows, chunks(rows)):
+    for (_, units, tiles, shares, least), chunk in zip(rows, chunks(rows)):
         assert chunk >= least
         assert units * max(1, -(-tiles // chunk)) <= shares + units, (units, tiles, shares, least, chunk)
         assert chunk == least or units * tiles > (chunk - 1) * shares, (units, tiles, shares, least, chunk)      # (no longer than need be)
+
+
+def _workgroups(lens, heads, keys):
+    return heads * sum(max(1, -(-n // keys)) for n in lens)
+
+
+def test_least_shares(chunks):
+    """128, 256 or 384 keys, the first with which 256 compute units have a workgroup each at most; otherwise 768 where that fills whole rounds of them by four fifths,
+    and 384 where it does not."""
+    rows, want = [], []
+    for lens, heads in (([2049], 8), ([4096], 8), ([4097], 8), ([8192], 8), ([8193], 8), ([12288], 8), ([12289], 8), ([4000] * 2, 8), ([4000] * 8, 8), ([8193] * 4, 8), ([700, 3000, 6000] * 3, 8),
+                        ([100, 900, 2500] * 8, 8), ([0] * 1024, 1), ([0, 5], 64), ([65536], 8), ([700, 1400] * 20, 2), ([], 8)):
+        at = {n: _workgroups(lens, heads, 128 * n) for n in (1, 2, 3, 6)}
+        rows.append(("l", *at.values()))
+        rounds = -(-at[6] // 256)
+        want.append(next((n for n in (1, 2, 3) if at[n] <= 256), 6 if at[6] >= 0.8 * 256 * rounds else 3))
+    assert chunks(rows) == want and set(want) == {1, 2, 3, 6}
