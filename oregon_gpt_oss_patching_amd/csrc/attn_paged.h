@@ -746,14 +746,14 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
                 const int page = paged_page(a, sp.b, key);
                 if (page < 0) continue;
                 const char *row = v_base + a.vp.at(page, key & in_page);
-                uint32_t power = 0;
-                if constexpr (Tile::kCodes) power = (uint8_t)ve_base[a.ve.at(page, key & in_page)];
+                float power = 1.0f;
+                if constexpr (Tile::kCodes) power = factor_of_byte((uint8_t)ve_base[a.ve.at(page, key & in_page)]);
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float x = stored_number(reinterpret_cast<const ST *>(row) + Tile::column(d, e, quad));
-                        if constexpr (Tile::kCodes) x = times_exp(x, power);
+                        if constexpr (Tile::kCodes) x *= power;
                         if ((__float_as_uint(x) & 0x7f800000u) != 0x7f800000u) continue;
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb)

@@ -108,9 +108,10 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const PagedArgs a) {
         load8<true>(reinterpret_cast<const ST *>(a.kp.head(g) + a.kp.at(page, at)) + c8, k);
         load8<true>(reinterpret_cast<const ST *>(a.vp.head(g) + a.vp.at(page, at)) + c8, v);
         if constexpr (sizeof(ST) == 1) {
-            const uint32_t ke = *reinterpret_cast<const uint8_t *>(a.ke.head(g) + a.ke.at(page, at)), ve = *reinterpret_cast<const uint8_t *>(a.ve.head(g) + a.ve.at(page, at));
+            const float ke = factor_of_byte(*reinterpret_cast<const uint8_t *>(a.ke.head(g) + a.ke.at(page, at)));
+            const float ve = factor_of_byte(*reinterpret_cast<const uint8_t *>(a.ve.head(g) + a.ve.at(page, at)));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { k[e] = times_exp(k[e], ke); v[e] = times_exp(v[e], ve); }
+            for (int e = 0; e < 8; ++e) { k[e] *= ke; v[e] *= ve; }
         }
     }
     store8<true>(reinterpret_cast<T *>(a.k) + b * a.ks.b + g * a.ks.h + i * a.ks.s + c8, k);

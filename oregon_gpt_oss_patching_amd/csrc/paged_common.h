@@ -76,9 +76,8 @@ __device__ __forceinline__ int paged_length(const PagedArgs &a, int b) {
 
 __device__ __forceinline__ float exp_of_byte(uint32_t e) { return __uint_as_float(e << 23); }        // 2^(e - 127), 1 <= e <= 254
 
-// A code's number times 2^(e - 127), NaN for 255: what the scaling conversions give for exp_of_byte(e), whatever e is.  (2^-127 is no normal number of 32 bits: as a
-// factor it would be 0.)
-__device__ __forceinline__ float times_exp(float x, uint32_t e) { return e == 255 ? __uint_as_float(0x7fc00000u) : __builtin_ldexpf(x, (int)e - kExpBias); }
+// 2^(e - 127) as a factor of any byte e, NaN for 255: what the scaling conversions take exp_of_byte(e) for.  (2^-127 is half of 32 bits' smallest normal number.)
+__device__ __forceinline__ float factor_of_byte(uint32_t e) { return __uint_as_float(e == 0 ? 0x00400000u : e == 255 ? 0x7fc00000u : e << 23); }
 
 struct e4m3 { uint8_t code; };
 
