@@ -43,14 +43,15 @@ struct PagedCall {
 
 // As int32 on the cache's GPU; what is so already does not go through the dispatcher (half a microsecond each).  Wider numbers that int32 does not hold become its
 // ends, which are no page, in front of every position and behind each (cut off, 2^32 + 3 would be page 3).
+bool is_integers(const Tensor &t) { return at::isIntegralType(t.scalar_type(), /*includeBool=*/true) && t.scalar_type() != at::kUInt64; }
 Tensor int32_on(const Tensor &t, const Tensor &pages) {
     if (t.scalar_type() == at::kInt && t.device() == pages.device()) return t;
-    const bool wide = t.scalar_type() == at::kLong || t.scalar_type() == at::kUInt32 || t.scalar_type() == at::kUInt64;
+    const bool wide = t.scalar_type() == at::kLong || t.scalar_type() == at::kUInt32;
     return (wide ? t.to(at::kLong).clamp(INT_MIN, INT_MAX) : t).to(pages.device(), at::kInt);
 }
 
 Tensor lengths_of(const Tensor &t, const Tensor &pages, int64_t batch, const char *name) {
-    TORCH_CHECK(t.numel() == batch && !at::isFloatingType(t.scalar_type()), name, " must hold one integer per batch row");
+    TORCH_CHECK(t.numel() == batch && is_integers(t), name, " must hold one integer per batch row");
     return int32_on(t, pages).contiguous();
 }
 
@@ -89,7 +90,7 @@ void fill(PagedCall &c, const Tensor &k_pages, const Tensor &v_pages, const OptT
     p.v_pages = const_cast<void *>(v_pages.const_data_ptr());
     set3(p.k_page_stride, k_pages);
     set3(p.v_page_stride, v_pages);
-    TORCH_CHECK(page_table.dim() == 2 && page_table.size(0) == batch && !at::isFloatingType(page_table.scalar_type()), "page_table must be (B, pages of a row) integers, got ",
+    TORCH_CHECK(page_table.dim() == 2 && page_table.size(0) == batch && is_integers(page_table), "page_table must be (B, pages of a row) integers, got ",
                 page_table.sizes(), " for ", batch, " rows");
     c.table = int32_on(page_table, k_pages);
     if (c.table.stride(1) != 1 && c.table.size(1) > 1) c.table = c.table.contiguous();

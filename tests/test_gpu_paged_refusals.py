@@ -49,3 +49,32 @@ def test_written_caches_have_a_new_version(A):  # noqa: F811
     before = [t._version for t in cache]
     A.paged_cache_write(cache, k, k, table, [0])
     assert all(t._version == v + 1 for t, v in zip(cache, before))
+
+
+@pytest.mark.parametrize("dtype", [torch.complex64, torch.float16, torch.uint64])
+def test_tables_and_lengths_that_are_no_integers(A, dtype):  # noqa: F811
+    """Complex numbers lost their imaginary part, numbers of 64 bits without a sign theirs above 2^63."""
+    cache, table, n = A.paged_cache(4, 2, 16), torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    q, k = torch.ones(1, 16, 1, 64, dtype=BF16, device=DEV), torch.ones(1, 2, 1, 64, dtype=BF16, device=DEV)
+    odd = lambda x: x.cpu().to(dtype).to(DEV)
+    for text, call in (("integer", lambda: A.paged_attention(q, cache, odd(table), n, None, SCALE)),
+                       ("integer", lambda: A.paged_attention(q, cache, table, odd(n), None, SCALE)),
+                       ("integer", lambda: A.paged_attention(q, cache, table, n, None, SCALE, None, odd(n))),
+                       ("integer", lambda: A.paged_cache_read(cache, table, odd(n), 4)),
+                       ("integer", lambda: A.paged_cache_write(cache, k, k, table, odd(n))),
+                       ("integer", lambda: A.paged_cache_write(cache, k, k, table, n, odd(n)))):
+        with pytest.raises(RuntimeError, match=text):
+            call()
+    assert not cache.k.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.uint16, torch.uint32, torch.int64])
+def test_integers_of_other_widths(A, dtype):  # noqa: F811
+    cache, n = A.paged_cache(4, 2, 16), torch.full((1,), 20, dtype=torch.int32, device=DEV)
+    table = torch.tensor([[3, 1]], dtype=torch.int32, device=DEV)
+    k = torch.randn(1, 2, 20, 64, device=DEV).to(BF16)
+    q = torch.randn(1, 16, 1, 64, device=DEV).to(BF16)
+    as_is = lambda x: x.cpu().to(dtype).to(DEV)
+    A.paged_cache_write(cache, k, k, as_is(table), as_is(n - 20), as_is(n))
+    assert torch.equal(A.paged_cache_read(cache, as_is(table), as_is(n), 20)[0], k)
+    assert torch.equal(A.paged_attention(q, cache, as_is(table), as_is(n), None, SCALE), A.paged_attention(q, cache, table, n, None, SCALE))
