@@ -349,8 +349,8 @@ typedef struct gptoss_attn_paged_params {
     int32_t B, H, G, Sq, D; /* Sq: query rows (fwd), new tokens of a row (write), rows of the result (read); H: fwd only */
     int32_t pages, page_size, table_width;
     int32_t window;         /* fwd: 0 = full causal; else sliding window length */
-    int32_t max_len;        /* fwd: a length that no sequence passes, if the caller knows one (0: not).  Only the division
-                               of the work goes by it; longer sequences are right too */
+    int32_t max_len;        /* fwd: a length that no sequence passes, if the caller knows one (0: not).  Only the choice of
+                               one launch for short rows and the scratch go by it; longer sequences are right too */
     float scale;            /* fwd: softmax scale */
     int32_t reserved0;
 
@@ -391,8 +391,8 @@ int gptoss_attn_paged_read(const gptoss_attn_paged_params *params, void *stream)
  * j <= p, j < n, window == 0 or j > p - window, and j's page exists, n = min(seqlens[b], table_width * page_size).  A query behind
  * the sequence (p >= n), in front of it (p < 0) or without a visible key gives O = 0, lse = sink.  What stands in rows that a query
  * does not see has no part in its result, infinities and NaN included.
- * Any number of queries is right; the cache is read once for each 64 (query, head of the group) pairs, so the many queries of a
- * prompt's chunk are better served by gptoss_attn_paged_read and gptoss_attn_fwd.
+ * Any number of queries is right; the cache is read once for each 64 (query, head of the group) pairs, 32 of float32 queries, so the
+ * many queries of a prompt's chunk are better served by gptoss_attn_paged_read and gptoss_attn_fwd.
  */
 int gptoss_attn_paged_fwd(const gptoss_attn_paged_params *params, void *stream);
 

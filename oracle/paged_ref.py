@@ -102,8 +102,8 @@ def bounds(o, lse, terms, dtype):
     68 u * scale * sum |q k| <= 68 u S; the exponent, taken to base 2, adds the rounding of an argument of at most S + |lse| (times log2 e, back
     times ln 2: (S + |lse|) u, twice, for logit and maximum) and two steps of the exponential itself, 4 u.  So each weight is off
     by at most E = (70 S + 2 |lse| + 4) u of itself, numerator and denominator both: 2 E.  Sums of n such weights and products add n u each.
-    bfloat16 kernels round each weight once before the second product, half a step of bfloat16: 2^-8 of it, and o once, 2^-8 of o;
-    float32 kernels round o once more, u.  E and n u stay far below 1 in the tests (their second orders: the factor 1.01)."""
+    For bfloat16 there is room for one rounding of each weight before the second product, half a step of bfloat16: 2^-8 of it (kernels that hold the
+    weights in two terms stay far below), and o is rounded once, 2^-8 of o; float32 kernels round o once more, u.  E and n u stay far below 1 in the tests (their second orders: the factor 1.01)."""
     amount, size, count = terms
     u = 2.0 ** -24
     logit = (70 * size + 2 * lse.abs().nan_to_num(posinf=0.0) + 4) * u

@@ -339,7 +339,8 @@ def hip_flash_attention(
     `position_ids` the model passes along are used.
 
     With `paged=` (a `PagedState`) the layer's new keys and values go into a cache in pages, and the queries attend to what
-    stands there."""
+    stands there.  `key` and `value` are then the new tokens' alone, the state says how long rows are, and there are no documents: `position_ids`
+    are not looked at."""
     paged = kwargs.get("paged")
     if paged is not None:
         if kwargs.get("doc_start") is not None or kwargs.get("seqlens") is not None or _is_lengths(attention_mask):

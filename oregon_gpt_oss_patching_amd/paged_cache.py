@@ -10,8 +10,8 @@ the pool (-1, say) names no page.  The pool holds the model's type, or 8-bit e4m
     out = paged_attention(q, cache, page_table, start + S, sinks, scale, window)      # (B, S, H, 64), as attention()
     k, v = paged_cache_read(cache, page_table, seqlens, max_len)          # rows back, for attention() of a long prompt's chunk
 
-Everything that says where tokens stand (`page_table`, `start`, `seqlens`) stays on the GPU and is read there: the calls do not
-synchronise and can be captured into a graph that is replayed with other contents.  None has a gradient.
+Everything that says where tokens stand (`page_table`, `start`, `seqlens`: integers, numbers beyond int32 being beyond every table) stays on the GPU and
+is read there: the calls do not synchronise and can be captured into a graph that is replayed with other contents.  None has a gradient, of either mode.
 
 A patched model takes all of this as one argument, a `PagedState`: `model(ids, position_ids=..., use_cache=False, paged=state)`.
 
@@ -167,10 +167,11 @@ def paged_attention(q, cache: PagedCache, page_table, seqlens, sinks, sm_scale, 
     and sees the keys at and before it, with `bandwidth` the last so many of them.  Queries at or behind seqlens[b] are padding: they
     give 0, as does a query that sees no key.  What stands in rows that a query does not see has no part in its result.
     `sinks`, `sm_scale`, `bandwidth`: as in `attention` (sinks=None: a logit of 0; logits of -inf: no sink).
-    `max_len`: a length that no row passes, if the caller knows one shorter than the table; it only helps to divide the work.
+    `max_len`: a length that no row passes, if the caller knows one shorter than the table; it only helps to divide the work: rows that are known to be short (up
+    to some 1000 to 3000 tokens, by their type and number) take one launch and not two.
 
-    The cache is read once for each 64 pairs of a query and a head of its KV head's group; the many queries of a prompt's chunk are better
-    served by `paged_cache_read` and `attention`."""
+    The cache is read once for each 64 pairs of a query and a head of its KV head's group (32 in float32); the many queries of a prompt's chunk are
+    better served by `paged_cache_read` and `attention`."""
     if not _ready:
         _register_ops()
     out = NotImplemented if _compiling() else _fwd_now(q, *cache, page_table, seqlens, start, sinks, sm_scale, bandwidth, max_len, False)
