@@ -146,8 +146,8 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int slot, 
     // numbers of shares of n times 128 keys, two at a time in 16 bits (which they fit wherever they are used: at most six times a.shares, and one for each unit)
     constexpr int k128 = 128 / KEYS;
     auto numbers = [&](int u, int tiles, int n, int m) __attribute__((always_inline)) {
-        const int x = max(1, (tiles + n * k128 - 1) / (n * k128)), y = max(1, (tiles + m * k128 - 1) / (m * k128));
-        return __builtin_amdgcn_readlane(wave_scan(u < a.units ? x + (y << 16) : 0), 63);
+        const uint32_t x = max(1, (tiles + n * k128 - 1) / (n * k128)), y = max(1, (tiles + m * k128 - 1) / (m * k128));
+        return (uint32_t)__builtin_amdgcn_readlane(wave_scan(u < a.units ? (int)(x + (y << 16)) : 0), 63);
     };
     uint32_t of12 = numbers(lane, tiles0, 1, 2), of36 = numbers(lane, tiles0, 3, 6);
     for (int u0 = 64; u0 < a.units; u0 += 64) {
