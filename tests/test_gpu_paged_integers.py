@@ -58,3 +58,32 @@ def test_lengths_and_positions(A, storage, far):  # noqa: F811
     A.paged_cache_write(other, -k, -k, table, [0, 0], torch.tensor([48 if far > 0 else 0, 0], dtype=torch.int32, device=DEV))
     for x, y in zip(cache, other):
         assert x is None or torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def test_a_graph_follows_them(A):  # noqa: F811
+    """Tables, lengths and positions in 64 bits are narrowed inside a captured call: replays follow what they hold then."""
+    cache, table, n, q, sinks, k, v = make(A, 63, [400, 90], 8, 2, 1, 16, BF16, E4M3)
+    q, sinks = q.to(DEV), sinks.to(DEV)
+    wide, lens, start = table.long(), n.long(), n.long() - 1
+
+    def call(*x):
+        return (*A.paged_attention_forward(q, cache, x[0], x[1], sinks, SCALE, None, x[2]), *A.paged_cache_read(cache, x[0], x[1], 30, x[2]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(wide, lens, start)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(wide, lens, start)
+    for a, b, first, entry in ((400, 90, 380, 2 ** 40), (2 ** 33, 5, 399, -1), (100, -2 ** 35, 2 ** 32 + 7, 1), (350, 90, 10, 2 ** 32)):
+        lens.copy_(torch.tensor([a, b]))
+        start.copy_(torch.tensor([first, b - 1]))
+        wide[0, 3] = entry
+        graph.replay()
+        got = [x.clone() for x in out]
+        fit = lambda x: x.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+        want = call(fit(wide), fit(lens), fit(start))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), (a, b, first, entry)
