@@ -402,6 +402,38 @@ size_t gptoss_attn_paged_workspace_bytes(const gptoss_attn_paged_params *params)
 /* Host-only argument check that each of the three calls starts with; `call`: 0 fwd, 1 write, 2 read. */
 int gptoss_attn_paged_validate(const gptoss_attn_paged_params *params, int call);
 
+/* ---- rotary positions --------------------------------------------------------------------------------------------
+ *
+ * The embedding that the model applies to q and k in front of the attention (the reference leaves it to transformers'
+ * apply_rotary_pos_emb).  Token (b, s) has an angle for each pair i < R/2 of a head's first R numbers:
+ *   angle = positions[b][s] * frequencies[i] (radians, in 64 bits), c = scale * cos(angle), s = scale * sin(angle),
+ * or c and s come from tables; with x1, x2 = numbers i and R/2 + i of the head (`interleaved`: 2i and 2i + 1),
+ *   y1 = c x1 - s x2,  y2 = c x2 + s x1
+ * in 32 bits, rounded once.  `inverse`: with -s, which is what gradients go through (and, with a scale of 1, the way
+ * back).  Numbers behind the first R are copied.
+ */
+typedef struct gptoss_attn_rotary_params {
+    uint32_t struct_size;   /* sizeof(gptoss_attn_rotary_params) */
+    int32_t dtype;          /* GPTOSS_ATTN_BF16 or GPTOSS_ATTN_FP32: q, k and the results */
+    int32_t table_dtype;    /* of cos_table and sin_table: GPTOSS_ATTN_BF16 or GPTOSS_ATTN_FP32 */
+    int32_t position_bytes; /* 4 or 8: positions are int32 or int64 */
+    int32_t B, H, G, S, D, R;       /* H heads in q, G in k; D <= 256, R even, 2 to D */
+    int32_t interleaved, inverse;
+    double scale;                   /* (of positions; tables hold theirs) */
+    const void *q, *k;              /* (B, H, S, D), (B, G, S, D): any strides, rows of D contiguous */
+    void *q_out, *k_out;            /* may be q and k themselves with the same strides; no other overlap */
+    const void *positions;          /* [b * position_stride_b + s * position_stride_s], or NULL: */
+    const double *frequencies;      /* (R/2) */
+    const void *cos_table, *sin_table;      /* rows of R/2 at [b * cos_stride_b + s * cos_stride_s] */
+    gptoss_attn_strides q_stride, k_stride, q_out_stride, k_out_stride;
+    int64_t position_stride_b, position_stride_s, cos_stride_b, cos_stride_s, sin_stride_b, sin_stride_s;
+} gptoss_attn_rotary_params;
+
+int gptoss_attn_rotary(const gptoss_attn_rotary_params *params, void *stream);
+
+/* Host-only argument check that the call starts with. */
+int gptoss_attn_rotary_validate(const gptoss_attn_rotary_params *params);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,7 +21,15 @@ from .paged_cache import (  # noqa: F401
     paged_cache_read,
     paged_cache_write,
 )
+from .rotary_positions import (  # noqa: F401
+    Rotary,
+    hip_rotary_pos_emb,
+    rotary,
+    rotary_frequencies,
+    rotary_tables,
+)
 
 __all__ = ["attention", "attention_forward", "attention_backward", "doc_start_from_position_ids",
            "hip_flash_attention", "triton_flash_attention",
-           "PagedCache", "PagedState", "paged_cache", "paged_cache_write", "paged_cache_read", "paged_attention", "paged_attention_forward"]
+           "PagedCache", "PagedState", "paged_cache", "paged_cache_write", "paged_cache_read", "paged_attention", "paged_attention_forward",
+           "Rotary", "rotary", "rotary_frequencies", "rotary_tables", "hip_rotary_pos_emb"]

@@ -43,6 +43,8 @@ EXPORTS = (
     "gptoss_attn_paged_read",
     "gptoss_attn_paged_workspace_bytes",
     "gptoss_attn_paged_validate",
+    "gptoss_attn_rotary",
+    "gptoss_attn_rotary_validate",
     "gptoss_attn_mfma_rate_probe",
     "gptoss_attn_stream_probe",
 )
@@ -107,6 +109,24 @@ class PagedParams(ctypes.Structure):
         ("q_stride", Strides), ("o_stride", Strides), ("k_stride", Strides), ("v_stride", Strides),
         ("k_page_stride", Strides), ("v_page_stride", Strides), ("k_exp_stride", Strides), ("v_exp_stride", Strides),
         ("table_stride", ctypes.c_int64),
+    ]
+
+
+class RotaryParams(ctypes.Structure):
+    """Mirror of `gptoss_attn_rotary_params`; field order and types must match the header."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32), ("table_dtype", ctypes.c_int32), ("position_bytes", ctypes.c_int32),
+        ("B", ctypes.c_int32), ("H", ctypes.c_int32), ("G", ctypes.c_int32), ("S", ctypes.c_int32), ("D", ctypes.c_int32), ("R", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("scale", ctypes.c_double),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p), ("frequencies", ctypes.c_void_p),
+        ("cos_table", ctypes.c_void_p), ("sin_table", ctypes.c_void_p),
+        ("q_stride", Strides), ("k_stride", Strides), ("q_out_stride", Strides), ("k_out_stride", Strides),
+        ("position_stride_b", ctypes.c_int64), ("position_stride_s", ctypes.c_int64), ("cos_stride_b", ctypes.c_int64), ("cos_stride_s", ctypes.c_int64),
+        ("sin_stride_b", ctypes.c_int64), ("sin_stride_s", ctypes.c_int64),
     ]
 
 
@@ -175,6 +195,10 @@ def load() -> ctypes.CDLL:
         lib.gptoss_attn_paged_workspace_bytes.argtypes = [ctypes.POINTER(PagedParams)]
         lib.gptoss_attn_paged_validate.restype = ctypes.c_int
         lib.gptoss_attn_paged_validate.argtypes = [ctypes.POINTER(PagedParams), ctypes.c_int]
+        lib.gptoss_attn_rotary.restype = ctypes.c_int
+        lib.gptoss_attn_rotary.argtypes = [ctypes.POINTER(RotaryParams), ctypes.c_void_p]
+        lib.gptoss_attn_rotary_validate.restype = ctypes.c_int
+        lib.gptoss_attn_rotary_validate.argtypes = [ctypes.POINTER(RotaryParams)]
         if lib.gptoss_attn_version() != ABI_VERSION:
             raise RuntimeError("libgptoss_attn.so ABI version mismatch; rebuild the library")
         _lib = lib
@@ -192,9 +216,10 @@ def load_torch_ops() -> None:
     torch.ops.load_library(TORCH_LIBRARY)
 
 
-def direct_calls():
-    """(paged_write, paged_read, paged_fwd) of libgptoss_torch.so as Python functions that do not go through the dispatcher."""
-    f = ctypes.PyDLL(TORCH_LIBRARY).gptoss_paged_direct
+def direct_calls(name: str = "gptoss_paged_direct"):
+    """Calls of libgptoss_torch.so as Python functions that do not go through the dispatcher: (paged_write, paged_read, paged_fwd), or the
+    rotary call ("gptoss_rotary_direct")."""
+    f = getattr(ctypes.PyDLL(TORCH_LIBRARY), name)
     f.restype = ctypes.py_object
     return f()
 

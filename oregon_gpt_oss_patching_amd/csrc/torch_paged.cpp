@@ -5,23 +5,9 @@
 //
 // Native for the same reason as attention() (torch_ops.cpp): a decoding step makes two of these calls for each layer, and each takes
 // a few microseconds on the GPU.
-#include <climits>
-
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <ATen/record_function.h>
-#include <torch/csrc/Dtype.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-
-#include "torch_common.h"
+#include "torch_direct.h"
 
 namespace {
-
-int32_t size32(int64_t n) {
-    TORCH_CHECK(n <= INT_MAX, "a dimension of ", n, " is too long");
-    return static_cast<int32_t>(n);
-}
 
 int abi_dtype(at::ScalarType t) { return t == at::kFloat ? GPTOSS_ATTN_FP32 : t == at::kBFloat16 ? GPTOSS_ATTN_BF16 : t == at::kFloat8_e4m3fn ? GPTOSS_ATTN_E4M3 : -1; }
 
@@ -40,15 +26,6 @@ struct PagedCall {
     gptoss_attn_paged_params p{};
     Tensor table, seqlens, start, sinks, q, k, v, scratch;
 };
-
-// As int32 on the cache's GPU; what is so already does not go through the dispatcher (half a microsecond each).  Wider numbers that int32 does not hold become its
-// ends, which are no page, in front of every position and behind each (cut off, 2^32 + 3 would be page 3).
-bool is_integers(const Tensor &t) { return at::isIntegralType(t.scalar_type(), /*includeBool=*/true) && t.scalar_type() != at::kUInt64; }
-Tensor int32_on(const Tensor &t, const Tensor &pages) {
-    if (t.scalar_type() == at::kInt && t.device() == pages.device()) return t;
-    const bool wide = t.scalar_type() == at::kLong || t.scalar_type() == at::kUInt32;
-    return (wide ? t.to(at::kLong).clamp(INT_MIN, INT_MAX) : t).to(pages.device(), at::kInt);
-}
 
 Tensor lengths_of(const Tensor &t, const Tensor &pages, int64_t batch, const char *name) {
     TORCH_CHECK(t.numel() == batch && is_integers(t), name, " must hold one integer per batch row");
@@ -224,35 +201,6 @@ std::tuple<Tensor, Tensor> paged_fwd(const Tensor &q, const Tensor &k_pages, con
     return {o, need_lse ? lse : new_tensor({0}, at::kFloat, o)};
 }
 
-using Pair = std::tuple<Tensor, Tensor>;
-
-// What a tensor asks for (most have no record of either): a gradient, which torch.no_grad() takes back, or the tangent of forward mode, which it does not.
-bool wants_gradient(const Tensor &t) { return t.unsafeGetTensorImpl()->autograd_meta() && t.requires_grad(); }
-bool has_tangent(const Tensor &t) { return t.unsafeGetTensorImpl()->autograd_meta() && t._fw_grad(0).defined(); }
-
-// Tensors with either are refused, as these calls would drop it without a word.
-void refuse_gradients(const c10::OperatorHandle &op, c10::DispatchKeySet keys, torch::jit::Stack *stack) {
-    const size_t n = op.schema().arguments().size();
-    for (size_t i = stack->size() - n; i < stack->size(); ++i) {
-        if (!(*stack)[i].isTensor()) continue;
-        const Tensor &t = (*stack)[i].toTensor();
-        TORCH_CHECK(!at::GradMode::is_enabled() || !wants_gradient(t), op.schema().name(), " has no gradient: call it under torch.no_grad() (argument ",
-                    op.schema().arguments()[i + n - stack->size()].name(), " requires one)");
-        TORCH_CHECK(!has_tangent(t), op.schema().name(), " has no gradient, forward mode's neither: argument ", op.schema().arguments()[i + n - stack->size()].name(),
-                    " has a tangent");
-    }
-    const at::AutoDispatchBelowADInplaceOrView below;
-    op.redispatchBoxed(keys & c10::after_ADInplaceOrView_keyset, stack);
-}
-
-void refuse_cpu(const c10::OperatorHandle &, torch::jit::Stack *) {
-    TORCH_CHECK(false, "gptoss attention runs on the GPU only (HIP kernels); got CPU tensors");
-}
-
-void refuse_vmap(const c10::OperatorHandle &, torch::jit::Stack *) {
-    TORCH_CHECK(false, "gptoss attention cannot be vmapped: its tensors have a batch dimension of their own");
-}
-
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(gptoss_attn, m) {
@@ -284,43 +232,6 @@ GPTOSS_PAGED_IMPL(FuncTorchBatched, refuse_vmap)
 // from Python, through the operator / so: write 4.25 / 3.45, attention 5.8 / 4.2 (with an empty result less), read 6.2 / 4.75.
 namespace {
 
-// Whether what is dispatched now reaches the GPU's kernel as it is.
-bool direct_now() {
-    return (c10::impl::tls_local_dispatch_key_set().included_ - c10::default_included_set).empty() && !at::impl::torch_function_mode_enabled() && !torch::jit::tracer::isTracing() &&
-           !at::getStepCallbacksUnlessEmpty(at::RecordScope::FUNCTION).has_value();
-}
-
-// Arguments from Python; `ok` falls where one is not what a direct call takes.
-struct Arguments {
-    PyObject *const *args;
-    const bool grad = at::GradMode::is_enabled();
-    bool ok = true;
-
-    const Tensor &tensor(int i) {
-        static const Tensor none;
-        static const c10::DispatchKeySet plain = c10::DispatchKeySet(c10::DispatchKey::CUDA) | c10::autograd_dispatch_keyset_with_ADInplaceOrView | c10::autocast_dispatch_keyset |
-                                                 c10::getAutogradRelatedKeySetFromBackend(c10::BackendComponent::CUDABit);
-        if (!THPVariable_CheckExact(args[i])) return ok = false, none;
-        const Tensor &t = THPVariable_Unpack(args[i]);
-        if ((t.key_set().raw_repr() & ~plain.raw_repr()) != 0 || (grad && wants_gradient(t)) || has_tangent(t)) ok = false;
-        return t;
-    }
-    OptTensor optional(int i) { return args[i] == Py_None ? OptTensor() : OptTensor(tensor(i)); }
-    int64_t integer(int i) {        // None: 0
-        if (args[i] == Py_None) return 0;
-        if (!PyLong_CheckExact(args[i])) return ok = false, 0;
-        int overflow = 0;
-        const long long x = PyLong_AsLongLongAndOverflow(args[i], &overflow);
-        if (overflow) ok = false;
-        return x;
-    }
-    double number(int i) { return PyFloat_CheckExact(args[i]) ? PyFloat_AS_DOUBLE(args[i]) : (ok = false, 0.0); }
-    bool truth(int i) { return PyBool_Check(args[i]) ? args[i] == Py_True : (ok = false); }
-    at::ScalarType dtype(int i) { return THPDtype_Check(args[i]) ? reinterpret_cast<THPDtype *>(args[i])->scalar_type : (ok = false, at::kBFloat16); }
-};
-
-PyObject *not_implemented() { Py_RETURN_NOTIMPLEMENTED; }
-
 PyObject *write_now(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     if (n != 9 || !direct_now()) return not_implemented();
@@ -334,12 +245,6 @@ PyObject *write_now(PyObject *, PyObject *const *args, Py_ssize_t n) {
     }
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
-}
-
-PyObject *pair(const Pair &x) {
-    const pybind11::object a = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::get<0>(x))),
-                           b = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::get<1>(x)));
-    return a && b ? PyTuple_Pack(2, a.ptr(), b.ptr()) : nullptr;
 }
 
 PyObject *read_now(PyObject *, PyObject *const *args, Py_ssize_t n) {
