@@ -20,10 +20,11 @@ struct RotaryArgs {
     int64_t items;                       // threads with work: (token, slot, chunk), chunks fastest
     int H, heads, D, R, pairs, chunks;   // heads: H + G; pairs: chunks that are turned, the others are copied
     int slots;                           // threads that share a token's heads
-    Div by_chunks, by_slots, by_s;
+    int inner;                           // what runs behind the chunks: the slots of a token, or (along_tokens) the tokens of a slot
+    Div by_chunks, by_inner, by_s;
     int S;
     float scale;                         // of the angles' cosine and sine; of tables 1
-    bool wide, f32_tables, inverse;
+    bool wide, f32_tables, whole_tables, inverse, along_tokens;
 };
 
 // c = cos(u pi / 2), s = sin(u pi / 2).  The whole quarters come off in 64 bits, what is left is at most half of one: polynomials (the Taylor series, whose
@@ -71,8 +72,29 @@ template <> struct RotaryPiece<bf16, 1> {
     __device__ __forceinline__ void set(int, float v) { x = (bf16)v; }
 };
 
-__device__ __forceinline__ float table_number(const void *p, int64_t i, bool f32) {
-    return f32 ? static_cast<const float *>(p)[i] : (float)static_cast<const bf16 *>(p)[i];
+// V numbers of a table row of either type; `whole`: its pieces of V lie on boundaries of their own size (of 16 bytes at most).
+template <int V>
+__device__ __forceinline__ void table_numbers(const void *p, int64_t at, bool f32, bool whole, float (&x)[V]) {
+    if constexpr (V > 1) {
+        if (whole) {
+            if (f32) {
+                constexpr int n = V < 4 ? V : 4;
+#pragma unroll
+                for (int i = 0; i < V; i += n) {
+                    const auto y = *reinterpret_cast<const RotaryPiece<float, n> *>(static_cast<const float *>(p) + at + i);
+#pragma unroll
+                    for (int e = 0; e < n; ++e) x[i + e] = y.get(e);
+                }
+            } else {
+                const auto y = *reinterpret_cast<const RotaryPiece<bf16, V> *>(static_cast<const bf16 *>(p) + at);
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[e] = y.get(e);
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = f32 ? static_cast<const float *>(p)[at + i] : (float)static_cast<const bf16 *>(p)[at + i];
 }
 
 // PAIRED: numbers 2i and 2i + 1 are a pair, otherwise i and i + R/2.
@@ -83,7 +105,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (item >= a.items) return;
     const int line = a.by_chunks.quotient((int)item), chunk = (int)item - line * a.chunks;
-    const int token = a.by_slots.quotient(line), slot = line - token * a.slots;
+    const int quotient = a.by_inner.quotient(line), inner = line - quotient * a.inner;
+    const int token = a.along_tokens ? inner : quotient, slot = a.along_tokens ? quotient : inner;
     const int b = a.by_s.quotient(token), s = token - b * a.S;
     const bool turned = chunk < a.pairs;
     // the two pieces of a head's row (of what is copied: one)
@@ -106,12 +129,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     float c[V], sn[V];
     if (turned) {
         if constexpr (TABLES) {
-            const int64_t cp = b * a.cos_b + s * a.cos_s + V * chunk, sp = b * a.sin_b + s * a.sin_s + V * chunk;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                c[i] = table_number(a.cos, cp + i, a.f32_tables);
-                sn[i] = table_number(a.sin, sp + i, a.f32_tables);
-            }
+            table_numbers<V>(a.cos, b * a.cos_b + s * a.cos_s + V * chunk, a.f32_tables, a.whole_tables, c);
+            table_numbers<V>(a.sin, b * a.sin_b + s * a.sin_s + V * chunk, a.f32_tables, a.whole_tables, sn);
         } else {
             const int64_t at = b * a.pos_b + s * a.pos_s;
             const double p = a.wide ? (double)static_cast<const int64_t *>(a.positions)[at] : (double)static_cast<const int32_t *>(a.positions)[at];

@@ -22,9 +22,11 @@ Tensor heads_of(const Tensor &t, gptoss_attn_strides &s) {
 }
 
 Tensor new_heads(const Tensor &like, gptoss_attn_strides &s) {
-    const Tensor t = new_tensor({like.size(0), like.size(2), like.size(1), like.size(3)}, like.scalar_type(), like).transpose(1, 2);
-    set(s, t, false);
-    return t;
+    const int64_t b = like.size(0), h = like.size(1), n = like.size(2), d = like.size(3);
+    s.b = n * h * d;
+    s.h = d;
+    s.s = h * d;
+    return Tensor(at::detail::empty_strided_cuda({b, h, n, d}, {s.b, s.h, s.s, 1}, like.scalar_type(), like.device()));
 }
 
 Pair turn(const Tensor &q_, const Tensor &k_, const OptTensor &positions, const OptTensor &frequencies, const OptTensor &cos, const OptTensor &sin, double scale,

@@ -89,12 +89,10 @@ _compiling = torch.compiler.is_compiling
 
 
 def _call(q, k, positions, frequencies, cos, sin, scale, interleaved):
-    if not _ready:
-        _register_ops()
-    out = NotImplemented if _compiling() else _now(q, k, positions, frequencies, cos, sin, scale, interleaved)
-    if out is NotImplemented:
-        out = _op(q, k, positions, frequencies, cos, sin, float(scale), bool(interleaved))
-    return out
+    """Through the dispatcher."""
+    if positions is not None and not isinstance(positions, torch.Tensor):
+        positions = torch.as_tensor(positions, device=q.device)
+    return _op(q, k, positions, frequencies, cos, sin, float(scale), bool(interleaved))
 
 
 def rotary(q, k, positions, rope: Rotary):
@@ -102,14 +100,18 @@ def rotary(q, k, positions, rope: Rotary):
     memory is (B, S, heads, D).  `positions`: (B, S), (1, S) or (S) integers, any numbers, negative ones too.
 
     Differentiable in q and k, any number of times.  float16 goes through float32."""
-    if not isinstance(positions, torch.Tensor):
-        positions = torch.as_tensor(positions, device=q.device)
-    return _call(q, k, positions, rope.frequencies, None, None, rope.scale, rope.interleaved)
+    if not _ready:
+        _register_ops()
+    out = NotImplemented if _compiling() else _now(q, k, positions, rope.frequencies, None, None, rope.scale, rope.interleaved)
+    return _call(q, k, positions, rope.frequencies, None, None, rope.scale, rope.interleaved) if out is NotImplemented else out
 
 
 def rotary_tables(q, k, cos, sin, interleaved=False):
     """`rotary` with tables of the angles' cosines and sines, (B, S, R / 2) or (1, S, R / 2), whatever factor they hold."""
-    return _call(q, k, None, None, cos, sin, 1.0, interleaved)
+    if not _ready:
+        _register_ops()
+    out = NotImplemented if _compiling() else _now(q, k, None, None, cos, sin, 1.0, interleaved)
+    return _call(q, k, None, None, cos, sin, 1.0, interleaved) if out is NotImplemented else out
 
 
 def hip_rotary_pos_emb(q, k, cos, sin, unsqueeze_dim=1):
