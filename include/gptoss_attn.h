@@ -399,8 +399,56 @@ int gptoss_attn_paged_fwd(const gptoss_attn_paged_params *params, void *stream);
 /* Bytes of scratch gptoss_attn_paged_fwd needs for this block (0: none; 0 for a NULL or shapeless block).  Host-only. */
 size_t gptoss_attn_paged_workspace_bytes(const gptoss_attn_paged_params *params);
 
-/* Host-only argument check that each of the three calls starts with; `call`: 0 fwd, 1 write, 2 read. */
+/*
+ * New tokens to slots of their own: token i of the Sq tokens of k and v (B = 1) goes to slot slots[i], that is to token
+ * slots[i] % page_size of page slots[i] / page_size.  Slots below 0 or behind the pool are dropped.  Of the block's page table, start and
+ * seqlens nothing is read.
+ */
+int gptoss_attn_paged_write_slots(const gptoss_attn_paged_params *params, const int64_t *slots, void *stream);
+
+/* Host-only argument check that each of the four calls starts with; `call`: 0 fwd, 1 write, 2 read, 3 write_slots. */
 int gptoss_attn_paged_validate(const gptoss_attn_paged_params *params, int call);
+
+/* ---- page tables -------------------------------------------------------------------------------------------------
+ *
+ * Which pages rows have, and where the tokens of a call go, from lengths on the device (the reference has no counterpart).
+ * Tables are those of the cache above: page_table (B, table_width) int32, rows table_stride apart, page_size a power of two from
+ * 16 to 1024; at most 16384 rows.  Lengths below 0 count as 0.
+ */
+typedef struct gptoss_attn_table_params {
+    uint32_t struct_size;           /* sizeof(gptoss_attn_table_params) */
+    int32_t B, table_width, page_size;
+    int32_t pages;                  /* update: of the pool, at most 2^30 */
+    int32_t total;                  /* map: entries of its results, at most 2^30 */
+    int64_t table_stride;
+    int32_t *page_table;            /* written by update */
+    const int32_t *have, *want;     /* (B), update: tokens that the rows' pages hold and shall hold; map: position of a row's first
+                                       new token (have) and how many it has (want) */
+    int32_t *seqlens, *left;        /* update: (B), (1) */
+    int32_t *row, *position, *first;        /* map: (total) each */
+    int64_t *slot;
+    int32_t *used;                  /* map: (1) */
+} gptoss_attn_table_params;
+
+/*
+ * Rows of have[b] tokens get pages for want[b].  A row keeps its first ceil(min(have, want) / page_size) entries; every page that no
+ * kept entry names is free, so rows that share one keep it until the last of them gives it back.  Rows that grow get the free pages
+ * in ascending order, row by row; seqlens[b] = want[b].  Where the pages a row wants, with those of the rows in front of it, are more
+ * than are free, the row gets none, nor does any behind it that wants some: their entries stay and seqlens[b] = have[b], as where a row wants
+ * more than its table holds (which no other row suffers from).  Entries that a row gives back become -1; others are not touched.
+ * left: free pages afterwards.  One workgroup: the order of nothing depends on the time.
+ */
+int gptoss_attn_page_table_update(const gptoss_attn_table_params *params, void *stream);
+
+/*
+ * Tokens of a call that has want[b] of each row, back to back in the order of the rows.  For token t: its row, its position
+ * have[row] + i (i: its number among the row's), first = t - i, slot = page * page_size + position % page_size, -1 where it has no page.
+ * Behind the last token: row -1, position 0, slot -1, first = used, the number of tokens (at most total).
+ */
+int gptoss_attn_token_map(const gptoss_attn_table_params *params, void *stream);
+
+/* Host-only argument check that both start with; `call`: 0 update, 1 map. */
+int gptoss_attn_table_validate(const gptoss_attn_table_params *params, int call);
 
 /* ---- rotary positions --------------------------------------------------------------------------------------------
  *

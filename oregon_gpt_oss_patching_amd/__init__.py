@@ -12,6 +12,11 @@ from .attention_kernel import (  # noqa: F401
     hip_flash_attention,
     triton_flash_attention,
 )
+from .page_tables import (  # noqa: F401
+    TokenMap,
+    page_table_update,
+    token_map,
+)
 from .paged_cache import (  # noqa: F401
     PagedCache,
     PagedState,
@@ -20,6 +25,7 @@ from .paged_cache import (  # noqa: F401
     paged_cache,
     paged_cache_read,
     paged_cache_write,
+    paged_cache_write_tokens,
 )
 from .rotary_positions import (  # noqa: F401
     Rotary,
@@ -31,5 +37,5 @@ from .rotary_positions import (  # noqa: F401
 
 __all__ = ["attention", "attention_forward", "attention_backward", "doc_start_from_position_ids",
            "hip_flash_attention", "triton_flash_attention",
-           "PagedCache", "PagedState", "paged_cache", "paged_cache_write", "paged_cache_read", "paged_attention", "paged_attention_forward",
-           "Rotary", "rotary", "rotary_frequencies", "rotary_tables", "hip_rotary_pos_emb"]
+           "PagedCache", "PagedState", "paged_cache", "paged_cache_write", "paged_cache_write_tokens", "paged_cache_read", "paged_attention", "paged_attention_forward",
+           "TokenMap", "page_table_update", "token_map", "Rotary", "rotary", "rotary_frequencies", "rotary_tables", "hip_rotary_pos_emb"]

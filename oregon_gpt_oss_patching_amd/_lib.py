@@ -43,6 +43,10 @@ EXPORTS = (
     "gptoss_attn_paged_read",
     "gptoss_attn_paged_workspace_bytes",
     "gptoss_attn_paged_validate",
+    "gptoss_attn_paged_write_slots",
+    "gptoss_attn_page_table_update",
+    "gptoss_attn_token_map",
+    "gptoss_attn_table_validate",
     "gptoss_attn_rotary",
     "gptoss_attn_rotary_validate",
     "gptoss_attn_mfma_rate_probe",
@@ -109,6 +113,19 @@ class PagedParams(ctypes.Structure):
         ("q_stride", Strides), ("o_stride", Strides), ("k_stride", Strides), ("v_stride", Strides),
         ("k_page_stride", Strides), ("v_page_stride", Strides), ("k_exp_stride", Strides), ("v_exp_stride", Strides),
         ("table_stride", ctypes.c_int64),
+    ]
+
+
+class TableParams(ctypes.Structure):
+    """Mirror of `gptoss_attn_table_params`; field order and types must match the header."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("B", ctypes.c_int32), ("table_width", ctypes.c_int32), ("page_size", ctypes.c_int32), ("pages", ctypes.c_int32), ("total", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64),
+        ("page_table", ctypes.c_void_p), ("have", ctypes.c_void_p), ("want", ctypes.c_void_p),
+        ("seqlens", ctypes.c_void_p), ("left", ctypes.c_void_p),
+        ("row", ctypes.c_void_p), ("position", ctypes.c_void_p), ("first", ctypes.c_void_p), ("slot", ctypes.c_void_p), ("used", ctypes.c_void_p),
     ]
 
 
@@ -195,6 +212,14 @@ def load() -> ctypes.CDLL:
         lib.gptoss_attn_paged_workspace_bytes.argtypes = [ctypes.POINTER(PagedParams)]
         lib.gptoss_attn_paged_validate.restype = ctypes.c_int
         lib.gptoss_attn_paged_validate.argtypes = [ctypes.POINTER(PagedParams), ctypes.c_int]
+        lib.gptoss_attn_paged_write_slots.restype = ctypes.c_int
+        lib.gptoss_attn_paged_write_slots.argtypes = [ctypes.POINTER(PagedParams), ctypes.c_void_p, ctypes.c_void_p]
+        for name in ("gptoss_attn_page_table_update", "gptoss_attn_token_map"):
+            fn = getattr(lib, name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(TableParams), ctypes.c_void_p]
+        lib.gptoss_attn_table_validate.restype = ctypes.c_int
+        lib.gptoss_attn_table_validate.argtypes = [ctypes.POINTER(TableParams), ctypes.c_int]
         lib.gptoss_attn_rotary.restype = ctypes.c_int
         lib.gptoss_attn_rotary.argtypes = [ctypes.POINTER(RotaryParams), ctypes.c_void_p]
         lib.gptoss_attn_rotary_validate.restype = ctypes.c_int
@@ -217,8 +242,8 @@ def load_torch_ops() -> None:
 
 
 def direct_calls(name: str = "gptoss_paged_direct"):
-    """Calls of libgptoss_torch.so as Python functions that do not go through the dispatcher: (paged_write, paged_read, paged_fwd), or the
-    rotary call ("gptoss_rotary_direct")."""
+    """Calls of libgptoss_torch.so as Python functions that do not go through the dispatcher: (paged_write, paged_read, paged_fwd,
+    paged_write_slots), (page_table_update, token_map) ("gptoss_tables_direct") or the rotary call ("gptoss_rotary_direct")."""
     f = getattr(ctypes.PyDLL(TORCH_LIBRARY), name)
     f.restype = ctypes.py_object
     return f()

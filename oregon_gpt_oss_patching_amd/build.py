@@ -20,6 +20,7 @@ ROTARY_SOURCE = os.path.join(_HERE, "csrc", "gptoss_rotary.hip")
 LIBRARY = os.path.join(_HERE, "libgptoss_attn.so")
 TORCH_SOURCE = os.path.join(_HERE, "csrc", "torch_ops.cpp")
 TORCH_PAGED_SOURCE = os.path.join(_HERE, "csrc", "torch_paged.cpp")
+TORCH_TABLES_SOURCE = os.path.join(_HERE, "csrc", "torch_tables.cpp")
 TORCH_ROTARY_SOURCE = os.path.join(_HERE, "csrc", "torch_rotary.cpp")
 TORCH_LIBRARY = os.path.join(_HERE, "libgptoss_torch.so")
 
@@ -78,7 +79,7 @@ def build_torch_ops(verbose: bool = False) -> str:
     flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
              "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
              "-isystem", os.path.join(rocm, "include"), "-isystem", sysconfig.get_paths()["include"]]
-    with _objects(lambda s, o: [gxx, *flags, "-c", "-o", o, s], (TORCH_SOURCE, TORCH_PAGED_SOURCE, TORCH_ROTARY_SOURCE), verbose) as objects:
+    with _objects(lambda s, o: [gxx, *flags, "-c", "-o", o, s], (TORCH_SOURCE, TORCH_PAGED_SOURCE, TORCH_TABLES_SOURCE, TORCH_ROTARY_SOURCE), verbose) as objects:
         _run([gxx, "-shared", "-o", TORCH_LIBRARY, *objects, "-L" + os.path.join(root, "lib"), "-lc10", "-ltorch_cpu", "-lc10_hip", "-ltorch_hip", "-ltorch_python",
               "-L" + _HERE, "-lgptoss_attn", "-Wl,-rpath,$ORIGIN"], verbose)
     return TORCH_LIBRARY

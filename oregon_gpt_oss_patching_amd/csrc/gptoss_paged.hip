@@ -3,13 +3,16 @@
 
 #include "../../include/gptoss_attn.h"
 #include "attn_paged.h"
+#include "page_tables.h"
 #include "paged_cache.h"
 
 using namespace gptoss;
 
 namespace {
 
-enum Call { kFwd = 0, kWrite = 1, kRead = 2 };
+enum Call { kFwd = 0, kWrite = 1, kRead = 2, kWriteSlots = 3 };
+
+bool page_size_ok(int n) { return n >= 16 && n <= 1024 && (n & (n - 1)) == 0; }
 
 bool aligned(const void *p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -57,11 +60,27 @@ PagedArgs make_args(const gptoss_attn_paged_params *p) {
     return a;
 }
 
+TableArgs table_args(const gptoss_attn_table_params *p) {
+    TableArgs a{};
+    a.table = p->page_table;
+    a.have = p->have; a.want = p->want;
+    a.seqlens = p->seqlens; a.left = p->left;
+    a.row = p->row; a.position = p->position; a.first = p->first; a.used = p->used;
+    a.slot = p->slot;
+    a.stride = p->table_stride;
+    a.B = p->B; a.width = p->table_width; a.pages = p->pages; a.total = p->total;
+    a.page_shift = __builtin_ctz((unsigned)p->page_size);
+    // a row's entries are read by all threads where there is one row, by sixteen from 64 rows on
+    a.row_threads_shift = 10;
+    for (int rows = 1; rows < p->B && rows < 64; rows *= 2) --a.row_threads_shift;
+    return a;
+}
+
 // One launch; a launch that fails reports its own status.
-template <typename Kernel>
-int launch(Kernel kernel, int64_t workgroups, int threads, void *stream, const PagedArgs &a) {
+template <typename Kernel, typename Args>
+int launch(Kernel kernel, int64_t workgroups, int threads, void *stream, const Args &a) {
     if (workgroups <= 0 || workgroups > 0x7fffffff) return GPTOSS_ATTN_ERR_SHAPE;
-    void *args[] = {const_cast<PagedArgs *>(&a)};
+    void *args[] = {const_cast<Args *>(&a)};
     const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3((unsigned)workgroups), dim3((unsigned)threads), args, 0,
                                          static_cast<hipStream_t>(stream));
     return e == hipSuccess ? GPTOSS_ATTN_OK : static_cast<int>(e);
@@ -162,19 +181,22 @@ int gptoss_attn_paged_validate(const gptoss_attn_paged_params *p, int call) {
     if (p->D != kD) return GPTOSS_ATTN_ERR_HEAD_DIM;
     if (p->G <= 0 || (call == kFwd && (p->H <= 0 || p->H % p->G))) return GPTOSS_ATTN_ERR_HEADS;
     if (p->B <= 0 || p->Sq <= 0 || p->Sq > (1 << 30)) return GPTOSS_ATTN_ERR_SHAPE;
-    if (p->pages <= 0 || p->table_width <= 0 || p->table_stride < 0 || p->page_size < 16 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)) ||
-        (int64_t)p->table_width * p->page_size > (1 << 30))
-        return GPTOSS_ATTN_ERR_PAGES;
+    if (p->pages <= 0 || !page_size_ok(p->page_size)) return GPTOSS_ATTN_ERR_PAGES;
+    const bool table = call != kWriteSlots;
+    if (table && (p->table_width <= 0 || p->table_stride < 0 || (int64_t)p->table_width * p->page_size > (1 << 30))) return GPTOSS_ATTN_ERR_PAGES;
+    if (!table && p->B != 1) return GPTOSS_ATTN_ERR_SHAPE;
     const int eb = p->dtype == GPTOSS_ATTN_FP32 ? 4 : 2;
     const bool codes = p->storage == GPTOSS_ATTN_E4M3;
     int rc;
     if ((rc = check_rows(p->k_pages, p->k_page_stride, codes ? 1 : eb))) return rc;
     if ((rc = check_rows(p->v_pages, p->v_page_stride, codes ? 1 : eb))) return rc;
-    if (!p->page_table || (codes && (!p->k_exp || !p->v_exp))) return GPTOSS_ATTN_ERR_NULL_TENSOR;
+    if ((table && !p->page_table) || (codes && (!p->k_exp || !p->v_exp))) return GPTOSS_ATTN_ERR_NULL_TENSOR;
     if (!pool_fits(p->k_page_stride, codes ? 1 : eb) || !pool_fits(p->v_page_stride, codes ? 1 : eb)) return GPTOSS_ATTN_ERR_STRIDE;
     if (codes && (!pool_fits(p->k_exp_stride, 1) || !pool_fits(p->v_exp_stride, 1))) return GPTOSS_ATTN_ERR_STRIDE;
-    if (!aligned(p->page_table, 4) || !aligned(p->seqlens, 4) || !aligned(p->start, 4)) return GPTOSS_ATTN_ERR_ALIGNMENT;
-    if (call == kWrite ? !p->start : !p->seqlens) return GPTOSS_ATTN_ERR_NULL_TENSOR;
+    if (table) {
+        if (!aligned(p->page_table, 4) || !aligned(p->seqlens, 4) || !aligned(p->start, 4)) return GPTOSS_ATTN_ERR_ALIGNMENT;
+        if (call == kWrite ? !p->start : !p->seqlens) return GPTOSS_ATTN_ERR_NULL_TENSOR;
+    }
     if (call != kFwd) {
         if ((rc = check_rows(p->k, p->k_stride, eb))) return rc;
         return check_rows(p->v, p->v_stride, eb);
@@ -249,6 +271,54 @@ int gptoss_attn_paged_read(const gptoss_attn_paged_params *p, void *stream) {
     if (p->dtype == GPTOSS_ATTN_BF16)
         return codes ? launch(paged_read_kernel<bf16, e4m3>, grid, 256, stream, a) : launch(paged_read_kernel<bf16, bf16>, grid, 256, stream, a);
     return codes ? launch(paged_read_kernel<float, e4m3>, grid, 256, stream, a) : launch(paged_read_kernel<float, float>, grid, 256, stream, a);
+}
+
+int gptoss_attn_paged_write_slots(const gptoss_attn_paged_params *p, const int64_t *slots, void *stream) {
+    const int rc = gptoss_attn_paged_validate(p, kWriteSlots);
+    if (rc) return rc;
+    if (!slots) return GPTOSS_ATTN_ERR_NULL_TENSOR;
+    if (!aligned(slots, 8)) return GPTOSS_ATTN_ERR_ALIGNMENT;
+    PagedArgs a = make_args(p);
+    const int64_t rows = (int64_t)a.Sq * a.G;
+    if (rows > (1 << 30)) return GPTOSS_ATTN_ERR_SHAPE;
+    a.by_g = div_by(a.G);
+    const bool codes = p->storage == GPTOSS_ATTN_E4M3;
+    const void *kernel = p->dtype == GPTOSS_ATTN_BF16
+                             ? (codes ? reinterpret_cast<const void *>(paged_write_slots_kernel<bf16, true>) : reinterpret_cast<const void *>(paged_write_slots_kernel<bf16, false>))
+                             : (codes ? reinterpret_cast<const void *>(paged_write_slots_kernel<float, true>) : reinterpret_cast<const void *>(paged_write_slots_kernel<float, false>));
+    void *args[] = {&a, const_cast<int64_t **>(&slots)};
+    const hipError_t e = hipLaunchKernel(kernel, dim3((unsigned)((rows + 31) / 32)), dim3(256), args, 0, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? GPTOSS_ATTN_OK : static_cast<int>(e);
+}
+
+int gptoss_attn_table_validate(const gptoss_attn_table_params *p, int call) {
+    if (!p) return GPTOSS_ATTN_ERR_NULL_PARAMS;
+    if (p->struct_size != sizeof(gptoss_attn_table_params)) return GPTOSS_ATTN_ERR_ABI;
+    if (p->B <= 0 || p->B > kTableRows) return GPTOSS_ATTN_ERR_SHAPE;
+    // (rows of a table that is written must not overlap)
+    if (!page_size_ok(p->page_size) || p->table_width <= 0 || (int64_t)p->table_width * p->page_size > (1 << 30) || p->table_stride < (call || p->B == 1 ? 0 : p->table_width))
+        return GPTOSS_ATTN_ERR_PAGES;
+    if (call ? p->total < 0 || p->total > (1 << 30) : p->pages <= 0 || p->pages > (1 << 30)) return call ? GPTOSS_ATTN_ERR_SHAPE : GPTOSS_ATTN_ERR_PAGES;
+    for (const void *t : {static_cast<const void *>(p->page_table), static_cast<const void *>(p->have), static_cast<const void *>(p->want),
+                          static_cast<const void *>(call ? p->row : p->seqlens), static_cast<const void *>(call ? p->position : p->left),
+                          static_cast<const void *>(call ? p->first : p->left), static_cast<const void *>(call ? p->used : p->left)}) {
+        if (!t) return GPTOSS_ATTN_ERR_NULL_TENSOR;
+        if (!aligned(t, 4)) return GPTOSS_ATTN_ERR_ALIGNMENT;
+    }
+    if (call && !p->slot) return GPTOSS_ATTN_ERR_NULL_TENSOR;
+    return call && !aligned(p->slot, 8) ? GPTOSS_ATTN_ERR_ALIGNMENT : GPTOSS_ATTN_OK;
+}
+
+int gptoss_attn_page_table_update(const gptoss_attn_table_params *p, void *stream) {
+    const int rc = gptoss_attn_table_validate(p, 0);
+    return rc ? rc : launch(page_table_update_kernel, 1, kTableThreads, stream, table_args(p));
+}
+
+int gptoss_attn_token_map(const gptoss_attn_table_params *p, void *stream) {
+    const int rc = gptoss_attn_table_validate(p, 1);
+    if (rc) return rc;
+    const int blocks = (p->total + kMapTokens - 1) / kMapTokens;
+    return launch(token_map_kernel, blocks ? blocks : 1, kMapThreads, stream, table_args(p));
 }
 
 }  // extern "C"

@@ -90,6 +90,21 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const PagedArgs a) {
     write_piece<T, E4M3>(a.vp, a.ve, page, at, g, c8, v);
 }
 
+// The same of one batch row whose tokens have slots of their own.
+template <typename T, bool E4M3>
+__global__ __launch_bounds__(256) void paged_write_slots_kernel(const PagedArgs a, const int64_t *slots) {
+    const int row = blockIdx.x * 32 + (threadIdx.x >> 3), c8 = (threadIdx.x & 7) * 8;
+    const int i = a.by_g.quotient(row), g = row - i * a.G;
+    if (i >= a.Sq) return;                                           // (all eight lanes of the row)
+    const Piece<T> k = load_piece(reinterpret_cast<const T *>(a.k) + g * a.ks.h + i * a.ks.s + c8);
+    const Piece<T> v = load_piece(reinterpret_cast<const T *>(a.v) + g * a.vs.h + i * a.vs.s + c8);
+    const int64_t slot = slots[i], page = slot >> a.page_shift;
+    if (slot < 0 || page >= a.pages) return;
+    const int at = (int)slot & ((1 << a.page_shift) - 1);
+    write_piece<T, E4M3>(a.kp, a.ke, (int)page, at, g, c8, k);
+    write_piece<T, E4M3>(a.vp, a.ve, (int)page, at, g, c8, v);
+}
+
 // Rows of a (batch row, KV head), which lie side by side in the result; one to a lane (two: eight prompts of up to 12000 tokens in e4m3, and their
 // last chunks written, 58 us and not 52).  The result is streamed past the caches' retention (the same 56.7 us without that), as are rows of whole
 // cache lines on their way in (16000 tokens of eight rows in bfloat16 106 us with neither, 97 with the first, 90 with both; codes 46 and 56).

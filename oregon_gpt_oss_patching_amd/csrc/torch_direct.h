@@ -29,6 +29,11 @@ inline Tensor int32_on(const Tensor &t, const Tensor &pages) {
     return (wide ? t.to(at::kLong).clamp(INT_MIN, INT_MAX) : t).to(pages.device(), at::kInt);
 }
 
+// Before a launch that writes into tensors of the caller: this refuses those that were made in inference mode and are written outside of it.
+inline void about_to_write(std::initializer_list<const Tensor *> tensors) {
+    for (const Tensor *t : tensors)
+        if (t) t->unsafeGetTensorImpl()->bump_version();
+}
 
 // What a tensor asks for (most have no record of either): a gradient, which torch.no_grad() takes back, or the tangent of forward mode, which it does not.
 inline bool wants_gradient(const Tensor &t) { return t.unsafeGetTensorImpl()->autograd_meta() && t.requires_grad(); }
@@ -98,6 +103,18 @@ inline PyObject *pair(const Pair &x) {
     const pybind11::object a = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::get<0>(x))),
                            b = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::get<1>(x)));
     return a && b ? PyTuple_Pack(2, a.ptr(), b.ptr()) : nullptr;
+}
+
+// A tuple of Python functions.
+template <size_t N>
+inline PyObject *functions_of(PyMethodDef (&defs)[N]) {
+    PyObject *out = PyTuple_New(N);
+    for (size_t i = 0; out && i < N; ++i) {
+        PyObject *f = PyCFunction_New(&defs[i], nullptr);
+        if (!f) { Py_DECREF(out); return nullptr; }
+        PyTuple_SET_ITEM(out, i, f);
+    }
+    return out;
 }
 
 }  // namespace

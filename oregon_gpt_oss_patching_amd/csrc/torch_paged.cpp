@@ -1,7 +1,7 @@
 // PyTorch operators of the key / value cache in pages (gptoss_attn_paged_* in include/gptoss_attn.h): argument checks, allocation and launch.
 //
-//   gptoss_attn::paged_write, paged_read, paged_fwd      the three library calls; none has a gradient (an operator cannot return None: an empty
-//                                                        lse stands for "not requested")
+//   gptoss_attn::paged_write, paged_write_slots, paged_read, paged_fwd      the four library calls; none has a gradient (an operator cannot return None: an
+//                                                        empty lse stands for "not requested")
 //
 // Native for the same reason as attention() (torch_ops.cpp): a decoding step makes two of these calls for each layer, and each takes
 // a few microseconds on the GPU.
@@ -32,9 +32,8 @@ Tensor lengths_of(const Tensor &t, const Tensor &pages, int64_t batch, const cha
     return int32_on(t, pages).contiguous();
 }
 
-// The cache, the table and what all calls have; `dtype`: the model's type.
-void fill(PagedCall &c, const Tensor &k_pages, const Tensor &v_pages, const OptTensor &k_exp, const OptTensor &v_exp, const Tensor &page_table,
-          at::ScalarType dtype, int64_t batch) {
+// The cache; `dtype`: the model's type.
+void fill_cache(PagedCall &c, const Tensor &k_pages, const Tensor &v_pages, const OptTensor &k_exp, const OptTensor &v_exp, at::ScalarType dtype, int64_t batch) {
     TORCH_CHECK(k_pages.is_cuda(), "gptoss attention runs on the GPU only (HIP kernels); the cache is on ", k_pages.device());
     require_near(k_pages, "v of the cache", v_pages);
     const auto storage = k_pages.scalar_type();
@@ -67,6 +66,13 @@ void fill(PagedCall &c, const Tensor &k_pages, const Tensor &v_pages, const OptT
     p.v_pages = const_cast<void *>(v_pages.const_data_ptr());
     set3(p.k_page_stride, k_pages);
     set3(p.v_page_stride, v_pages);
+}
+
+// The cache, the table and what all calls with one have.
+void fill(PagedCall &c, const Tensor &k_pages, const Tensor &v_pages, const OptTensor &k_exp, const OptTensor &v_exp, const Tensor &page_table,
+          at::ScalarType dtype, int64_t batch) {
+    fill_cache(c, k_pages, v_pages, k_exp, v_exp, dtype, batch);
+    gptoss_attn_paged_params &p = c.p;
     TORCH_CHECK(page_table.dim() == 2 && page_table.size(0) == batch && is_integers(page_table), "page_table must be (B, pages of a row) integers, got ",
                 page_table.sizes(), " for ", batch, " rows");
     c.table = int32_on(page_table, k_pages);
@@ -88,6 +94,19 @@ Tensor rows_of(const Tensor &t, gptoss_attn_strides &s) {
         return t;
     const Tensor r = t.clone(at::MemoryFormat::Contiguous);
     set3(s, r);
+    return r;
+}
+
+// Tokens (T, G, 64) as a batch row of theirs.
+Tensor tokens_of(const Tensor &t, gptoss_attn_strides &s) {
+    const int64_t per16 = 16 / t.element_size();
+    s.b = 0;
+    s.h = t.size(1) == 1 ? 0 : t.stride(1);
+    s.s = t.size(0) == 1 ? 64 : t.stride(0);
+    if (t.stride(2) == 1 && s.h % per16 == 0 && s.s % per16 == 0 && s.s >= 64 && s.s <= kMaxSeqStride && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0) return t;
+    const Tensor r = t.clone(at::MemoryFormat::Contiguous);
+    s.h = r.stride(1);
+    s.s = r.stride(0);
     return r;
 }
 
@@ -115,10 +134,33 @@ void paged_write(const Tensor &k_pages, const Tensor &v_pages, const OptTensor &
         c.seqlens = lengths_of(*seqlens, k_pages, c.p.B, "seqlens");
         c.p.seqlens = c.seqlens.const_data_ptr<int32_t>();
     }
-    // (this refuses a cache that was made in inference mode and is written outside of it: before the launch, not after)
-    for (const Tensor *t : {&k_pages, &v_pages, k_exp ? &*k_exp : nullptr, v_exp ? &*v_exp : nullptr})
-        if (t) t->unsafeGetTensorImpl()->bump_version();
+    about_to_write({&k_pages, &v_pages, k_exp ? &*k_exp : nullptr, v_exp ? &*v_exp : nullptr});
     check("gptoss_attn_paged_write", gptoss_attn_paged_write(&c.p, stream_of(k_pages)));
+}
+
+// k, v (T, G, 64) to slots of their own.
+void paged_write_slots(const Tensor &k_pages, const Tensor &v_pages, const OptTensor &k_exp, const OptTensor &v_exp, const Tensor &k_, const Tensor &v_, const Tensor &slots_) {
+    const c10::OptionalDeviceGuard guard(k_pages.device());
+    TORCH_CHECK(k_.scalar_type() == v_.scalar_type(), "k and v must be of one type, got ", k_.scalar_type(), " and ", v_.scalar_type());
+    TORCH_CHECK(k_.dim() == 3 && k_.sizes() == v_.sizes(), "k and v must both be (T, G, 64), got ", k_.sizes(), " and ", v_.sizes());
+    const bool half = k_.scalar_type() == at::kHalf;
+    PagedCall c;
+    fill_cache(c, k_pages, v_pages, k_exp, v_exp, half ? at::kBFloat16 : k_.scalar_type(), 1);
+    TORCH_CHECK(k_.size(1) == c.p.G && k_.size(2) == 64, "k and v must be (T, ", c.p.G, ", 64) for this cache, got ", k_.sizes());
+    TORCH_CHECK(slots_.dim() == 1 && slots_.size(0) == k_.size(0) && is_integers(slots_), "slots must hold one integer per token, got ", slots_.scalar_type(), " ", slots_.sizes(),
+                " for ", k_.size(0));
+    require_near(k_pages, "k", k_);
+    require_near(k_pages, "v", v_);
+    if (k_.size(0) == 0) return;
+    c.k = tokens_of(half ? k_.to(at::kBFloat16) : k_, c.p.k_stride);
+    c.v = tokens_of(half ? v_.to(at::kBFloat16) : v_, c.p.v_stride);
+    c.p.k = const_cast<void *>(c.k.const_data_ptr());
+    c.p.v = const_cast<void *>(c.v.const_data_ptr());
+    c.p.Sq = size32(k_.size(0));
+    c.start = slots_.scalar_type() == at::kLong && slots_.device() == k_pages.device() ? slots_ : slots_.to(k_pages.device(), at::kLong);
+    if (c.start.stride(0) != 1) c.start = c.start.contiguous();
+    about_to_write({&k_pages, &v_pages, k_exp ? &*k_exp : nullptr, v_exp ? &*v_exp : nullptr});
+    check("gptoss_attn_paged_write_slots", gptoss_attn_paged_write_slots(&c.p, c.start.const_data_ptr<int64_t>(), stream_of(k_pages)));
 }
 
 std::tuple<Tensor, Tensor> paged_read(const Tensor &k_pages, const Tensor &v_pages, const OptTensor &k_exp, const OptTensor &v_exp, const Tensor &page_table,
@@ -206,6 +248,7 @@ std::tuple<Tensor, Tensor> paged_fwd(const Tensor &q, const Tensor &k_pages, con
 TORCH_LIBRARY_FRAGMENT(gptoss_attn, m) {
     m.def("paged_write(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_exp, Tensor(d!)? v_exp, Tensor k, Tensor v, Tensor page_table, Tensor start, "
           "Tensor? seqlens) -> ()");
+    m.def("paged_write_slots(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_exp, Tensor(d!)? v_exp, Tensor k, Tensor v, Tensor slots) -> ()");
     m.def("paged_read(Tensor k_pages, Tensor v_pages, Tensor? k_exp, Tensor? v_exp, Tensor page_table, Tensor seqlens, SymInt max_len, Tensor? start, "
           "ScalarType dtype) -> (Tensor, Tensor)");
     m.def("paged_fwd(Tensor q, Tensor k_pages, Tensor v_pages, Tensor? k_exp, Tensor? v_exp, Tensor page_table, Tensor seqlens, Tensor? start, Tensor? sinks, "
@@ -213,13 +256,14 @@ TORCH_LIBRARY_FRAGMENT(gptoss_attn, m) {
 }
 TORCH_LIBRARY_IMPL(gptoss_attn, CUDA, m) {
     m.impl("paged_write", &paged_write);
+    m.impl("paged_write_slots", &paged_write_slots);
     m.impl("paged_read", &paged_read);
     m.impl("paged_fwd", &paged_fwd);
 }
-#define GPTOSS_PAGED_IMPL(KEY, FN)                                                        \
-    TORCH_LIBRARY_IMPL(gptoss_attn, KEY, m) {                                             \
-        for (const char *name : {"paged_write", "paged_read", "paged_fwd"})               \
-            m.impl(name, torch::CppFunction::makeFromBoxedFunction<&FN>());               \
+#define GPTOSS_PAGED_IMPL(KEY, FN)                                                               \
+    TORCH_LIBRARY_IMPL(gptoss_attn, KEY, m) {                                                    \
+        for (const char *name : {"paged_write", "paged_write_slots", "paged_read", "paged_fwd"}) \
+            m.impl(name, torch::CppFunction::makeFromBoxedFunction<&FN>());                      \
     }
 GPTOSS_PAGED_IMPL(Autograd, refuse_gradients)
 GPTOSS_PAGED_IMPL(CPU, refuse_cpu)
@@ -242,6 +286,21 @@ PyObject *write_now(PyObject *, PyObject *const *args, Py_ssize_t n) {
     {
         const pybind11::gil_scoped_release free;
         paged_write(k_pages, v_pages, k_exp, v_exp, k, v, table, start, seqlens);
+    }
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *write_slots_now(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7 || !direct_now()) return not_implemented();
+    Arguments a{args};
+    const Tensor &k_pages = a.tensor(0), &v_pages = a.tensor(1), &k = a.tensor(4), &v = a.tensor(5), &slots = a.tensor(6);
+    const OptTensor k_exp = a.optional(2), v_exp = a.optional(3);
+    if (!a.ok) return not_implemented();
+    {
+        const pybind11::gil_scoped_release free;
+        paged_write_slots(k_pages, v_pages, k_exp, v_exp, k, v, slots);
     }
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
@@ -288,17 +347,10 @@ PyMethodDef kDirect[] = {
     {"paged_write_now", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&write_now)), METH_FASTCALL, nullptr},
     {"paged_read_now", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&read_now)), METH_FASTCALL, nullptr},
     {"paged_fwd_now", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&fwd_now)), METH_FASTCALL, nullptr},
+    {"paged_write_slots_now", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&write_slots_now)), METH_FASTCALL, nullptr},
 };
 
 }  // namespace
 
-// (paged_write, paged_read, paged_fwd) for Python
-extern "C" PyObject *gptoss_paged_direct() {
-    PyObject *out = PyTuple_New(3);
-    for (int i = 0; out && i < 3; ++i) {
-        PyObject *f = PyCFunction_New(&kDirect[i], nullptr);
-        if (!f) { Py_DECREF(out); return nullptr; }
-        PyTuple_SET_ITEM(out, i, f);
-    }
-    return out;
-}
+// (paged_write, paged_read, paged_fwd, paged_write_slots) for Python
+extern "C" PyObject *gptoss_paged_direct() { return functions_of(kDirect); }

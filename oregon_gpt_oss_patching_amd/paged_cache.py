@@ -25,8 +25,9 @@ import torch
 
 from . import _lib
 from . import attention_kernel as _ak
+from .page_tables import TokenMap
 
-__all__ = ["PagedCache", "PagedState", "paged_cache", "paged_cache_write", "paged_cache_read", "paged_attention", "paged_attention_forward"]
+__all__ = ["PagedCache", "PagedState", "paged_cache", "paged_cache_write", "paged_cache_write_tokens", "paged_cache_read", "paged_attention", "paged_attention_forward"]
 
 
 class PagedCache(NamedTuple):
@@ -46,19 +47,27 @@ class PagedState(NamedTuple):
     caches: a `PagedCache` for each layer, by its `layer_idx`.  page_table (B, width): the same pages in each layer's pool.
     start (B): position of each row's first new token; None: the rows begin with this call, and attend to the new tokens as they came.
     seqlens (B): tokens of each row with the new ones.  counts (B): how many of the call's S tokens a row has, where not all have S, the rest being
-    padding (start=None: seqlens).  max_len: as in `paged_attention`."""
+    padding (start=None: seqlens).  max_len: as in `paged_attention`.
+    tokens: a `TokenMap` where the call is one batch row that holds new rows' tokens back to back (start=None, and the map made with starts of 0): the model gets
+    tokens.position as its position ids."""
     caches: Sequence[PagedCache]
     page_table: torch.Tensor
     start: Optional[torch.Tensor]
     seqlens: torch.Tensor
     counts: Optional[torch.Tensor] = None
     max_len: Optional[int] = None
+    tokens: Optional[TokenMap] = None
 
     def attend(self, module, q, k, v, sm_scale) -> torch.Tensor:
         """A layer's new keys and values into its cache, and its queries' attention."""
         if k.shape[2] != q.shape[2]:
             raise RuntimeError(f"paged= writes the new tokens' keys, as many as queries, got {k.shape[2]} for {q.shape[2]}: the pages hold the past, pass no past_key_values")
         cache, window = self.caches[module.layer_idx], module.sliding_window
+        if self.tokens is not None:
+            if self.start is not None or q.shape[0] != 1:
+                raise RuntimeError(f"tokens= is one batch row of rows that begin with this call: start must be None, got {'one' if self.start is not None else 'none'} and {q.shape[0]} batch rows")
+            paged_cache_write_tokens(cache, k[0].transpose(0, 1), v[0].transpose(0, 1), self.tokens.slot)
+            return _ak.attention(q, k, v, module.sinks, sm_scale, window, None, self.tokens.used, self.tokens.first[None])
         if self.start is None:
             n = _ints(self.seqlens, q)
             paged_cache_write(cache, k, v, self.page_table, torch.zeros_like(n), n)
@@ -81,17 +90,21 @@ def paged_cache(pages, kv_heads, page_size=64, storage=torch.bfloat16, device="c
 
 
 _ready = False
-_write = _read = _fwd = None
-_write_now = _read_now = _fwd_now = None        # the same without the dispatcher, NotImplemented where it is needed
+_write = _read = _fwd = _write_slots = None
+_write_now = _read_now = _fwd_now = _write_slots_now = None        # the same without the dispatcher, NotImplemented where it is needed
 
 
 def _register_ops() -> None:
-    global _ready, _write, _read, _fwd, _write_now, _read_now, _fwd_now
+    global _ready, _write, _read, _fwd, _write_slots, _write_now, _read_now, _fwd_now, _write_slots_now
     _lib.load_torch_ops()
     ops = torch.ops.gptoss_attn
 
     @torch.library.register_fake(f"{_ak.OP_NAMESPACE}::paged_write")
     def _write_fake(k_pages, v_pages, k_exp, v_exp, k, v, page_table, start, seqlens):
+        return None
+
+    @torch.library.register_fake(f"{_ak.OP_NAMESPACE}::paged_write_slots")
+    def _write_slots_fake(k_pages, v_pages, k_exp, v_exp, k, v, slots):
         return None
 
     @torch.library.register_fake(f"{_ak.OP_NAMESPACE}::paged_read")
@@ -104,8 +117,8 @@ def _register_ops() -> None:
         b, h, s, d = q.shape
         return q.new_empty((b, s, h, d)), q.new_empty((b, h, s) if need_lse else (0,), dtype=torch.float32)
 
-    _write_now, _read_now, _fwd_now = _lib.direct_calls()
-    _write, _read, _fwd = ops.paged_write.default, ops.paged_read.default, ops.paged_fwd.default
+    _write_now, _read_now, _fwd_now, _write_slots_now = _lib.direct_calls()
+    _write, _read, _fwd, _write_slots = ops.paged_write.default, ops.paged_read.default, ops.paged_fwd.default, ops.paged_write_slots.default
     _ready = True
 
 
@@ -133,6 +146,16 @@ def paged_cache_write(cache: PagedCache, k, v, page_table, start, seqlens=None) 
         _register_ops()
     if _compiling() or _write_now(*cache, k, v, page_table, start, seqlens) is NotImplemented:
         _write(*cache, k, v, _ints(page_table, cache.k), _ints(start, cache.k), _ints(seqlens, cache.k))
+
+
+def paged_cache_write_tokens(cache: PagedCache, k, v, slots) -> None:
+    """`paged_cache_write` of tokens that lie back to back, whatever rows they are of: k, v (T, G, 64), any strides; token t goes to slot
+    slots[t], that is to token slots[t] % page_size of page slots[t] // page_size (`token_map` says which).  Slots below 0 or behind the pool are dropped."""
+    if not _ready:
+        _register_ops()
+    if _compiling() or _write_slots_now(*cache, k, v, slots) is NotImplemented:
+        slots = slots if isinstance(slots, _Tensor) else torch.as_tensor(slots, dtype=torch.int64, device=cache.k.device)
+        _write_slots(*cache, k, v, slots)
 
 
 def paged_cache_read(cache: PagedCache, page_table, seqlens, max_len, start=None, dtype=None):
