@@ -61,8 +61,10 @@ enum gptoss_attn_dtype {
     GPTOSS_ATTN_FP32 = 1, /* 4-byte float tensors, fp32 MFMA products (the reference's fp32 mode,
                              attention_kernel.py is dtype-generic), at a sixteenth of the bf16 matrix rate;
                              larger calls with scratch: gptoss_attn_split_bytes */
-    GPTOSS_ATTN_E4M3 = 2  /* storage of a paged cache only: 8-bit numbers (sign, 4 exponent and 3 mantissa bits, largest
+    GPTOSS_ATTN_E4M3 = 2, /* storage of a paged cache only: 8-bit numbers (sign, 4 exponent and 3 mantissa bits, largest
                              448, no infinity) with a power of two for each row of 64 */
+    GPTOSS_ATTN_E2M1 = 3  /* storage of a paged cache only: 4-bit numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+                             negatives) with a power of two for each 32 of them */
 };
 
 enum gptoss_attn_status {
@@ -326,9 +328,10 @@ int gptoss_attn_validate(const gptoss_attn_params *params, int need_bwd);
  *
  * The serving side of the same layer; the reference has no counterpart (its generate.py leaves the cache to transformers,
  * one contiguous tensor per layer).  Keys and values of all sequences live in one pool of pages:
- *   k_pages, v_pages (pages, G, page_size, 64) in `storage`: the model's type (`dtype`), or GPTOSS_ATTN_E4M3
+ *   k_pages, v_pages (pages, G, page_size, 64) in `storage`: the model's type (`dtype`), or GPTOSS_ATTN_E4M3;
+ *                    GPTOSS_ATTN_E2M1: (pages, G, page_size, 32) bytes, number 2i of a row in the lower half of byte i
  *   k_exp, v_exp     (pages, G, page_size) bytes, E4M3 only: row values are code * 2^(byte - 127), infinite from 2^128 on; NaN
- *                    where the byte is 255
+ *                    where the byte is 255.  E2M1: (pages, G, page_size, 2) bytes, one for each half of a row, side by side
  *   page_table       (B, table_width) int32, rows table_stride apart: token t of row b is slot t % page_size of page
  *                    page_table[b][t / page_size].  An entry outside 0 .. pages - 1 names no page: what would be written
  *                    there is dropped, what would be read from there is 0, its keys are invisible.
@@ -339,11 +342,15 @@ int gptoss_attn_validate(const gptoss_attn_params *params, int need_bwd);
  * E4M3: a row's power of two is the smallest 2^s (s >= -64) with its largest finite number at most 448 * 2^s; the numbers
  * divided by it are rounded to nearest, ties to even, so each is within 2^-4 of itself, or 2^(s-10) where that is more.
  * Numbers that would come back as 2^128 are stored as 1.875 * 2^127, infinities and NaN as NaN.  What is read back is exact in bfloat16 as in float32.
+ *
+ * E2M1: the power of two of 32 numbers is the smallest 2^s (-64 <= s <= 125) with the largest of them at most 7 * 2^s; the numbers divided
+ * by it are rounded to nearest, ties to even, those above 6 to 6, so each is within 2^-2 of itself, or 2^(s-2) where that is more.  32 numbers
+ * with an infinity or a NaN among them are stored with the byte 255, as NaN.
  */
 typedef struct gptoss_attn_paged_params {
     uint32_t struct_size;   /* sizeof(gptoss_attn_paged_params), checked by every call */
     int32_t dtype;          /* GPTOSS_ATTN_BF16 or GPTOSS_ATTN_FP32: type of q, o, k and v */
-    int32_t storage;        /* = dtype, or GPTOSS_ATTN_E4M3 */
+    int32_t storage;        /* = dtype, or GPTOSS_ATTN_E4M3, or GPTOSS_ATTN_E2M1 (whose page strides are in bytes) */
     int32_t sinks_dtype;    /* GPTOSS_ATTN_FP32 or GPTOSS_ATTN_BF16 */
 
     int32_t B, H, G, Sq, D; /* Sq: query rows (fwd), new tokens of a row (write), rows of the result (read); H: fwd only */

@@ -23,8 +23,39 @@ def quantise(x):
     return torch.where((s == 120) & (y.abs() > 240.0), torch.sign(y) * 240.0, y), s[..., 0]
 
 
+GRID4 = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
+
+
+def quantise4(x):
+    """(numbers in units of their power of two, exponents (..., 2)) of rows (..., 64), 32 numbers at a time: the smallest s from -64 to 125 with the largest at most
+    7 * 2^s, the nearest number of the grid (of two equally near the one whose code is even), at most 6; where one is not finite all are NaN and s is 128."""
+    x = x.double().unflatten(-1, (2, 32))
+    finite = torch.isfinite(x).all(-1, keepdim=True)
+    top = x.abs().amax(-1, keepdim=True)
+    s = torch.full(top.shape, -64, dtype=torch.int64)
+    for e in range(-64, 125):
+        s = torch.where(top > 7.0 * 2.0 ** e, torch.full_like(s, e + 1), s)
+    y = x / torch.exp2(s.double())
+    distance = (y.abs()[..., None] - GRID4).abs()
+    nearest = distance == distance.amin(-1, keepdim=True)
+    code = (nearest * torch.tensor([8, 1, 7, 2, 6, 3, 5, 4])).argmax(-1)       # (even codes come first)
+    y = torch.where(finite, torch.sign(y) * GRID4[code], torch.full_like(y, float("nan")))
+    return y.flatten(-2), torch.where(finite, s, torch.full_like(s, 128))[..., 0]
+
+
+def values4(codes, exps):
+    """What bytes of codes (..., 32), two numbers each, with bytes of exponents (..., 2) stand for, in 64 bits: infinite from 2^128 on, NaN under 255."""
+    code = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).long()
+    x = torch.cat((GRID4, -GRID4))[code].unflatten(-1, (2, 32)) * torch.exp2(exps.double() - 127)[..., None]
+    x = torch.where(x.abs() >= 2.0 ** 128, torch.sign(x) * float("inf"), x)
+    return torch.where((exps == 255)[..., None], torch.full_like(x, float("nan")), x).flatten(-2)
+
+
 def stored_rows(x, storage):
     """What rows of x stand for once they are in a cache of `storage`."""
+    if storage == torch.float4_e2m1fn_x2:
+        y, s = quantise4(x)
+        return y * torch.exp2(s.double()).repeat_interleave(32, -1)
     if storage != torch.float8_e4m3fn:
         return x.double()
     y, s = quantise(x)

@@ -17,6 +17,7 @@ ABI_VERSION = 4
 DTYPE_BF16 = 0
 DTYPE_FP32 = 1
 DTYPE_E4M3 = 2          # storage of a paged cache only
+DTYPE_E2M1 = 3          # the same
 
 EXPORTS = (
     "gptoss_attn_version",

@@ -244,46 +244,26 @@ __device__ __forceinline__ void split_weights(const float (&x)[8], bf16x8 &hi, b
 // Of float32 queries over codes too: a code times its power of two is a bfloat16 number, and a float32 number is the sum of three (its 24 bits, eight
 // at a time), so three products of each kind take the place of the fp32 MFMA's, in a fifth of their time: 32 rows of 6000 to 16384 tokens 69 us, and 135 with those.
 // The smaller terms are added first, to 0: their roundings are then 2^-8 of the sum's.
-template <typename T, typename ST, int NB, int KB>
-struct PagedTile16 {
-    static constexpr bool kCodes = sizeof(ST) == 1, kOnce = NB < (sizeof(T) == 4 ? 2 : 4), kStagedK = !kCodes;
+// What the tiles share: the queries and the sums, and both products.
+template <typename T, int NB, int KB>
+struct PagedProducts16 {
     static constexpr int kTerms = sizeof(T) == 4 ? 3 : 1;
     static constexpr int kStage = 16 * KB * kRowBytes;           // LDS bytes of a wavefront
-    static constexpr int kVecs = kCodes ? 1 : 2;                 // 16-byte loads per lane and block
-    u32x4 k[KB][kVecs], v[KB][kVecs];
-    uint32_t ke[KB], ve[KB];
+    static constexpr bool kOnce = NB < (sizeof(T) == 4 ? 2 : 4);
     bf16x8 q[NB][kTerms][2];     // the largest term first
     f32x4 o[NB][4];
-    uint32_t tr[4], wr[2], nat[2], k_at[kVecs], v_at[kVecs], ke_at, ve_at;
+    uint32_t tr[4];
 
-    // (codes: rows 0, 1, 4, 5 and so on for each 16 lanes, which then write to distinct banks)
-    __device__ __forceinline__ static int v_row(int lane, int i) {
-        const int q = lane >> 2;
-        return kCodes ? (q & 9) | (q & 2) << 1 | (q & 4) >> 1 : (lane >> 3) + 8 * i;
-    }
-
-    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage, int lane) {
+    __device__ __forceinline__ void init_products(uint32_t stage, int lane) {
         const int i = lane & 15, quad = lane >> 4, row = 4 * quad + (i >> 2);
 #pragma unroll
         for (int d = 0; d < 4; ++d) tr[d] = stage + row * kRowBytes + (((2 * d + ((i & 3) >> 1)) ^ swz(row)) * 16) + (i & 1) * 8;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int r = v_row(lane, e), c = kCodes ? 2 * (lane & 3) + e : lane & 7;
-            wr[e] = stage + r * kRowBytes + ((c ^ swz(r)) * 16);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) nat[e] = stage + i * kRowBytes + (((4 * e + quad) ^ swz(i)) * 16);
-#pragma unroll
-        for (int e = 0; e < kVecs; ++e) k_at[e] = kCodes ? i * a.kp.s + 16 * quad : v_row(lane, e) * a.kp.s + 16 * (lane & 7);
-#pragma unroll
-        for (int e = 0; e < kVecs; ++e) v_at[e] = v_row(lane, e) * a.vp.s + 16 * (kCodes ? lane & 3 : lane & 7);
-        ke_at = i * a.ke.s;
-        ve_at = v_row(lane, 0) * a.ve.s;
     }
-    __device__ __forceinline__ void load_q(int nb, const T *row, bool there, int quad) {
+    // The lane's numbers of a query: eight from number at0 on, eight from at1 on.
+    __device__ __forceinline__ void load_numbers(int nb, const T *row, bool there, int at0, int at1) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const T *at = row + (kCodes ? 16 * quad + 8 * s : 32 * s + 8 * quad);
+            const T *at = row + (s ? at1 : at0);
             if constexpr (kTerms == 1) {
                 const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
                 q[nb][0][s] = as_bf16x8(there ? x : u32x4{0, 0, 0, 0});
@@ -302,6 +282,102 @@ struct PagedTile16 {
         }
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[nb][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // A block's keys `f`, in the queries' order, times the queries.
+    __device__ __forceinline__ void block_logits(const bf16x8 (&f)[2], int blk, f32x4 (&s)[NB][KB]) const {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int t = kTerms - 1; t >= 0; --t) {
+                z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[0], q[nb][t][0], z, 0, 0, 0);
+                z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[1], q[nb][t][1], z, 0, 0, 0);
+            }
+            s[nb][blk] = z;
+        }
+    }
+    __device__ __forceinline__ void product(const f32x4 (&s)[NB][KB]) {
+#pragma unroll
+        for (int h = 0; h < KB / 2; ++h) {
+            // A bfloat16 query's weights go in as two terms: one alone, half a step of bfloat16 of each weight, adds as much to the result's error as
+            // rounding it does (relative, 2-norm: 2.2e-3 in all and not 1.7e-3).  us, one term / two: 16 x 8192 tokens 48.7 / 48.9, in e4m3 30.7 / 31.1, one row of 2049 8.5 / 8.6,
+            // five queries on eight rows of 700 to 6000 17.6 / 18.3; where the arithmetic counts, eight queries on 16 x 8192 in e4m3, 43.0 / 49.5.
+            constexpr int kWeightTerms = kTerms == 1 ? 2 : kTerms;
+            bf16x8 p[NB][kWeightTerms];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = s[nb][2 * h + (e >> 2)][e & 3];
+                if constexpr (kTerms == 1) {
+                    split_weights(x, p[nb][0], p[nb][1]);
+                } else {
+#pragma unroll
+                    for (int t = 0; t < kTerms; ++t) p[nb][t] = take_upper(x);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                union { struct { s16x4 a, b; } s; bf16x8 v; } x;
+                x.s.a = lds_load_tr64(tr[d], 32 * h * kRowBytes);
+                x.s.b = lds_load_tr64(tr[d], (32 * h + 16) * kRowBytes);
+                if constexpr (kTerms == 1) {
+#pragma unroll
+                    for (int t = kWeightTerms - 1; t >= 0; --t)
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) o[nb][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb][t], o[nb][d], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int t = kTerms - 1; t >= 0; --t) z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb][t], z, 0, 0, 0);
+                        o[nb][d] += z;
+                    }
+                }
+            }
+        }
+    }
+    // column of o[.][d][e] in the lane's row
+    __device__ __forceinline__ static int column(int d, int e, int quad) { return 16 * d + 4 * quad + e; }
+};
+
+template <typename T, typename ST, int NB, int KB>
+struct PagedTile16 : PagedProducts16<T, NB, KB> {
+    using Base = PagedProducts16<T, NB, KB>;
+    using Base::kOnce;
+    static constexpr bool kCodes = sizeof(ST) == 1, kStagedK = !kCodes;
+    static constexpr int kVecs = kCodes ? 1 : 2;                 // 16-byte loads per lane and block
+    u32x4 k[KB][kVecs], v[KB][kVecs];
+    uint32_t ke[KB], ve[KB];
+    uint32_t wr[2], nat[2], k_at[kVecs], v_at[kVecs], ke_at, ve_at;
+
+    // (codes: rows 0, 1, 4, 5 and so on for each 16 lanes, which then write to distinct banks)
+    __device__ __forceinline__ static int v_row(int lane, int i) {
+        const int q = lane >> 2;
+        return kCodes ? (q & 9) | (q & 2) << 1 | (q & 4) >> 1 : (lane >> 3) + 8 * i;
+    }
+
+    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage, int lane) {
+        const int i = lane & 15, quad = lane >> 4;
+        Base::init_products(stage, lane);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = v_row(lane, e), c = kCodes ? 2 * (lane & 3) + e : lane & 7;
+            wr[e] = stage + r * kRowBytes + ((c ^ swz(r)) * 16);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) nat[e] = stage + i * kRowBytes + (((4 * e + quad) ^ swz(i)) * 16);
+#pragma unroll
+        for (int e = 0; e < kVecs; ++e) k_at[e] = kCodes ? i * a.kp.s + 16 * quad : v_row(lane, e) * a.kp.s + 16 * (lane & 7);
+#pragma unroll
+        for (int e = 0; e < kVecs; ++e) v_at[e] = v_row(lane, e) * a.vp.s + 16 * (kCodes ? lane & 3 : lane & 7);
+        ke_at = i * a.ke.s;
+        ve_at = v_row(lane, 0) * a.ve.s;
+    }
+    __device__ __forceinline__ void load_q(int nb, const T *row, bool there, int quad) {
+        if constexpr (kCodes) Base::load_numbers(nb, row, there, 16 * quad, 16 * quad + 8);
+        else Base::load_numbers(nb, row, there, 8 * quad, 32 + 8 * quad);
     }
     // `mask`: all ones, or 0 where there is no next tile (one address instead of a branch)
     __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb, uint32_t mask) {
@@ -332,16 +408,7 @@ struct PagedTile16 {
                 f[0] = as_bf16x8(lds_load128(nat[0], 16 * blk * kRowBytes));
                 f[1] = as_bf16x8(lds_load128(nat[1], 16 * blk * kRowBytes));
             }
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int t = kTerms - 1; t >= 0; --t) {
-                    z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[0], q[nb][t][0], z, 0, 0, 0);
-                    z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[1], q[nb][t][1], z, 0, 0, 0);
-                }
-                s[nb][blk] = z;
-            }
+            Base::block_logits(f, blk, s);
         }
     }
     // V into the stage.  Where `edge`: rows outside first .. last - 1 of the tile as zeros; with `several` queries, what is not finite in the
@@ -399,53 +466,123 @@ struct PagedTile16 {
             }
         return odd;
     }
-    __device__ __forceinline__ void product(const f32x4 (&s)[NB][KB]) {
+};
+
+// e2m1 pages: rows of 32 bytes and two bytes of exponents.  A load takes 32 rows, two blocks of keys, 16 bytes (32 numbers, which share a power) to a lane: of K, lanes below 32
+// halves of the first block's rows, those above of the second's, which one exchange between the two turns into both blocks' operands (quarter rows 0, 2, 1, 3 by quad: the queries come in that order);
+// of V, rows in the order in which 16 lanes write to distinct banks.  The two blocks may lie in different pages.
+template <typename T, int NB, int KB>
+struct PagedTile4 : PagedProducts16<T, NB, KB> {
+    using Base = PagedProducts16<T, NB, KB>;
+    using Base::kOnce;
+    static constexpr bool kCodes = true, kStagedK = false;
+    static constexpr int kPairs = KB / 2;
+    static_assert(KB % 2 == 0, "two blocks to a load");
+    u32x4 k[kPairs], v[kPairs];
+    uint32_t ke[kPairs], ve[kPairs];
+    uint32_t wr[4], k_at, v_at, ke_at, ve_at;
+    bool upper;
+    const char *first_row, *first_exp;           // of the pair's first block, until its second is known
+
+    // of the pair's 32 rows
+    __device__ __forceinline__ static int v_row(int lane) {
+        const int i = lane >> 1;
+        return (i & 17) | (i & 6) << 1 | (i & 8) >> 2;
+    }
+    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage, int lane) {
+        Base::init_products(stage, lane);
+        const int i = lane & 15, half = lane >> 4 & 1, r = v_row(lane), in_block = r & 15;
 #pragma unroll
-        for (int h = 0; h < KB / 2; ++h) {
-            // A bfloat16 query's weights go in as two terms: one alone, half a step of bfloat16 of each weight, adds as much to the result's error as
-            // rounding it does (relative, 2-norm: 2.2e-3 in all and not 1.7e-3).  us, one term / two: 16 x 8192 tokens 48.7 / 48.9, in e4m3 30.7 / 31.1, one row of 2049 8.5 / 8.6,
-            // five queries on eight rows of 700 to 6000 17.6 / 18.3; where the arithmetic counts, eight queries on 16 x 8192 in e4m3, 43.0 / 49.5.
-            constexpr int kWeightTerms = kTerms == 1 ? 2 : kTerms;
-            bf16x8 p[NB][kWeightTerms];
+        for (int w = 0; w < 4; ++w) wr[w] = stage + r * kRowBytes + (((4 * (lane & 1) + w) ^ swz(r)) * 16);
+        k_at = i * a.kp.s + 16 * half;
+        ke_at = i * a.ke.s + half;
+        v_at = in_block * a.vp.s + 16 * (lane & 1);
+        ve_at = in_block * a.ve.s + (lane & 1);
+        upper = lane >= 32;
+    }
+    __device__ __forceinline__ void load_q(int nb, const T *row, bool there, int quad) {
+        const int at = 32 * (quad & 1) + 16 * (quad >> 1);
+        Base::load_numbers(nb, row, there, at, at + 8);
+    }
+    __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb, uint32_t mask) {
+        load(blk, kb, eb, lane_offset(k_at, mask), lane_offset(ke_at, mask), k[blk >> 1], ke[blk >> 1]);
+    }
+    __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb, uint32_t mask) {
+        load(blk, vb, eb, lane_offset(v_at, mask), lane_offset(ve_at, mask), v[blk >> 1], ve[blk >> 1]);
+    }
+    __device__ __forceinline__ void load(int blk, const char *rows, const char *exps, uint32_t at, uint32_t e_at, u32x4 &x, uint32_t &e) {
+        if ((blk & 1) == 0) {
+            first_row = rows;
+            first_exp = exps;
+        } else {
+            x = load16<kOnce>((upper ? rows : first_row) + at);
+            e = (uint8_t)(upper ? exps : first_exp)[e_at];
+        }
+    }
+    __device__ __forceinline__ void stage_k() const {}
+    __device__ __forceinline__ static bf16x8 widen(uint32_t w, float f) {
+        union { bf16x2 p[4]; bf16x8 v; } x;
+        x.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0);
+        x.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1);
+        x.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2);
+        x.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3);
+        return x.v;
+    }
+    __device__ __forceinline__ void logits(f32x4 (&s)[NB][KB]) const {
+        typedef __attribute__((ext_vector_type(2))) unsigned u32x2_t;
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                float x[8];
+        for (int i = 0; i < kPairs; ++i) {
+            // (the upper half of the first for the lower half of the second)
+            const u32x2_t w0 = __builtin_amdgcn_permlane32_swap(k[i][0], k[i][2], false, false), w1 = __builtin_amdgcn_permlane32_swap(k[i][1], k[i][3], false, false);
+            const u32x2_t e = __builtin_amdgcn_permlane32_swap(ke[i], ke[i], false, false);
+            const float p = exp_of_byte(e.x), p2 = exp_of_byte(e.y);
+            const bf16x8 f[2] = {widen(w0.x, p), widen(w1.x, p)}, f2[2] = {widen(w0.y, p2), widen(w1.y, p2)};
+            Base::block_logits(f, 2 * i, s);
+            Base::block_logits(f2, 2 * i + 1, s);
+        }
+    }
+    // As PagedTile16's.
+    __device__ __forceinline__ bool stage_v(bool edge, bool several, int first, int last, unsigned there, int lane) {
+        bool odd = false;
+        if (edge) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = s[nb][2 * h + (e >> 2)][e & 3];
-                if constexpr (kTerms == 1) {
-                    split_weights(x, p[nb][0], p[nb][1]);
-                } else {
+            for (int i = 0; i < kPairs; ++i) {
+                const int r = 32 * i + v_row(lane);
+                const bool in = r >= first && r < last && (there >> (2 * i + (upper ? 1 : 0)) & 1);
+                ve[i] = in ? ve[i] : (uint32_t)kExpBias;
 #pragma unroll
-                    for (int t = 0; t < kTerms; ++t) p[nb][t] = take_upper(x);
-                }
-            }
+                for (int e = 0; e < 4; ++e) v[i][e] = in ? v[i][e] : 0u;
+                if (several) {
+                    // Added to the magnitudes of codes, what carries those that are not finite into the sign's bit: under 2^126 4 and 6 (codes 6 and 7), under 2^127 2 and more
+                    // (from code 4 on), under the byte 255 all of them.
+                    const uint32_t carry = ve[i] < 253u ? 0u : ve[i] == 255u ? 0x88888888u : 0x22222222u * (ve[i] - 252u);
+                    ve[i] = ve[i] == 255u ? (uint32_t)kExpBias : ve[i];
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                union { struct { s16x4 a, b; } s; bf16x8 v; } x;
-                x.s.a = lds_load_tr64(tr[d], 32 * h * kRowBytes);
-                x.s.b = lds_load_tr64(tr[d], (32 * h + 16) * kRowBytes);
-                if constexpr (kTerms == 1) {
-#pragma unroll
-                    for (int t = kWeightTerms - 1; t >= 0; --t)
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) o[nb][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb][t], o[nb][d], 0, 0, 0);
-                } else {
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int t = kTerms - 1; t >= 0; --t) z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, p[nb][t], z, 0, 0, 0);
-                        o[nb][d] += z;
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t bad = ((((v[i][e] & 0x77777777u) + carry) & 0x88888888u) >> 3) * 0xfu;
+                        odd = odd || bad != 0u;
+                        v[i][e] &= ~bad;
                     }
                 }
             }
         }
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            const float p = exp_of_byte(ve[i]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                union { bf16x8 b; u32x4 u; } x;
+                x.b = widen(v[i][w], p);
+                *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>((uintptr_t)(wr[w] + 32 * i * kRowBytes)) = x.u;
+            }
+        }
+        return odd;
     }
-    // column of o[.][d][e] in the lane's row
-    __device__ __forceinline__ static int column(int d, int e, int quad) { return 16 * d + 4 * quad + e; }
 };
 template <typename ST, int NB, int KB> struct PagedTile<bf16, ST, NB, KB> : PagedTile16<bf16, ST, NB, KB> {};
 template <int NB, int KB> struct PagedTile<float, e4m3, NB, KB> : PagedTile16<float, e4m3, NB, KB> {};
+template <int NB, int KB> struct PagedTile<bf16, e2m1, NB, KB> : PagedTile4<bf16, NB, KB> {};
+template <int NB, int KB> struct PagedTile<float, e2m1, NB, KB> : PagedTile4<float, NB, KB> {};
 
 // ---- float32 products ------------------------------------------------------------------------------------------------
 template <int NB, int KB>
@@ -746,14 +883,19 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
                 const int page = paged_page(a, sp.b, key);
                 if (page < 0) continue;
                 const char *row = v_base + a.vp.at(page, key & in_page);
-                float power = 1.0f;
-                if constexpr (Tile::kCodes) power = factor_of_byte((uint8_t)ve_base[a.ve.at(page, key & in_page)]);
+                float power[2] = {1.0f, 1.0f};                   // of the first 32 numbers and the others
+                if constexpr (Tile::kCodes) {
+                    const char *e = ve_base + a.ve.at(page, key & in_page);
+                    power[0] = factor_of_byte((uint8_t)e[0]);
+                    power[1] = is_e2m1<ST> ? factor_of_byte((uint8_t)e[1]) : power[0];
+                }
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float x = stored_number(reinterpret_cast<const ST *>(row) + Tile::column(d, e, quad));
-                        if constexpr (Tile::kCodes) x *= power;
+                        const int column = Tile::column(d, e, quad);
+                        float x = stored_number(reinterpret_cast<const ST *>(row), column);
+                        if constexpr (Tile::kCodes) x *= power[column >> 5];
                         if ((__float_as_uint(x) & 0x7f800000u) != 0x7f800000u) continue;
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb)

@@ -16,13 +16,16 @@ bool page_size_ok(int n) { return n >= 16 && n <= 1024 && (n & (n - 1)) == 0; }
 
 bool aligned(const void *p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-// Rows of 64 elements of `eb` bytes, each on a 16-byte boundary.
-int check_rows(const void *p, const gptoss_attn_strides &s, int eb) {
+// Rows of 64 elements of `eb` bytes (of `n` elements), each on a 16-byte boundary.
+int check_rows(const void *p, const gptoss_attn_strides &s, int eb, int n = kD) {
     if (!p) return GPTOSS_ATTN_ERR_NULL_TENSOR;
     const int64_t per16 = 16 / eb;
     if (!aligned(p, 16) || s.b % per16 || s.h % per16 || s.s % per16) return GPTOSS_ATTN_ERR_ALIGNMENT;
-    return s.s < kD || s.s > (1 << 24) ? GPTOSS_ATTN_ERR_STRIDE : GPTOSS_ATTN_OK;
+    return s.s < n || s.s > (1 << 24) ? GPTOSS_ATTN_ERR_STRIDE : GPTOSS_ATTN_OK;
 }
+
+// Rows of codes with bytes of exponents.
+bool is_codes(const gptoss_attn_paged_params *p) { return p->storage == GPTOSS_ATTN_E4M3 || p->storage == GPTOSS_ATTN_E2M1; }
 
 Strides cvt(const gptoss_attn_strides &s) { return Strides{s.b, s.h, s.s}; }
 
@@ -37,7 +40,7 @@ PagedArgs make_args(const gptoss_attn_paged_params *p) {
     a.sinks = p->sinks;
     a.o = p->o;
     a.lse = p->lse;
-    const int eb = p->storage == GPTOSS_ATTN_E4M3 ? 1 : p->storage == GPTOSS_ATTN_FP32 ? 4 : 2;
+    const int eb = is_codes(p) ? 1 : p->storage == GPTOSS_ATTN_FP32 ? 4 : 2;
     a.kp = pool(p->k_pages, p->k_page_stride, eb);
     a.vp = pool(p->v_pages, p->v_page_stride, eb);
     a.ke = pool(p->k_exp, p->k_exp_stride, 1);
@@ -86,6 +89,13 @@ int launch(Kernel kernel, int64_t workgroups, int threads, void *stream, const A
     return e == hipSuccess ? GPTOSS_ATTN_OK : static_cast<int>(e);
 }
 
+// call(number of the model's type, number as it is stored) for the block's types.
+template <typename F>
+auto of_types(const gptoss_attn_paged_params *p, F call) {
+    if (p->dtype == GPTOSS_ATTN_BF16) return p->storage == GPTOSS_ATTN_E2M1 ? call(bf16{}, e2m1{}) : p->storage == GPTOSS_ATTN_E4M3 ? call(bf16{}, e4m3{}) : call(bf16{}, bf16{});
+    return p->storage == GPTOSS_ATTN_E2M1 ? call(float{}, e2m1{}) : p->storage == GPTOSS_ATTN_E4M3 ? call(float{}, e4m3{}) : call(float{}, float{});
+}
+
 // How the attention's work is divided: column blocks of 16 pairs, blocks of pairs of a row, (row, block) units, shares of all units'
 // tiles for each KV head that there are at most beside one for each unit (0: units stay whole, each walked by `alone` wavefronts), how many are to be expected, and
 // the scratch that takes; `across`: a slot's KV heads on one XCD.  How long shares are is the kernel's to find, from the lengths (PagedShare).
@@ -96,7 +106,7 @@ template <typename T, typename ST, int NB> constexpr int per_simd() { return pag
 
 PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     PagedDivision d{};
-    const bool codes = p->storage == GPTOSS_ATTN_E4M3, f32 = p->storage == GPTOSS_ATTN_FP32;      // f32: the fp32 MFMA
+    const bool codes = is_codes(p), four = p->storage == GPTOSS_ATTN_E2M1, f32 = p->storage == GPTOSS_ATTN_FP32;      // f32: the fp32 MFMA
     const int64_t r = p->H / p->G, pairs = (int64_t)p->Sq * r;
     const int most = p->dtype == GPTOSS_ATTN_FP32 ? paged_pairs<float>() : paged_pairs<bf16>();
     d.nb = pairs <= 16 ? 1 : pairs <= 32 || most == 32 ? 2 : pairs <= 48 ? 3 : 4;
@@ -129,7 +139,7 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     // least half of the workgroups are shares all the same, so that a long row among many is cut.  No more than the units can have.  us with half as many,
     // as many, twice as many: 16 x 8192 tokens 46.3 / 47.5 / 50.1, 64 x 3540 73.9 / 77.4 / 80.3, but 64 rows of 150 to 16384 103 / 81.6 / 83.5, 32 of 6000 to
     // 16384 137 / 112 / 114, and four queries on each of those in e4m3 44.3 / 33.4 / 41.2.
-#define GPTOSS_HELD(T, NB) (codes ? per_simd<T, e4m3, NB>() : per_simd<T, T, NB>())
+#define GPTOSS_HELD(T, NB) (four ? per_simd<T, e2m1, NB>() : codes ? per_simd<T, e4m3, NB>() : per_simd<T, T, NB>())
     const int at_a_time = p->dtype == GPTOSS_ATTN_FP32 ? (d.nb == 1 ? GPTOSS_HELD(float, 1) : GPTOSS_HELD(float, 2))
                            : d.nb == 1 ? GPTOSS_HELD(bf16, 1) : d.nb == 2 ? GPTOSS_HELD(bf16, 2) : d.nb == 3 ? GPTOSS_HELD(bf16, 3) : GPTOSS_HELD(bf16, 4);
 #undef GPTOSS_HELD
@@ -177,7 +187,7 @@ int gptoss_attn_paged_validate(const gptoss_attn_paged_params *p, int call) {
     if (!p) return GPTOSS_ATTN_ERR_NULL_PARAMS;
     if (p->struct_size != sizeof(gptoss_attn_paged_params)) return GPTOSS_ATTN_ERR_ABI;
     if (p->dtype != GPTOSS_ATTN_BF16 && p->dtype != GPTOSS_ATTN_FP32) return GPTOSS_ATTN_ERR_DTYPE;
-    if (p->storage != p->dtype && p->storage != GPTOSS_ATTN_E4M3) return GPTOSS_ATTN_ERR_DTYPE;
+    if (p->storage != p->dtype && !is_codes(p)) return GPTOSS_ATTN_ERR_DTYPE;
     if (p->D != kD) return GPTOSS_ATTN_ERR_HEAD_DIM;
     if (p->G <= 0 || (call == kFwd && (p->H <= 0 || p->H % p->G))) return GPTOSS_ATTN_ERR_HEADS;
     if (p->B <= 0 || p->Sq <= 0 || p->Sq > (1 << 30)) return GPTOSS_ATTN_ERR_SHAPE;
@@ -186,10 +196,11 @@ int gptoss_attn_paged_validate(const gptoss_attn_paged_params *p, int call) {
     if (table && (p->table_width <= 0 || p->table_stride < 0 || (int64_t)p->table_width * p->page_size > (1 << 30))) return GPTOSS_ATTN_ERR_PAGES;
     if (!table && p->B != 1) return GPTOSS_ATTN_ERR_SHAPE;
     const int eb = p->dtype == GPTOSS_ATTN_FP32 ? 4 : 2;
-    const bool codes = p->storage == GPTOSS_ATTN_E4M3;
+    const bool codes = is_codes(p);
+    const int row = p->storage == GPTOSS_ATTN_E2M1 ? kD / 2 : kD;
     int rc;
-    if ((rc = check_rows(p->k_pages, p->k_page_stride, codes ? 1 : eb))) return rc;
-    if ((rc = check_rows(p->v_pages, p->v_page_stride, codes ? 1 : eb))) return rc;
+    if ((rc = check_rows(p->k_pages, p->k_page_stride, codes ? 1 : eb, row))) return rc;
+    if ((rc = check_rows(p->v_pages, p->v_page_stride, codes ? 1 : eb, row))) return rc;
     if ((table && !p->page_table) || (codes && (!p->k_exp || !p->v_exp))) return GPTOSS_ATTN_ERR_NULL_TENSOR;
     if (!pool_fits(p->k_page_stride, codes ? 1 : eb) || !pool_fits(p->v_page_stride, codes ? 1 : eb)) return GPTOSS_ATTN_ERR_STRIDE;
     if (codes && (!pool_fits(p->k_exp_stride, 1) || !pool_fits(p->v_exp_stride, 1))) return GPTOSS_ATTN_ERR_STRIDE;
@@ -231,13 +242,13 @@ int gptoss_attn_paged_fwd(const gptoss_attn_paged_params *p, void *stream) {
         a.plan = static_cast<int *>(p->scratch);
         a.partial = reinterpret_cast<float *>(static_cast<char *>(p->scratch) + d.plan_bytes);
     }
-    const bool codes = p->storage == GPTOSS_ATTN_E4M3;
+    const bool codes = is_codes(p), four = p->storage == GPTOSS_ATTN_E2M1;
     if (p->dtype == GPTOSS_ATTN_BF16) {
-#define GPTOSS_PAGED(NB) (codes ? attend<bf16, e4m3, NB>(d, stream, a) : attend<bf16, bf16, NB>(d, stream, a))
+#define GPTOSS_PAGED(NB) (four ? attend<bf16, e2m1, NB>(d, stream, a) : codes ? attend<bf16, e4m3, NB>(d, stream, a) : attend<bf16, bf16, NB>(d, stream, a))
         return d.nb == 1 ? GPTOSS_PAGED(1) : d.nb == 2 ? GPTOSS_PAGED(2) : d.nb == 3 ? GPTOSS_PAGED(3) : GPTOSS_PAGED(4);
 #undef GPTOSS_PAGED
     }
-#define GPTOSS_PAGED(NB) (codes ? attend<float, e4m3, NB>(d, stream, a) : attend<float, float, NB>(d, stream, a))
+#define GPTOSS_PAGED(NB) (four ? attend<float, e2m1, NB>(d, stream, a) : codes ? attend<float, e4m3, NB>(d, stream, a) : attend<float, float, NB>(d, stream, a))
     return d.nb == 1 ? GPTOSS_PAGED(1) : GPTOSS_PAGED(2);
 #undef GPTOSS_PAGED
 }
@@ -252,10 +263,7 @@ int gptoss_attn_paged_write(const gptoss_attn_paged_params *p, void *stream) {
     a.blocks = (int)blocks;
     a.by_blocks = div_by(blocks);
     a.by_g = div_by(a.G);
-    const bool codes = p->storage == GPTOSS_ATTN_E4M3;
-    if (p->dtype == GPTOSS_ATTN_BF16)
-        return codes ? launch(paged_write_kernel<bf16, true>, grid, 256, stream, a) : launch(paged_write_kernel<bf16, false>, grid, 256, stream, a);
-    return codes ? launch(paged_write_kernel<float, true>, grid, 256, stream, a) : launch(paged_write_kernel<float, false>, grid, 256, stream, a);
+    return of_types(p, [&](auto t, auto st) { return launch(paged_write_kernel<decltype(t), decltype(st)>, grid, 256, stream, a); });
 }
 
 int gptoss_attn_paged_read(const gptoss_attn_paged_params *p, void *stream) {
@@ -267,10 +275,7 @@ int gptoss_attn_paged_read(const gptoss_attn_paged_params *p, void *stream) {
     a.blocks = (int)blocks;
     a.by_blocks = div_by(blocks);
     a.by_g = div_by(a.G);
-    const bool codes = p->storage == GPTOSS_ATTN_E4M3;
-    if (p->dtype == GPTOSS_ATTN_BF16)
-        return codes ? launch(paged_read_kernel<bf16, e4m3>, grid, 256, stream, a) : launch(paged_read_kernel<bf16, bf16>, grid, 256, stream, a);
-    return codes ? launch(paged_read_kernel<float, e4m3>, grid, 256, stream, a) : launch(paged_read_kernel<float, float>, grid, 256, stream, a);
+    return of_types(p, [&](auto t, auto st) { return launch(paged_read_kernel<decltype(t), decltype(st)>, grid, 256, stream, a); });
 }
 
 int gptoss_attn_paged_write_slots(const gptoss_attn_paged_params *p, const int64_t *slots, void *stream) {
@@ -282,10 +287,7 @@ int gptoss_attn_paged_write_slots(const gptoss_attn_paged_params *p, const int64
     const int64_t rows = (int64_t)a.Sq * a.G;
     if (rows > (1 << 30)) return GPTOSS_ATTN_ERR_SHAPE;
     a.by_g = div_by(a.G);
-    const bool codes = p->storage == GPTOSS_ATTN_E4M3;
-    const void *kernel = p->dtype == GPTOSS_ATTN_BF16
-                             ? (codes ? reinterpret_cast<const void *>(paged_write_slots_kernel<bf16, true>) : reinterpret_cast<const void *>(paged_write_slots_kernel<bf16, false>))
-                             : (codes ? reinterpret_cast<const void *>(paged_write_slots_kernel<float, true>) : reinterpret_cast<const void *>(paged_write_slots_kernel<float, false>));
+    const void *kernel = of_types(p, [](auto t, auto st) { return reinterpret_cast<const void *>(paged_write_slots_kernel<decltype(t), decltype(st)>); });
     void *args[] = {&a, const_cast<int64_t **>(&slots)};
     const hipError_t e = hipLaunchKernel(kernel, dim3((unsigned)((rows + 31) / 32)), dim3(256), args, 0, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? GPTOSS_ATTN_OK : static_cast<int>(e);

@@ -36,6 +36,30 @@ __device__ __forceinline__ uint2 e4m3_codes(const float (&x)[8], int s) {
     return make_uint2((uint32_t)lo, (uint32_t)hi);
 }
 
+// The power of two of 32 numbers (over the four lanes that hold them): the smallest 2^s with the largest at most 7 * 2^s, which is where rounding to the format's next
+// number, 8, would begin; s = 128, the byte that means NaN, where one of them is not finite.
+__device__ __forceinline__ int block_exponent(const float (&x)[8]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);      // magnitudes compare as their bits do
+    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+    if (top >= 0x7f800000u) return 128;
+    // 7 = 1.75 * 2^2 (numbers below 2^-126: as in row_exponent)
+    return min(max((int)(top >> 23) - 127 - 2 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0), kMinExp), kMaxExp4);
+}
+
+__device__ __forceinline__ uint32_t e2m1_codes(const float (&x)[8], int s) {
+    const float inv = exp_of_byte((uint32_t)(kExpBias - min(s, kMaxExp4)));      // 2^-s: as in e4m3_codes
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i] * inv, -6.0f, 6.0f);
+    uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], y[1], 1.0f, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], 1.0f, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], 1.0f, 2);
+    return s == 128 ? 0u : __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], 1.0f, 3);
+}
+
 // Eight numbers of a row as they travel.
 template <typename T> struct Piece { u32x4 u[sizeof(T) / 2]; };
 template <typename T>
@@ -57,10 +81,16 @@ __device__ __forceinline__ void numbers_of(const Piece<T> &p, float (&x)[8]) {
     }
 }
 
-template <typename T, bool E4M3>
+template <typename T, typename ST>
 __device__ __forceinline__ void write_piece(const PagedPool &rows, const PagedPool &exps, int page, int at, int g, int c8, const Piece<T> &p) {
     char *row = rows.head(g) + rows.at(page, at);
-    if constexpr (E4M3) {
+    if constexpr (is_e2m1<ST>) {
+        float x[8];
+        numbers_of(p, x);
+        const int s = block_exponent(x);
+        *reinterpret_cast<uint32_t *>(row + (c8 >> 1)) = e2m1_codes(x, s);
+        if ((c8 & 31) == 0) *(exps.head(g) + exps.at(page, at) + (c8 >> 5)) = (char)(s + kExpBias);
+    } else if constexpr (sizeof(ST) == 1) {
         float x[8];
         numbers_of(p, x);
         const int s = row_exponent(x);
@@ -74,7 +104,7 @@ __device__ __forceinline__ void write_piece(const PagedPool &rows, const PagedPo
 
 // Rows (token, KV head) of a batch row, the KV head fastest: the model's keys and values have a token's heads side by side.  The rows are under
 // way while their page is looked up.  One row to a lane: with two, 8 x 4096 tokens of 8 KV heads took 27.9 us and not 26.2 (134 MB moved).
-template <typename T, bool E4M3>
+template <typename T, typename ST>
 __global__ __launch_bounds__(256) void paged_write_kernel(const PagedArgs a) {
     const int b = a.by_blocks.quotient(blockIdx.x), row = (blockIdx.x - b * a.blocks) * 32 + (threadIdx.x >> 3), c8 = (threadIdx.x & 7) * 8;
     const int n = a.seqlens ? min(a.seqlens[b], a.Sq) : a.Sq;
@@ -86,12 +116,12 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const PagedArgs a) {
     const int page = pos < 0 || pos > 0x7fffffff ? -1 : paged_page(a, b, (int)pos);
     if (page < 0) return;
     const int at = (int)pos & ((1 << a.page_shift) - 1);
-    write_piece<T, E4M3>(a.kp, a.ke, page, at, g, c8, k);
-    write_piece<T, E4M3>(a.vp, a.ve, page, at, g, c8, v);
+    write_piece<T, ST>(a.kp, a.ke, page, at, g, c8, k);
+    write_piece<T, ST>(a.vp, a.ve, page, at, g, c8, v);
 }
 
 // The same of one batch row whose tokens have slots of their own.
-template <typename T, bool E4M3>
+template <typename T, typename ST>
 __global__ __launch_bounds__(256) void paged_write_slots_kernel(const PagedArgs a, const int64_t *slots) {
     const int row = blockIdx.x * 32 + (threadIdx.x >> 3), c8 = (threadIdx.x & 7) * 8;
     const int i = a.by_g.quotient(row), g = row - i * a.G;
@@ -101,8 +131,8 @@ __global__ __launch_bounds__(256) void paged_write_slots_kernel(const PagedArgs 
     const int64_t slot = slots[i], page = slot >> a.page_shift;
     if (slot < 0 || page >= a.pages) return;
     const int at = (int)slot & ((1 << a.page_shift) - 1);
-    write_piece<T, E4M3>(a.kp, a.ke, (int)page, at, g, c8, k);
-    write_piece<T, E4M3>(a.vp, a.ve, (int)page, at, g, c8, v);
+    write_piece<T, ST>(a.kp, a.ke, (int)page, at, g, c8, k);
+    write_piece<T, ST>(a.vp, a.ve, (int)page, at, g, c8, v);
 }
 
 // Rows of a (batch row, KV head), which lie side by side in the result; one to a lane (two: eight prompts of up to 12000 tokens in e4m3, and their
@@ -120,11 +150,12 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const PagedArgs a) {
     for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.0f;
     if (page >= 0) {
         const int at = (int)pos & ((1 << a.page_shift) - 1);
-        load8<true>(reinterpret_cast<const ST *>(a.kp.head(g) + a.kp.at(page, at)) + c8, k);
-        load8<true>(reinterpret_cast<const ST *>(a.vp.head(g) + a.vp.at(page, at)) + c8, v);
+        load8<true>(reinterpret_cast<const ST *>(a.kp.head(g) + a.kp.at(page, at)), c8, k);
+        load8<true>(reinterpret_cast<const ST *>(a.vp.head(g) + a.vp.at(page, at)), c8, v);
         if constexpr (sizeof(ST) == 1) {
-            const float ke = factor_of_byte(*reinterpret_cast<const uint8_t *>(a.ke.head(g) + a.ke.at(page, at)));
-            const float ve = factor_of_byte(*reinterpret_cast<const uint8_t *>(a.ve.head(g) + a.ve.at(page, at)));
+            const int half = is_e2m1<ST> ? c8 >> 5 : 0;              // which of a row's bytes
+            const float ke = factor_of_byte(*reinterpret_cast<const uint8_t *>(a.ke.head(g) + a.ke.at(page, at) + half));
+            const float ve = factor_of_byte(*reinterpret_cast<const uint8_t *>(a.ve.head(g) + a.ve.at(page, at) + half));
 #pragma unroll
             for (int e = 0; e < 8; ++e) { k[e] *= ke; v[e] *= ve; }
         }

@@ -1,6 +1,7 @@
 // A key / value cache in pages: what its kernels share (the arguments, the page of a token, rows of 64 as they are stored).
 //
-// A stored row is 64 numbers of the model's type, or 64 e4m3 codes and a byte e: the row is code * 2^(e - 127).  A power of two
+// A stored row is 64 numbers of the model's type, or 64 e4m3 codes and a byte e: the row is code * 2^(e - 127); or 64 e2m1 codes, two to a byte, and a byte e for
+// each 32 of them.  A power of two
 // makes both directions exact but for the one rounding to e4m3: codes widen to bf16 (four significant bits), and so do their
 // products with 2^s.  A divisor of largest / 448, which fills the format's range, would save at most one bit in the numbers below
 // 2^-15 of the row's largest, and cost a rounding in each direction.
@@ -54,7 +55,7 @@ struct PagedArgs {
     bool sinks_bf16;
 };
 
-constexpr int kExpBias = 127, kMinExp = -64, kMaxExp = 120;       // exponent bytes; the powers of two of rows
+constexpr int kExpBias = 127, kMinExp = -64, kMaxExp = 120, kMaxExp4 = 125;       // exponent bytes; the powers of two of e4m3 rows, and of 32 e2m1 numbers
 constexpr float kLowest = -3.0e38f;                // start of a running maximum: finite, so that -inf - (it) is -inf and not NaN
 
 __device__ __forceinline__ float paged_sink(const PagedArgs &a, int head) {
@@ -80,11 +81,20 @@ __device__ __forceinline__ float exp_of_byte(uint32_t e) { return __uint_as_floa
 __device__ __forceinline__ float factor_of_byte(uint32_t e) { return __uint_as_float(e == 0 ? 0x00400000u : e == 255 ? 0x7fc00000u : e << 23); }
 
 struct e4m3 { uint8_t code; };
+struct e2m1 { uint8_t pair; };                     // numbers 2i (lower half) and 2i + 1
+template <typename ST> constexpr bool is_e2m1 = false;
+template <> inline constexpr bool is_e2m1<e2m1> = true;
 
-// A number of a row (of a code: without its power of two).
-__device__ __forceinline__ float stored_number(const bf16 *p) { return (float)*p; }
-__device__ __forceinline__ float stored_number(const float *p) { return *p; }
-__device__ __forceinline__ float stored_number(const e4m3 *p) { return __builtin_amdgcn_cvt_f32_fp8((int)p->code, 0); }
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+
+// Number i of a row (of a code: without its power of two).
+__device__ __forceinline__ float stored_number(const bf16 *row, int i) { return (float)row[i]; }
+__device__ __forceinline__ float stored_number(const float *row, int i) { return row[i]; }
+__device__ __forceinline__ float stored_number(const e4m3 *row, int i) { return __builtin_amdgcn_cvt_f32_fp8((int)row[i].code, 0); }
+__device__ __forceinline__ float stored_number(const e2m1 *row, int i) {
+    const f32x2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((uint32_t)row[i >> 1].pair, 1.0f, 0);
+    return i & 1 ? x.y : x.x;
+}
 
 // 16 bytes; ONCE: past the caches' retention, for what a kernel streams through.
 template <bool ONCE>
@@ -98,22 +108,29 @@ __device__ __forceinline__ void store16(void *p, const u32x4 x) {
     else *static_cast<u32x4 *>(p) = x;
 }
 
-// Eight numbers of a row.
+// Eight numbers of a row, from number c on.
 template <bool ONCE = false>
-__device__ __forceinline__ void load8(const bf16 *p, float (&x)[8]) {
-    const bf16x8 v = as_bf16x8(load16<ONCE>(p));
+__device__ __forceinline__ void load8(const bf16 *row, int c, float (&x)[8]) {
+    const bf16x8 v = as_bf16x8(load16<ONCE>(row + c));
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
 }
 template <bool ONCE = false>
-__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
-    const u32x4 u = load16<ONCE>(p), w = load16<ONCE>(p + 4);
+__device__ __forceinline__ void load8(const float *row, int c, float (&x)[8]) {
+    const u32x4 u = load16<ONCE>(row + c), w = load16<ONCE>(row + c + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) { x[i] = __uint_as_float(u[i]); x[4 + i] = __uint_as_float(w[i]); }
 }
 template <bool ONCE = false>
-__device__ __forceinline__ void load8(const e4m3 *p, float (&x)[8]) {
-    const uint2 w = *reinterpret_cast<const uint2 *>(p);
+__device__ __forceinline__ void load8(const e2m1 *row, int c, float (&x)[8]) {
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(row + (c >> 1));
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
+    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = d.x; x[5] = d.y; x[6] = e.x; x[7] = e.y;
+}
+template <bool ONCE = false>
+__device__ __forceinline__ void load8(const e4m3 *row, int c, float (&x)[8]) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(row + c);
     x[0] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 0);
     x[1] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 1);
     x[2] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 2);

@@ -9,7 +9,11 @@
 
 namespace {
 
-int abi_dtype(at::ScalarType t) { return t == at::kFloat ? GPTOSS_ATTN_FP32 : t == at::kBFloat16 ? GPTOSS_ATTN_BF16 : t == at::kFloat8_e4m3fn ? GPTOSS_ATTN_E4M3 : -1; }
+constexpr auto kPairs = at::ScalarType::Float4_e2m1fn_x2;        // two e2m1 numbers to an element
+
+int abi_dtype(at::ScalarType t) {
+    return t == at::kFloat ? GPTOSS_ATTN_FP32 : t == at::kBFloat16 ? GPTOSS_ATTN_BF16 : t == at::kFloat8_e4m3fn ? GPTOSS_ATTN_E4M3 : t == kPairs ? GPTOSS_ATTN_E2M1 : -1;
+}
 
 void set3(gptoss_attn_strides &s, const Tensor &t) {
     s.b = t.stride(0);
@@ -38,20 +42,24 @@ void fill_cache(PagedCall &c, const Tensor &k_pages, const Tensor &v_pages, cons
     require_near(k_pages, "v of the cache", v_pages);
     const auto storage = k_pages.scalar_type();
     TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "unsupported dtype ", dtype, ": bfloat16 or float32");
-    TORCH_CHECK(v_pages.scalar_type() == storage && (storage == dtype || storage == at::kFloat8_e4m3fn), "a cache of ", storage, "/", v_pages.scalar_type(),
-                " does not go with tensors of ", dtype, ": it holds their type or float8_e4m3fn");
-    TORCH_CHECK(k_pages.dim() == 4 && k_pages.sizes() == v_pages.sizes() && k_pages.size(3) == 64, "the cache's k and v must both be (pages, G, page_size, 64), got ",
+    const bool pairs = storage == kPairs, codes = pairs || storage == at::kFloat8_e4m3fn;
+    TORCH_CHECK(v_pages.scalar_type() == storage && (storage == dtype || codes), "a cache of ", storage, "/", v_pages.scalar_type(),
+                " does not go with tensors of ", dtype, ": it holds their type, float8_e4m3fn or float4_e2m1fn_x2");
+    const int64_t row = pairs ? 32 : 64;
+    TORCH_CHECK(k_pages.dim() == 4 && k_pages.sizes() == v_pages.sizes() && k_pages.size(3) == row, "the cache's k and v must both be (pages, G, page_size, ", row, "), got ",
                 k_pages.sizes(), " and ", v_pages.sizes());
-    TORCH_CHECK(k_pages.stride(3) == 1 && v_pages.stride(3) == 1, "the cache's rows of 64 must be contiguous, got strides ", k_pages.strides(), " and ", v_pages.strides());
+    TORCH_CHECK(k_pages.stride(3) == 1 && v_pages.stride(3) == 1, "the cache's rows of ", row, " must be contiguous, got strides ", k_pages.strides(), " and ", v_pages.strides());
     gptoss_attn_paged_params &p = c.p;
     p.struct_size = sizeof(p);
     p.dtype = abi_dtype(dtype);
     p.storage = abi_dtype(storage);
-    if (storage == at::kFloat8_e4m3fn) {
-        TORCH_CHECK(k_exp && v_exp, "a float8_e4m3fn cache needs its exponents");
+    if (codes) {
+        TORCH_CHECK(k_exp && v_exp, "a ", pairs ? "float4_e2m1fn_x2" : "float8_e4m3fn", " cache needs its exponents");
         for (const auto &[name, t, e] : {std::tuple<const char *, const Tensor &, uint8_t **>("k_exp", *k_exp, &p.k_exp), {"v_exp", *v_exp, &p.v_exp}}) {
             require_near(k_pages, name, t);
-            TORCH_CHECK(t.scalar_type() == at::kByte && t.sizes() == k_pages.sizes().slice(0, 3), name, " must be uint8 (pages, G, page_size), got ", t.scalar_type(), " ", t.sizes());
+            TORCH_CHECK(t.scalar_type() == at::kByte && t.dim() == (pairs ? 4 : 3) && t.sizes().slice(0, 3) == k_pages.sizes().slice(0, 3) &&
+                            (!pairs || (t.size(3) == 2 && t.stride(3) == 1)),
+                        name, " must be uint8 (pages, G, page_size", pairs ? ", 2), a row's bytes side by side, got " : "), got ", t.scalar_type(), " ", t.sizes());
             *e = const_cast<uint8_t *>(t.const_data_ptr<uint8_t>());
         }
         set3(p.k_exp_stride, *k_exp);

@@ -3,9 +3,10 @@
 The sequences of a serving batch share one pool of pages per layer, `PagedCache`, and each has a row of page numbers in a
 `page_table` (B, pages of a row): token t stands in slot t % page_size of page page_table[b, t // page_size].  An entry outside
 the pool (-1, say) names no page.  The pool holds the model's type, or 8-bit e4m3 numbers with a power of two for each row of
-64: half of bfloat16's memory and traffic, each number within 2^-4 of itself.
+64: half of bfloat16's memory and traffic, each number within 2^-4 of itself; or 4-bit e2m1 numbers with a power of two for each 32 of them: 34 bytes for 128, each
+number within a quarter of itself or of that power.
 
-    cache = paged_cache(pages, kv_heads, page_size=64, storage=torch.float8_e4m3fn)
+    cache = paged_cache(pages, kv_heads, page_size=64, storage=torch.float8_e4m3fn)      # or torch.float4_e2m1fn_x2
     paged_cache_write(cache, k, v, page_table, start)                     # new tokens' keys and values, (B, G, S, 64)
     out = paged_attention(q, cache, page_table, start + S, sinks, scale, window)      # (B, S, H, 64), as attention()
     k, v = paged_cache_read(cache, page_table, seqlens, max_len)          # rows back, for attention() of a long prompt's chunk
@@ -33,7 +34,8 @@ __all__ = ["PagedCache", "PagedState", "paged_cache", "paged_cache_write", "page
 class PagedCache(NamedTuple):
     """k, v: (pages, G, page_size, 64), bfloat16, float32 or float8_e4m3fn, page_size a power of two from 16 to 1024; rows of 64 must be
     contiguous and start on 16-byte boundaries, the other strides are free.  k_exp, v_exp: float8_e4m3fn only, (pages, G, page_size)
-    uint8, a row's values are its numbers times 2^(byte - 127), NaN where the byte is 255."""
+    uint8, a row's values are its numbers times 2^(byte - 127), NaN where the byte is 255.
+    float4_e2m1fn_x2: (pages, G, page_size, 32), two numbers to an element, the first in its lower half; exponents (pages, G, page_size, 2), a byte for each half of a row."""
     k: torch.Tensor
     v: torch.Tensor
     k_exp: Optional[torch.Tensor] = None
@@ -78,11 +80,14 @@ class PagedState(NamedTuple):
 
 def paged_cache(pages, kv_heads, page_size=64, storage=torch.bfloat16, device="cuda") -> PagedCache:
     """An empty cache (all zeros) of one layer."""
-    if storage not in (torch.bfloat16, torch.float32, torch.float8_e4m3fn):
-        raise RuntimeError(f"unsupported storage {storage}: bfloat16, float32 or float8_e4m3fn")
+    if storage not in (torch.bfloat16, torch.float32, torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
+        raise RuntimeError(f"unsupported storage {storage}: bfloat16, float32, float8_e4m3fn or float4_e2m1fn_x2")
     if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
         raise RuntimeError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
     shape = (pages, kv_heads, page_size)
+    if storage == torch.float4_e2m1fn_x2:
+        k, v = (torch.zeros((*shape, 32), dtype=torch.uint8, device=device).view(storage) for _ in range(2))
+        return PagedCache(k, v, *(torch.zeros((*shape, 2), dtype=torch.uint8, device=device) for _ in range(2)))
     k, v = (torch.zeros((*shape, 64), dtype=storage, device=device) for _ in range(2))
     if storage != torch.float8_e4m3fn:
         return PagedCache(k, v)
@@ -160,13 +165,13 @@ def paged_cache_write_tokens(cache: PagedCache, k, v, slots) -> None:
 
 def paged_cache_read(cache: PagedCache, page_table, seqlens, max_len, start=None, dtype=None):
     """Rows back out of the pages: k, v (B, G, max_len, 64), row i being position start[b] + i (start: 0).  Zero at and behind seqlens[b], in
-    front of 0 and where an entry names no page.  `dtype`: the cache's, or of an e4m3 cache bfloat16 (exact), float32 or float16.
+    front of 0 and where an entry names no page.  `dtype`: the cache's, or of a cache of codes bfloat16 (exact), float32 or float16.
 
     The keys and values that a chunk of a long prompt sees, for `attention(q, k, v, sinks, scale, window, start_q)`."""
     if not _ready:
         _register_ops()
     if dtype is None:
-        dtype = torch.bfloat16 if cache.k.dtype == torch.float8_e4m3fn else cache.k.dtype
+        dtype = torch.bfloat16 if cache.k.dtype in (torch.float8_e4m3fn, torch.float4_e2m1fn_x2) else cache.k.dtype
     out = NotImplemented if _compiling() else _read_now(*cache, page_table, seqlens, max_len, start, dtype)
     if out is NotImplemented:
         out = _read(*cache, _ints(page_table, cache.k), _ints(seqlens, cache.k), int(max_len), _ints(start, cache.k), dtype)
