@@ -37,11 +37,11 @@ constexpr int kPagedWaves = 4;
 // Blocks of 16 keys in a tile: what a wavefront has under way is a tile, so rows of fewer bytes come more at a time; two columns' worth of
 // float32 numbers leave registers for one block.
 template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_tile_blocks() {
-    return sizeof(ST) == 4 ? (NB > 1 ? 1 : 2) : sizeof(ST) == 1 && NB == 1 && NW == kPagedWaves ? 4 : 2;
+    return sizeof(ST) == 4 ? (NB > 1 ? 1 : 2) : sizeof(ST) == 1 && !is_e2m1<ST> && NB == 1 && NW == kPagedWaves ? 4 : 2;
 }
 // Wavefronts per SIMD, of what the registers leave.
 template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_occupancy() {
-    return sizeof(ST) == 4 ? (NB == 2 && NW == kPagedWaves ? 3 : 2) : sizeof(T) == 4 ? 3 : NB == 1 ? 4 : NB == 2 || (NB == 3 && sizeof(ST) == 1) ? 3 : 2;
+    return sizeof(ST) == 4 ? (NB == 2 && NW == kPagedWaves ? 3 : 2) : sizeof(T) == 4 ? 3 : NB == 1 ? (is_e2m1<ST> && NW == kPagedWaves ? 5 : 4) : NB == 2 || (NB == 3 && sizeof(ST) == 1) ? 3 : 2;
 }
 // Pairs (query, head of the group) that one workgroup may take.
 template <typename T> __host__ __device__ constexpr int paged_pairs() { return sizeof(T) == 2 ? 64 : 32; }
@@ -349,7 +349,7 @@ struct PagedTile16 : PagedProducts16<T, NB, KB> {
     static constexpr bool kCodes = sizeof(ST) == 1, kStagedK = !kCodes;
     static constexpr int kVecs = kCodes ? 1 : 2;                 // 16-byte loads per lane and block
     u32x4 k[KB][kVecs], v[KB][kVecs];
-    uint32_t ke[KB], ve[KB];
+    uint8_t ke[KB], ve[KB];      // (bytes: widened as 32 bits are where they are loaded, they would be waited for there)
     uint32_t wr[2], nat[2], k_at[kVecs], v_at[kVecs], ke_at, ve_at;
 
     // (codes: rows 0, 1, 4, 5 and so on for each 16 lanes, which then write to distinct banks)
@@ -358,7 +358,7 @@ struct PagedTile16 : PagedProducts16<T, NB, KB> {
         return kCodes ? (q & 9) | (q & 2) << 1 | (q & 4) >> 1 : (lane >> 3) + 8 * i;
     }
 
-    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage, int lane) {
+    __device__ __forceinline__ void init(const PagedArgs &a, int, uint32_t stage, int lane) {
         const int i = lane & 15, quad = lane >> 4;
         Base::init_products(stage, lane);
 #pragma unroll
@@ -375,7 +375,8 @@ struct PagedTile16 : PagedProducts16<T, NB, KB> {
         ke_at = i * a.ke.s;
         ve_at = v_row(lane, 0) * a.ve.s;
     }
-    __device__ __forceinline__ void load_q(int nb, const T *row, bool there, int quad) {
+    __device__ __forceinline__ void load_q(int nb, const T *row, bool there, int lane) {
+        const int quad = lane >> 4;
         if constexpr (kCodes) Base::load_numbers(nb, row, there, 16 * quad, 16 * quad + 8);
         else Base::load_numbers(nb, row, there, 8 * quad, 32 + 8 * quad);
     }
@@ -422,7 +423,7 @@ struct PagedTile16 : PagedProducts16<T, NB, KB> {
                 for (int i = 0; i < kVecs; ++i) {
                     const int r = 16 * blk + v_row(lane, i);
                     const bool in = r >= first && r < last && (there >> blk & 1);
-                    if constexpr (kCodes) ve[blk] = in ? ve[blk] : (uint32_t)kExpBias;
+                    if constexpr (kCodes) ve[blk] = in ? ve[blk] : (uint8_t)kExpBias;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[blk][i][e] = in ? v[blk][i][e] : 0u;
                 }
@@ -434,7 +435,7 @@ struct PagedTile16 : PagedProducts16<T, NB, KB> {
                     uint32_t carry = 0x01010101u;
                     if constexpr (kCodes) {
                         carry = ve[blk] < 247u ? carry : ve[blk] == 255u ? 0x80808080u : 0x08080808u * (ve[blk] - 246u);
-                        ve[blk] = ve[blk] == 255u ? (uint32_t)kExpBias : ve[blk];
+                        ve[blk] = ve[blk] == 255u ? (uint8_t)kExpBias : ve[blk];
                     }
 #pragma unroll
                     for (int i = 0; i < kVecs; ++i)
@@ -469,57 +470,65 @@ struct PagedTile16 : PagedProducts16<T, NB, KB> {
 };
 
 // e2m1 pages: rows of 32 bytes and two bytes of exponents.  A load takes 32 rows, two blocks of keys, 16 bytes (32 numbers, which share a power) to a lane: of K, lanes below 32
-// halves of the first block's rows, those above of the second's, which one exchange between the two turns into both blocks' operands (quarter rows 0, 2, 1, 3 by quad: the queries come in that order);
-// of V, rows in the order in which 16 lanes write to distinct banks.  The two blocks may lie in different pages.
-template <typename T, int NB, int KB>
-struct PagedTile4 : PagedProducts16<T, NB, KB> {
-    using Base = PagedProducts16<T, NB, KB>;
-    using Base::kOnce;
+// have halves of the first block's rows, those above of the second's; of V, rows in the order in which 16 lanes write to distinct banks.  In pages of 16 tokens (ST = e2m1_of_16)
+// the two blocks lie in two of them, and each lane's addresses are of its half's page: 48 rows of 300 to 30000 tokens 46.0 us, in pages of 64, whose addresses are scalar, 44.1.
+// Tiles of 32 keys and five wavefronts a SIMD: with 64 and four one row of 2049 tokens takes 9.3 us and not 8.5 (two of four wavefronts have a tile of a share), 16 x 8192 23.1 / 22.8,
+// 32 x 16384 59.1 / 59.4.  Measured and not kept: a second tile under way (24.5 for 22.8: registers and no gain, the wait is not for memory), eight pairs in sixteen columns by
+// taking two blocks' keys into one contraction (a third fewer vector operations, 22.9).
+template <typename ST, int KB, bool ONCE>
+struct PagedRows4 {
     static constexpr bool kCodes = true, kStagedK = false;
-    static constexpr int kPairs = KB / 2;
+    static constexpr int kLoads = KB / 2;
     static_assert(KB % 2 == 0, "two blocks to a load");
-    u32x4 k[kPairs], v[kPairs];
-    uint32_t ke[kPairs], ve[kPairs];
+    u32x4 k[kLoads], v[kLoads];
+    uint8_t ke[kLoads], ve[kLoads];              // (as in PagedTile16)
+    static constexpr bool kTwoPages = std::is_same_v<ST, e2m1_of_16>;
     uint32_t wr[4], k_at, v_at, ke_at, ve_at;
+    const char *k_lane, *v_lane, *ke_lane, *ve_lane;         // two pages: where the lane's numbers of page 0 are
     bool upper;
-    const char *first_row, *first_exp;           // of the pair's first block, until its second is known
 
-    // of the pair's 32 rows
+    // of the load's 32 rows
     __device__ __forceinline__ static int v_row(int lane) {
         const int i = lane >> 1;
         return (i & 17) | (i & 6) << 1 | (i & 8) >> 2;
     }
-    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage, int lane) {
-        Base::init_products(stage, lane);
+    __device__ __forceinline__ void init_rows(const PagedArgs &a, int g, uint32_t stage, int lane) {
         const int i = lane & 15, half = lane >> 4 & 1, r = v_row(lane), in_block = r & 15;
 #pragma unroll
         for (int w = 0; w < 4; ++w) wr[w] = stage + r * kRowBytes + (((4 * (lane & 1) + w) ^ swz(r)) * 16);
-        k_at = i * a.kp.s + 16 * half;
-        ke_at = i * a.ke.s + half;
-        v_at = in_block * a.vp.s + 16 * (lane & 1);
-        ve_at = in_block * a.ve.s + (lane & 1);
         upper = lane >= 32;
-    }
-    __device__ __forceinline__ void load_q(int nb, const T *row, bool there, int quad) {
-        const int at = 32 * (quad & 1) + 16 * (quad >> 1);
-        Base::load_numbers(nb, row, there, at, at + 8);
-    }
-    __device__ __forceinline__ void load_k(int blk, const char *kb, const char *eb, uint32_t mask) {
-        load(blk, kb, eb, lane_offset(k_at, mask), lane_offset(ke_at, mask), k[blk >> 1], ke[blk >> 1]);
-    }
-    __device__ __forceinline__ void load_v(int blk, const char *vb, const char *eb, uint32_t mask) {
-        load(blk, vb, eb, lane_offset(v_at, mask), lane_offset(ve_at, mask), v[blk >> 1], ve[blk >> 1]);
-    }
-    __device__ __forceinline__ void load(int blk, const char *rows, const char *exps, uint32_t at, uint32_t e_at, u32x4 &x, uint32_t &e) {
-        if ((blk & 1) == 0) {
-            first_row = rows;
-            first_exp = exps;
-        } else {
-            x = load16<kOnce>((upper ? rows : first_row) + at);
-            e = (uint8_t)(upper ? exps : first_exp)[e_at];
+        const int second = upper && std::is_same_v<ST, e2m1> ? 16 : 0;       // (otherwise its rows are a page's first)
+        k_at = (second + i) * a.kp.s + 16 * half;
+        ke_at = (second + i) * a.ke.s + half;
+        v_at = (second + in_block) * a.vp.s + 16 * (lane & 1);
+        ve_at = (second + in_block) * a.ve.s + (lane & 1);
+        if constexpr (kTwoPages) {
+            k_lane = a.kp.head(g) + k_at;
+            v_lane = a.vp.head(g) + v_at;
+            ke_lane = a.ke.head(g) + ke_at;
+            ve_lane = a.ve.head(g) + ve_at;
         }
     }
+    // Two pages: the page of the lane's half.
+    __device__ __forceinline__ void load_k(int i, int page, const PagedArgs &a) {
+        k[i] = load16<ONCE>(k_lane + a.kp.at(page, 0));
+        ke[i] = (uint8_t)ke_lane[a.ke.at(page, 0)];
+    }
+    __device__ __forceinline__ void load_v(int i, int page, const PagedArgs &a) {
+        v[i] = load16<ONCE>(v_lane + a.vp.at(page, 0));
+        ve[i] = (uint8_t)ve_lane[a.ve.at(page, 0)];
+    }
+    // `kb`, `vb`: where the load's rows begin, for each lane its block's where they lie in two pages
+    __device__ __forceinline__ void load_k(int i, const char *kb, const char *eb, uint32_t mask) {
+        k[i] = load16<ONCE>(kb + lane_offset(k_at, mask));
+        ke[i] = (uint8_t)eb[lane_offset(ke_at, mask)];
+    }
+    __device__ __forceinline__ void load_v(int i, const char *vb, const char *eb, uint32_t mask) {
+        v[i] = load16<ONCE>(vb + lane_offset(v_at, mask));
+        ve[i] = (uint8_t)eb[lane_offset(ve_at, mask)];
+    }
     __device__ __forceinline__ void stage_k() const {}
+    // Eight codes as bf16 numbers times the power of two `f`: exact.
     __device__ __forceinline__ static bf16x8 widen(uint32_t w, float f) {
         union { bf16x2 p[4]; bf16x8 v; } x;
         x.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0);
@@ -528,10 +537,67 @@ struct PagedTile4 : PagedProducts16<T, NB, KB> {
         x.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3);
         return x.v;
     }
+    // Rows of V outside first .. last - 1 as zeros.
+    __device__ __forceinline__ void clear_rows(int first, int last, unsigned there, int lane) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = 32 * i + v_row(lane);
+            const bool in = r >= first && r < last && (there >> (2 * i + (upper ? 1 : 0)) & 1);
+            ve[i] = in ? ve[i] : (uint8_t)kExpBias;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = in ? v[i][e] : 0u;
+        }
+    }
+    // What is not finite as zeros, and whether there was such a thing.  Added to the magnitudes of codes, what carries those that are not finite into the sign's bit: under 2^126 4 and 6
+    // (codes 6 and 7), under 2^127 2 and more (from code 4 on), under the byte 255 all of them.
+    __device__ __forceinline__ bool clear_not_finite() {
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t carry = ve[i] < 253u ? 0u : ve[i] == 255u ? 0x88888888u : 0x22222222u * (ve[i] - 252u);
+            ve[i] = ve[i] == 255u ? (uint8_t)kExpBias : ve[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t bad = ((((v[i][e] & 0x77777777u) + carry) & 0x88888888u) >> 3) * 0xfu;
+                odd = odd || bad != 0u;
+                v[i][e] &= ~bad;
+            }
+        }
+        return odd;
+    }
+    __device__ __forceinline__ void stage_rows() const {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const float p = exp_of_byte(ve[i]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                union { bf16x8 b; u32x4 u; } x;
+                x.b = widen(v[i][w], p);
+                *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>((uintptr_t)(wr[w] + 32 * i * kRowBytes)) = x.u;
+            }
+        }
+    }
+};
+
+// One exchange between the wavefront's halves turns a load of K into both blocks' operands (quarter rows 0, 2, 1, 3 by quad: the queries come in that order).
+template <typename T, typename ST, int NB, int KB>
+struct PagedTile4 : PagedProducts16<T, NB, KB>, PagedRows4<ST, KB, PagedProducts16<T, NB, KB>::kOnce> {
+    using Base = PagedProducts16<T, NB, KB>;
+    using Rows = PagedRows4<ST, KB, Base::kOnce>;
+    using Rows::k, Rows::ke, Rows::widen;
+
+    __device__ __forceinline__ void init(const PagedArgs &a, int g, uint32_t stage, int lane) {
+        Base::init_products(stage, lane);
+        Rows::init_rows(a, g, stage, lane);
+    }
+    __device__ __forceinline__ void load_q(int nb, const T *row, bool there, int lane) {
+        const int quad = lane >> 4, at = 32 * (quad & 1) + 16 * (quad >> 1);
+        Base::load_numbers(nb, row, there, at, at + 8);
+    }
     __device__ __forceinline__ void logits(f32x4 (&s)[NB][KB]) const {
         typedef __attribute__((ext_vector_type(2))) unsigned u32x2_t;
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
+        for (int i = 0; i < Rows::kLoads; ++i) {
             // (the upper half of the first for the lower half of the second)
             const u32x2_t w0 = __builtin_amdgcn_permlane32_swap(k[i][0], k[i][2], false, false), w1 = __builtin_amdgcn_permlane32_swap(k[i][1], k[i][3], false, false);
             const u32x2_t e = __builtin_amdgcn_permlane32_swap(ke[i], ke[i], false, false);
@@ -545,44 +611,20 @@ struct PagedTile4 : PagedProducts16<T, NB, KB> {
     __device__ __forceinline__ bool stage_v(bool edge, bool several, int first, int last, unsigned there, int lane) {
         bool odd = false;
         if (edge) {
-#pragma unroll
-            for (int i = 0; i < kPairs; ++i) {
-                const int r = 32 * i + v_row(lane);
-                const bool in = r >= first && r < last && (there >> (2 * i + (upper ? 1 : 0)) & 1);
-                ve[i] = in ? ve[i] : (uint32_t)kExpBias;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[i][e] = in ? v[i][e] : 0u;
-                if (several) {
-                    // Added to the magnitudes of codes, what carries those that are not finite into the sign's bit: under 2^126 4 and 6 (codes 6 and 7), under 2^127 2 and more
-                    // (from code 4 on), under the byte 255 all of them.
-                    const uint32_t carry = ve[i] < 253u ? 0u : ve[i] == 255u ? 0x88888888u : 0x22222222u * (ve[i] - 252u);
-                    ve[i] = ve[i] == 255u ? (uint32_t)kExpBias : ve[i];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t bad = ((((v[i][e] & 0x77777777u) + carry) & 0x88888888u) >> 3) * 0xfu;
-                        odd = odd || bad != 0u;
-                        v[i][e] &= ~bad;
-                    }
-                }
-            }
+            Rows::clear_rows(first, last, there, lane);
+            if (several) odd = Rows::clear_not_finite();
         }
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-            const float p = exp_of_byte(ve[i]);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                union { bf16x8 b; u32x4 u; } x;
-                x.b = widen(v[i][w], p);
-                *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>((uintptr_t)(wr[w] + 32 * i * kRowBytes)) = x.u;
-            }
-        }
+        Rows::stage_rows();
         return odd;
     }
 };
+
 template <typename ST, int NB, int KB> struct PagedTile<bf16, ST, NB, KB> : PagedTile16<bf16, ST, NB, KB> {};
 template <int NB, int KB> struct PagedTile<float, e4m3, NB, KB> : PagedTile16<float, e4m3, NB, KB> {};
-template <int NB, int KB> struct PagedTile<bf16, e2m1, NB, KB> : PagedTile4<bf16, NB, KB> {};
-template <int NB, int KB> struct PagedTile<float, e2m1, NB, KB> : PagedTile4<float, NB, KB> {};
+template <int NB, int KB> struct PagedTile<bf16, e2m1, NB, KB> : PagedTile4<bf16, e2m1, NB, KB> {};
+template <int NB, int KB> struct PagedTile<bf16, e2m1_of_16, NB, KB> : PagedTile4<bf16, e2m1_of_16, NB, KB> {};
+template <int NB, int KB> struct PagedTile<float, e2m1, NB, KB> : PagedTile4<float, e2m1, NB, KB> {};
+template <int NB, int KB> struct PagedTile<float, e2m1_of_16, NB, KB> : PagedTile4<float, e2m1_of_16, NB, KB> {};
 
 // ---- float32 products ------------------------------------------------------------------------------------------------
 template <int NB, int KB>
@@ -597,7 +639,7 @@ struct PagedTile<float, float, NB, KB> {
     f32x4 w[KB][4];              // V without what is masked
     uint32_t k_at[kVecs], wr[kVecs], nat[kVecs], v_at[4];
 
-    __device__ __forceinline__ void init(const PagedArgs &a, uint32_t stage, int lane) {
+    __device__ __forceinline__ void init(const PagedArgs &a, int, uint32_t stage, int lane) {
         const int l16 = lane & 15, quad = lane >> 4;
 #pragma unroll
         for (int e = 0; e < kVecs; ++e) {
@@ -610,7 +652,8 @@ struct PagedTile<float, float, NB, KB> {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v_at[e] = (4 * quad + e) * a.vp.s + 16 * l16;
     }
-    __device__ __forceinline__ void load_q(int nb, const float *row, bool there, int quad) {
+    __device__ __forceinline__ void load_q(int nb, const float *row, bool there, int lane) {
+        const int quad = lane >> 4;
 #pragma unroll
         for (int t = 0; t < 16; t += 4) {
             const f32x4 x = *reinterpret_cast<const f32x4 *>(row + 4 * t + 4 * quad);
@@ -759,7 +802,7 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
 
     Tile tile;
     const uint32_t stage = lds_addr(smem) + w * Tile::kStage;
-    tile.init(a, stage, lane);
+    tile.init(a, g, stage, lane);
     int pq[NB];                // position of the column's query
     float m[NB], l[NB];
 #pragma unroll
@@ -767,7 +810,7 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
         const bool ok = 16 * nb + l16 < pairs;
         const int pair = sp.pair0 + (ok ? 16 * nb + l16 : 0), row = a.by_r.quotient(pair), head = g * a.r + pair - row * a.r;
         pq[nb] = sp.base + row;
-        tile.load_q(nb, static_cast<const T *>(a.q) + sp.b * a.qs.b + head * a.qs.h + row * a.qs.s, ok, quad);
+        tile.load_q(nb, static_cast<const T *>(a.q) + sp.b * a.qs.b + head * a.qs.h + row * a.qs.s, ok, lane);
         m[nb] = kLowest;
         l[nb] = 0.0f;
     }
@@ -777,6 +820,15 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
     // (page, slot) -> load(block, address of the rows, of their exponents); blocks behind the first of a page follow it
     auto fetch = [&](int j, const char *base, const PagedPool &rows, const char *ebase, const PagedPool &exps, auto load) __attribute__((always_inline)) {
         const int n0 = (t_lo + w + NW * j) * kKeys;
+        if constexpr (is_e2m1<ST>) {
+            // two blocks to a load
+#pragma unroll
+            for (int i = 0; i < KB / 2; ++i) {
+                const int page = max(page_of(j, 2 * i), 0), at = (n0 + 32 * i) & in_page;
+                load(i, base + rows.at(page, at), ebase + exps.at(page, at));
+            }
+            return;
+        }
         const char *p = nullptr, *e = nullptr;
 #pragma unroll
         for (int blk = 0; blk < KB; ++blk) {
@@ -791,8 +843,38 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
             load(blk, p, e);
         }
     };
-    auto fetch_k = [&](int j, uint32_t mask) __attribute__((always_inline)) { fetch(j, k_base, a.kp, ke_base, a.ke, [&](int blk, const char *p, const char *e) { tile.load_k(blk, p, e, mask); }); };
-    auto fetch_v = [&](int j, uint32_t mask) __attribute__((always_inline)) { fetch(j, v_base, a.vp, ve_base, a.ve, [&](int blk, const char *p, const char *e) { tile.load_v(blk, p, e, mask); }); };
+    constexpr bool kTwoPages = std::is_same_v<ST, e2m1_of_16>;
+    int lane_page[(KB + 1) / 2];             // two pages to a load: the lane's
+    int pages = 0;                           // of the tile under way: negative where a block has no page
+    unsigned there = 0;                      // which of them have one
+    auto fetch_k = [&](int j, uint32_t mask) __attribute__((always_inline)) {
+        pages = 0;
+        there = 0;
+#pragma unroll
+        for (int blk = 0; blk < KB; ++blk) {
+            pages |= page_of(j, blk);
+            there |= page_of(j, blk) >= 0 ? 1u << blk : 0u;
+        }
+        if constexpr (kTwoPages) {
+#pragma unroll
+            for (int i = 0; i < KB / 2; ++i) {
+                const int first = max(page_of(j, 2 * i), 0), second = max(page_of(j, 2 * i + 1), 0);
+                lane_page[i] = tile.upper ? second : first;
+                tile.load_k(i, lane_page[i], a);
+            }
+        } else {
+            fetch(j, k_base, a.kp, ke_base, a.ke, [&](int blk, const char *p, const char *e) { tile.load_k(blk, p, e, mask); });
+        }
+    };
+    // (of the tile whose K was fetched last)
+    auto fetch_v = [&](int j, uint32_t mask) __attribute__((always_inline)) {
+        if constexpr (kTwoPages) {
+#pragma unroll
+            for (int i = 0; i < KB / 2; ++i) tile.load_v(i, lane_page[i], a);
+        } else {
+            fetch(j, v_base, a.vp, ve_base, a.ve, [&](int blk, const char *p, const char *e) { tile.load_v(blk, p, e, mask); });
+        }
+    };
 
     if (n_it > 0) {
         fetch_k(0, ~0u);
@@ -802,13 +884,7 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
     bool odd = false;
     for (int j = 0; j < n_it; ++j) {
         const int n0 = (t_lo + w + NW * j) * kKeys;
-        int pages = 0;                       // negative where a block of the tile has no page
-        unsigned there = 0;                  // which of them have one
-#pragma unroll
-        for (int blk = 0; blk < KB; ++blk) {
-            pages |= page_of(j, blk);
-            there |= page_of(j, blk) >= 0 ? 1u << blk : 0u;
-        }
+        const unsigned there_now = there;
         const bool edge = n0 + kKeys - 1 > sp.pos0 || n0 <= sp.pos1 - weff || pages < 0;
         // The next tile; behind the last one the same loads from one line of it, so that the waits for what is under way can be counted: with a branch
         // around them every tile began with a wait for all of it.
@@ -826,7 +902,7 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
             tile.logits(s);
             fetch_k(next, mask);
         }
-        odd = tile.stage_v(edge, several, sp.lo - n0, sp.hi - n0, there, lane) || odd;
+        odd = tile.stage_v(edge, several, sp.lo - n0, sp.hi - n0, there_now, lane) || odd;
         fetch_v(next, mask);
         if (edge) {
 #pragma unroll
@@ -836,7 +912,7 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int key = n0 + 16 * blk + 4 * quad + e;
-                        s[nb][blk][e] = key <= pq[nb] && key > pq[nb] - weff && (there >> blk & 1) ? s[nb][blk][e] : -INFINITY;
+                        s[nb][blk][e] = key <= pq[nb] && key > pq[nb] - weff && (there_now >> blk & 1) ? s[nb][blk][e] : -INFINITY;
                     }
         }
 #pragma unroll

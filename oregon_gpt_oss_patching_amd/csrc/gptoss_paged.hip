@@ -131,7 +131,7 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     //   32 bits: 1 x 300 10.2 / 9.6, 8 x 300 11.0 / 9.9, but 1 x 500 10.4 / 11.6; 128 x 500 on two KV heads 21.7 / 16.4
     const int64_t wgs = d.units * p->G;
     const bool full = wgs > (f32 ? 128 : 256), half = wgs >= 128;
-    d.alone = d.nb > 1 || keys <= 128 || wgs > (f32 ? 256 : 512) ? kPagedWaves : f32 || full || keys <= 256 ? 8 : 16;
+    d.alone = d.nb > 1 || keys <= 128 || wgs > (f32 ? 256 : 512) ? kPagedWaves : f32 || four || full || keys <= 256 ? 8 : 16;
     const int most_alone = f32 ? (full ? 576 : 288) : d.nb > 1 ? (full ? 2304 : half ? 1152 : 832) : codes ? (full ? 3456 : half ? 2304 : 1536) : full ? 2304 : 1152;
     if (d.units > kPagedMaxUnits || keys <= most_alone) return d;
     d.alone = kPagedWaves;
@@ -162,7 +162,7 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
 template <typename T, typename ST, int NB>
 int attend(const PagedDivision &d, void *stream, PagedArgs &a) {
     if constexpr (NB == 1) {
-        if constexpr (sizeof(ST) < 4)
+        if constexpr (sizeof(ST) < 4 && !is_e2m1<ST>)
             if (d.alone == 16) return launch(attn_paged_kernel<T, ST, NB, 16>, d.units * a.G, 1024, stream, a);
         if (d.alone == 8) return launch(attn_paged_kernel<T, ST, NB, 8>, d.units * a.G, 512, stream, a);
     }
@@ -243,12 +243,14 @@ int gptoss_attn_paged_fwd(const gptoss_attn_paged_params *p, void *stream) {
         a.partial = reinterpret_cast<float *>(static_cast<char *>(p->scratch) + d.plan_bytes);
     }
     const bool codes = is_codes(p), four = p->storage == GPTOSS_ATTN_E2M1;
+    // (of rows of 32 bytes a load takes two blocks of keys, see PagedTile4)
+    const bool of_16 = p->page_size == 16;
     if (p->dtype == GPTOSS_ATTN_BF16) {
-#define GPTOSS_PAGED(NB) (four ? attend<bf16, e2m1, NB>(d, stream, a) : codes ? attend<bf16, e4m3, NB>(d, stream, a) : attend<bf16, bf16, NB>(d, stream, a))
+#define GPTOSS_PAGED(NB) (four ? (of_16 ? attend<bf16, e2m1_of_16, NB>(d, stream, a) : attend<bf16, e2m1, NB>(d, stream, a)) : codes ? attend<bf16, e4m3, NB>(d, stream, a) : attend<bf16, bf16, NB>(d, stream, a))
         return d.nb == 1 ? GPTOSS_PAGED(1) : d.nb == 2 ? GPTOSS_PAGED(2) : d.nb == 3 ? GPTOSS_PAGED(3) : GPTOSS_PAGED(4);
 #undef GPTOSS_PAGED
     }
-#define GPTOSS_PAGED(NB) (four ? attend<float, e2m1, NB>(d, stream, a) : codes ? attend<float, e4m3, NB>(d, stream, a) : attend<float, float, NB>(d, stream, a))
+#define GPTOSS_PAGED(NB) (four ? (of_16 ? attend<float, e2m1_of_16, NB>(d, stream, a) : attend<float, e2m1, NB>(d, stream, a)) : codes ? attend<float, e4m3, NB>(d, stream, a) : attend<float, float, NB>(d, stream, a))
     return d.nb == 1 ? GPTOSS_PAGED(1) : GPTOSS_PAGED(2);
 #undef GPTOSS_PAGED
 }

@@ -82,8 +82,10 @@ __device__ __forceinline__ float factor_of_byte(uint32_t e) { return __uint_as_f
 
 struct e4m3 { uint8_t code; };
 struct e2m1 { uint8_t pair; };                     // numbers 2i (lower half) and 2i + 1
+struct e2m1_of_16 : e2m1 {};                       // the same in pages of 16 tokens, to the attention
 template <typename ST> constexpr bool is_e2m1 = false;
 template <> inline constexpr bool is_e2m1<e2m1> = true;
+template <> inline constexpr bool is_e2m1<e2m1_of_16> = true;
 
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 
