@@ -435,6 +435,8 @@ typedef struct gptoss_attn_table_params {
     int32_t *row, *position, *first;        /* map: (total) each */
     int64_t *slot;
     int32_t *used;                  /* map: (1) */
+    void *scratch;                  /* update: gptoss_attn_table_workspace_bytes() bytes, 4-byte aligned, of this call alone until it has run */
+    size_t scratch_bytes;
 } gptoss_attn_table_params;
 
 /*
@@ -443,7 +445,7 @@ typedef struct gptoss_attn_table_params {
  * in ascending order, row by row; seqlens[b] = want[b].  Where the pages a row wants, with those of the rows in front of it, are more
  * than are free, the row gets none, nor does any behind it that wants some: their entries stay and seqlens[b] = have[b], as where a row wants
  * more than its table holds (which no other row suffers from).  Entries that a row gives back become -1; others are not touched.
- * left: free pages afterwards.  One workgroup: the order of nothing depends on the time.
+ * left: free pages afterwards.  Nothing depends on the order in which workgroups run.
  */
 int gptoss_attn_page_table_update(const gptoss_attn_table_params *params, void *stream);
 
@@ -453,6 +455,9 @@ int gptoss_attn_page_table_update(const gptoss_attn_table_params *params, void *
  * Behind the last token: row -1, position 0, slot -1, first = used, the number of tokens (at most total).
  */
 int gptoss_attn_token_map(const gptoss_attn_table_params *params, void *stream);
+
+/* Bytes of scratch gptoss_attn_page_table_update needs for this block (0: none; 0 for a NULL or shapeless block).  Host-only. */
+size_t gptoss_attn_table_workspace_bytes(const gptoss_attn_table_params *params);
 
 /* Host-only argument check that both start with; `call`: 0 update, 1 map. */
 int gptoss_attn_table_validate(const gptoss_attn_table_params *params, int call);

@@ -47,6 +47,7 @@ EXPORTS = (
     "gptoss_attn_paged_write_slots",
     "gptoss_attn_page_table_update",
     "gptoss_attn_token_map",
+    "gptoss_attn_table_workspace_bytes",
     "gptoss_attn_table_validate",
     "gptoss_attn_rotary",
     "gptoss_attn_rotary_validate",
@@ -127,6 +128,7 @@ class TableParams(ctypes.Structure):
         ("page_table", ctypes.c_void_p), ("have", ctypes.c_void_p), ("want", ctypes.c_void_p),
         ("seqlens", ctypes.c_void_p), ("left", ctypes.c_void_p),
         ("row", ctypes.c_void_p), ("position", ctypes.c_void_p), ("first", ctypes.c_void_p), ("slot", ctypes.c_void_p), ("used", ctypes.c_void_p),
+        ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_size_t),
     ]
 
 
@@ -219,6 +221,8 @@ def load() -> ctypes.CDLL:
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int
             fn.argtypes = [ctypes.POINTER(TableParams), ctypes.c_void_p]
+        lib.gptoss_attn_table_workspace_bytes.restype = ctypes.c_size_t
+        lib.gptoss_attn_table_workspace_bytes.argtypes = [ctypes.POINTER(TableParams)]
         lib.gptoss_attn_table_validate.restype = ctypes.c_int
         lib.gptoss_attn_table_validate.argtypes = [ctypes.POINTER(TableParams), ctypes.c_int]
         lib.gptoss_attn_rotary.restype = ctypes.c_int

@@ -73,9 +73,6 @@ TableArgs table_args(const gptoss_attn_table_params *p) {
     a.stride = p->table_stride;
     a.B = p->B; a.width = p->table_width; a.pages = p->pages; a.total = p->total;
     a.page_shift = __builtin_ctz((unsigned)p->page_size);
-    // a row's entries are read by all threads where there is one row, by sixteen from 64 rows on
-    a.row_threads_shift = 10;
-    for (int rows = 1; rows < p->B && rows < 64; rows *= 2) --a.row_threads_shift;
     return a;
 }
 
@@ -309,13 +306,33 @@ int gptoss_attn_table_validate(const gptoss_attn_table_params *p, int call) {
         if (!t) return GPTOSS_ATTN_ERR_NULL_TENSOR;
         if (!aligned(t, 4)) return GPTOSS_ATTN_ERR_ALIGNMENT;
     }
-    if (call && !p->slot) return GPTOSS_ATTN_ERR_NULL_TENSOR;
-    return call && !aligned(p->slot, 8) ? GPTOSS_ATTN_ERR_ALIGNMENT : GPTOSS_ATTN_OK;
+    if (!call) {
+        const size_t need = gptoss_attn_table_workspace_bytes(p);
+        if (!aligned(p->scratch, 4)) return GPTOSS_ATTN_ERR_ALIGNMENT;
+        return p->scratch_bytes < need || (need && !p->scratch) ? GPTOSS_ATTN_ERR_WORKSPACE : GPTOSS_ATTN_OK;
+    }
+    if (!p->slot) return GPTOSS_ATTN_ERR_NULL_TENSOR;
+    return !aligned(p->slot, 8) ? GPTOSS_ATTN_ERR_ALIGNMENT : GPTOSS_ATTN_OK;
+}
+
+size_t gptoss_attn_table_workspace_bytes(const gptoss_attn_table_params *p) {
+    if (!p || p->B <= 0 || p->table_width <= 0 || p->pages <= 0 || p->pages > kPoolBits) return 0;
+    // A launch for the bits alone where one workgroup would take more than two rounds for the runs that the table has room for (the lengths are the device's).  us, one launch / two: 128
+    // rows of 1000 tokens (two rounds) 6.9 / 7.1, 128 of 4000 9.0 / 10.0, 64 of 4000 (one) 6.9 / 8.6; 256 of 1000 (four) 10.0 / 7.5, 64 of 16000 12.8 / 11.1, 1024 of 300 28.8 / 8.1.
+    const int lanes = mark_lanes(p->table_width), runs = mark_runs(p->table_width);
+    if ((int64_t)p->B * runs <= 2 * (kTableThreads / lanes)) return 0;
+    return (size_t)kMarkers * ((p->pages + 31) / 32) * sizeof(uint32_t);
 }
 
 int gptoss_attn_page_table_update(const gptoss_attn_table_params *p, void *stream) {
-    const int rc = gptoss_attn_table_validate(p, 0);
-    return rc ? rc : launch(page_table_update_kernel, 1, kTableThreads, stream, table_args(p));
+    int rc = gptoss_attn_table_validate(p, 0);
+    if (rc) return rc;
+    TableArgs a = table_args(p);
+    if (gptoss_attn_table_workspace_bytes(p)) {
+        a.marks = static_cast<uint32_t *>(p->scratch);
+        if ((rc = launch(page_table_mark_kernel, kMarkers, kTableThreads, stream, a))) return rc;
+    }
+    return launch(page_table_update_kernel, 1, kTableThreads, stream, a);
 }
 
 int gptoss_attn_token_map(const gptoss_attn_table_params *p, void *stream) {

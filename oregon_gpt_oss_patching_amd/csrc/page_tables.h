@@ -1,8 +1,9 @@
 // Whose page is whose (gptoss_attn_page_table_update) and where the tokens of a call go (gptoss_attn_token_map): whole numbers only.
 //
-// What bounds both: latencies.  A decoding step's update reads some ten thousand entries and writes a dozen; what it takes is a launch and a chain of
-// dependent loads and barriers, so it is one workgroup with its counts and the pool's bits in LDS, and no list of free pages is kept
-// from call to call: a page is free iff no row's kept entry names it.
+// No list of free pages is kept from call to call: a page is free iff no row's kept entry names it, so each update reads all of them.  What bounds it is not their bytes but latencies, and the
+// LDS atomics that set a bit for each (some 1.3 a cycle): one workgroup has its counts and the pool's bits in LDS; where a table may be large, sixteen others set the bits first, each of its
+// share of the entries, in a launch of its own.  256 rows of 40 to 9000 tokens: 9.8 us, 3 of them the first launch;
+// 4096 of 500 18.6; 8 of 1000, in one launch, 4.7.
 #pragma once
 #include "paged_common.h"
 
@@ -10,6 +11,8 @@ namespace gptoss {
 
 constexpr int kTableRows = 16384;                  // rows of a call: a number of 32 bits each in LDS
 constexpr int kTableThreads = 1024;
+constexpr int kMarkers = 16;                       // workgroups that set bits in a launch of their own
+constexpr int kFresh = 4096;                       // pages that are handed out together: 16 KB
 constexpr int kPoolBits = 1 << 19;                 // pages that are looked at together: 64 KB of LDS
 constexpr int kPoolGroup = 64 * 32;                // pages of a wavefront's word each
 constexpr uint32_t kMany = (1u << 30) + 1;         // sums stay here: more than there are pages or tokens
@@ -20,9 +23,9 @@ struct TableArgs {
     int32_t *seqlens, *left;
     int32_t *row, *position, *first, *used;        // map
     int64_t *slot;
+    uint32_t *marks;                               // update: the bits that page_table_mark_kernel has set, or NULL
     int64_t stride;
     int B, width, pages, page_shift, total;
-    int row_threads_shift;                         // update: 2^this threads read a row's entries
 };
 
 __device__ __forceinline__ uint32_t add_up(uint32_t x, uint32_t y) { return min(x + y, kMany); }      // (2 kMany is below 2^32)
@@ -38,24 +41,51 @@ __device__ __forceinline__ uint32_t wave_scan_up(uint32_t x) {
     return x;
 }
 
-// ends[i] = value(0) + ... + value(i) for i < n, by all THREADS; `part`: a number for each wavefront.  Ends with a barrier.
-template <int THREADS, typename F>
-__device__ __forceinline__ void block_sums(uint32_t *ends, uint32_t *part, int n, F value) {
+// the largest of the lanes up to this one, of numbers from 0 on
+__device__ __forceinline__ int wave_scan_max(int x) {
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));        // as in wave_scan_up
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+    return x;
+}
+
+// ends[i] = value(0) + ... + value(i) for i < n, by all THREADS, EACH numbers a thread at a time; `part`: a number for each wavefront.  Ends with a barrier.
+template <int THREADS, int EACH, typename F>
+__device__ __forceinline__ void sums_of(uint32_t *ends, uint32_t *part, int n, F value) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     uint32_t before = 0;
-    for (int i0 = 0; i0 < n; i0 += THREADS) {
-        const uint32_t x = wave_scan_up(i0 + tid < n ? min(value(i0 + tid), kMany) : 0u);
-        if (lane == 63) part[w] = x;
+    for (int i0 = 0; i0 < n; i0 += EACH * THREADS) {
+        uint32_t x[EACH];
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) x[k] = i0 + EACH * tid + k < n ? min(value(i0 + EACH * tid + k), kMany) : 0u;
+#pragma unroll
+        for (int k = 1; k < EACH; ++k) x[k] = add_up(x[k], x[k - 1]);
+        const uint32_t incl = wave_scan_up(x[EACH - 1]);
+        if (lane == 63) part[w] = incl;
         __syncthreads();
+        // what stands in front of the thread's: earlier rounds, wavefronts and lanes (sums that stay at kMany come to kMany here too)
         uint32_t mine = before;
         for (int k = 0; k < THREADS / 64; ++k) {
             const uint32_t p = part[k];
             mine = k < w ? add_up(mine, p) : mine;
             before = add_up(before, p);
         }
-        if (i0 + tid < n) ends[i0 + tid] = add_up(mine, x);
+        const uint32_t lower = (uint32_t)__shfl_up((int)incl, 1);
+        mine = add_up(mine, lane ? lower : 0u);
+#pragma unroll
+        for (int k = 0; k < EACH; ++k)
+            if (i0 + EACH * tid + k < n) ends[i0 + EACH * tid + k] = add_up(mine, x[k]);
         __syncthreads();
     }
+}
+// (four at a time where one each would take several rounds: 4096 rows 4.5 us, so 2.9; one round 1.0 and 1.5)
+template <int THREADS, typename F>
+__device__ __forceinline__ void block_sums(uint32_t *ends, uint32_t *part, int n, F value) {
+    if (n <= THREADS) sums_of<THREADS, 1>(ends, part, n, value);
+    else sums_of<THREADS, 4>(ends, part, n, value);
 }
 
 // The first i < n with ends[i] > x, n where there is none.
@@ -76,33 +106,57 @@ __device__ __forceinline__ RowPages row_pages(const TableArgs &a, int b) {
     return RowPages{(int)min(has, (int64_t)a.width), (int)min(wants, (int64_t)a.width), wants <= a.width};
 }
 
-// Bits of the pages lo .. lo + kPoolBits - 1 that rows keep.  Ends with a barrier.
-__device__ __forceinline__ void mark_kept(const TableArgs &a, uint32_t *bits, int lo, int words) {
-    constexpr int kAtOnce = 16;                    // loads under way
-    for (int i = threadIdx.x; i < words; i += kTableThreads) bits[i] = 0;
-    __syncthreads();
-    const int n = 1 << a.row_threads_shift, lane = threadIdx.x & (n - 1);
-    for (int b = threadIdx.x >> a.row_threads_shift; b < a.B; b += kTableThreads >> a.row_threads_shift) {
+// Lanes that read a run of a row's entries, sixteen each, and how many runs rows of a table have: where they have one of sixteen lanes at most, four rows to a wavefront.
+constexpr int kMarkEach = 16;
+__host__ __device__ __forceinline__ int mark_lanes(int width) { return width <= 16 * kMarkEach ? 16 : 64; }
+__host__ __device__ __forceinline__ int mark_runs(int width) { return (width + kMarkEach * mark_lanes(width) - 1) / (kMarkEach * mark_lanes(width)); }
+
+// Bits of the pages lo .. lo + kPoolBits - 1 that rows keep: runs in turn among the `waves` of which this is number `wave` (4096 rows
+// of 500 tokens with a wavefront each 34.6 us in all, so 18.6).  `bits` of LDS, zeros already; ends with a barrier.
+__device__ __forceinline__ void mark_kept(const TableArgs &a, uint32_t *bits, int lo, int wave, int waves) {
+    constexpr int kEach = kMarkEach;
+    const int lanes = mark_lanes(a.width), lane = threadIdx.x & (lanes - 1), per_wave = 64 / lanes;
+    const int runs = mark_runs(a.width), groups = waves * per_wave, group = wave * per_wave + (threadIdx.x & 63) / lanes;
+    int b = group / runs, run = group - b * runs;
+    const int rows_on = groups / runs, runs_on = groups - rows_on * runs;
+    while (b < a.B) {
         const RowPages r = row_pages(a, b);
-        const int kept = min(r.has, r.wants);
+        const int first = run * kEach * lanes + lane, kept = min(r.has, r.wants);
         const int32_t *row = a.table + b * a.stride;
-        for (int i0 = lane; i0 < kept; i0 += kAtOnce * n) {
-            int page[kAtOnce];
+        int page[kEach];
 #pragma unroll
-            for (int k = 0; k < kAtOnce; ++k) page[k] = i0 + k * n < kept ? row[i0 + k * n] : -1;
+        for (int k = 0; k < kEach; ++k) page[k] = first + k * lanes < kept ? row[first + k * lanes] : -1;
 #pragma unroll
-            for (int k = 0; k < kAtOnce; ++k) {
-                const int at = page[k] - lo;
-                if (page[k] >= 0 && page[k] < a.pages && at >= 0 && at < kPoolBits) atomicOr(bits + (at >> 5), 1u << (at & 31));
-            }
+        for (int k = 0; k < kEach; ++k) {
+            const int at = page[k] - lo;
+            if (page[k] >= 0 && page[k] < a.pages && at >= 0 && at < kPoolBits) atomicOr(bits + (at >> 5), 1u << (at & 31));
         }
+        b += rows_on;
+        run += runs_on;
+        if (run >= runs) { run -= runs; ++b; }
     }
     __syncthreads();
 }
 
+__device__ __forceinline__ void clear_bits(uint32_t *bits, int words) {
+    for (int i = threadIdx.x; i < words; i += kTableThreads) bits[i] = 0;
+    __syncthreads();
+}
+
+// The bits of a share of the kept entries, to a.marks + blockIdx.x * words.
+__global__ __launch_bounds__(kTableThreads) void page_table_mark_kernel(const TableArgs a) {
+    __shared__ uint32_t bits[kPoolBits / 32];
+    const int words = (a.pages + 31) / 32;
+    clear_bits(bits, words);
+    mark_kept(a, bits, 0, __builtin_amdgcn_readfirstlane(blockIdx.x * (kTableThreads / 64) + (threadIdx.x >> 6)), kMarkers * (kTableThreads / 64));
+    uint32_t *out = a.marks + (int64_t)blockIdx.x * words;
+    for (int i = threadIdx.x; i < words; i += kTableThreads) out[i] = bits[i];
+}
+
 __global__ __launch_bounds__(kTableThreads) void page_table_update_kernel(const TableArgs a) {
-    __shared__ uint32_t ends[kTableRows], bits[kPoolBits / 32], base[kPoolBits / kPoolGroup], part[kTableThreads / 64];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    __shared__ uint32_t ends[kTableRows], bits[kPoolBits / 32], base[kPoolBits / kPoolGroup + 1], fresh[kFresh], part[kTableThreads / 64];
+    __shared__ uint16_t row_at[kFresh];            // row + 1, 0: none begins here
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     block_sums<kTableThreads>(ends, part, a.B, [&](int b) __attribute__((always_inline)) {
         const RowPages r = row_pages(a, b);
         return r.fits && r.wants > r.has ? (uint32_t)(r.wants - r.has) : 0u;
@@ -118,74 +172,127 @@ __global__ __launch_bounds__(kTableThreads) void page_table_update_kernel(const 
             if (lane == 63) base[g] = incl;
         }
         __syncthreads();
-        uint32_t all = 0;
         if (w == 0) {
+            uint32_t all = 0;
             for (int g0 = 0; g0 < groups; g0 += 64) {
                 const uint32_t x = g0 + lane < groups ? base[g0 + lane] : 0u, incl = wave_scan_up(x);
                 if (g0 + lane < groups) base[g0 + lane] = all + incl - x;
                 all += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
             }
-            if (lane == 0) part[0] = all;
+            if (lane == 0) base[groups] = all;
         }
         __syncthreads();
-        all = part[0];
-        __syncthreads();
-        return all;
+        return base[groups];
     };
     auto span_of = [&](int lo) { return min(a.pages - lo, kPoolBits); };
+    auto mark = [&](int lo) __attribute__((always_inline)) {
+        const int words = (span_of(lo) + 31) / 32;
+        if (a.marks) {                             // (the pool is one part then)
+            for (int i = tid; i < words; i += kTableThreads) {
+                uint32_t x[kMarkers];
+#pragma unroll
+                for (int k = 0; k < kMarkers; ++k) x[k] = a.marks[k * words + i];
+#pragma unroll
+                for (int k = 1; k < kMarkers; ++k) x[0] |= x[k];
+                bits[i] = x[0];
+            }
+            __syncthreads();
+        } else {
+            clear_bits(bits, words);
+            mark_kept(a, bits, lo, w, kTableThreads / 64);
+        }
+    };
     uint32_t free = 0;
     for (int lo = 0; lo < a.pages; lo += kPoolBits) {        // (pages <= 2^30: lo stays below 2^31)
-        mark_kept(a, bits, lo, (span_of(lo) + 31) / 32);
+        mark(lo);
         free += count(lo, span_of(lo));
+        __syncthreads();
     }
     // Rows in their order: whoever's demand, with those in front of it, passes what is free gets nothing, nor does any behind it that wants pages.
-    const bool enough = demand <= free;
-    const int served_rows = enough ? a.B : first_above(ends, a.B, free);
-    const uint32_t given = enough ? demand : served_rows ? ends[served_rows - 1] : 0u;
+    uint32_t given = demand;
+    if (demand > free) {
+        const int served = first_above(ends, a.B, free);
+        given = served ? ends[served - 1] : 0u;
+    }
     uint32_t before = 0;
     for (int lo = 0; lo < a.pages && before < given; lo += kPoolBits) {
         uint32_t here = free;
         if (a.pages > kPoolBits) {                 // (otherwise the bits are there)
-            mark_kept(a, bits, lo, (span_of(lo) + 31) / 32);
+            mark(lo);
             here = count(lo, span_of(lo));
         }
         const int span = span_of(lo), groups = (span + kPoolGroup - 1) / kPoolGroup;
-        for (int g = w; g < groups; g += kTableThreads / 64) {
-            const uint32_t from = before + base[g];
-            if (from >= given) break;
-            const int first = g * kPoolGroup + 32 * lane, there = min(max(span - first, 0), 32);
-            uint32_t set = there ? ~bits[first >> 5] & (~0u >> (32 - there)) : 0u;
-            const uint32_t number = __popc(set);
-            uint32_t rank = from + wave_scan_up(number) - number;
-            if (!set || rank >= given) continue;
-            int b = first_above(ends, a.B, rank);
-            while (set && rank < given) {
-                while (ends[b] <= rank) ++b;
-                const RowPages r = row_pages(a, b);
-                const uint32_t row_first = b ? ends[b - 1] : 0u;
-                // (the row's pages that this word holds)
-                int32_t *to = a.table + b * a.stride + r.has;
-                do {
-                    const int bit = __ffs(set) - 1;
-                    set &= set - 1;
-                    to[rank - row_first] = lo + first + bit;
-                    ++rank;
-                } while (set && rank < ends[b]);
+        const uint32_t end = min(before + here, given);
+        // kFresh pages at a time into LDS by their rank, and the rows at the first of their ranks; a rank's row is then the last one at or before it.
+        for (uint32_t c0 = before; c0 < end; c0 += kFresh) {
+            constexpr int kEach = kFresh / kTableThreads;
+            const uint32_t c1 = min(c0 + kFresh, end);
+            const bool few = c1 - c0 <= kTableThreads;           // (a search for each is quicker then: 256 rows 1.8 us, and 2.4)
+            if (!few) {
+                for (int i = tid; i < kFresh; i += kTableThreads) row_at[i] = 0;
+                __syncthreads();
+                for (int b = tid; b < a.B; b += kTableThreads) {
+                    const uint32_t r0 = max(b ? ends[b - 1] : 0u, c0);
+                    if (r0 < min(ends[b], c1)) row_at[r0 - c0] = (uint16_t)(b + 1);
+                }
             }
+            for (int g = w; g < groups; g += kTableThreads / 64) {
+                if (before + base[g + 1] <= c0 || before + base[g] >= c1) continue;
+                const int first = g * kPoolGroup + 32 * lane, there = min(max(span - first, 0), 32);
+                uint32_t set = there ? ~bits[first >> 5] & (~0u >> (32 - there)) : 0u;
+                const uint32_t number = __popc(set);
+                uint32_t rank = before + base[g] + wave_scan_up(number) - number;
+                for (; set; set &= set - 1, ++rank)
+                    if (rank >= c0 && rank < c1) fresh[rank - c0] = (uint32_t)(lo + first + __ffs(set) - 1);
+            }
+            __syncthreads();
+            if (few) {
+                if (c0 + tid < c1) {
+                    const int b = first_above(ends, a.B, c0 + tid);
+                    a.table[b * a.stride + row_pages(a, b).has + (c0 + tid - (b ? ends[b - 1] : 0u))] = (int32_t)fresh[tid];
+                }
+                __syncthreads();
+                continue;
+            }
+            // the thread's kEach ranks
+            int row[kEach], has[kEach];
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) row[k] = max((int)row_at[kEach * tid + k], k ? row[k - 1] : 0);
+            const int incl = wave_scan_max(row[kEach - 1]);
+            if (lane == 63) part[w] = (uint32_t)incl;
+            __syncthreads();
+            int front = __shfl_up(incl, 1);
+            front = lane ? front : 0;
+            for (int k = 0; k < w; ++k) front = max(front, (int)part[k]);
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                row[k] = max(row[k], front) - 1;
+                has[k] = c0 + kEach * tid + k < c1 ? row_pages(a, row[k]).has : 0;
+            }
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const uint32_t i = kEach * tid + k;
+                if (c0 + i < c1) a.table[row[k] * a.stride + has[k] + (c0 + i - (row[k] ? ends[row[k] - 1] : 0u))] = (int32_t)fresh[i];
+            }
+            __syncthreads();
         }
         before += here;
-        __syncthreads();
-    }
-    for (int b = tid; b < a.B; b += kTableThreads) {
-        const RowPages r = row_pages(a, b);
-        a.seqlens[b] = max(r.fits && (r.wants <= r.has || ends[b] <= free) ? a.want[b] : a.have[b], 0);
     }
     if (tid == 0) *a.left = (int32_t)(free - given);
-    // what rows give back
-    const int n = 1 << a.row_threads_shift, l = tid & (n - 1);
-    for (int b = tid >> a.row_threads_shift; b < a.B; b += kTableThreads >> a.row_threads_shift) {
-        const RowPages r = row_pages(a, b);
-        for (int i = r.wants + l; i < r.has; i += n) a.table[b * a.stride + i] = -1;
+    for (int b0 = w * 64; b0 < a.B; b0 += kTableThreads) {
+        const int b = b0 + lane;
+        RowPages r{0, 0, true};
+        if (b < a.B) {
+            r = row_pages(a, b);
+            a.seqlens[b] = max(r.fits && (r.wants <= r.has || ends[b] <= free) ? a.want[b] : a.have[b], 0);
+        }
+        // what rows give back, the wavefront's one after the other
+        unsigned long long back = __builtin_amdgcn_ballot_w64(r.has > r.wants);
+        while (back) {
+            const int l = __builtin_ctzll(back), has = __builtin_amdgcn_readlane(r.has, l), wants = __builtin_amdgcn_readlane(r.wants, l);
+            back &= back - 1;
+            for (int i = wants + lane; i < has; i += 64) a.table[(int64_t)(b0 + l) * a.stride + i] = -1;
+        }
     }
 }
 

@@ -42,6 +42,9 @@ Pair page_table_update(const Tensor &page_table, const Tensor &have, const Tenso
     Tensor seqlens = new_tensor({page_table.size(0)}, at::kInt, page_table), left = new_tensor({1}, at::kInt, page_table);
     c.p.seqlens = seqlens.data_ptr<int32_t>();
     c.p.left = left.data_ptr<int32_t>();
+    c.p.scratch_bytes = gptoss_attn_table_workspace_bytes(&c.p);
+    const Tensor scratch = c.p.scratch_bytes ? new_tensor({static_cast<int64_t>(c.p.scratch_bytes / sizeof(int32_t))}, at::kInt, page_table) : Tensor();
+    if (c.p.scratch_bytes) c.p.scratch = scratch.data_ptr();
     about_to_write({&page_table});
     check("gptoss_attn_page_table_update", gptoss_attn_page_table_update(&c.p, stream_of(page_table)));
     return {seqlens, left};

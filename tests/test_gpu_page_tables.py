@@ -340,3 +340,37 @@ def test_refusals(A):
     ):
         with pytest.raises(RuntimeError, match=what):
             call()
+
+
+@pytest.mark.parametrize("rows,width,pages", [(128, 256, 3000), (129, 256, 3000), (32, 257, 9000), (33, 257, 9000), (33, 1025, 1 << 19), (33, 1025, (1 << 19) + 1), (700, 40, 40000), (5, 20000, 100000)])
+def test_one_launch_or_two(A, rows, width, pages):
+    """Tables on both sides of what decides whether a launch of its own sets the bits, and how many lanes read a run; as many new pages as are given out together, and more."""
+    print(f"case rows={rows} width={width} pages={pages}", flush=True)
+    rng = random.Random(rows + width)
+    longest = min(16 * width, 16 * (pages // rows) // 2)
+    have = [rng.choice((0, rng.randint(1, longest))) for _ in range(rows)]
+    table = tables_of(rng, have, 16, pages, width)
+    for new in (0, 40, 900):
+        want = [min(n + rng.randint(0, new), 16 * width) if rng.random() < 0.9 else 0 for n in have]
+        table, have = check_update(A, table, have, want, pages, 16)
+
+
+def test_two_updates_at_once(A):
+    """Tables of their own on two streams, with scratch of their own: what they give alone."""
+    rng = random.Random(8)
+    have = [rng.randint(1, 3000) for _ in range(300)]
+    want = [n + rng.randint(0, 40) for n in have]
+    pages = sum(T.pages_for(n, 16) for n in want) + 50
+    table = tables_of(rng, have, 16, pages, 200)
+    ref = T.update(table, have, want, pages, 16)
+    tables = [ints(table) for _ in range(8)]
+    h, w = ints(have), ints(want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    out = []
+    for i, t in enumerate(tables):
+        with torch.cuda.stream(streams[i % 2]):
+            out.append(A.page_table_update(t, h, w, pages, 16))
+    torch.cuda.synchronize()
+    for t, (got, left) in zip(tables, out):
+        assert t.tolist() == ref[0] and got.tolist() == ref[1] and left.tolist() == [ref[2]]

@@ -55,6 +55,24 @@ def test_validate(field, value, code, calls):
     assert _lib.load().gptoss_attn_table_validate(None, 0) == -1
 
 
+@pytest.mark.parametrize("rows,width,pages,need", [
+    (128, 256, 1000, 0), (129, 256, 1000, 16 * 32 * 4), (32, 257, 1000, 0), (33, 257, 1000, 16 * 32 * 4), (16, 2048, 33, 0), (17, 2048, 33, 16 * 2 * 4), (5000, 100, 1 << 19, 16 << 16),
+    (5000, 100, (1 << 19) + 1, 0), (0, 100, 100, 0),
+])
+def test_update_scratch(rows, width, pages, need):
+    """A launch that sets the pool's bits takes sixteen copies of them; pools of more than 2^19 pages are looked at in parts, by one workgroup."""
+    p = _params()
+    p.B, p.table_width, p.table_stride, p.pages = rows, width, width, pages
+    lib = _lib.load()
+    assert lib.gptoss_attn_table_workspace_bytes(ctypes.byref(p)) == need and lib.gptoss_attn_table_workspace_bytes(None) == 0
+    if need:
+        assert lib.gptoss_attn_table_validate(ctypes.byref(p), UPDATE) == lib.gptoss_attn_page_table_update(ctypes.byref(p), None) == -10
+        p.scratch, p.scratch_bytes = 0x1000, need - 1
+        assert lib.gptoss_attn_table_validate(ctypes.byref(p), UPDATE) == -10
+        p.scratch_bytes = need
+        assert lib.gptoss_attn_table_validate(ctypes.byref(p), UPDATE) == 0
+
+
 @pytest.mark.parametrize("mutate,code", [
     (lambda p: None, 0), (lambda p: setattr(p, "page_table", None), 0), (lambda p: setattr(p, "start", None), 0), (lambda p: setattr(p, "table_width", 0), 0), (lambda p: setattr(p, "B", 2), -5),
     (lambda p: setattr(p, "Sq", 0), -5), (lambda p: setattr(p, "k", None), -2), (lambda p: setattr(p, "pages", 0), -11), (lambda p: setattr(p, "page_size", 24), -11),
