@@ -199,7 +199,7 @@ def test_second_derivative_and_differences(A):
     with torch.no_grad():
         e = 2.0 ** -6
         slope = (f(q + e * v, k).double() - f(q - e * v, k).double()) / (2 * e)      # (quadratic: exact but for the roundings, 2^-24 of sums below 2^7, over 2^-5)
-    assert abs(float(slope - (g.double() * v.double()).sum())) < 2e-3
+    assert abs(float(slope - (g.detach().double() * v.double()).sum())) < 2e-3
 
 
 def test_captured_and_replayed(A):
@@ -294,3 +294,48 @@ def test_patched_layer(A):
     assert M.apply_rotary_pos_emb is before and len(found[0]) == 9
     for x, y in zip(*found):
         assert float((x - y).norm()) <= 1e-4 * float(x.norm())
+
+
+def test_both_directions_captured(A):
+    """The call and its way back (what a gradient goes through) in one graph, replayed with other positions between eager calls."""
+    rope = A.rotary_frequencies(64, 150000.0, factor=32.0, original_length=4096)
+    gen = torch.Generator().manual_seed(12)
+    q, k, gq, gk = (torch.randn(2, n, 70, 64, generator=gen).to(BF16).to(DEV) for n in (8, 2, 8, 2))
+    at = torch.arange(70, device=DEV).expand(2, 70).clone()
+
+    def both():
+        out = A.rotary(q, k, at, rope)
+        return (*out, *torch.ops.gptoss_attn.rotary(gq, gk, at, rope.frequencies, None, None, rope.scale, False, True))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = both()
+    for step in range(3):
+        at += 977 * step
+        for t in outs:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        x, y = q.clone().requires_grad_(), k.clone().requires_grad_()
+        a, b = A.rotary(x, y, at, rope)
+        want = (a, b, *torch.autograd.grad((a, b), (x, y), (gq, gk)))
+        assert all(torch.equal(s, t) for s, t in zip(outs, want)), step
+
+
+def test_transforms_and_changed_positions_are_refused(A):
+    rope = A.rotary_frequencies(64, 10000.0)
+    q, at = torch.randn(1, 2, 3, 64, device=DEV), torch.arange(3, device=DEV)
+    for call in (lambda: torch.func.grad(lambda a: (A.rotary(a, q, at, rope)[0] ** 2).sum())(q), lambda: torch.func.jvp(lambda a: A.rotary(a, q, at, rope)[0], (q,), (q,)),
+                 lambda: torch.vmap(lambda a: A.rotary(a, a, at, rope)[0])(q[None])):
+        with pytest.raises(RuntimeError):
+            call()
+    x = q.clone().requires_grad_()
+    out = A.rotary(x, q, at, rope)[0]
+    at += 1                                    # the gradient would be turned by other angles
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(out.sum(), x)
