@@ -107,14 +107,24 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     const int64_t r = p->H / p->G, pairs = (int64_t)p->Sq * r;
     const int most = p->dtype == GPTOSS_ATTN_FP32 ? paged_pairs<float>() : paged_pairs<bf16>();
     d.nb = pairs <= 16 ? 1 : pairs <= 32 || most == 32 ? 2 : pairs <= 48 ? 3 : 4;
+    // the most keys that a unit of 16 * nb pairs can see
+    const auto seen = [&](int nb) {
+        int64_t keys = (int64_t)p->table_width * p->page_size;
+        if (p->max_len > 0 && p->max_len < keys) keys = p->max_len;
+        const int64_t queries = (16 * nb - 1) / r + 2;                 // that a unit's pairs touch
+        return p->window > 0 && p->window + queries < keys ? p->window + queries : keys;
+    };
+    // Of rows in 4 bits a step's reads are few: where all units' are, what counts is how long a workgroup takes for its own, and units of fewer pairs, which read the same rows
+    // again, end sooner.  us, as many pairs as there are (up to 64) / at most 32 / 16, eight heads on each of 8 KV heads: windows of 128 keys, 24 rows of five queries 8.7 / 8.3 / 7.3, 4 of
+    // eight 9.5 / 6.8 / 6.0, 64 of eight 12.4 / 11.3 / 13.7; 8 x 300 tokens with eight 10.1 / 7.3 / 6.1, 2 x 700 with 64 13.6 / 10.0 / 10.2, 1 x 3000 with eight 13.8 / 11.3 / 10.3, 32 x 300
+    // with four 7.5 / - / 7.9; but 24 rows of 500 to 9000 with five 31.2 / 34.3 / 35.2, 16 x 8192 with eight 45.2 / 49.8 / 61.9
+    if (four)
+        for (int nb = 1; nb < d.nb; ++nb)
+            if ((double)((pairs + 16 * nb - 1) / (16 * nb)) * p->B * p->G * seen(nb) <= 1 << 18) d.nb = nb;
     const int64_t blocks = (pairs + 16 * d.nb - 1) / (16 * d.nb);
     d.blocks = (int)(blocks < 0x7fffffff ? blocks : 0x7fffffff);
     d.units = blocks * p->B;
-    // the most keys that a unit can see
-    int64_t keys = (int64_t)p->table_width * p->page_size;
-    if (p->max_len > 0 && p->max_len < keys) keys = p->max_len;
-    const int64_t queries = (16 * d.nb - 1) / r + 2;                   // that a unit's pairs touch
-    if (p->window > 0 && p->window + queries < keys) keys = p->window + queries;
+    const int64_t keys = seen(d.nb);
     // Short rows: a workgroup walks a unit alone, as many wavefronts as its keys and the compute unit's share of the workgroups have room for, and
     // there is nothing to add in a second launch.  What counts is what the host knows of the lengths: in a table far wider than the rows, without max_len, these are cut too, 32 x 1000
     // tokens 18.7 and not 15.3, with four queries 23.1 / 15.7, 32 x 2000 in codes 21.8 / 16.0.  Rows of few bytes, and workgroups that fill the chip by themselves, go alone for longer.  us, cut / alone, 64
@@ -125,6 +135,8 @@ PagedDivision paged_division(const gptoss_attn_paged_params *p) {
     //   16 to 3500 12.6 / 15.7; more than one: 64 to 3500 21.1 / 18.4, 40 to 3500 17.0 / 17.2, 40 to 4500 17.9 / 20.4
     //   four queries a row (four wavefronts): 3 to 800 10.2 / 10.1, 3 to 1000 10.3 / 11.4, 32 x 500 16.3 / 9.4; 16 to 1000 11.4 / 10.9, 16 to 1300 12.9 / 13.2; 64 to 2000 24.9 / 20.2, 40 to
     //   3000 22.4 / 23.5
+    //   e2m1 (eight wavefronts, us with 8 / 16: 1 x 600 6.2 / 7.4, 1 x 1100 7.8 / 8.5, 40 x 1100 11.5 / 15.8, 64 x 1100 12.0 / 16.2, but 1 x 3000 14.1 / 13.4): 1 x 1500 9.2 / 9.3, 8 x 1500
+    //   10.9 / 9.7; 16 x 2000 14.3 / 11.5, 32 x 2000 17.0 / 11.8, 16 x 3000 14.6 / 14.8; 64 x 3000 28.5 / 22.4
     //   32 bits: 1 x 300 10.2 / 9.6, 8 x 300 11.0 / 9.9, but 1 x 500 10.4 / 11.6; 128 x 500 on two KV heads 21.7 / 16.4
     const int64_t wgs = d.units * p->G;
     const bool full = wgs > (f32 ? 128 : 256), half = wgs >= 128;
