@@ -81,7 +81,8 @@ enum gptoss_attn_status {
     GPTOSS_ATTN_ERR_ALIGNMENT = -7,     /* a tensor base or stride breaks 16-byte row alignment */
     GPTOSS_ATTN_ERR_STRIDE = -8,        /* a sequence stride smaller than D or larger than 2^24 elements; of pages also a stride from page to page below 0 or of 2^32 bytes and more */
     GPTOSS_ATTN_ERR_ABI = -9,           /* struct_size does not match this library */
-    GPTOSS_ATTN_ERR_WORKSPACE = -10,    /* gptoss_attn_bwd_static: 24*B*H*Sq bytes do not fit the built-in scratch */
+    GPTOSS_ATTN_ERR_WORKSPACE = -10,    /* gptoss_attn_bwd_static: 24*B*H*Sq bytes do not fit the built-in scratch; calls
+                                           that take one: scratch_bytes is less than they need */
     GPTOSS_ATTN_ERR_PAGES = -11         /* paged cache: page_size no power of two from 16 to 1024, pages or table_width <= 0,
                                            table_stride < 0, or table_width * page_size above 2^30 */
 };
@@ -408,8 +409,8 @@ size_t gptoss_attn_paged_workspace_bytes(const gptoss_attn_paged_params *params)
 
 /*
  * New tokens to slots of their own: token i of the Sq tokens of k and v (B = 1) goes to slot slots[i], that is to token
- * slots[i] % page_size of page slots[i] / page_size.  Slots below 0 or behind the pool are dropped.  Of the block's page table, start and
- * seqlens nothing is read.
+ * slots[i] % page_size of page slots[i] / page_size.  Slots below 0 or behind the pool are dropped; no two tokens may have the same.  Of the
+ * block's page table, start and seqlens nothing is read.
  */
 int gptoss_attn_paged_write_slots(const gptoss_attn_paged_params *params, const int64_t *slots, void *stream);
 
@@ -445,7 +446,7 @@ typedef struct gptoss_attn_table_params {
  * in ascending order, row by row; seqlens[b] = want[b].  Where the pages a row wants, with those of the rows in front of it, are more
  * than are free, the row gets none, nor does any behind it that wants some: their entries stay and seqlens[b] = have[b], as where a row wants
  * more than its table holds (which no other row suffers from).  Entries that a row gives back become -1; others are not touched.
- * left: free pages afterwards.  Nothing depends on the order in which workgroups run.
+ * left: free pages afterwards.  Nothing depends on the order in which workgroups run.  seqlens may be have or want itself.
  */
 int gptoss_attn_page_table_update(const gptoss_attn_table_params *params, void *stream);
 

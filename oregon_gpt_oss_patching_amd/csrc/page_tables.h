@@ -128,8 +128,8 @@ __device__ __forceinline__ void mark_kept(const TableArgs &a, uint32_t *bits, in
         for (int k = 0; k < kEach; ++k) page[k] = first + k * lanes < kept ? row[first + k * lanes] : -1;
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
-            const int at = page[k] - lo;
-            if (page[k] >= 0 && page[k] < a.pages && at >= 0 && at < kPoolBits) atomicOr(bits + (at >> 5), 1u << (at & 31));
+            const uint32_t at = (uint32_t)page[k] - (uint32_t)lo;                // (pages in front of lo come to 2^31 and more)
+            if (page[k] >= 0 && page[k] < a.pages && at < (uint32_t)kPoolBits) atomicOr(bits + (at >> 5), 1u << (at & 31));
         }
         b += rows_on;
         run += runs_on;

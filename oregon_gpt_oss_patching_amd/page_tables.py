@@ -79,6 +79,8 @@ def page_table_update(page_table, have, want, pages, page_size):
     grow in ascending order, row by row.  Where there are too few, the first row that does not get all it wants gets none, nor does any behind it
     that wants some; a row that wants more than its table holds gets none either.  Entries behind a row's pages are left as they are.
 
+    Nothing that runs at the same time may read or write the table; rows of it must not overlap.
+
     Returns (seqlens (B) int32, left (1) int32): `want` of the rows that have their pages, `have` of the others; the pages that are free now."""
     if not _ready:
         _register_ops()

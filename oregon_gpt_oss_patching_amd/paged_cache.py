@@ -155,7 +155,9 @@ def paged_cache_write(cache: PagedCache, k, v, page_table, start, seqlens=None) 
 
 def paged_cache_write_tokens(cache: PagedCache, k, v, slots) -> None:
     """`paged_cache_write` of tokens that lie back to back, whatever rows they are of: k, v (T, G, 64), any strides; token t goes to slot
-    slots[t], that is to token slots[t] % page_size of page slots[t] // page_size (`token_map` says which).  Slots below 0 or behind the pool are dropped."""
+    slots[t], that is to token slots[t] % page_size of page slots[t] // page_size (`token_map` says which).  Slots below 0 or behind the pool are dropped.
+
+    Two tokens of one call must not have the same slot, and nothing that runs at the same time may read what is being written."""
     if not _ready:
         _register_ops()
     if _compiling() or _write_slots_now(*cache, k, v, slots) is NotImplemented:

@@ -374,3 +374,30 @@ def test_two_updates_at_once(A):
     torch.cuda.synchronize()
     for t, (got, left) in zip(tables, out):
         assert t.tolist() == ref[0] and got.tolist() == ref[1] and left.tolist() == [ref[2]]
+
+
+@pytest.mark.parametrize("rows", [5, 700, 5000])
+@pytest.mark.parametrize("onto", ["have", "want"])
+def test_lengths_replaced_where_they_are(A, rows, onto):
+    """Through the C interface: seqlens is have or want itself."""
+    import ctypes
+
+    from oregon_gpt_oss_patching_amd import _lib
+    print(f"case rows={rows} onto={onto}", flush=True)
+    rng, ps, width = random.Random(rows), 16, 12
+    have = [rng.randint(0, 100) for _ in range(rows)]
+    want = [rng.choice((0, n, n + 1, n + 40, 200)) for n in have]
+    pages = sum(T.pages_for(n, ps) for n in have) + rows // 3
+    table = tables_of(rng, have, ps, pages, width)
+    t, h, w, left = ints(table), ints(have), ints(want), ints([0])
+    p = _lib.TableParams()
+    p.struct_size = ctypes.sizeof(p)
+    p.B, p.table_width, p.page_size, p.pages, p.table_stride = rows, width, ps, pages, width
+    p.page_table, p.have, p.want, p.left = t.data_ptr(), h.data_ptr(), w.data_ptr(), left.data_ptr()
+    p.seqlens = {"have": h, "want": w}[onto].data_ptr()
+    need = _lib.load().gptoss_attn_table_workspace_bytes(ctypes.byref(p))
+    scratch = torch.empty(max(need, 4) // 4, dtype=torch.int32, device=DEV)
+    p.scratch, p.scratch_bytes = scratch.data_ptr(), need
+    assert _lib.load().gptoss_attn_page_table_update(ctypes.byref(p), torch.cuda.current_stream().cuda_stream) == 0
+    ref, seqlens, free = T.update(table, have, want, pages, ps)
+    assert t.tolist() == ref and {"have": h, "want": w}[onto].tolist() == seqlens and left.tolist() == [free]

@@ -230,6 +230,33 @@ def test_attention_divisions(A, dtype, lens, h, g, sq, width, w):  # noqa: F811
 
 
 @BOTH
+@pytest.mark.parametrize("ps", [16, 64])
+@pytest.mark.parametrize("lens,h,g,sq,keys,w", [
+    # pairs (a query and a head of a KV head's group) of a row: 20, 40, 64, 65, 96; few keys in all, then so many that each unit has all pairs that fit
+    ([500, 90], 8, 2, 5, 512, 0), ([500, 90], 8, 2, 5, 1 << 18, 0),
+    ([500, 90], 8, 1, 5, 512, 0), ([500, 90], 8, 1, 5, 1 << 18, 0),
+    ([700, 8, 0], 8, 1, 8, 704, 0), ([700, 8, 0], 8, 1, 8, 1 << 18, 0),
+    ([700, 66], 5, 1, 13, 704, 0), ([700, 66], 5, 1, 13, 1 << 18, 0),
+    ([130, 300], 24, 2, 8, 320, 0), ([130, 300], 24, 2, 8, 1 << 18, 0),
+    # no unit is cut
+    ([830, 3, 64] + [5] * 50, 24, 8, 7, 832, 0),
+    ([830, 3, 64] + [5] * 50, 40, 8, 8, 832, 0),
+    ([830, 3, 64] + [5] * 50, 56, 8, 8, 832, 0),
+    ([830, 3, 64] + [5] * 50, 64, 8, 8, 832, 0),
+    # windows
+    ([1000, 140, 128, 129], 64, 8, 8, 1024, 128),
+    ([600, 140, 128, 129] + [9] * 260, 32, 8, 8, 640, 128),
+    ([600, 140, 128, 129] + [9] * 260, 64, 8, 8, 640, 128),
+])
+def test_attention_units_of_few_and_many_pairs(A, dtype, lens, h, g, sq, keys, w, ps):  # noqa: F811
+    print(f"case {dtype} rows={len(lens)} H={h} G={g} Sq={sq} keys={keys} window={w} page={ps}", flush=True)
+    cache, table, n, q, sinks, _, _ = make(A, 29 + sum(lens) + sq, lens, h, g, sq, ps, dtype, E2M1)
+    wide = torch.full((len(lens), keys // ps), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    check(A, cache, wide, n, q, sinks, w)
+
+
+@BOTH
 def test_missing_pages_and_lengths_beyond_the_table(A, dtype):  # noqa: F811
     lens = [200, 150, 96, 300]
     cache, table, n, q, sinks, _, _ = make(A, 9, lens, 8, 2, 2, 16, dtype, E2M1)
