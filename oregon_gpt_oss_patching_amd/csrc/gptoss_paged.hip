@@ -344,14 +344,16 @@ int gptoss_attn_page_table_update(const gptoss_attn_table_params *p, void *strea
         a.marks = static_cast<uint32_t *>(p->scratch);
         if ((rc = launch(page_table_mark_kernel, kMarkers, kTableThreads, stream, a))) return rc;
     }
-    return launch(page_table_update_kernel, 1, kTableThreads, stream, a);
+    // (lengths that are replaced are read by one workgroup, which is done with a row's before it writes them)
+    return launch(page_table_update_kernel, a.seqlens == a.have || a.seqlens == a.want ? 1 : kGivers, kTableThreads, stream, a);
 }
 
 int gptoss_attn_token_map(const gptoss_attn_table_params *p, void *stream) {
     const int rc = gptoss_attn_table_validate(p, 1);
     if (rc) return rc;
-    const int blocks = (p->total + kMapTokens - 1) / kMapTokens;
-    return launch(token_map_kernel, blocks ? blocks : 1, kMapThreads, stream, table_args(p));
+    const int blocks = p->total ? (p->total + kMapThreads - 1) / kMapThreads : 1;
+    return p->B <= kMapFewRows ? launch(token_map_kernel<kMapFewRows>, blocks, kMapThreads, stream, table_args(p))
+                               : launch(token_map_kernel<kTableRows>, blocks, kMapThreads, stream, table_args(p));
 }
 
 }  // extern "C"

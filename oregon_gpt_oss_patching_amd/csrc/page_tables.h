@@ -1,9 +1,10 @@
 // Whose page is whose (gptoss_attn_page_table_update) and where the tokens of a call go (gptoss_attn_token_map): whole numbers only.
 //
 // No list of free pages is kept from call to call: a page is free iff no row's kept entry names it, so each update reads all of them.  What bounds it is not their bytes but latencies, and the
-// LDS atomics that set a bit for each (some 1.3 a cycle): one workgroup has its counts and the pool's bits in LDS; where a table may be large, sixteen others set the bits first, each of its
-// share of the entries, in a launch of its own.  256 rows of 40 to 9000 tokens: 9.8 us, 3 of them the first launch;
-// 4096 of 500 18.6; 8 of 1000, in one launch, 4.7.
+// LDS atomics that set a bit for each (some 1.3 a cycle).  A workgroup has all counts and the pool's bits in LDS; where a table may be large, others set the bits first, each of its
+// share of the entries, in a launch of its own.  What is given out goes to sixteen workgroups, 1024 pages at a time, each of which makes the same counts: they read kept entries, lengths and bits,
+// and write others.  us: 256 rows of 40 to 9000 tokens 10.6, 3 of them the first launch; 96 of up to 16384 of which 32 begin (8284 pages) 11.3, by one workgroup 28.6; 4096 of 500
+// 18.4; 8 of 1000, in one launch, 4.9.
 #pragma once
 #include "paged_common.h"
 
@@ -12,7 +13,7 @@ namespace gptoss {
 constexpr int kTableRows = 16384;                  // rows of a call: a number of 32 bits each in LDS
 constexpr int kTableThreads = 1024;
 constexpr int kMarkers = 16;                       // workgroups that set bits in a launch of their own
-constexpr int kFresh = 4096;                       // pages that are handed out together: 16 KB
+constexpr int kGivers = 16;                        // workgroups that give pages out (4, 8, 32 for the 8284 above: 15.3, 13.3, 11.3 us)
 constexpr int kPoolBits = 1 << 19;                 // pages that are looked at together: 64 KB of LDS
 constexpr int kPoolGroup = 64 * 32;                // pages of a wavefront's word each
 constexpr uint32_t kMany = (1u << 30) + 1;         // sums stay here: more than there are pages or tokens
@@ -38,17 +39,6 @@ __device__ __forceinline__ uint32_t wave_scan_up(uint32_t x) {
     x = add_up(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false));
     x = add_up(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));      // row_bcast:15 into rows 1 and 3
     x = add_up(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));      // row_bcast:31 into rows 2 and 3
-    return x;
-}
-
-// the largest of the lanes up to this one, of numbers from 0 on
-__device__ __forceinline__ int wave_scan_max(int x) {
-    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));        // as in wave_scan_up
-    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
-    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
-    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
-    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
-    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
     return x;
 }
 
@@ -154,8 +144,7 @@ __global__ __launch_bounds__(kTableThreads) void page_table_mark_kernel(const Ta
 }
 
 __global__ __launch_bounds__(kTableThreads) void page_table_update_kernel(const TableArgs a) {
-    __shared__ uint32_t ends[kTableRows], bits[kPoolBits / 32], base[kPoolBits / kPoolGroup + 1], fresh[kFresh], part[kTableThreads / 64];
-    __shared__ uint16_t row_at[kFresh];            // row + 1, 0: none begins here
+    __shared__ uint32_t ends[kTableRows], bits[kPoolBits / 32], base[kPoolBits / kPoolGroup + 1], fresh[kTableThreads], part[kTableThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     block_sums<kTableThreads>(ends, part, a.B, [&](int b) __attribute__((always_inline)) {
         const RowPages r = row_pages(a, b);
@@ -223,19 +212,9 @@ __global__ __launch_bounds__(kTableThreads) void page_table_update_kernel(const 
         }
         const int span = span_of(lo), groups = (span + kPoolGroup - 1) / kPoolGroup;
         const uint32_t end = min(before + here, given);
-        // kFresh pages at a time into LDS by their rank, and the rows at the first of their ranks; a rank's row is then the last one at or before it.
-        for (uint32_t c0 = before; c0 < end; c0 += kFresh) {
-            constexpr int kEach = kFresh / kTableThreads;
-            const uint32_t c1 = min(c0 + kFresh, end);
-            const bool few = c1 - c0 <= kTableThreads;           // (a search for each is quicker then: 256 rows 1.8 us, and 2.4)
-            if (!few) {
-                for (int i = tid; i < kFresh; i += kTableThreads) row_at[i] = 0;
-                __syncthreads();
-                for (int b = tid; b < a.B; b += kTableThreads) {
-                    const uint32_t r0 = max(b ? ends[b - 1] : 0u, c0);
-                    if (r0 < min(ends[b], c1)) row_at[r0 - c0] = (uint16_t)(b + 1);
-                }
-            }
+        // A page for each thread at a time, into LDS by its rank; who gets a rank is found in the sums.
+        for (uint32_t c0 = before + blockIdx.x * kTableThreads; c0 < end; c0 += gridDim.x * kTableThreads) {
+            const uint32_t c1 = min(c0 + kTableThreads, end);
             for (int g = w; g < groups; g += kTableThreads / 64) {
                 if (before + base[g + 1] <= c0 || before + base[g] >= c1) continue;
                 const int first = g * kPoolGroup + 32 * lane, there = min(max(span - first, 0), 32);
@@ -246,40 +225,16 @@ __global__ __launch_bounds__(kTableThreads) void page_table_update_kernel(const 
                     if (rank >= c0 && rank < c1) fresh[rank - c0] = (uint32_t)(lo + first + __ffs(set) - 1);
             }
             __syncthreads();
-            if (few) {
-                if (c0 + tid < c1) {
-                    const int b = first_above(ends, a.B, c0 + tid);
-                    a.table[b * a.stride + row_pages(a, b).has + (c0 + tid - (b ? ends[b - 1] : 0u))] = (int32_t)fresh[tid];
-                }
-                __syncthreads();
-                continue;
-            }
-            // the thread's kEach ranks
-            int row[kEach], has[kEach];
-#pragma unroll
-            for (int k = 0; k < kEach; ++k) row[k] = max((int)row_at[kEach * tid + k], k ? row[k - 1] : 0);
-            const int incl = wave_scan_max(row[kEach - 1]);
-            if (lane == 63) part[w] = (uint32_t)incl;
-            __syncthreads();
-            int front = __shfl_up(incl, 1);
-            front = lane ? front : 0;
-            for (int k = 0; k < w; ++k) front = max(front, (int)part[k]);
-#pragma unroll
-            for (int k = 0; k < kEach; ++k) {
-                row[k] = max(row[k], front) - 1;
-                has[k] = c0 + kEach * tid + k < c1 ? row_pages(a, row[k]).has : 0;
-            }
-#pragma unroll
-            for (int k = 0; k < kEach; ++k) {
-                const uint32_t i = kEach * tid + k;
-                if (c0 + i < c1) a.table[row[k] * a.stride + has[k] + (c0 + i - (row[k] ? ends[row[k] - 1] : 0u))] = (int32_t)fresh[i];
+            if (c0 + tid < c1) {
+                const int b = first_above(ends, a.B, c0 + tid);
+                a.table[b * a.stride + row_pages(a, b).has + (c0 + tid - (b ? ends[b - 1] : 0u))] = (int32_t)fresh[tid];
             }
             __syncthreads();
         }
         before += here;
     }
-    if (tid == 0) *a.left = (int32_t)(free - given);
-    for (int b0 = w * 64; b0 < a.B; b0 += kTableThreads) {
+    if (tid == 0 && blockIdx.x == 0) *a.left = (int32_t)(free - given);
+    for (int b0 = (blockIdx.x * (kTableThreads / 64) + w) * 64; b0 < a.B; b0 += gridDim.x * kTableThreads) {
         const int b = b0 + lane;
         RowPages r{0, 0, true};
         if (b < a.B) {
@@ -296,35 +251,34 @@ __global__ __launch_bounds__(kTableThreads) void page_table_update_kernel(const 
     }
 }
 
-// Tokens t = kMapTokens blockIdx.x + ... of a call that has counts[b] of each row, back to back.
-constexpr int kMapThreads = 256, kMapTokens = 1024;
+// Tokens of a call that has counts[b] of each row, back to back: one to a thread (two, four: what a token waits for adds up, 96 rows of 132000 tokens 3.9 us, so 4.4, 5.7; 1024 rows of one
+// 4.0, 4.8, 7.1; only a million tokens of 1000 rows 11.8, 10.4, 10.4).  ROWS: sums that LDS has room for, with few of them more workgroups run at a time: 270000 tokens 4.6 and not 6.7 us.
+constexpr int kMapThreads = 256, kMapFewRows = 2048;
+template <int ROWS>
 __global__ __launch_bounds__(kMapThreads) void token_map_kernel(const TableArgs a) {
-    __shared__ uint32_t ends[kTableRows], part[kMapThreads / 64];
+    __shared__ uint32_t ends[ROWS], part[kMapThreads / 64];
     block_sums<kMapThreads>(ends, part, a.B, [&](int b) __attribute__((always_inline)) { return (uint32_t)max(a.want[b], 0); });
     const uint32_t all = ends[a.B - 1], used = min(all, (uint32_t)a.total);
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.used = (int32_t)used;
-#pragma unroll
-    for (int k = 0; k < kMapTokens / kMapThreads; ++k) {
-        const int t = blockIdx.x * kMapTokens + k * kMapThreads + threadIdx.x;
-        if (t >= a.total) return;
-        int row = -1, position = 0, first = (int)used;
-        int64_t slot = -1;
-        if ((uint32_t)t < used) {
-            row = first_above(ends, a.B, (uint32_t)t);
-            first = row ? (int)ends[row - 1] : 0;
-            const int64_t at = (int64_t)a.have[row] + (t - first);
-            position = (int)min(at, (int64_t)0x7fffffff);
-            const int64_t entry = at >> a.page_shift;
-            if (at >= 0 && entry < a.width) {
-                const int page = a.table[row * a.stride + entry];
-                if (page >= 0) slot = ((int64_t)page << a.page_shift) + (at & ((1 << a.page_shift) - 1));
-            }
+    const int t = blockIdx.x * kMapThreads + threadIdx.x;
+    if (t >= a.total) return;
+    int row = -1, position = 0, first = (int)used;
+    int64_t slot = -1;
+    if ((uint32_t)t < used) {
+        row = first_above(ends, a.B, (uint32_t)t);
+        first = row ? (int)ends[row - 1] : 0;
+        const int64_t at = (int64_t)a.have[row] + (t - first);
+        position = (int)min(at, (int64_t)0x7fffffff);
+        const int64_t entry = at >> a.page_shift;
+        if (at >= 0 && entry < a.width) {
+            const int page = a.table[row * a.stride + entry];
+            if (page >= 0) slot = ((int64_t)page << a.page_shift) + (at & ((1 << a.page_shift) - 1));
         }
-        a.row[t] = row;
-        a.position[t] = position;
-        a.first[t] = first;
-        a.slot[t] = slot;
     }
+    a.row[t] = row;
+    a.position[t] = position;
+    a.first[t] = first;
+    a.slot[t] = slot;
 }
 
 }  // namespace gptoss

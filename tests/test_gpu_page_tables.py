@@ -401,3 +401,25 @@ def test_lengths_replaced_where_they_are(A, rows, onto):
     assert _lib.load().gptoss_attn_page_table_update(ctypes.byref(p), torch.cuda.current_stream().cuda_stream) == 0
     ref, seqlens, free = T.update(table, have, want, pages, ps)
     assert t.tolist() == ref and {"have": h, "want": w}[onto].tolist() == seqlens and left.tolist() == [free]
+
+
+@pytest.mark.parametrize("rows,longest,spare", [(70, 16384, 500), (40, 30000, -900), (300, 4000, 20), (1, 600000, 5)])
+@pytest.mark.parametrize("pool", [0, 700001])
+def test_many_new_pages(A, rows, longest, spare, pool):
+    """More pages given out than one workgroup has threads, in pools that are looked at in one part and in two."""
+    print(f"case rows={rows} longest={longest} spare={spare} pool={pool}", flush=True)
+    rng, ps = random.Random(rows + longest), 16
+    have = [rng.choice((0, 0, rng.randint(1, longest // 2))) for _ in range(rows)]
+    want = [rng.choice((0, longest, rng.randint(longest // 2, longest))) if rows > 1 else longest for _ in range(rows)]
+    kept, grown = sum(T.pages_for(min(a, b), ps) for a, b in zip(have, want)), sum(T.pages_for(b, ps) for b in want)
+    pages = max(grown + spare, sum(T.pages_for(a, ps) for a in have), kept + 1)
+    if pool:                                          # all but as many are one row's, which stays
+        held = pool - pages
+        t = [x + [-1] * (held + 1) for x in tables_of(rng, have, ps, pages, longest // ps + 1)]
+        move = rng.randint(0, pages)                  # (the others lie on both sides of it)
+        t = [[y if y < move else y + held for y in x] for x in t]
+        t.append(list(range(move, move + held)) + [-1] * (len(t[0]) - held))
+        have, want, pages = [*have, held * ps], [*want, held * ps], pool
+    else:
+        t = tables_of(rng, have, ps, pages, longest // ps + 1)
+    check_update(A, t, have, want, pages, ps)
