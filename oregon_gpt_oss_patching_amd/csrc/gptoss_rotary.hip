@@ -101,7 +101,7 @@ int gptoss_attn_rotary(const gptoss_attn_rotary_params *p, void *stream) {
     const void *kernel = f32 ? (v == 4 ? kernel_of<float, 4>(paired, tables) : v == 2 ? kernel_of<float, 2>(paired, tables) : kernel_of<float, 1>(paired, tables))
                              : (v == 8 ? kernel_of<bf16, 8>(paired, tables) : v == 2 ? kernel_of<bf16, 2>(paired, tables) : kernel_of<bf16, 1>(paired, tables));
     void *args[] = {&a};
-    const hipError_t e = hipLaunchKernel(kernel, dim3((unsigned)((a.items + 255) / 256)), dim3(256), args, 0, static_cast<hipStream_t>(stream));
+    const hipError_t e = hipLaunchKernel(kernel, dim3((unsigned)((a.items + kRotaryThreads - 1) / kRotaryThreads)), dim3(kRotaryThreads), args, 0, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? GPTOSS_ATTN_OK : static_cast<int>(e);
 }
 
