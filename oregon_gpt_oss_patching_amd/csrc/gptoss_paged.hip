@@ -300,7 +300,7 @@ int gptoss_attn_paged_write_slots(const gptoss_attn_paged_params *p, const int64
     a.by_g = div_by(a.G);
     const void *kernel = of_types(p, [](auto t, auto st) { return reinterpret_cast<const void *>(paged_write_slots_kernel<decltype(t), decltype(st)>); });
     void *args[] = {&a, const_cast<int64_t **>(&slots)};
-    const hipError_t e = hipLaunchKernel(kernel, dim3((unsigned)((rows + 31) / 32)), dim3(256), args, 0, static_cast<hipStream_t>(stream));
+    const hipError_t e = hipLaunchKernel(kernel, dim3((unsigned)((rows + 255) / 256 * 8)), dim3(256), args, 0, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? GPTOSS_ATTN_OK : static_cast<int>(e);
 }
 

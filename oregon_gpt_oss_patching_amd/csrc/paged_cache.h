@@ -120,10 +120,11 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const PagedArgs a) {
     write_piece<T, ST>(a.vp, a.ve, page, at, g, c8, v);
 }
 
-// The same of one batch row whose tokens have slots of their own.
+// The same of one batch row whose tokens have slots of their own.  Workgroups go to the eight XCDs in turn: each XCD has a run of rows, so that its L2 has whole lines of a page's short rows and exponents to write back (in the
+// order of the workgroups 7666 tokens in e2m1 7.0 us and not 6.6, 30000 20.6 / 20.3, up to 2000 the same).  The grid is a multiple of eight.
 template <typename T, typename ST>
 __global__ __launch_bounds__(256) void paged_write_slots_kernel(const PagedArgs a, const int64_t *slots) {
-    const int row = blockIdx.x * 32 + (threadIdx.x >> 3), c8 = (threadIdx.x & 7) * 8;
+    const int row = ((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) * 32 + (threadIdx.x >> 3), c8 = (threadIdx.x & 7) * 8;
     const int i = a.by_g.quotient(row), g = row - i * a.G;
     if (i >= a.Sq) return;                                           // (all eight lanes of the row)
     const Piece<T> k = load_piece(reinterpret_cast<const T *>(a.k) + g * a.ks.h + i * a.ks.s + c8);
