@@ -423,3 +423,16 @@ def test_many_new_pages(A, rows, longest, spare, pool):
     else:
         t = tables_of(rng, have, ps, pages, longest // ps + 1)
     check_update(A, t, have, want, pages, ps)
+
+
+@pytest.mark.parametrize("rows", [255, 256, 257, 2048, 2049])
+def test_token_map_of_many_rows(A, rows):
+    """On both sides of the rows that one round of sums and the smaller kernel take, with tokens that fill workgroups and do not."""
+    print(f"case rows={rows}", flush=True)
+    rng, ps = random.Random(rows), 16
+    start = [rng.randint(0, 90) for _ in range(rows)]
+    counts = [rng.choice((0, 1, 1, 1, 40)) for _ in range(rows)]
+    have = [a + b for a, b in zip(start, counts)]
+    table = tables_of(rng, have, ps, sum(T.pages_for(n, ps) for n in have) + 3, 10)
+    for total in (sum(counts), sum(counts) - 1, sum(counts) // 256 * 256, sum(counts) + 300):
+        check_map(A, table, start, counts, total, ps)
