@@ -68,6 +68,8 @@ class PagedState(NamedTuple):
         if self.tokens is not None:
             if self.start is not None or q.shape[0] != 1:
                 raise RuntimeError(f"tokens= is one batch row of rows that begin with this call: start must be None, got {'one' if self.start is not None else 'none'} and {q.shape[0]} batch rows")
+            if self.counts is not None:
+                raise RuntimeError("counts= says how many of a batch row's tokens are its own; with tokens= the map says it")
             paged_cache_write_tokens(cache, k[0].transpose(0, 1), v[0].transpose(0, 1), self.tokens.slot)
             return _ak.attention(q, k, v, module.sinks, sm_scale, window, None, self.tokens.used, self.tokens.first[None])
         if self.start is None:

@@ -436,3 +436,35 @@ def test_token_map_of_many_rows(A, rows):
     table = tables_of(rng, have, ps, sum(T.pages_for(n, ps) for n in have) + 3, 10)
     for total in (sum(counts), sum(counts) - 1, sum(counts) // 256 * 256, sum(counts) + 300):
         check_map(A, table, start, counts, total, ps)
+
+
+def test_two_launches_captured(A):
+    """A table large enough for a launch of its own for the bits, captured twice, replayed in turn with eager updates of another table between."""
+    ps, rows, width = 16, 300, 64
+    rng = random.Random(77)
+    lens = [rng.randint(0, 600) for _ in range(rows)]
+    pages = sum(T.pages_for(n, ps) for n in lens) + 200
+    ref = tables_of(rng, lens, ps, pages, width)
+    table, have, want = ints(ref), ints(lens), ints(lens)
+    other = tables_of(rng, lens, ps, pages, width)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(stream):
+        A.page_table_update(table, have, want, pages, ps)
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                out = A.page_table_update(table, have, want, pages, ps)
+            graphs.append((g, out))
+    torch.cuda.current_stream().wait_stream(stream)
+    for i in range(6):
+        new = [rng.choice((0, n, n + 1, min(n + rng.randint(0, 60), ps * width))) for n in lens]
+        have.copy_(ints(lens))
+        want.copy_(ints(new))
+        g, (got, left) = graphs[i % 2]
+        g.replay()
+        torch.cuda.synchronize()
+        ref, lens, free = T.update(ref, lens, new, pages, ps)
+        assert table.tolist() == ref and got.tolist() == lens and left.tolist() == [free], i
+        check_update(A, other, [0] * rows, [rng.randint(0, 90) for _ in lens], pages, ps)

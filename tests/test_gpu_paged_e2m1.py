@@ -596,3 +596,21 @@ def test_layers_with_a_paged_state(A):  # noqa: F811
             ref, ref_lse, terms = P.attention(q.cpu(), *values(cache), table.cpu(), n.cpu(), sinks.cpu(), SCALE, module.sliding_window or 0)
             assert bool(((o.cpu().double() - ref).abs() <= bounds(ref, ref_lse, terms, BF16)[0]).all()), (step, module.layer_idx)
         have, lens = n, n + 1
+
+
+def test_float16_goes_through_bfloat16(A):  # noqa: F811
+    """Tokens and queries in float16 are those in bfloat16, rounded; results come back in float16."""
+    lens, g, ps = [70, 33], 2, 16
+    cache, table, n, q, sinks, _, _ = make(A, 41, lens, 8, g, 1, ps, BF16, E2M1)
+    gen = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(40, g, 64, generator=gen).to(torch.float16).to(DEV) for _ in range(2))
+    a, b = A.paged_cache(4, g, ps, E2M1), A.paged_cache(4, g, ps, E2M1)
+    slots = torch.randperm(64, generator=gen)[:40].to(DEV)
+    A.paged_cache_write_tokens(a, k, v, slots)
+    A.paged_cache_write_tokens(b, k.to(BF16), v.to(BF16), slots)
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+    half, sinks = q.to(DEV, torch.float16), sinks.to(DEV)
+    o = A.paged_attention(half, cache, table, n, sinks, 0.125)
+    assert o.dtype == torch.float16 and torch.equal(o, A.paged_attention(half.to(BF16), cache, table, n, sinks, 0.125).to(torch.float16))
+    got = A.paged_cache_read(cache, table, n, 70, dtype=torch.float16)
+    assert all(x.dtype == torch.float16 and torch.equal(x, y.to(torch.float16)) for x, y in zip(got, A.paged_cache_read(cache, table, n, 70)))

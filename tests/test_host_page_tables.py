@@ -117,3 +117,15 @@ def test_traced_shapes():
         assert [tuple(x.shape) for x in m] == [(7,), (7,), (7,), (7,), (1,)] and m.slot.dtype == torch.int64
         cache, k = A.paged_cache(4, 2, 16), torch.zeros(7, 2, 64, dtype=torch.bfloat16, device="cuda")
         assert A.paged_cache_write_tokens(cache, k, k, m.slot) is None
+
+
+def test_states_of_packed_rows_are_refused_what_the_map_says_already():
+    from types import SimpleNamespace
+    module, n = SimpleNamespace(layer_idx=0, sliding_window=None, sinks=None), torch.zeros(2, dtype=torch.int32)
+    cache, table = A.paged_cache(4, 2, 16, device="cpu"), torch.zeros(2, 3, dtype=torch.int32)
+    tokens = A.TokenMap(*(torch.zeros(5, dtype=torch.int32) for _ in range(5)))
+    q, k = torch.zeros(1, 4, 5, 64, dtype=torch.bfloat16), torch.zeros(1, 2, 5, 64, dtype=torch.bfloat16)
+    for state, rows, match in ((A.PagedState([cache], table, n, n, tokens=tokens), 1, "start must be None"), (A.PagedState([cache], table, None, n, tokens=tokens), 2, "one batch row"),
+                               (A.PagedState([cache], table, None, n, counts=n, tokens=tokens), 1, "counts=")):
+        with pytest.raises(RuntimeError, match=match):
+            state.attend(module, q.expand(rows, -1, -1, -1), k.expand(rows, -1, -1, -1), k.expand(rows, -1, -1, -1), 0.125)
