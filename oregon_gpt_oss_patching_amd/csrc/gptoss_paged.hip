@@ -93,6 +93,9 @@ auto of_types(const gptoss_attn_paged_params *p, F call) {
     return p->storage == GPTOSS_ATTN_E2M1 ? call(float{}, e2m1{}) : p->storage == GPTOSS_ATTN_E4M3 ? call(float{}, e4m3{}) : call(float{}, float{});
 }
 
+// Workgroups for so many of write_group's.
+template <typename ST> int64_t write_grid(int64_t groups) { return is_e2m1<ST> ? (groups + 7) / 8 * 8 : groups; }
+
 // How the attention's work is divided: column blocks of 16 pairs, blocks of pairs of a row, (row, block) units, shares of all units'
 // tiles for each KV head that there are at most beside one for each unit (0: units stay whole, each walked by `alone` wavefronts), how many are to be expected, and
 // the scratch that takes; `across`: a slot's KV heads on one XCD.  How long shares are is the kernel's to find, from the lengths (PagedShare).
@@ -274,7 +277,7 @@ int gptoss_attn_paged_write(const gptoss_attn_paged_params *p, void *stream) {
     a.blocks = (int)blocks;
     a.by_blocks = div_by(blocks);
     a.by_g = div_by(a.G);
-    return of_types(p, [&](auto t, auto st) { return launch(paged_write_kernel<decltype(t), decltype(st)>, grid, 256, stream, a); });
+    return of_types(p, [&](auto t, auto st) { return launch(paged_write_kernel<decltype(t), decltype(st)>, write_grid<decltype(st)>(grid), 256, stream, a); });
 }
 
 int gptoss_attn_paged_read(const gptoss_attn_paged_params *p, void *stream) {
@@ -298,10 +301,12 @@ int gptoss_attn_paged_write_slots(const gptoss_attn_paged_params *p, const int64
     const int64_t rows = (int64_t)a.Sq * a.G;
     if (rows > (1 << 30)) return GPTOSS_ATTN_ERR_SHAPE;
     a.by_g = div_by(a.G);
-    const void *kernel = of_types(p, [](auto t, auto st) { return reinterpret_cast<const void *>(paged_write_slots_kernel<decltype(t), decltype(st)>); });
-    void *args[] = {&a, const_cast<int64_t **>(&slots)};
-    const hipError_t e = hipLaunchKernel(kernel, dim3((unsigned)((rows + 255) / 256 * 8)), dim3(256), args, 0, static_cast<hipStream_t>(stream));
-    return e == hipSuccess ? GPTOSS_ATTN_OK : static_cast<int>(e);
+    return of_types(p, [&](auto t, auto st) {
+        void *args[] = {&a, const_cast<int64_t **>(&slots)};
+        const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(paged_write_slots_kernel<decltype(t), decltype(st)>), dim3((unsigned)write_grid<decltype(st)>((rows + 31) / 32)),
+                                             dim3(256), args, 0, static_cast<hipStream_t>(stream));
+        return e == hipSuccess ? static_cast<int>(GPTOSS_ATTN_OK) : static_cast<int>(e);
+    });
 }
 
 int gptoss_attn_table_validate(const gptoss_attn_table_params *p, int call) {

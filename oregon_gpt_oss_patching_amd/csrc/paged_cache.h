@@ -102,11 +102,19 @@ __device__ __forceinline__ void write_piece(const PagedPool &rows, const PagedPo
     }
 }
 
+// Which 32 rows a workgroup writes.  Workgroups go to the eight XCDs in turn; of 4-bit rows each XCD has a run, so that its L2 has whole lines of them and of their exponents to write back (the grid is a multiple of
+// eight).  us, in the order of the workgroups / so: 8 x 4096 tokens of 8 KV heads 24.1 / 22.4, 4 x 3001 9.8 / 9.5, by slots 7666 tokens 7.0 / 6.6, 30000 20.6 / 20.3; but in e4m3 8 x 4096 27.3 / 27.8, in bfloat16 27.9 / 28.8.
+template <typename ST>
+__device__ __forceinline__ int write_group() {
+    return is_e2m1<ST> ? (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+}
+
 // Rows (token, KV head) of a batch row, the KV head fastest: the model's keys and values have a token's heads side by side.  The rows are under
 // way while their page is looked up.  One row to a lane: with two, 8 x 4096 tokens of 8 KV heads took 27.9 us and not 26.2 (134 MB moved).
 template <typename T, typename ST>
 __global__ __launch_bounds__(256) void paged_write_kernel(const PagedArgs a) {
-    const int b = a.by_blocks.quotient(blockIdx.x), row = (blockIdx.x - b * a.blocks) * 32 + (threadIdx.x >> 3), c8 = (threadIdx.x & 7) * 8;
+    const int wg = write_group<ST>(), b = a.by_blocks.quotient(wg), row = (wg - b * a.blocks) * 32 + (threadIdx.x >> 3), c8 = (threadIdx.x & 7) * 8;
+    if (is_e2m1<ST> && b >= a.B) return;
     const int n = a.seqlens ? min(a.seqlens[b], a.Sq) : a.Sq;
     const int i = a.by_g.quotient(row), g = row - i * a.G;
     if (i >= n) return;                                              // (all eight lanes of the row)
@@ -120,11 +128,10 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const PagedArgs a) {
     write_piece<T, ST>(a.vp, a.ve, page, at, g, c8, v);
 }
 
-// The same of one batch row whose tokens have slots of their own.  Workgroups go to the eight XCDs in turn: each XCD has a run of rows, so that its L2 has whole lines of a page's short rows and exponents to write back (in the
-// order of the workgroups 7666 tokens in e2m1 7.0 us and not 6.6, 30000 20.6 / 20.3, up to 2000 the same).  The grid is a multiple of eight.
+// The same of one batch row whose tokens have slots of their own.
 template <typename T, typename ST>
 __global__ __launch_bounds__(256) void paged_write_slots_kernel(const PagedArgs a, const int64_t *slots) {
-    const int row = ((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) * 32 + (threadIdx.x >> 3), c8 = (threadIdx.x & 7) * 8;
+    const int row = write_group<ST>() * 32 + (threadIdx.x >> 3), c8 = (threadIdx.x & 7) * 8;
     const int i = a.by_g.quotient(row), g = row - i * a.G;
     if (i >= a.Sq) return;                                           // (all eight lanes of the row)
     const Piece<T> k = load_piece(reinterpret_cast<const T *>(a.k) + g * a.ks.h + i * a.ks.s + c8);
