@@ -845,16 +845,22 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
     };
     constexpr bool kTwoPages = std::is_same_v<ST, e2m1_of_16>;
     int lane_page[(KB + 1) / 2];             // two pages to a load: the lane's
-    int pages = 0;                           // of the tile under way: negative where a block has no page
-    unsigned there = 0;                      // which of them have one
-    auto fetch_k = [&](int j, uint32_t mask) __attribute__((always_inline)) {
-        pages = 0;
-        there = 0;
+    struct Blocks { int pages; unsigned there; };            // of a tile: negative where a block of 16 keys has no page; which of them have one
+    auto blocks_of = [&](int j) __attribute__((always_inline)) {
+        Blocks x{0, 0};
 #pragma unroll
         for (int blk = 0; blk < KB; ++blk) {
-            pages |= page_of(j, blk);
-            there |= page_of(j, blk) >= 0 ? 1u << blk : 0u;
+            x.pages |= page_of(j, blk);
+            x.there |= page_of(j, blk) >= 0 ? 1u << blk : 0u;
         }
+        return x;
+    };
+    // Where they are looked up: with the addresses of K, a tile ahead, or where the tile begins.  us, so / so: e2m1, five queries on 24 rows of 500 to 9000 tokens 32.2 / 32.4, four on
+    // 16 x 8192 31.5 / 32.5; but 16 windows of 128 keys in bfloat16 5.7 / 5.4, in e4m3 6.1 / 5.9, 32 x 1000 tokens in e4m3 10.7 / 10.4 (scalar registers: two numbers more live over the loop).
+    constexpr bool kBlocksAhead = is_e2m1<ST>;
+    Blocks ahead{0, 0};
+    auto fetch_k = [&](int j, uint32_t mask) __attribute__((always_inline)) {
+        if constexpr (kBlocksAhead) ahead = blocks_of(j);
         if constexpr (kTwoPages) {
 #pragma unroll
             for (int i = 0; i < KB / 2; ++i) {
@@ -884,8 +890,10 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
     bool odd = false;
     for (int j = 0; j < n_it; ++j) {
         const int n0 = (t_lo + w + NW * j) * kKeys;
-        const unsigned there_now = there;
-        const bool edge = n0 + kKeys - 1 > sp.pos0 || n0 <= sp.pos1 - weff || pages < 0;
+        Blocks now;
+        if constexpr (kBlocksAhead) now = ahead;
+        else now = blocks_of(j);
+        const bool edge = n0 + kKeys - 1 > sp.pos0 || n0 <= sp.pos1 - weff || now.pages < 0;
         // The next tile; behind the last one the same loads from one line of it, so that the waits for what is under way can be counted: with a branch
         // around them every tile began with a wait for all of it.
         const int next = min(j + 1, n_it - 1);
@@ -902,7 +910,7 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
             tile.logits(s);
             fetch_k(next, mask);
         }
-        odd = tile.stage_v(edge, several, sp.lo - n0, sp.hi - n0, there_now, lane) || odd;
+        odd = tile.stage_v(edge, several, sp.lo - n0, sp.hi - n0, now.there, lane) || odd;
         fetch_v(next, mask);
         if (edge) {
 #pragma unroll
@@ -912,7 +920,7 @@ __global__ __launch_bounds__(64 * NW, (paged_occupancy<T, ST, NB, NW>())) void a
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int key = n0 + 16 * blk + 4 * quad + e;
-                        s[nb][blk][e] = key <= pq[nb] && key > pq[nb] - weff && (there_now >> blk & 1) ? s[nb][blk][e] : -INFINITY;
+                        s[nb][blk][e] = key <= pq[nb] && key > pq[nb] - weff && (now.there >> blk & 1) ? s[nb][blk][e] : -INFINITY;
                     }
         }
 #pragma unroll
