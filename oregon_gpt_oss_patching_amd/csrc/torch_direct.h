@@ -84,14 +84,14 @@ struct Arguments {
         return t;
     }
     OptTensor optional(int i) { return args[i] == Py_None ? OptTensor() : OptTensor(tensor(i)); }
-    int64_t integer(int i) {        // None: 0
-        if (args[i] == Py_None) return 0;
+    int64_t integer(int i) {
         if (!PyLong_CheckExact(args[i])) return ok = false, 0;
         int overflow = 0;
         const long long x = PyLong_AsLongLongAndOverflow(args[i], &overflow);
         if (overflow) ok = false;
         return x;
     }
+    int64_t integer_or_none(int i) { return args[i] == Py_None ? 0 : integer(i); }        // None: 0, where that says the same
     double number(int i) { return PyFloat_CheckExact(args[i]) ? PyFloat_AS_DOUBLE(args[i]) : (ok = false, 0.0); }
     bool truth(int i) { return PyBool_Check(args[i]) ? args[i] == Py_True : (ok = false); }
     at::ScalarType dtype(int i) { return THPDtype_Check(args[i]) ? reinterpret_cast<THPDtype *>(args[i])->scalar_type : (ok = false, at::kBFloat16); }

@@ -339,7 +339,7 @@ PyObject *fwd_now(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Tensor &q = a.tensor(0), &k_pages = a.tensor(1), &v_pages = a.tensor(2), &table = a.tensor(5), &seqlens = a.tensor(6);
     const OptTensor k_exp = a.optional(3), v_exp = a.optional(4), start = a.optional(7), sinks = a.optional(8);
     const double scale = a.number(9);
-    const int64_t window = a.integer(10), max_len = a.integer(11);
+    const int64_t window = a.integer_or_none(10), max_len = a.integer_or_none(11);
     const bool need_lse = a.truth(12);
     if (!a.ok) return not_implemented();
     Pair out;

@@ -468,3 +468,16 @@ def test_two_launches_captured(A):
         ref, lens, free = T.update(ref, lens, new, pages, ps)
         assert table.tolist() == ref and got.tolist() == lens and left.tolist() == [free], i
         check_update(A, other, [0] * rows, [rng.randint(0, 90) for _ in lens], pages, ps)
+
+
+def test_a_number_left_out_is_refused(A):
+    """None where a whole number belongs (as a window or max_len it means that there is none)."""
+    table, n = ints([[0, 1], [2, -1]]), ints([20, 5])
+    cache = A.paged_cache(4, 2, 16)
+    for call in (lambda: A.token_map(table, n, n, None, 16), lambda: A.token_map(table, n, n, 50, None), lambda: A.page_table_update(table, n, n, None, 16),
+                 lambda: A.page_table_update(table, n, n, 4, None), lambda: A.paged_cache_read(cache, table, n, None)):
+        with pytest.raises(TypeError):
+            call()
+    assert table.tolist() == [[0, 1], [2, -1]]
+    q = torch.randn(2, 4, 1, 64, device=DEV, dtype=BF16)
+    assert torch.equal(A.paged_attention(q, cache, table, n, None, 0.125, None, None, None), A.paged_attention(q, cache, table, n, None, 0.125, 0, None, 0))
