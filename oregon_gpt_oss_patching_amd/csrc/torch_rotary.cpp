@@ -5,8 +5,11 @@
 //
 // Angles come from positions and frequencies, or from tables of their cosines and sines.  Results lie as (B, S, heads, D): the layout of the projection in
 // front of the call and of its gradient, which then need no copy; the attention takes either layout in the same time (16384 tokens and less, both directions).
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include "torch_direct.h"
 
@@ -142,6 +145,19 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     }
 };
 
+// While a graph is recorded, a gradient goes into the autograd node that its tensor has.  A leaf keeps its node, and the stream that it was made on, for as long as any result of
+// the leaf lives; torch lets that stream wait for the gradient.  A node of another stream than the recording one (of an eager result of the same leaf, or of an eager call that made
+// the tensor) so draws that stream into the recording; with the default stream this has ended the process.  Refused where it can be seen: before the forward call.
+void require_recorded(const char *name, const Tensor &t) {
+    if (!at::GradMode::is_enabled() || !wants_gradient(t)) return;
+    const auto node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    if (!stream || *stream == c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device())) return;
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, "rotary: the gradient of ", name,
+                " would leave the graph that is being recorded, for a stream on which ", name, " has an eager result that is still alive (or was made): drop it before recording, ",
+                "or run it on the recording stream");
+}
+
 Pair rotary(const Tensor &q, const Tensor &k, const OptTensor &positions, const OptTensor &frequencies, const OptTensor &cos, const OptTensor &sin, double scale,
             bool interleaved, bool inverse) {
     for (const auto &[name, t] : {std::pair<const char *, const OptTensor &>("frequencies", frequencies), {"cos", cos}, {"sin", sin}})
@@ -152,6 +168,8 @@ Pair rotary(const Tensor &q, const Tensor &k, const OptTensor &positions, const 
         const at::AutoDispatchBelowADInplaceOrView below;
         return call_turn(q, k, positions, frequencies, cos, sin, scale, interleaved, inverse);
     }
+    require_recorded("q", q);
+    require_recorded("k", k);
     const auto out = RotaryFunction::apply(q, k, positions, frequencies, cos, sin, scale, interleaved, inverse);
     return {out[0], out[1]};
 }

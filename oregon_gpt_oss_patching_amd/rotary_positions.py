@@ -99,7 +99,8 @@ def rotary(q, k, positions, rope: Rotary):
     """q (B, H, S, D) and k (B, G, S, D), any strides, D up to 256, turned by their positions' angles: new tensors of the same shapes, whose
     memory is (B, S, heads, D).  `positions`: (B, S), (1, S) or (S) integers, any numbers, negative ones too.
 
-    Differentiable in q and k, any number of times.  float16 goes through float32."""
+    Differentiable in q and k, any number of times.  float16 goes through float32.  While a graph is recorded with a gradient wanted, q and k must not have eager results
+    that are still alive, nor come from an eager call on another stream."""
     if not _ready:
         _register_ops()
     out = NotImplemented if _compiling() else _now(q, k, positions, rope.frequencies, None, None, rope.scale, rope.interleaved)

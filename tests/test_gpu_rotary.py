@@ -339,3 +339,75 @@ def test_transforms_and_changed_positions_are_refused(A):
     at += 1                                    # the gradient would be turned by other angles
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         torch.autograd.grad(out.sum(), x)
+
+
+def test_a_recorded_gradient_that_would_leave_its_graph_is_refused(A):
+    """A leaf with an eager result alive, and a tensor of an eager call: their autograd nodes belong to another stream than the one that records.  The forward call
+    raises, in front of any launch; what else is recorded stays whole, and without a gradient wanted the same tensors are taken."""
+    rope = A.rotary_frequencies(64, 10000.0)
+    gen = torch.Generator().manual_seed(21)
+    at = torch.arange(9, device=DEV)
+    x, k = torch.randn(1, 4, 9, 64, generator=gen).to(DEV).requires_grad_(), torch.randn(1, 2, 9, 64, generator=gen).to(DEV)
+    alive = A.rotary(x, k, at, rope)
+    product = k.clone().requires_grad_() * 2
+    other = torch.randn(1, 4, 9, 64, generator=gen).to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        with pytest.raises(RuntimeError, match="gradient of q .* recorded"):
+            A.rotary(x, k, at, rope)
+        with pytest.raises(RuntimeError, match="gradient of k .* recorded"):
+            A.rotary(other, product, at, rope)
+        with pytest.raises(RuntimeError, match="gradient of q .* recorded"):
+            A.rotary_tables(x, k, torch.ones(1, 9, 32, device=DEV), torch.ones(1, 9, 32, device=DEV))
+        with torch.no_grad():
+            out = A.rotary(x, product, at, rope)
+    for step in range(3):
+        at += step
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            assert all(torch.equal(a, b) for a, b in zip(out, A.rotary(x, product, at, rope))), step
+    # eager, they have their gradients
+    (d,) = torch.autograd.grad(A.rotary(x, k, torch.arange(9, device=DEV), rope)[0], x, other)
+    within(d, other, R.of_positions(torch.arange(9)[None], rope.frequencies.cpu()).conj(), FP32)
+    assert alive[0].requires_grad
+
+
+def test_a_training_step_recorded(A):
+    """Call and gradients by the engine in one graph, of leaves without an eager result, replayed with other inputs, positions and gradients between eager steps of other leaves."""
+    rope = A.rotary_frequencies(64, 150000.0, factor=32.0, original_length=4096)
+    gen = torch.Generator().manual_seed(22)
+
+    def numbers():
+        return [torch.randn(2, n, 33, 64, generator=gen).to(BF16).to(DEV) for n in (8, 2, 8, 2)]
+
+    at = torch.arange(33, device=DEV).expand(2, 33).clone()
+
+    def step(q, k, gq, gk):
+        out = A.rotary(q, k, at, rope)
+        return (*out, *torch.autograd.grad(out, (q, k), (gq, gk)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        q, k, gq, gk = numbers()
+        step(q.requires_grad_(), k.requires_grad_(), gq, gk)
+    side.synchronize()
+    q, k, gq, gk = numbers()
+    q.requires_grad_(), k.requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = step(q, k, gq, gk)
+    for i in range(4):
+        with torch.no_grad():
+            for t, new in zip((q, k, gq, gk), numbers()):
+                t.copy_(new)
+        at += 311 * i
+        for t in out:
+            t.detach().fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(q.detach().clone().requires_grad_(), k.detach().clone().requires_grad_(), gq, gk)
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), i
