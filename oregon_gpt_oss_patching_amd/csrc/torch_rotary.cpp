@@ -131,6 +131,11 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["interleaved"] = interleaved;
         ctx->saved_data["inverse"] = inverse;
+        // (a result asks for a gradient where its own tensor does: keys that go into a cache while the queries are trained must not)
+        torch::autograd::variable_list plain;
+        if (!wants_gradient(q)) plain.push_back(qo);
+        if (!wants_gradient(k)) plain.push_back(ko);
+        ctx->mark_non_differentiable(plain);
         return {qo, ko};
     }
 

@@ -180,6 +180,24 @@ def test_one_gradient_of_two(A):
     assert float((d.cpu().double() - want).abs().max()) < 10 * 31 * 2.0 ** -24 * max(float(gq.abs().max()), float(g.abs().max()))
 
 
+def test_one_tensor_of_two_with_a_gradient(A):
+    """The other's result has none: it can go into a cache while gradients are on, and the one gradient is what it is beside the other."""
+    rope = A.rotary_frequencies(64, 10000.0)
+    gen = torch.Generator().manual_seed(29)
+    at, z = torch.arange(16, device=DEV), R.of_positions(torch.arange(16)[None], rope.frequencies.cpu())
+    q, k = torch.randn(1, 4, 16, 64, generator=gen).to(BF16).to(DEV).requires_grad_(), torch.randn(1, 2, 16, 64, generator=gen).to(BF16).to(DEV)
+    g = torch.randn(1, 4, 16, 64, generator=gen).to(BF16).to(DEV)
+    for call in (A.rotary, torch.compile(A.rotary, backend="aot_eager", fullgraph=True)):
+        oq, ok = call(q, k, at, rope)
+        assert oq.requires_grad and not ok.requires_grad
+        within(ok, k, z, BF16)
+        (d,) = torch.autograd.grad(oq, q, g)
+        within(d, g, z.conj(), BF16)
+    cache = A.paged_cache(1, 2, 16)
+    A.paged_cache_write(cache, ok, k, torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV))
+    assert torch.equal(cache.k[0], ok[0]) and torch.equal(cache.v[0], k[0])
+
+
 def test_second_derivative_and_differences(A):
     rope = A.rotary_frequencies(8, 100.0, attention_factor=1.3, interleaved=True)
     gen = torch.Generator().manual_seed(10)

@@ -135,6 +135,15 @@ def test_traced_shapes_stay_symbols():
     assert not env.replacements and not [g for g in env.guards if "Eq" in str(g.expr)]
 
 
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_result_asks_for_a_gradient_where_its_tensor_does(which):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = [torch.empty((2, n, 5, 64), dtype=torch.bfloat16, device="cuda", requires_grad=i == which) for i, n in enumerate((8, 2))]
+        out = A.rotary(*x, torch.empty((2, 5), dtype=torch.int64, device="cuda"), A.Rotary(torch.empty(32, dtype=torch.float64, device="cuda")))
+    assert [y.requires_grad for y in out] == [which == 0, which == 1]
+
+
 def test_the_models_function_is_swapped_and_put_back():
     M = pytest.importorskip("transformers.models.gpt_oss.modeling_gpt_oss")
     from oregon_gpt_oss_patching_amd.patching import patch_flash_attention, unpatch_flash_attention
