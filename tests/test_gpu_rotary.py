@@ -429,3 +429,46 @@ def test_a_training_step_recorded(A):
         torch.cuda.synchronize()
         want = step(q.detach().clone().requires_grad_(), k.detach().clone().requires_grad_(), gq, gk)
         assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+def _c_call(q, k, qo, ko, positions, frequencies, scale, interleaved, inverse, stride_of_one=None):
+    """The C interface on tensors (B, heads, S, D) as they lie; `stride_of_one`: what is said of the tokens' stride where a row has one token."""
+    import ctypes
+
+    from oregon_gpt_oss_patching_amd import _lib
+    p = _lib.RotaryParams()
+    p.struct_size = ctypes.sizeof(p)
+    p.dtype = _lib.DTYPE_FP32 if q.dtype == FP32 else _lib.DTYPE_BF16
+    p.B, p.H, p.S, p.D = q.shape
+    p.G, p.R, p.position_bytes = k.shape[1], 2 * frequencies.numel(), positions.element_size()
+    p.interleaved, p.inverse, p.scale = interleaved, inverse, scale
+    p.positions, p.frequencies = positions.data_ptr(), frequencies.data_ptr()
+    p.position_stride_b, p.position_stride_s = positions.stride()
+    for name, t in (("q", q), ("k", k), ("q_out", qo), ("k_out", ko)):
+        assert t.stride(3) == 1
+        setattr(p, name, t.data_ptr())
+        s = getattr(p, name + "_stride")
+        s.b, s.h, s.s = t.stride(0), t.stride(1), t.stride(2) if stride_of_one is None else stride_of_one
+    rc = _lib.load().gptoss_attn_rotary(ctypes.byref(p), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0, rc
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "pairs"])
+@pytest.mark.parametrize("b,h,g,s,d,r", [(5, 7, 3, 1, 64, 64), (1, 1, 1, 1, 64, 32), (2, 7, 3, 33, 80, 32), (3, 3, 2, 17, 66, 6), (1, 13, 5, 2500, 64, 64), (2, 13, 5, 3000, 64, 48)])
+def test_in_place_through_the_c_interface(A, b, h, g, s, d, r, interleaved, dtype):
+    """q and k themselves as results, tokens or heads outermost, both directions: the bits of results of their own."""
+    print(f"case B={b} H={h} G={g} S={s} D={d} R={r} interleaved={interleaved} {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(b + s)
+    rope = A.rotary_frequencies(r, 150000.0, attention_factor=1.25, interleaved=interleaved)
+    positions = torch.randint(0, 9000, (b, s), generator=gen).to(DEV)
+    for tokens_outermost in (True, False):
+        def numbers(n):
+            x = torch.randn(b, s, n, d, generator=gen).to(dtype).to(DEV)
+            return x.transpose(1, 2) if tokens_outermost else x.transpose(1, 2).contiguous()
+        q, k = numbers(h), numbers(g)
+        want = A.rotary(q, k, positions, rope)
+        back = torch.ops.gptoss_attn.rotary(*want, positions, rope.frequencies, None, None, rope.scale, interleaved, True)
+        for inverse, expect in ((False, want), (True, back)):
+            _c_call(q, k, q, k, positions, rope.frequencies, rope.scale, interleaved, inverse)
+            assert torch.equal(q, expect[0]) and torch.equal(k, expect[1]), (tokens_outermost, inverse)
