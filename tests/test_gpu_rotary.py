@@ -472,3 +472,21 @@ def test_in_place_through_the_c_interface(A, b, h, g, s, d, r, interleaved, dtyp
         for inverse, expect in ((False, want), (True, back)):
             _c_call(q, k, q, k, positions, rope.frequencies, rope.scale, interleaved, inverse)
             assert torch.equal(q, expect[0]) and torch.equal(k, expect[1]), (tokens_outermost, inverse)
+
+
+@pytest.mark.parametrize("stride", [0, 64, 4096, 1 << 30])
+def test_rows_of_one_token_whatever_their_stride(A, stride):
+    """Of one token a row, what is said of the way to the next one is not looked at."""
+    rope = A.rotary_frequencies(64, 150000.0)
+    gen = torch.Generator().manual_seed(31)
+    positions = torch.randint(0, 9000, (300, 1), generator=gen).to(DEV)
+    for transposed in (True, False):
+        q, k = (torch.randn(300, n, 1, 64, generator=gen).to(BF16).to(DEV) for n in (64, 8))
+        if transposed:                             # heads far apart, rows next to each other
+            q, k = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k))
+        want = A.rotary(q, k, positions, rope)
+        out = [torch.full_like(x, float("nan")) for x in (q, k)]
+        _c_call(q, k, *out, positions, rope.frequencies, rope.scale, False, False, stride)
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+        for got, x in zip(want, (q, k)):
+            within(got, x, R.of_positions(positions.cpu(), rope.frequencies.cpu()), BF16)
