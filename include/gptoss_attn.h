@@ -442,7 +442,9 @@ typedef struct gptoss_attn_table_params {
 
 /*
  * Rows of have[b] tokens get pages for want[b].  A row keeps its first ceil(min(have, want) / page_size) entries; every page that no
- * kept entry names is free, so rows that share one keep it until the last of them gives it back.  Rows that grow get the free pages
+ * kept entry names is free, so rows that share one keep it until the last of them gives it back.  (Only full pages may be shared by rows
+ * that grow: a row's next token goes into its last page where that has room, whoever else has it.  Nothing is copied, and nothing checks
+ * it; a row that has shrunk into a shared page must not grow again.)  Rows that grow get the free pages
  * in ascending order, row by row; seqlens[b] = want[b].  Where the pages a row wants, with those of the rows in front of it, are more
  * than are free, the row gets none, nor does any behind it that wants some: their entries stay and seqlens[b] = have[b], as where a row wants
  * more than its table holds (which no other row suffers from).  Entries that a row gives back become -1; others are not touched.

@@ -7,7 +7,9 @@ A scheduler that keeps its lengths on the GPU never has to wait for it: pages ar
     paged_cache_write_tokens(cache, k, v, tokens.slot)                                 # k, v (total, G, 64)
 
 A page is free iff no row keeps an entry that names it: there is no list of free pages beside the tables, and rows may share pages (a common prefix
-copied from one row of the table into another) until the last of them gives them back.
+copied from one row of the table into another) until the last of them gives them back.  Only full pages: a row's next token goes into its last page where that has room, whoever else
+has it.  Where a common prefix ends inside a page, give the new row a page of its own for the rest (an update from the full pages' tokens on) and copy that page's rows in the caches;
+and do not let a row that has shrunk into a shared page grow again.  Nothing checks this: such rows overwrite each other's keys and values.
 
 The reference has no counterpart (its generate.py:1-30 leaves the cache to transformers).
 """

@@ -481,3 +481,46 @@ def test_a_number_left_out_is_refused(A):
     assert table.tolist() == [[0, 1], [2, -1]]
     q = torch.randn(2, 4, 1, 64, device=DEV, dtype=BF16)
     assert torch.equal(A.paged_attention(q, cache, table, n, None, 0.125, None, None, None), A.paged_attention(q, cache, table, n, None, 0.125, 0, None, 0))
+
+
+@pytest.mark.parametrize("storage", [BF16, E4M3, torch.float4_e2m1fn_x2], ids=["bf16", "e4m3", "e2m1"])
+def test_rows_that_share_whole_pages_grow_apart(A, storage):
+    """Two rows over one prefix of whole pages, a third over a prefix whose last page, not full, it has copied: all grow by update, map and write, then the first ends.
+    Each reads back the prefix as it was and its own tokens."""
+    ps, g, pages, gen = 16, 2, 24, torch.Generator().manual_seed(17)
+    cache, prefix = A.paged_cache(pages, g, ps, storage), 40
+    table, zero = torch.full((3, 6), -1, dtype=torch.int32, device=DEV), ints([0])
+    first, _ = A.page_table_update(table[:1], zero, ints([prefix]), pages, ps)
+    common = torch.randn(2, prefix, g, 64, generator=gen).to(BF16).to(DEV)
+    at = A.token_map(table[:1], zero, first, prefix, ps)
+    A.paged_cache_write_tokens(cache, common[0], common[1], at.slot)
+    # rows 1 and 2 begin with row 0's two full pages; row 2 has the 8 tokens behind them in a page of its own
+    table[1:, :2] = table[0, :2]
+    have = ints([prefix, 32, 32])
+    have, _ = A.page_table_update(table, have, ints([prefix, 32, prefix]), pages, ps)
+    own = table[2, 2].item()
+    assert own not in table[0].tolist()
+    for pool in cache:
+        if pool is not None:
+            pool = pool.view(torch.uint8) if pool.element_size() == 1 else pool
+            pool[own] = pool[table[0, 2].long()]
+    lens = [40, 32, 40]
+    rows = [common[:, :n] for n in lens]
+    for want in ([53, 61, 40], [54, 90, 71], [0, 91, 96]):
+        counts = [max(0, w - n) for n, w in zip(lens, want)]
+        got, _ = A.page_table_update(table, have, ints(want), pages, ps)
+        assert got.tolist() == want
+        new = torch.randn(2, sum(counts), g, 64, generator=gen).to(BF16).to(DEV)
+        tokens = A.token_map(table, have, ints(counts), sum(counts) + 1, ps)
+        A.paged_cache_write_tokens(cache, torch.cat((new[0], new[0, :1])), torch.cat((new[1], new[1, :1])), tokens.slot)
+        pieces = list(new.split(counts, 1))
+        rows = [torch.cat((r, p), 1) if w else r[:, :0] for r, p, w in zip(rows, pieces, want)]
+        have, lens = got, want
+        k, v = A.paged_cache_read(cache, table, have, 96)
+        for b, n in enumerate(lens):
+            for read, x in ((k, rows[b][0]), (v, rows[b][1])):
+                # (what a cache of its own makes of the same tokens)
+                alone = A.paged_cache(6, g, ps, storage)
+                A.paged_cache_write_tokens(alone, x, x, torch.arange(n, device=DEV))
+                want_b = A.paged_cache_read(alone, torch.arange(6, dtype=torch.int32, device=DEV)[None], ints([n]), 96)[0][0]
+                assert torch.equal(read[b], want_b), (b, n)
