@@ -470,7 +470,7 @@ int gptoss_attn_table_validate(const gptoss_attn_table_params *params, int call)
  * The embedding that the model applies to q and k in front of the attention (the reference leaves it to transformers'
  * apply_rotary_pos_emb).  Token (b, s) has an angle for each pair i < R/2 of a head's first R numbers:
  *   angle = positions[b][s] * frequencies[i] (radians, in 64 bits), c = scale * cos(angle), s = scale * sin(angle),
- * or c and s come from tables; with x1, x2 = numbers i and R/2 + i of the head (`interleaved`: 2i and 2i + 1),
+ * or c and s come from tables (an angle's roundings, 3 * 2^-53 of it, are 2^-24 at 2^27 radians and grow with it); with x1, x2 = numbers i and R/2 + i of the head (`interleaved`: 2i and 2i + 1),
  *   y1 = c x1 - s x2,  y2 = c x2 + s x1
  * in 32 bits, rounded once.  `inverse`: with -s, which is what gradients go through (and, with a scale of 1, the way
  * back).  Numbers behind the first R are copied.

@@ -39,7 +39,8 @@ constexpr int kPagedWaves = 4;
 template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_tile_blocks() {
     return sizeof(ST) == 4 ? (NB > 1 ? 1 : 2) : sizeof(ST) == 1 && !is_e2m1<ST> && NB == 1 && NW == kPagedWaves ? 4 : 2;
 }
-// Wavefronts per SIMD, of what the registers leave.
+// Wavefronts per SIMD that a kernel's registers have to leave room for, and that the division of the work counts with.  (Over e2m1 pages two column blocks take 117 registers, and float32
+// queries on one 116: a fourth fits there, which is not counted.)
 template <typename T, typename ST, int NB, int NW> __host__ __device__ constexpr int paged_occupancy() {
     return sizeof(ST) == 4 ? (NB == 2 && NW == kPagedWaves ? 3 : 2) : sizeof(T) == 4 ? 3 : NB == 1 ? (is_e2m1<ST> && NW == kPagedWaves ? 5 : 4) : NB == 2 || (NB == 3 && sizeof(ST) == 1) ? 3 : 2;
 }
@@ -213,7 +214,8 @@ __device__ __forceinline__ uint32_t lane_offset(uint32_t at, uint32_t mask) {
 
 // kOnce: rows that no other workgroup reads bypass the caches' retention, us without / with: 16 x 8192 tokens 54.6 / 47.3, 4 x 65536 101 / 87.2 (6.2 TB/s), 64 rows of 150
 // to 16384 96.7 / 84.8, 32 of 6000 to 16384 in e4m3 74.8 / 66.2.  A row of more pairs than a workgroup takes is read again by the next one (NB = 4, and two
-// blocks in 32 bits).
+// blocks in 32 bits).  Short calls over e2m1 pages, whose units have fewer pairs (paged_division), have their rows read again as well, and the caches have them either way: us without / with,
+// 2 x 700 tokens with 64 queries of eight heads on each KV head 10.1 / 10.0, 64 windows of 128 keys with eight queries 11.2 / 11.2, 8 x 300 tokens with eight 5.9 / 5.9.
 // A tile's K and V as they are loaded, and what is done with them.  `kb` / `vb`: scalar addresses of the first row of a block of 16 keys;
 // lanes: l16 = lane % 16, quad = lane / 16.
 template <typename T, typename ST, int NB, int KB> struct PagedTile;
@@ -471,7 +473,8 @@ struct PagedTile16 : PagedProducts16<T, NB, KB> {
 
 // e2m1 pages: rows of 32 bytes and two bytes of exponents.  A load takes 32 rows, two blocks of keys, 16 bytes (32 numbers, which share a power) to a lane: of K, lanes below 32
 // have halves of the first block's rows, those above of the second's; of V, rows in the order in which 16 lanes write to distinct banks.  In pages of 16 tokens (ST = e2m1_of_16)
-// the two blocks lie in two of them, and each lane's addresses are of its half's page: 48 rows of 300 to 30000 tokens 46.0 us, in pages of 64, whose addresses are scalar, 44.1.
+// the two blocks lie in two of them, and each lane's addresses are of its half's page: 48 rows of 300 to 30000 tokens, three caches in turn, 47.0 us, in pages of 64 or 32, whose addresses are scalar,
+// 45.3.
 // Tiles of 32 keys and five wavefronts a SIMD: with 64 and four one row of 2049 tokens takes 9.3 us and not 8.5 (two of four wavefronts have a tile of a share), 16 x 8192 23.1 / 22.8,
 // 32 x 16384 59.1 / 59.4.  Measured and not kept: a second tile under way (24.5 for 22.8: registers and no gain, the wait is not for memory), eight pairs in sixteen columns by
 // taking two blocks' keys into one contraction (a third fewer vector operations, 22.9).

@@ -35,7 +35,8 @@ struct RotaryArgs {
 
 // c = cos(u pi / 2), s = sin(u pi / 2).  The whole quarters come off in 64 bits, what is left is at most half of one: polynomials (the Taylor series, whose
 // first term left out is below 2^-29 there) in 32 bits.  Off by at most 4 * 2^-24: the argument's rounding, the leading constant's and the last
-// multiplication's and addition's.
+// multiplication's and addition's.  u itself, a position times (a frequency times 2 / pi), has been rounded three times in 64 bits: the angle is off by up to 3 * 2^-53 of itself, which
+// is 2^-24 more at 2^27 radians and grows with them (and positions beyond 2^53 are not held exactly).
 __device__ __forceinline__ void quarter_turns(double u, float &c, float &s) {
     const double n = __builtin_rint(u);
     const float f = (float)(u - n), f2 = f * f;

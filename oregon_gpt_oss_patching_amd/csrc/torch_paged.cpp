@@ -90,6 +90,9 @@ void fill(PagedCall &c, const Tensor &k_pages, const Tensor &v_pages, const OptT
     p.page_table = c.table.const_data_ptr<int32_t>();
 }
 
+// (float16 is bfloat16 to these calls, which the attention computes with in any case.  Into codes that rounds twice: a number within 2^-9 of itself of the middle between two codes counts as
+// that middle, so it may come back 2^-9 of itself further off than from the nearer one; the code's own half step is 2^-4 or 2^-2.)
+
 // Rows (B, G, S, 64) or (B, H, S, 64) as the kernels take them, and their strides; a dimension of one element has a stride that says nothing.  What is laid out
 // otherwise is copied (a copy that is one: `contiguous` gives such a tensor back as it is, on whatever address).
 Tensor rows_of(const Tensor &t, gptoss_attn_strides &s) {

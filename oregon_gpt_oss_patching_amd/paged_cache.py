@@ -51,7 +51,7 @@ class PagedState(NamedTuple):
     seqlens (B): tokens of each row with the new ones.  counts (B): how many of the call's S tokens a row has, where not all have S, the rest being
     padding (start=None: seqlens).  max_len: as in `paged_attention`.
     tokens: a `TokenMap` where the call is one batch row that holds new rows' tokens back to back (start=None, and the map made with starts of 0): the model gets
-    tokens.position as its position ids."""
+    tokens.position as its position ids.  (A chunk behind a row's past is a batch row of its own, with start and counts: the attention over pages takes no queries back to back.)"""
     caches: Sequence[PagedCache]
     page_table: torch.Tensor
     start: Optional[torch.Tensor]
@@ -146,7 +146,8 @@ def _ints(x, like):
 def paged_cache_write(cache: PagedCache, k, v, page_table, start, seqlens=None) -> None:
     """Writes new tokens: k, v (B, G, S, 64), any strides; token i of row b goes to position start[b] + i.  `seqlens`: how many of its S
     tokens each row has, the rest being padding, which is not written.  Positions in front of 0, behind the table, or on an entry that
-    names no page are dropped; nothing else of the cache is touched.  float16 tensors are rounded to bfloat16 on the way in.
+    names no page are dropped; nothing else of the cache is touched.  float16 tensors are rounded to bfloat16 on the way in, in front of the rounding to codes as well (what is said of a code's
+    distance is of the bfloat16 number; a caller who wants float16 numbers rounded once passes them as float32).
 
     Two rows of one call must not write the same slot, and nothing that runs at the same time may read what is being written."""
     if not _ready:

@@ -117,7 +117,8 @@ def rotary_tables(q, k, cos, sin, interleaved=False):
 
 def hip_rotary_pos_emb(q, k, cos, sin, unsqueeze_dim=1):
     """Drop-in for transformers' `modeling_gpt_oss.apply_rotary_pos_emb`: cos and sin (B, S, D / 2); q and k (B, heads, S, D), or with
-    `unsqueeze_dim=2` (B, S, heads, D).  The products are in 32 bits and rounded once, where the eager code rounds each to the model's type."""
+    `unsqueeze_dim=2` (B, S, heads, D).  The products are in 32 bits and rounded once, where the eager code rounds each to the model's type.
+    Results are of q's and k's type, whatever the tables' (the eager code's are of the wider one: of bfloat16 under autocast with float32 tables, float32)."""
     if unsqueeze_dim == 1:
         return rotary_tables(q, k, cos, sin)
     if unsqueeze_dim != 2:

@@ -614,3 +614,16 @@ def test_float16_goes_through_bfloat16(A):  # noqa: F811
     assert o.dtype == torch.float16 and torch.equal(o, A.paged_attention(half.to(BF16), cache, table, n, sinks, 0.125).to(torch.float16))
     got = A.paged_cache_read(cache, table, n, 70, dtype=torch.float16)
     assert all(x.dtype == torch.float16 and torch.equal(x, y.to(torch.float16)) for x, y in zip(got, A.paged_cache_read(cache, table, n, 70)))
+
+
+def test_float16_beside_a_tie(A):  # noqa: F811
+    """What the documents say of float16 numbers next to the middle between two codes: as they are, rounded to bfloat16 first; as float32, to the nearest code of their own."""
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    row = torch.cat([t * (1 + torch.tensor([-2.0, -1.0, 1.0, 2.0]) * 2.0 ** -10) for t in ties] + [torch.tensor([6.0, 0.0, 1.0, 2.0])])
+    x = torch.cat([row, -row]).to(torch.float16).view(1, 1, 64).to(DEV)
+    table, n = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    for given, counts in ((x, x.to(BF16)), (x.float(), x)):
+        cache = A.paged_cache(1, 1, 16, E2M1)
+        A.paged_cache_write_tokens(cache, given, given, torch.zeros(1, dtype=torch.int64, device=DEV))
+        got = A.paged_cache_read(cache, table, n, 1, None, FP32)[0].cpu().double().view(64)
+        assert torch.equal(got, P.stored_rows(counts.cpu().view(1, 64), E2M1)[0])
