@@ -152,13 +152,21 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
 
 // While a graph is recorded, a gradient goes into the autograd node that its tensor has.  A leaf keeps its node, and the stream that it was made on, for as long as any result of
 // the leaf lives; torch lets that stream wait for the gradient.  A node of another stream than the recording one (of an eager result of the same leaf, or of an eager call that made
-// the tensor) so draws that stream into the recording; with the default stream this has ended the process.  Refused where it can be seen: before the forward call.
+// the tensor) so draws that stream into the recording; this has ended the process.  Refused where it can be seen: before the forward call.
 void require_recorded(const char *name, const Tensor &t) {
     if (!at::GradMode::is_enabled() || !wants_gradient(t)) return;
     const auto node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
     const auto stream = node ? node->stream() : std::nullopt;
-    if (!stream || *stream == c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device())) return;
-    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, "rotary: the gradient of ", name,
+    const c10::impl::VirtualGuardImpl streams(t.device().type());
+    const auto recorded = [] { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; };
+    if (!stream || *stream == streams.getStream(t.device()) || !recorded()) return;
+    // (a stream that has joined the recording is as good; the default stream cannot, and must not be asked)
+    bool joined = false;
+    if (*stream != streams.getDefaultStream(t.device())) {
+        const c10::StreamGuard on(*stream);
+        joined = recorded();
+    }
+    TORCH_CHECK(joined, "rotary: the gradient of ", name,
                 " would leave the graph that is being recorded, for a stream on which ", name, " has an eager result that is still alive (or was made): drop it before recording, ",
                 "or run it on the recording stream");
 }

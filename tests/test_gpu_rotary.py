@@ -490,3 +490,28 @@ def test_rows_of_one_token_whatever_their_stride(A, stride):
         assert all(torch.equal(x, y) for x, y in zip(out, want))
         for got, x in zip(want, (q, k)):
             within(got, x, R.of_positions(positions.cpu(), rope.frequencies.cpu()), BF16)
+
+
+def test_queries_of_a_stream_that_has_joined_the_recording(A):
+    """A graph over two streams: q is computed on one and turned on the other, with a gradient wanted."""
+    rope = A.rotary_frequencies(64, 10000.0)
+    gen = torch.Generator().manual_seed(23)
+    at = torch.arange(9, device=DEV)
+    x, k = (torch.randn(1, n, 9, 64, generator=gen).to(DEV) for n in (4, 2))
+    with torch.no_grad():
+        A.rotary(x * 2, k, at, rope)
+    leaf = x.clone().requires_grad_()
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        other.wait_stream(side)
+        with torch.cuda.stream(other):
+            q = leaf * 2
+        side.wait_stream(other)
+        out = A.rotary(q, k, at, rope)
+    for step in range(3):
+        at += step
+        graph.replay()
+        torch.cuda.synchronize()
+        assert out[0].requires_grad and all(torch.equal(a, b) for a, b in zip(out, A.rotary(x * 2, k, at, rope))), step
